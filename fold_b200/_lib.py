@@ -29,6 +29,10 @@ SIGNATURES = {
                           _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _vp],
     "fold_far_query": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _i32, _i32,
                        _i32, _i32, _vp, _vp],
+    "fold_rotary": [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i64,
+                    _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp],
+    "fold_append_paged": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _vp, _vp, _i64, _i32, _i64, _i64, _i64,
+                          _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp],
     "fold_rerope_query": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _i32,
                           _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _vp],
     "fold_far_read": [_vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i64, _i64, _vp, _vp, _i64, _i64, _vp,

@@ -1,0 +1,333 @@
+// Rotary positions (fold_rotary) and the append of keys and values to a paged cache with the
+// rotation applied on the way (fold_append_paged).
+//
+// A pair (lo, hi) of a row at position p turns by the angle p * f_i:
+//   lo' = lo cos - hi sin,   hi' = hi cos + lo sin      (inverse: sin negated, the transpose)
+// with cos and sin taken from a float32 table formed in float64 (row p: cos then sin, both times
+// the attention factor of scaled frequencies). Pairs are (i, i + rot/2) or, interleaved,
+// (2i, 2i+1); dims past rot pass through. Arithmetic is float32 with one rounding to the type.
+//
+// Bound: HBM bytes, each row read once and written once; a token's table row is shared by all its
+// heads. So one thread owns one unit, two 16-byte chunks that hold whole pairs (chunk c of each
+// half; two neighbouring chunks when interleaved or passed through), of HU heads of one token: the
+// table values are loaded once for the HU heads, and 2 * HU 16-byte loads are in flight.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "host_common.h"
+
+namespace fold {
+namespace {
+
+struct RopeRows {  // rows [n, heads, hd] with the innermost dim contiguous
+  const void* in;
+  void* out;
+  int64_t in_st, in_sh, out_st, out_sh;
+  int heads;
+};
+
+struct RopeParams {
+  RopeRows q, k, v;  // v.heads = 0 outside the append
+  const int64_t* positions;
+  const int64_t* slots;  // null: k goes to its out rows; else k and v go to the cache
+  int64_t num_slots, cs_block, cs_head, cs_slot;
+  int block_size;
+  const float* table;  // null: nothing is rotated
+  int64_t table_rows;
+  int n, hd, rot;
+  float sgn;  // -1: the transposed rotation
+  int* err;
+};
+
+template <class T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f32(float x) { return x; }
+template <class T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ float from_f32(float x) { return x; }
+
+template <class T>
+union Chunk {
+  uint4 raw;
+  T e[16 / sizeof(T)];
+};
+
+// The table row of token t (a position outside the table is clamped and reported).
+__device__ __forceinline__ const float* table_row(const RopeParams& p, int t) {
+  if (!p.table) return nullptr;
+  int64_t pos = __ldg(p.positions + t);
+  if (pos < 0 || pos >= p.table_rows) {
+    set_error(p.err, FOLD_DEVERR_ROPE_RANGE);
+    pos = pos < 0 ? 0 : p.table_rows - 1;
+  }
+  return p.table + pos * p.rot;
+}
+
+// Source and destination rows of head hh of token t, heads counted q, then k, then v. No
+// destination (false): the token's slot is negative or outside the cache.
+template <class T>
+__device__ __forceinline__ bool locate(const RopeParams& p, int t, int hh, const T*& src, T*& dst) {
+  const bool is_q = hh < p.q.heads;
+  const RopeRows& r = is_q ? p.q : hh < p.q.heads + p.k.heads ? p.k : p.v;
+  const int h = is_q ? hh : hh < p.q.heads + p.k.heads ? hh - p.q.heads : hh - p.q.heads - p.k.heads;
+  src = static_cast<const T*>(r.in) + t * r.in_st + h * r.in_sh;
+  if (is_q || !p.slots) {
+    dst = static_cast<T*>(r.out) + t * r.out_st + h * r.out_sh;
+    return true;
+  }
+  const int64_t slot = __ldg(p.slots + t);
+  if (slot < 0) return false;
+  if (slot >= p.num_slots) {
+    set_error(p.err, FOLD_DEVERR_APPEND_RANGE);
+    return false;
+  }
+  const int64_t block = (slot >> 32) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(slot) /
+                                                                 static_cast<uint32_t>(p.block_size))
+                                          : slot / p.block_size;
+  dst = static_cast<T*>(r.out) + block * p.cs_block + h * p.cs_head + (slot - block * p.block_size) * p.cs_slot;
+  return true;
+}
+
+// One thread per (token, group of HU heads, unit); neighbouring threads walk a row's units.
+template <class T, bool INTER, int HU>
+__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
+  constexpr int E = 16 / sizeof(T);
+  if (p.q.heads == 0) release_dependents();  // no query is written: a read behind may load its own early
+  const int units = p.hd / (2 * E), runits = p.table ? p.rot / (2 * E) : 0;
+  const int heads = p.q.heads + p.k.heads + p.v.heads, groups = (heads + HU - 1) / HU;
+  const int rotated = p.q.heads + p.k.heads;  // v is stored as it is
+  const int64_t total = static_cast<int64_t>(p.n) * groups * units;
+  for (int64_t idx = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; idx < total;
+       idx += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    // one 64-bit division a thread at most, none where the product fits 32 bits
+    int t, rest;
+    const int per = groups * units;
+    if ((idx >> 32) == 0) {
+      t = static_cast<int>(static_cast<uint32_t>(idx) / static_cast<uint32_t>(per));
+      rest = static_cast<int>(static_cast<uint32_t>(idx) - static_cast<uint32_t>(t) * static_cast<uint32_t>(per));
+    } else {
+      t = static_cast<int>(idx / per), rest = static_cast<int>(idx - static_cast<int64_t>(t) * per);
+    }
+    const int g = rest / units, c = rest - g * units;
+    const bool turn = c < runits;
+    // element offsets of the unit's two chunks
+    int a, b;
+    if (turn && !INTER) a = c * E, b = (p.rot >> 1) + c * E;
+    else if (turn) a = 2 * c * E, b = a + E;
+    else a = runits * 2 * E + 2 * (c - runits) * E, b = a + E;
+
+    Chunk<T> x[HU], y[HU];
+    T* dst[HU];
+    bool live[HU];
+#pragma unroll
+    for (int j = 0; j < HU; ++j) {
+      const T* src = nullptr;
+      const int hh = g * HU + j;
+      live[j] = hh < heads && locate<T>(p, t, hh, src, dst[j]);
+      if (live[j]) {
+        x[j].raw = *reinterpret_cast<const uint4*>(src + a);
+        y[j].raw = *reinterpret_cast<const uint4*>(src + b);
+      }
+    }
+    float cs[E], sn[E];
+    if (turn && g * HU < rotated) {
+      const float* row = table_row(p, t);
+      const float4* tc = reinterpret_cast<const float4*>(row + c * E);
+      const float4* ts = reinterpret_cast<const float4*>(row + (p.rot >> 1) + c * E);
+#pragma unroll
+      for (int i = 0; i < E / 4; ++i) {
+        const float4 u = __ldg(tc + i), w = __ldg(ts + i);
+        cs[4 * i] = u.x, cs[4 * i + 1] = u.y, cs[4 * i + 2] = u.z, cs[4 * i + 3] = u.w;
+        sn[4 * i] = p.sgn * w.x, sn[4 * i + 1] = p.sgn * w.y, sn[4 * i + 2] = p.sgn * w.z, sn[4 * i + 3] = p.sgn * w.w;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < HU; ++j) {
+      if (!live[j]) continue;
+      if (turn && g * HU + j < rotated) {
+        Chunk<T> ox, oy;
+        if constexpr (INTER) {  // pair i of the unit: elements 2i, 2i + 1 of the two chunks in a row
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            const Chunk<T>& s = i < E / 2 ? x[j] : y[j];
+            Chunk<T>& o = i < E / 2 ? ox : oy;
+            const int e = 2 * (i < E / 2 ? i : i - E / 2);
+            const float lo = to_f32(s.e[e]), hi = to_f32(s.e[e + 1]);
+            o.e[e] = from_f32<T>(lo * cs[i] - hi * sn[i]);
+            o.e[e + 1] = from_f32<T>(hi * cs[i] + lo * sn[i]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < E; ++i) {
+            const float lo = to_f32(x[j].e[i]), hi = to_f32(y[j].e[i]);
+            ox.e[i] = from_f32<T>(lo * cs[i] - hi * sn[i]);
+            oy.e[i] = from_f32<T>(hi * cs[i] + lo * sn[i]);
+          }
+        }
+        x[j] = ox, y[j] = oy;
+      }
+      *reinterpret_cast<uint4*>(dst[j] + a) = x[j].raw;
+      *reinterpret_cast<uint4*>(dst[j] + b) = y[j].raw;
+    }
+  }
+}
+
+// Rows that 16-byte units do not cover (odd head or rotated sizes, unaligned strides): one thread
+// per pair, and per passed-through element, of one head.
+template <class T, bool INTER>
+__global__ void __launch_bounds__(256) rope_scalar_kernel(const RopeParams p) {
+  if (p.q.heads == 0) release_dependents();
+  const int rot = p.table ? p.rot : 0, half = rot >> 1, units = half + p.hd - rot;
+  const int heads = p.q.heads + p.k.heads + p.v.heads, rotated = p.q.heads + p.k.heads;
+  const int64_t total = static_cast<int64_t>(p.n) * heads * units;
+  for (int64_t idx = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; idx < total;
+       idx += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t row = idx / units;
+    const int c = static_cast<int>(idx - row * units);
+    const int t = static_cast<int>(row / heads), hh = static_cast<int>(row - static_cast<int64_t>(t) * heads);
+    const T* src;
+    T* dst;
+    if (!locate<T>(p, t, hh, src, dst)) continue;
+    if (c >= half) {  // passed through
+      dst[rot + c - half] = src[rot + c - half];
+      continue;
+    }
+    const int a = INTER ? 2 * c : c, b = INTER ? 2 * c + 1 : c + half;
+    T x = src[a], y = src[b];
+    if (hh < rotated) {
+      const float* tr = table_row(p, t);
+      const float lo = to_f32(x), hi = to_f32(y), cs = __ldg(tr + c), sn = p.sgn * __ldg(tr + half + c);
+      x = from_f32<T>(lo * cs - hi * sn), y = from_f32<T>(hi * cs + lo * sn);
+    }
+    dst[a] = x, dst[b] = y;
+  }
+}
+
+// Whether every row of r starts on a 16-byte boundary (es: element size).
+bool rows_aligned(const RopeRows& r, int es, bool with_out) {
+  if (r.heads == 0) return true;
+  const int e = 16 / es;
+  return aligned16(r.in) && r.in_st % e == 0 && r.in_sh % e == 0 &&
+         (!with_out || (aligned16(r.out) && r.out_st % e == 0 && r.out_sh % e == 0));
+}
+
+template <class T, bool INTER>
+int launch_rope(const RopeParams& p, cudaStream_t stream) {
+  constexpr int E = 16 / sizeof(T);
+  const int heads = p.q.heads + p.k.heads + p.v.heads;
+  const bool to_cache = p.slots != nullptr;
+  bool vec = p.hd % (2 * E) == 0 && (!p.table || (p.rot % (2 * E) == 0 && aligned16(p.table))) &&
+             rows_aligned(p.q, sizeof(T), true) && rows_aligned(p.k, sizeof(T), !to_cache) &&
+             rows_aligned(p.v, sizeof(T), false);
+  if (to_cache)
+    vec = vec && aligned16(p.k.out) && aligned16(p.v.out) && p.cs_block % E == 0 && p.cs_head % E == 0 &&
+          p.cs_slot % E == 0;
+  int sms = device_sm_count();
+  if (sms <= 0) sms = 148;
+  const int threads = 256;
+  auto grid = [&](int64_t total, int per_sm) {
+    const int64_t want = (total + threads - 1) / threads, cap = static_cast<int64_t>(sms) * per_sm;
+    return static_cast<unsigned>(want < cap ? want : cap);
+  };
+  if (!vec) {
+    const int units = p.table ? p.hd - p.rot / 2 : p.hd;
+    rope_scalar_kernel<T, INTER><<<grid(static_cast<int64_t>(p.n) * heads * units, 64), threads, 0, stream>>>(p);
+    return check_launch("rope_scalar_kernel");
+  }
+  const int64_t units = static_cast<int64_t>(p.n) * heads * (p.hd / (2 * E));
+  if (units <= static_cast<int64_t>(sms) * 1024) {
+    // too few units to fill the SMs' threads with four heads each: one head a thread is the
+    // shortest chain of loads
+    rope_kernel<T, INTER, 1><<<grid(units, 64), threads, 0, stream>>>(p);
+  } else {
+    const int64_t total = static_cast<int64_t>(p.n) * ((heads + 3) / 4) * (p.hd / (2 * E));
+    rope_kernel<T, INTER, 4><<<grid(total, 64), threads, 0, stream>>>(p);
+  }
+  return check_launch("rope_kernel");
+}
+
+int dispatch_rope(const RopeParams& p, int dtype, int interleaved, cudaStream_t stream) {
+  switch (dtype) {
+    case FOLD_BF16:
+      return interleaved ? launch_rope<__nv_bfloat16, true>(p, stream) : launch_rope<__nv_bfloat16, false>(p, stream);
+    case FOLD_FP16: return interleaved ? launch_rope<__half, true>(p, stream) : launch_rope<__half, false>(p, stream);
+    default: return interleaved ? launch_rope<float, true>(p, stream) : launch_rope<float, false>(p, stream);
+  }
+}
+
+int check_rope(const float* table, int64_t table_rows, int rot_dim, int n, int hd, int dtype, const char* what) {
+  const std::string w(what);
+  if (n < 0 || hd < 1) return fail(FOLD_ERR_INVALID_ARGUMENT, w + ": bad sizes");
+  if (hd > 8192) return fail(FOLD_ERR_UNSUPPORTED, w + ": heads of at most 8192 elements");
+  if (dtype != FOLD_BF16 && dtype != FOLD_FP16 && dtype != FOLD_FP32)
+    return fail(FOLD_ERR_INVALID_ARGUMENT, w + ": unknown type");
+  if (table && (table_rows < 1 || rot_dim < 2 || rot_dim % 2 || rot_dim > hd))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, w + ": the table has rows of rot_dim floats, rot_dim even and at most hd");
+  return FOLD_OK;
+}
+
+}  // namespace
+}  // namespace fold
+
+extern "C" {
+
+int fold_rotary(const void* q, int64_t q_stride_tok, int64_t q_stride_head, void* q_out, int64_t qo_stride_tok,
+                int64_t qo_stride_head, int hq, const void* k, int64_t k_stride_tok, int64_t k_stride_head,
+                void* k_out, int64_t ko_stride_tok, int64_t ko_stride_head, int hk, const int64_t* positions,
+                const float* rope_table, int64_t table_rows, int rot_dim, int n, int hd, int dtype, int interleaved,
+                int inverse, int* err, void* stream) {
+  using namespace fold;
+  if (int s = check_rope(rope_table, table_rows, rot_dim, n, hd, dtype, "rotary")) return s;
+  if (hq < 0 || hk < 0 || hq > 16384 || hk > 16384) return fail(FOLD_ERR_INVALID_ARGUMENT, "rotary: bad sizes");
+  if (n == 0 || hq + hk == 0) return FOLD_OK;
+  if (!positions || !rope_table || (hq && (!q || !q_out)) || (hk && (!k || !k_out)))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "rotary: null pointer");
+  RopeParams p{};
+  p.q = RopeRows{q, q_out, q_stride_tok, q_stride_head, qo_stride_tok, qo_stride_head, hq};
+  p.k = RopeRows{k, k_out, k_stride_tok, k_stride_head, ko_stride_tok, ko_stride_head, hk};
+  // a call of keys alone still writes rows that a read behind it may load: count them as queries
+  if (hq == 0) p.q = p.k, p.k = RopeRows{};
+  p.positions = positions, p.table = rope_table, p.table_rows = table_rows;
+  p.n = n, p.hd = hd, p.rot = rot_dim, p.sgn = inverse ? -1.f : 1.f, p.err = err;
+  return dispatch_rope(p, dtype, interleaved, static_cast<cudaStream_t>(stream));
+}
+
+int fold_append_paged(const void* k, int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+                      int64_t v_stride_head, const int64_t* positions, const int64_t* slots, int n, void* k_cache,
+                      void* v_cache, int64_t num_blocks, int block_size, int64_t cache_stride_block,
+                      int64_t cache_stride_head, int64_t cache_stride_slot, const float* rope_table,
+                      int64_t table_rows, int rot_dim, int hkv, int hd, int dtype, int interleaved, const void* q,
+                      int64_t q_stride_tok, int64_t q_stride_head, void* q_out, int64_t qo_stride_tok,
+                      int64_t qo_stride_head, int hq, int* err, void* stream) {
+  using namespace fold;
+  if (int s = check_rope(rope_table, table_rows, rot_dim, n, hd, dtype, "paged append")) return s;
+  if (hkv < 1 || hkv > 16384 || hq < 0 || hq > 16384 || num_blocks < 1 || block_size < 1 ||
+      num_blocks > (int64_t(1) << 40))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "paged append: bad sizes");
+  if (n == 0) return FOLD_OK;
+  if (!k || !v || !slots || !k_cache || !v_cache || (rope_table && !positions) || (hq && (!q || !q_out)))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "paged append: null pointer");
+  if (hq && !rope_table) return fail(FOLD_ERR_INVALID_ARGUMENT, "paged append: queries are given only to be rotated");
+  RopeParams p{};
+  p.q = RopeRows{q, q_out, q_stride_tok, q_stride_head, qo_stride_tok, qo_stride_head, hq};
+  p.k = RopeRows{k, k_cache, k_stride_tok, k_stride_head, 0, 0, hkv};
+  p.v = RopeRows{v, v_cache, v_stride_tok, v_stride_head, 0, 0, hkv};
+  p.positions = positions, p.slots = slots, p.num_slots = num_blocks * block_size, p.block_size = block_size;
+  p.cs_block = cache_stride_block, p.cs_head = cache_stride_head, p.cs_slot = cache_stride_slot;
+  p.table = rope_table, p.table_rows = table_rows, p.rot = rope_table ? rot_dim : 0;
+  p.n = n, p.hd = hd, p.sgn = 1.f, p.err = err;
+  return dispatch_rope(p, dtype, interleaved, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -304,6 +304,139 @@ def merge_partials(o_wpart, lse_wpart, o_fpart, lse_fpart, out, qsl, seq_lens, *
               1.0 / float(alpha), _stream(out))
 
 
+# Element types of the operators that take more than bf16 (fold_dtype in include/fold_b200.h).
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _check_devices(what, first, *rest):
+    """All given tensors on one CUDA device."""
+    _require_cuda(first, *rest)
+    dev = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            raise FoldError(f"{what}: the tensors are on different devices")
+
+
+def _call_on(t, name, *args):
+    """Calls an entry point on t's device and that device's current stream (the last argument)."""
+    dev = t.get_device()
+    if dev == torch.cuda.current_device():
+        _lib.call(name, *args, _stream(t))
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, _stream(t))
+
+
+def _check_err(what, err):
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 1):
+        raise FoldError(f"{what}: err must be an int32 tensor of at least one element")
+
+
+def _check_table(what, table, d):
+    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] < 1:
+        raise FoldError(f"{what}: the rope table must be contiguous float32 [rows, rot_dim]")
+    rot = table.shape[1]
+    if rot < 2 or rot % 2 or rot > d:
+        raise FoldError(f"{what}: the table's rot_dim must be even and at most the head dimension")
+
+
+def _check_index(what, name, t, n):
+    if t.dim() != 1 or t.shape[0] != n:
+        raise FoldError(f"{what}: {name} needs one entry per token")
+    if t.dtype not in (torch.int64, torch.int32):
+        raise FoldError(f"{what}: {name} must be int64 or int32")
+    return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
+
+
+def _rotary_out(what, x, out):
+    """(x, out) with contiguous heads; a new output when none is given."""
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        if out is x:
+            raise FoldError(f"{what}: the head dimension must be contiguous")
+        x = x.contiguous()
+    if out is None:
+        return x, torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    if out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and out.shape[-1] > 1):
+        raise FoldError(f"{what}: an output has its input's shape and type and a contiguous head dimension")
+    return x, out
+
+
+def rotary(q, k, positions, table, *, interleaved=False, inverse=False, q_out=None, k_out=None, err=None):
+    """Rotary positions: q [n, Hq, D] and k [n, Hk, D] (or None), bf16, fp16 or float32, rotated by
+    positions [n] on the first rot_dim = table.shape[1] dims; returns (q_out, k_out). Pairs are
+    (i, i + rot_dim / 2), or (2i, 2i + 1) when `interleaved`. `table` is rope_table's, for native or
+    scaled frequencies. `inverse` applies the transposed rotation, which takes the outputs'
+    gradients to the inputs'. Outputs are new tensors unless given; one may be its own input.
+    A position outside the table is clamped and reported in err (int32 [1])."""
+    _check_devices("rotary", q, k, positions, table, q_out, k_out, err)
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+        raise FoldError("rotary: q and k must be [n, heads, head_dim] with equal n and head_dim")
+    if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
+        raise FoldError("rotary: q and k must both be bfloat16, float16 or float32")
+    n, hq, d = q.shape
+    _check_table("rotary", table, d)
+    _check_err("rotary", err)
+    positions = _check_index("rotary", "positions", positions, n)
+    q, q_out = _rotary_out("rotary", q, q_out)
+    hk, ks, kos = 0, (0, 0), (0, 0)
+    if k is not None:
+        k, k_out = _rotary_out("rotary", k, k_out)
+        hk, ks, kos = k.shape[1], k.stride(), k_out.stride()
+    _call_on(q, "fold_rotary", _p(q), q.stride(0), q.stride(1), _p(q_out), q_out.stride(0), q_out.stride(1), hq, _p(k),
+             ks[0], ks[1], _p(k_out), kos[0], kos[1], hk, _p(positions), _p(table), table.shape[0], table.shape[1], n,
+             d, _DTYPES[q.dtype], int(bool(interleaved)), int(bool(inverse)), _p(err))
+    return q_out, k_out
+
+
+def _check_planes(what, k_cache, v_cache):
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.stride() != v_cache.stride() \
+            or (k_cache.stride(-1) != 1 and k_cache.shape[-1] > 1):
+        raise FoldError(f"{what}: K and V planes must be [num_blocks, Hkv, block_size, head_dim] views with equal "
+                        "strides and a contiguous head dimension")
+    if v_cache.dtype != k_cache.dtype:
+        raise FoldError(f"{what}: K and V planes must have one type")
+
+
+def append_paged(k, v, positions, slots, k_cache, v_cache, table, *, interleaved=False, q=None, q_out=None, err=None):
+    """Writes K [n, Hkv, D] rotated by positions [n] (as rotary) and V [n, Hkv, D] into a paged cache
+    at slots [n] (block * block_size + offset; a negative slot skips the token): k_cache and v_cache
+    are [num_blocks, Hkv, block_size, D] planes with equal strides (paged_planes of vLLM's cache),
+    bf16, fp16 or float32 like K and V. With q [n, Hq, D] the tokens' queries are rotated in the
+    same launch and returned (q_out, a new tensor unless given; it may be q). table None stores the
+    keys as they are. The non-negative slots of a call must be distinct; a slot past the cache is
+    skipped and reported in err."""
+    _check_devices("append_paged", k, v, positions, slots, k_cache, v_cache, table, q, q_out, err)
+    _check_planes("append_paged", k_cache, v_cache)
+    nb, hkv, bs, d = k_cache.shape
+    if k.dim() != 3 or k.shape[1:] != (hkv, d) or v.shape != k.shape:
+        raise FoldError("append_paged: K and V must be [n, Hkv, head_dim] matching the cache planes")
+    if k.dtype not in _DTYPES or v.dtype != k.dtype or k_cache.dtype != k.dtype:
+        raise FoldError("append_paged: K, V and the cache must all be bfloat16, float16 or float32")
+    n = k.shape[0]
+    _check_err("append_paged", err)
+    if (k.stride(-1) != 1 or v.stride(-1) != 1) and d > 1:
+        raise FoldError("append_paged: the head dimension of K and V must be contiguous")
+    slots = _check_index("append_paged", "slots", slots, n)
+    if table is not None:
+        _check_table("append_paged", table, d)
+        positions = _check_index("append_paged", "positions", positions, n)
+    hq, qs, qos = 0, (0, 0), (0, 0)
+    if q is not None:
+        if table is None:
+            raise FoldError("append_paged: queries are given only to be rotated (table is None)")
+        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype:
+            raise FoldError("append_paged: q must be [n, Hq, head_dim] of the keys' type")
+        q, q_out = _rotary_out("append_paged", q, q_out)
+        hq, qs, qos = q.shape[1], q.stride(), q_out.stride()
+    rows, rot = (0, 0) if table is None else table.shape
+    _call_on(k, "fold_append_paged", _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1),
+             _p(positions) if table is not None else None, _p(slots), n, _p(k_cache), _p(v_cache), nb, bs,
+             k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), _p(table), rows, rot, hkv, d, _DTYPES[k.dtype],
+             int(bool(interleaved)), _p(q), qs[0], qs[1], _p(q_out) if q is not None else None, qos[0], qos[1], hq,
+             _p(err))
+    return q_out if q is not None else None
+
+
 def append(k, v, positions, slots, side, *, pos_lo=0, skip_foreign=False, err=None):
     """Writes K [ctx, Hkv, D] (before RoPE) and V [ctx, Hkv, D] of committed entries into the
     side cache at their positions (fold/attention.py:260-265); rows with slot < 0 go to the

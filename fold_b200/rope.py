@@ -47,15 +47,73 @@ def default_inv_freq(theta: float, rotary_dim: int, device=None) -> torch.Tensor
     return torch.from_numpy((1.0 / (theta ** (i / rotary_dim))).astype(np.float32)).to(device)
 
 
-def table_host(inv_freq, rows: int) -> np.ndarray:
-    """cos/sin table [rows, 2 * len(inv_freq)] float32, computed in float64."""
+def scaled_inv_freq(theta: float, rotary_dim: int, scaling=None, device=None):
+    """(frequencies float32 [rotary_dim / 2], attention factor) of a long-context rotary scaling, for
+    rope_table(inv_freq, rows, device, factor). `scaling` is None (native) or a dict in the form
+    model configurations give it:
+
+      {"rope_type": "linear", "factor": s}     positions interpolated: f / s
+      {"rope_type": "ntk", "factor": s}        base stretched: theta * s^(d / (d - 2))
+      {"rope_type": "llama3", "factor": s, "low_freq_factor": a, "high_freq_factor": b,
+       "original_max_position_embeddings": L}  f / s below a turns in L, f above b, linear between
+      {"rope_type": "yarn", "factor": s, "original_max_position_embeddings": L, "beta_fast": 32,
+       "beta_slow": 1}                         f above beta_fast turns in L, f / s below beta_slow,
+                                               a linear ramp over the dims between; the attention
+                                               factor is 0.1 ln s + 1 unless "attention_factor"
+    """
+    d = int(rotary_dim)
+    if d < 2 or d % 2 or not theta > 0:
+        raise ValueError("scaled_inv_freq: rotary_dim must be even and positive, theta positive")
+    i = np.arange(0, d, 2, dtype=np.float64)
+    f = 1.0 / (float(theta) ** (i / d))
+    attention = 1.0
+    if scaling is not None:
+        kind = scaling.get("rope_type", scaling.get("type"))
+        if kind not in ("linear", "ntk", "llama3", "yarn"):
+            raise ValueError(f"scaled_inv_freq: unknown rope_type {kind!r}")
+        s = float(scaling["factor"])
+        if not s >= 1.0:
+            raise ValueError("scaled_inv_freq: factor must be at least 1")
+        if kind == "linear":
+            f = f / s
+        elif kind == "ntk":
+            if d < 4:
+                raise ValueError("scaled_inv_freq: ntk needs a rotary_dim of at least 4")
+            f = 1.0 / ((float(theta) * s ** (d / (d - 2))) ** (i / d))
+        else:
+            ctx = float(scaling["original_max_position_embeddings"])
+            turns = ctx * f / (2.0 * np.pi)  # whole turns of each pair over the trained context
+            if kind == "llama3":
+                lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+                if not hi > lo > 0:
+                    raise ValueError("scaled_inv_freq: llama3 needs high_freq_factor > low_freq_factor > 0")
+                keep = np.clip((turns - lo) / (hi - lo), 0.0, 1.0)
+            else:
+                fast, slow = float(scaling.get("beta_fast", 32)), float(scaling.get("beta_slow", 1))
+                if not fast > slow > 0 or not theta > 1:
+                    raise ValueError("scaled_inv_freq: yarn needs beta_fast > beta_slow > 0 and theta > 1")
+
+                def dim_of(n):  # the (real-valued) pair index that makes n turns
+                    return d * np.log(ctx / (n * 2.0 * np.pi)) / (2.0 * np.log(float(theta)))
+
+                lo, hi = max(np.floor(dim_of(fast)), 0.0), min(np.ceil(dim_of(slow)), d - 1.0)
+                ramp = (np.arange(d // 2) - lo) / max(hi - lo, 1e-3)
+                keep = 1.0 - np.clip(ramp, 0.0, 1.0)
+                attention = scaling.get("attention_factor")
+                attention = 0.1 * np.log(s) + 1.0 if attention is None else float(attention)
+            f = f * keep + (f / s) * (1.0 - keep)
+    return torch.from_numpy(f.astype(np.float32)).to(device), float(attention)
+
+
+def table_host(inv_freq, rows: int, factor: float = 1.0) -> np.ndarray:
+    """cos/sin table [rows, 2 * len(inv_freq)] float32 times `factor`, computed in float64."""
     f = np.asarray(inv_freq.detach().cpu() if isinstance(inv_freq, torch.Tensor) else inv_freq, dtype=np.float64)
     out = np.empty((rows, 2 * f.size), dtype=np.float32)
     step = 1 << 16
     for a in range(0, rows, step):
         ang = np.arange(a, min(rows, a + step), dtype=np.float64)[:, None] * f[None, :]
-        out[a:a + ang.shape[0], :f.size] = np.cos(ang)
-        out[a:a + ang.shape[0], f.size:] = np.sin(ang)
+        out[a:a + ang.shape[0], :f.size] = np.cos(ang) * factor
+        out[a:a + ang.shape[0], f.size:] = np.sin(ang) * factor
     return out
 
 
@@ -63,13 +121,14 @@ _tables: dict = {}
 _tables_lock = threading.Lock()
 
 
-def rope_table(inv_freq: torch.Tensor, rows: int, device) -> torch.Tensor:
-    """Shared device table with at least `rows` rows for these frequencies."""
+def rope_table(inv_freq: torch.Tensor, rows: int, device, factor: float = 1.0) -> torch.Tensor:
+    """Shared device table with at least `rows` rows for these frequencies and this attention
+    factor (scaled_inv_freq)."""
     device = torch.device(device)
-    key = (np.asarray(inv_freq.detach().cpu(), dtype=np.float32).tobytes(), str(device))
+    key = (np.asarray(inv_freq.detach().cpu(), dtype=np.float32).tobytes(), str(device), float(factor))
     with _tables_lock:
         t = _tables.get(key)
         if t is None or t.shape[0] < rows:
-            t = torch.from_numpy(table_host(inv_freq, rows)).to(device)
+            t = torch.from_numpy(table_host(inv_freq, rows, factor)).to(device)
             _tables[key] = t
         return t

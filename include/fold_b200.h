@@ -39,6 +39,9 @@ enum fold_status {
   FOLD_ERR_TENSOR_MAP = 5        /* the TMA descriptor of the side cache could not be built */
 };
 
+/* Element types of the operators that take more than bf16. */
+enum fold_dtype { FOLD_BF16 = 0, FOLD_FP16 = 1, FOLD_FP32 = 2 };
+
 #define FOLD_DEVERR_APPEND_RANGE 1 /* an append/gather position lies outside the cache */
 #define FOLD_DEVERR_ROPE_RANGE 2   /* |rotation offset| beyond the rope table (offset clamped) */
 #define FOLD_DEVERR_TIMEOUT 4      /* a pipeline wait of the far read, or a wait for a peer, gave up */
@@ -90,6 +93,44 @@ int fold_far_query(const void* q, int64_t q_stride_tok, int64_t q_stride_head, v
                    int64_t qf_stride_head, const int* qsl, const int* seq_lens, const float* rope_table,
                    int table_rows, int rot_dim, int* far_len, int n, int hq, int hd, int window, int block,
                    int far_distance, int* err, void* stream);
+
+/* Rotary positions of queries and keys, for the rotation the reference leaves to vLLM's rotary op
+ * (fold/attention.py:245-246) and in more forms than its far query's: q [n, hq, hd] and k
+ * [n, hk, hd] of type `dtype` (fold_dtype), innermost dim contiguous, strides (tok, head) in
+ * elements, are rotated by their tokens' positions (int64[n]) on the first rot_dim dims into q_out
+ * and k_out; the other dims are copied. hq or hk may be 0 (their pointers are then not read).
+ * Pairs are (i, i + rot_dim/2), or (2i, 2i+1) when `interleaved`:
+ *   lo' = lo cos - hi sin, hi' = hi cos + lo sin.
+ * `inverse` negates sin: the transpose of the rotation, which takes the gradient of the outputs to
+ * the gradient of the inputs. rope_table: float32 [table_rows, rot_dim], row p holding
+ * c cos(p f_i) then c sin(p f_i), c the attention factor of scaled frequencies (1 otherwise); a
+ * position outside [0, table_rows) is clamped and sets FOLD_DEVERR_ROPE_RANGE. An output may be its
+ * input; any other overlap of inputs and outputs is not allowed. Rows are read 16 bytes at a time
+ * where rot_dim and hd are multiples of 32 bytes' elements and rows start on 16-byte boundaries,
+ * else element by element. hd at most 8192. */
+int fold_rotary(const void* q, int64_t q_stride_tok, int64_t q_stride_head, void* q_out, int64_t qo_stride_tok,
+                int64_t qo_stride_head, int hq, const void* k, int64_t k_stride_tok, int64_t k_stride_head,
+                void* k_out, int64_t ko_stride_tok, int64_t ko_stride_head, int hk, const int64_t* positions,
+                const float* rope_table, int64_t table_rows, int rot_dim, int n, int hd, int dtype, int interleaved,
+                int inverse, int* err, void* stream);
+
+/* Append to a paged cache with the rotation applied on the way: replaces the rotary op and the
+ * cache update behind it (fold/attention.py:245-246,256) by one launch. k, v [n, hkv, hd] of type
+ * `dtype`; token i goes to slot slots[i] = block * block_size + offset of the planes k_cache and
+ * v_cache ([num_blocks, hkv, block_size, hd], same type, given strides in elements, innermost dim
+ * contiguous, both planes share them), k rotated as by fold_rotary, v as it is. A token with a
+ * negative slot is skipped; one at or past num_blocks * block_size is skipped and sets
+ * FOLD_DEVERR_APPEND_RANGE. The non-negative slots of one call are distinct (of two tokens with
+ * one slot, which one's 16-byte pieces remain is not defined). rope_table NULL: keys are stored as
+ * they are, positions are not read. With hq > 0 the queries q [n, hq, hd] of the same tokens are
+ * rotated into q_out too (whatever their slots), in the same launch; q_out may be q. */
+int fold_append_paged(const void* k, int64_t k_stride_tok, int64_t k_stride_head, const void* v, int64_t v_stride_tok,
+                      int64_t v_stride_head, const int64_t* positions, const int64_t* slots, int n, void* k_cache,
+                      void* v_cache, int64_t num_blocks, int block_size, int64_t cache_stride_block,
+                      int64_t cache_stride_head, int64_t cache_stride_slot, const float* rope_table,
+                      int64_t table_rows, int rot_dim, int hkv, int hd, int dtype, int interleaved, const void* q,
+                      int64_t q_stride_tok, int64_t q_stride_head, void* q_out, int64_t qo_stride_tok,
+                      int64_t qo_stride_head, int hq, int* err, void* stream);
 
 /* ReRoPE query pair. Replaces rerope_queries / _rerope_query_kernel (fold/kernels.py:49-83,
  * 122-132): qs = q * max(1, log(H + t + 1) * inv_log_ref) when inv_log_ref > 0, else q;

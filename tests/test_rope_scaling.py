@@ -1,0 +1,144 @@
+"""Scaled rotary frequencies and their table on the CPU, and the refusals of the rotary and paged
+append entry points that need no GPU."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from fold_b200 import _lib, kernels, rope
+from fold_b200.errors import FoldError
+
+F32 = 2.0 ** -24  # half a step of float32, relative
+
+
+def native(theta, d):
+    return [theta ** (-2.0 * i / d) for i in range(d // 2)]
+
+
+def close(got, want):
+    got, want = got.numpy().astype(np.float64), np.asarray(want)
+    # the float64 formulas agree to far below float32's rounding: half a step, and a little
+    assert np.all(np.abs(got - want) <= 1.01 * F32 * np.abs(want))
+
+
+def test_native_matches_default():
+    f, c = rope.scaled_inv_freq(500000.0, 128)
+    assert c == 1.0
+    assert torch.equal(f, rope.default_inv_freq(500000.0, 128))
+
+
+def test_linear_and_ntk():
+    f, c = rope.scaled_inv_freq(10000.0, 64, {"rope_type": "linear", "factor": 4.0})
+    close(f, [x / 4 for x in native(10000.0, 64)])
+    assert c == 1.0
+    f, c = rope.scaled_inv_freq(10000.0, 64, {"rope_type": "ntk", "factor": 8.0})
+    close(f, native(10000.0 * 8.0 ** (64 / 62), 64))
+
+
+def test_llama3_bands():
+    L, s, a, b = 8192, 8.0, 1.0, 4.0
+    f, c = rope.scaled_inv_freq(500000.0, 128, {"rope_type": "llama3", "factor": s, "low_freq_factor": a,
+                                                "high_freq_factor": b, "original_max_position_embeddings": L})
+    want = []
+    for x in native(500000.0, 128):
+        wave = 2 * math.pi / x
+        if wave < L / b:
+            want.append(x)
+        elif wave > L / a:
+            want.append(x / s)
+        else:
+            t = (L / wave - a) / (b - a)
+            want.append((1 - t) * x / s + t * x)
+    close(f, want)
+    assert c == 1.0
+
+
+def test_yarn_ramp_and_attention_factor():
+    L, s, d, theta = 4096, 16.0, 128, 10000.0
+    cfg = {"rope_type": "yarn", "factor": s, "original_max_position_embeddings": L}
+    f, c = rope.scaled_inv_freq(theta, d, cfg)
+    assert c == pytest.approx(0.1 * math.log(s) + 1.0, abs=1e-15)
+    at = [d * math.log(L / (n * 2 * math.pi)) / (2 * math.log(theta)) for n in (32, 1)]
+    lo, hi = max(math.floor(at[0]), 0), min(math.ceil(at[1]), d - 1)
+    want = []
+    for i, x in enumerate(native(theta, d)):
+        r = min(max((i - lo) / (hi - lo), 0.0), 1.0)
+        want.append(x / s * r + x * (1 - r))
+    close(f, want)
+    assert f[0] == 1.0 and abs(float(f[-1]) * s / native(theta, d)[-1] - 1) < 1e-6
+    assert rope.scaled_inv_freq(theta, d, {**cfg, "attention_factor": 1.25})[1] == 1.25
+
+
+@pytest.mark.parametrize("theta,d,cfg", [
+    (1e4, 63, None), (0.0, 64, None), (1e4, 64, {"rope_type": "magic", "factor": 2}),
+    (1e4, 64, {"rope_type": "linear", "factor": 0.5}), (1e4, 2, {"rope_type": "ntk", "factor": 2}),
+    (1e4, 64, {"rope_type": "llama3", "factor": 2, "low_freq_factor": 4, "high_freq_factor": 4,
+               "original_max_position_embeddings": 100}),
+    (1e4, 64, {"rope_type": "yarn", "factor": 2, "beta_fast": 1, "beta_slow": 1,
+               "original_max_position_embeddings": 100})])
+def test_scaling_refusals(theta, d, cfg):
+    with pytest.raises(ValueError):
+        rope.scaled_inv_freq(theta, d, cfg)
+
+
+def test_table_carries_the_factor():
+    f = rope.default_inv_freq(10000.0, 16)
+    plain, scaled = rope.rope_table(f, 64, "cpu"), rope.rope_table(f, 64, "cpu", factor=1.25)
+    again = rope.rope_table(f, 64, "cpu")
+    assert again is plain
+    ang = np.arange(64)[:, None] * f.numpy().astype(np.float64)
+    want = np.concatenate([np.cos(ang), np.sin(ang)], 1)
+    assert np.abs(plain.numpy()[:64] - want).max() <= F32
+    assert np.abs(scaled.numpy()[:64] - 1.25 * want).max() <= 2 * F32
+
+
+def call_rotary(**kw):
+    a = dict(q=16, hq=2, k=16, hk=1, pos=16, table=16, rows=8, rot=16, n=3, hd=32, dtype=0)
+    a.update(kw)
+    _lib.call("fold_rotary", a["q"], 64, 32, a["q"], 64, 32, a["hq"], a["k"], 32, 32, a["k"], 32, 32, a["hk"], a["pos"],
+              a["table"], a["rows"], a["rot"], a["n"], a["hd"], a["dtype"], 0, 0, None, None)
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=5), dict(rot=15), dict(rot=34), dict(rot=0), dict(rows=0), dict(n=-1),
+                                 dict(hd=0), dict(hq=-1), dict(pos=None), dict(table=None), dict(q=None),
+                                 dict(k=None), dict(hd=16384)])
+def test_rotary_refusals(bad):
+    with pytest.raises(FoldError, match="rotary"):
+        call_rotary(**bad)
+
+
+def test_rotary_of_nothing_is_a_no_op():
+    call_rotary(n=0)
+    call_rotary(hq=0, hk=0)
+
+
+def call_append(**kw):
+    a = dict(k=16, v=16, pos=16, slots=16, kc=16, vc=16, nb=2, bs=16, table=16, rows=8, rot=16, hkv=1, hd=32, dtype=0,
+             q=None, hq=0, n=3)
+    a.update(kw)
+    _lib.call("fold_append_paged", a["k"], 32, 32, a["v"], 32, 32, a["pos"], a["slots"], a["n"], a["kc"], a["vc"],
+              a["nb"], a["bs"], 512, 512, 32, a["table"], a["rows"], a["rot"], a["hkv"], a["hd"], a["dtype"], 0, a["q"],
+              64, 32, a["q"], 64, 32, a["hq"], None, None)
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=-1), dict(rot=33), dict(hkv=0), dict(nb=0), dict(bs=0), dict(n=-2),
+                                 dict(k=None), dict(v=None), dict(slots=None), dict(kc=None), dict(vc=None),
+                                 dict(pos=None), dict(hq=2), dict(hq=2, q=16, table=None)])
+def test_append_refusals(bad):
+    with pytest.raises(FoldError, match="paged append"):
+        call_append(**bad)
+
+
+def test_append_of_nothing_is_a_no_op():
+    call_append(n=0)
+
+
+def test_wrappers_take_cuda_tensors_only():
+    x = torch.zeros(2, 1, 32)
+    t = rope.rope_table(rope.default_inv_freq(1e4, 32), 8, "cpu")
+    with pytest.raises(FoldError, match="CUDA"):
+        kernels.rotary(x, None, torch.zeros(2, dtype=torch.int64), t)
+    with pytest.raises(FoldError, match="CUDA"):
+        kernels.append_paged(x, x, torch.zeros(2, dtype=torch.int64), torch.zeros(2, dtype=torch.int64),
+                             torch.zeros(1, 1, 16, 32), torch.zeros(1, 1, 16, 32), t)
