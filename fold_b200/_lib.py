@@ -46,6 +46,10 @@ SIGNATURES = {
     "fold_allgather_partials": [_vp, _vp, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp],
     "fold_window_read": [_vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _i32, _i32, _i32,
                          _i32, _f32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp],
+    "fold_prefix_read": [_vp, _i64, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _i32, _vp,
+                         _i64, _i32, _i32, _f32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp,
+                         _vp],
+    "fold_prefix_read_workspace": [_i32, _i32, _i32, _i32],
     "fold_step_read": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i64, _i64, _vp, _vp,
                        _vp, _vp, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp,
                        _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _f32, _vp, _vp],
@@ -63,7 +67,8 @@ SIGNATURES = {
                                    _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                    _i32, _f32, _f32, _vp, _vp],
 }
-_RESTYPES = {"fold_status_string": ctypes.c_char_p, "fold_last_error": ctypes.c_char_p}
+_RESTYPES = {"fold_status_string": ctypes.c_char_p, "fold_last_error": ctypes.c_char_p,
+             "fold_prefix_read_workspace": _i64}
 
 _lock = threading.Lock()
 _lib = None
@@ -114,3 +119,7 @@ def default_splits(hkv: int, hd: int, n: int, hq: int) -> int:
 
 def far_read_kernel_for(hd: int, n: int, hq: int, hkv: int) -> int:
     return int(load().fold_far_read_kernel_for(hd, n, hq, hkv))
+
+
+def prefix_read_workspace(n: int, hq: int, hkv: int, hd: int) -> int:
+    return int(load().fold_prefix_read_workspace(n, hq, hkv, hd))

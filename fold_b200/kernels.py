@@ -437,6 +437,58 @@ def append_paged(k, v, positions, slots, k_cache, v_cache, table, *, interleaved
     return q_out if q is not None else None
 
 
+def prefix_workspace(n, hq, hkv, d, device):
+    """A workspace for prefix_read calls of up to these sizes (one per call that may overlap another)."""
+    with torch.cuda.device(device):
+        size = _lib.prefix_read_workspace(int(n), int(hq), int(hkv), int(d))
+    if size < 0:
+        raise FoldError(f"prefix_read: no kernel for n {n}, Hq {hq}, Hkv {hkv}, head_dim {d}")
+    return torch.empty(max(size, 16), device=device, dtype=torch.uint8)
+
+
+def prefix_read(q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, block_tables, out, *, softmax_scale,
+                causal=True, lse=None, workspace=None, err=None):
+    """Attention of a batch of sequences that share a prefix, the prefix read once for all of them.
+
+    q [n, Hq, D] bf16 or fp16 (RoPE'd): rows [qsl[i], qsl[i + 1]) belong to sequence i; rows from
+    qsl[b] on are left alone. Sequence i sees the first prefix_len[0] positions of the blocks in
+    prefix_table [blocks] and own_lens[i] positions of the blocks in block_tables[i] (causal: row r
+    of sequence i the first own_lens[i] - rows + r + 1 of them). k_cache and v_cache are
+    [num_blocks, Hkv, block_size, D] planes (paged_planes); lengths and tables are int32 on the
+    device. Writes out [n, Hq, D] and, when given, lse [Hq, n] float32; a row without a key gets
+    out 0 and lse -inf. `workspace` (prefix_workspace) is allocated per call when not given."""
+    _check_devices("prefix_read", q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, block_tables, out, lse,
+                   workspace, err)
+    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
+        raise FoldError("prefix_read: q and out must be [n, Hq, head_dim] of one type, out's head dimension contiguous")
+    n, hq, d = q.shape
+    _check_planes("prefix_read", k_cache, v_cache)
+    nb, hkv, bs, dk = k_cache.shape
+    if q.dtype not in (torch.bfloat16, torch.float16) or k_cache.dtype != q.dtype or dk != d:
+        raise FoldError("prefix_read: q and the cache must both be bfloat16 or float16 with one head dimension")
+    for name, t, dim in (("query_start_loc", qsl, 1), ("own_lens", own_lens, 1), ("prefix_len", prefix_len, 1),
+                         ("prefix_table", prefix_table, 1), ("block_tables", block_tables, 2)):
+        if t.dtype != torch.int32 or t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1):
+            raise FoldError(f"prefix_read: {name} must be int32 with {dim} dimension(s), the last one contiguous")
+    b = own_lens.shape[0]
+    if qsl.shape[0] != b + 1 or block_tables.shape[0] != b or prefix_len.shape[0] != 1:
+        raise FoldError("prefix_read: query_start_loc needs b + 1 entries, block_tables b rows and prefix_len one entry")
+    if lse is not None and (lse.shape != (hq, n) or lse.dtype != torch.float32 or not lse.is_contiguous()):
+        raise FoldError("prefix_read: lse must be contiguous float32 [Hq, n]")
+    _check_err("prefix_read", err)
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    if workspace is None:
+        workspace = prefix_workspace(n, hq, hkv, d, q.device)
+    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise FoldError("prefix_read: workspace must be a contiguous uint8 tensor (prefix_workspace)")
+    _call_on(q, "fold_prefix_read", _p(q), q.stride(0), q.stride(1), _p(qsl), _p(own_lens), _p(prefix_len), b,
+             _p(k_cache), _p(v_cache), nb, bs, k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), _p(prefix_table),
+             prefix_table.shape[0], _p(block_tables), block_tables.stride(0), block_tables.shape[1], int(bool(causal)),
+             float(softmax_scale), _p(out), out.stride(0), out.stride(1), _p(lse), _p(workspace), workspace.numel(), n,
+             hq, hkv, d, _DTYPES[q.dtype], _p(err))
+
+
 def append(k, v, positions, slots, side, *, pos_lo=0, skip_foreign=False, err=None):
     """Writes K [ctx, Hkv, D] (before RoPE) and V [ctx, Hkv, D] of committed entries into the
     side cache at their positions (fold/attention.py:260-265); rows with slot < 0 go to the

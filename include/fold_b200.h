@@ -184,6 +184,40 @@ int fold_window_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
                      float softmax_scale, float* o_part, float* lse_part, int splits, int n, int hq, int hkv, int hd,
                      int* err, void* stream);
 
+/* Attention of a batch of sequences that share a prefix; no reference counterpart (the reference
+ * serves one sequence; it refuses vLLM's cascade attention, fold/attention.py:137). The prefix's
+ * keys are read once for the rows of all sequences together, each sequence's own keys for its rows.
+ * Sequence i (of b) has the query rows [qsl[i], qsl[i+1]) of q [n, hq, hd] (qsl ascending; rows
+ * from qsl[b] on are not read and their outputs are left as they were) and own_lens[i] own keys.
+ * The prefix's position j < prefix_len[0] lies in block prefix_table[j / block_size]; own position
+ * j in block block_tables[i * block_tables_stride + j / block_size], both at offset
+ * j % block_size of the planes k_cache and v_cache ([num_blocks, hkv, block_size, hd] with the
+ * given strides, as fold_window_read; the block stride a multiple of the head stride). The keys
+ * already hold their rotation (fold_append_paged). Row r of sequence i sees the whole prefix and,
+ * of its own m = own_lens[i] keys, all, or when `causal` the first m - (query rows of i) + r + 1
+ * (bottom-right alignment). out [n, hq, hd] = the softmax-weighted values, lse [hq, n] (contiguous,
+ * may be NULL) the natural log of the sum of exp(softmax_scale * q.k); a row that sees no key has
+ * out 0 and lse -inf. Slots of a block that no length reaches may hold anything; a value row that
+ * some rows of its sequence see must be finite even for rows that do not. dtype FOLD_BF16 or
+ * FOLD_FP16 (q, cache and out); hd 64, 128 or 256; hq / hkv at most 128; block_size a multiple of
+ * 16; q, out and the planes on 16-byte boundaries with strides of whole 16 bytes. Lengths past the
+ * tables' capacity (table_len * block_size) are cut and set FOLD_DEVERR_CAPACITY; a table entry
+ * outside the cache is read as zeros and sets FOLD_DEVERR_BLOCK_TABLE. All lengths and tables are
+ * read on the device: b, n and the table lengths are what a captured call is fixed to. workspace:
+ * fold_prefix_read_workspace bytes of device memory, 16-byte aligned, not shared by calls that
+ * may overlap; nothing in it outlives the call. */
+int fold_prefix_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const int* qsl, const int* own_lens,
+                     const int* prefix_len, int b, const void* k_cache, const void* v_cache, int64_t num_blocks,
+                     int block_size, int64_t cache_stride_block, int64_t cache_stride_head, int64_t cache_stride_slot,
+                     const int* prefix_table, int prefix_table_len, const int* block_tables,
+                     int64_t block_tables_stride, int block_tables_len, int causal, float softmax_scale, void* out,
+                     int64_t o_stride_tok, int64_t o_stride_head, float* lse, void* workspace, int64_t workspace_bytes,
+                     int n, int hq, int hkv, int hd, int dtype, int* err, void* stream);
+
+/* Bytes of workspace fold_prefix_read takes for these sizes on the current device (-1: sizes it
+ * does not take). */
+int64_t fold_prefix_read_workspace(int n, int hq, int hkv, int hd);
+
 /* Far-memory read of an fp8 side cache (fold_append_fp8): the work of fold_far_read with the keys
  * and values dequantised by k_scale, v_scale (float [hkv], device): K and V of the side cache are
  * e4m3 (exact in f16), the tiles f16 MMAs with f32 accumulation, the query rotated in float32 and
