@@ -356,6 +356,7 @@ def test_refusals():
     bad(q, qsl, own, plen, k, v, pt, bt.t())
     bad(q, qsl, own, plen, k, v, pt, bt, o=out[:2])
     bad(q, qsl, own, plen, k, v, pt, bt, lse=torch.empty(3, 4, device="cuda"))
+    bad(q, qsl, own, plen, k, v, pt, bt, workspace=torch.empty(16, device="cuda", dtype=torch.uint8))
     bad(q[..., :64], qsl, own, plen, k, v, pt, bt, o=out[..., :64])
     bad(q, qsl, own, plen, k, v, pt, bt, err=own.float())
     kernels.prefix_read(q[:0], torch.zeros(3, dtype=torch.int32, device="cuda"), own, plen, k, v, pt, bt, out[:0],
