@@ -69,6 +69,7 @@ struct PrefixParams {
   int64_t o_st, o_sh;
   float* lse;
   int n, hq, hkv, group;
+  int half_toks;  // tokens whose rows fill a half of a wide row tile: 128 / group
   int ctas;
   // workspace
   int4* plan;       // [2][n][hkv]: first CTA, number of CTAs, first token of the row tile
@@ -113,7 +114,7 @@ constexpr int kTileCost = 4, kWideTileCost = 8, kItemCost = 4;
 
 struct Seg {
   int part;  // 0: prefix, 1: own keys, -1: no more work
-  int seq, head, tok0, rows;
+  int seq, head, tok0, ntok;
   int kb, ke;   // key tiles [kb, ke)
   int limit;    // keys any row of the item sees
   int lim0, lim_step;  // row of token tok0 + x sees min(limit, lim0 + x * lim_step) keys
@@ -121,16 +122,20 @@ struct Seg {
 };
 constexpr int kSegs = 4;
 
+// Q of up to this many tokens is copied row by row, of more as one box of the half tile (a box always
+// moves all of its rows).
+constexpr int kFewToks = 8;
+
 struct Bars {
   uint64_t full[12], empty[12];
   uint64_t s_full[2], p_full[2], pv_done;
   uint64_t q_full[2], q_empty[2];
   uint64_t seg_full[kSegs], seg_empty[kSegs];
-  uint64_t seg_done, o_free, stat_full;
+  uint64_t seg_done[2], o_free[2], stat_full, stat_free, drained;
   uint32_t tmem;
   int start_seq;
   int64_t start_base;
-  int64_t scan[16];
+  int64_t scan[12];
   Seg seg[kSegs];
 };
 static_assert(sizeof(Bars) <= 768, "barriers fit their place");
@@ -144,7 +149,9 @@ __device__ __forceinline__ int capped(int len, int cap, int* err) {
   return max(len, 0);
 }
 
-__device__ __forceinline__ int tile_cost(int rows) { return rows > 128 ? kWideTileCost : kTileCost; }
+__device__ __forceinline__ int tile_cost(const PrefixParams& p, int ntok) {
+  return ntok > p.half_toks ? kWideTileCost : kTileCost;
+}
 
 // Query rows of sequence s, [first, last), kept inside [0, n] whatever qsl holds.
 __device__ __forceinline__ void seq_rows(const PrefixParams& p, int s, int& first, int& last) {
@@ -159,12 +166,11 @@ __device__ __forceinline__ void own_limits(const PrefixParams& p, int first, int
   limit = p.causal ? max(min(m, lim0 + ntok - 1), 0) : m;
 }
 
-__device__ __forceinline__ int64_t item_cost(int tiles, int rows) {
-  return kItemCost + static_cast<int64_t>(tiles) * tile_cost(rows);
+__device__ __forceinline__ int64_t item_cost(const PrefixParams& p, int tiles, int ntok) {
+  return kItemCost + static_cast<int64_t>(tiles) * tile_cost(p, ntok);
 }
 
 // Cost of all own items of sequence s and one KV head.
-template <int ROWS>
 __device__ __forceinline__ int64_t seq_cost(const PrefixParams& p, int s, int per_tile) {
   int first, last;
   seq_rows(p, s, first, last);
@@ -174,7 +180,7 @@ __device__ __forceinline__ int64_t seq_cost(const PrefixParams& p, int s, int pe
     const int nt = min(per_tile, last - t0);
     int limit, lim0;
     own_limits(p, first, last, m, t0, nt, limit, lim0);
-    c += item_cost((limit + TK - 1) / TK, nt * p.group);
+    c += item_cost(p, (limit + TK - 1) / TK, nt);
   }
   return c;
 }
@@ -201,13 +207,36 @@ __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// D[tmem] (+)= A[tmem] x B[smem desc].
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// A value that is the same in all lanes, as the compiler can see. The MMA instructions take their
+// operands from uniform registers: issued from one lane's own values each of them first moves five
+// (a step's 16 MMAs then took 1830 cycles of that lane, and bounded the kernel).
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+// Low words of shared-memory matrix descriptors; the high words are constants of the layout.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
+constexpr uint32_t desc_hi(uint32_t sbo) { return (sbo >> 4) | 1u << 14 | kSwizzle128 << 29; }
+// D[tmem] (+)= A[smem] x B[smem] and D[tmem] (+)= A[tmem] x B[smem].
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                       uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, {%7, %7, %7, %7}, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, {%6, %6, %6, %6}, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(0u)
       : "memory");
 }
 // Instruction descriptor of kind::f16 for bf16 or f16 operands, f32 accumulation, M = 128.
@@ -221,6 +250,14 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, u
       "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_plain(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
+                                                  int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
 template <class T>
@@ -237,23 +274,35 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 
-// Ring position (in tiles' K or V) of K(j) and V(j) of a segment of T tiles: K runs one tile
-// ahead, K0 K1 V0 K2 V1 ... V(T-1), the order in which the MMAs first need them.
-__device__ __forceinline__ int k_pos(int j) { return j == 0 ? 0 : 2 * j - 1; }
-__device__ __forceinline__ int v_pos(int j, int T) { return min(2 * j + 2, 2 * T - 1); }
+// Ring position (in tiles' K or V) of K and V of the CTA's tile j, counted over all its segments:
+// K runs one tile ahead, K0 K1 V0 K2 V1 ..., the order in which the MMAs first need them.
+__device__ __forceinline__ uint32_t k_pos(uint32_t j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ uint32_t v_pos(uint32_t j) { return 2 * j + 2; }
+
+__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 // ---------------------------------------------------------------- the kernel
 template <class C>
 __global__ void __launch_bounds__(C::NTHREADS, 1)
-    prefix_read_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
-                       const PrefixParams p) {
+    prefix_read_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap, const PrefixParams p) {
   constexpr int HD = C::HD, KU = C::KU, NU = C::NU, NWG = C::NWG, NSW = C::NSW, QB = C::QB;
   using T = typename C::T;
   extern __shared__ __align__(1024) unsigned char smem[];
   Bars& B = *reinterpret_cast<Bars*>(smem + C::OFF_BAR);
   float2* stats = reinterpret_cast<float2*>(smem + C::OFF_STAT);  // [slot][row]: maximum, sum
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int per_tile = C::ROWS / p.group;  // tokens of a full row tile
+  const int per_tile = NWG * p.half_toks;  // tokens of a full row tile
 
   if (warp == NSW) {
     if (lane == 0) {
@@ -261,9 +310,11 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       for (int i = 0; i < 2; ++i) {
         mbar_init(&B.s_full[i], 1), mbar_init(&B.p_full[i], 4);
         mbar_init(&B.q_full[i], 1), mbar_init(&B.q_empty[i], 1);
+        mbar_init(&B.seg_done[i], 1), mbar_init(&B.o_free[i], NSW);
       }
-      for (int i = 0; i < kSegs; ++i) mbar_init(&B.seg_full[i], 1), mbar_init(&B.seg_empty[i], 2 + NSW);
-      mbar_init(&B.pv_done, 1), mbar_init(&B.seg_done, 1), mbar_init(&B.o_free, NSW), mbar_init(&B.stat_full, NSW);
+      for (int i = 0; i < kSegs; ++i) mbar_init(&B.seg_full[i], 1), mbar_init(&B.seg_empty[i], 3 + NSW);
+      mbar_init(&B.pv_done, 1), mbar_init(&B.stat_full, NSW), mbar_init(&B.stat_free, NSW);
+      mbar_init(&B.drained, 1);
       fence_mbar_init();
     }
     __syncwarp();
@@ -279,12 +330,12 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
   const int ptiles = (plen + TK - 1) / TK;
   const int prow_tiles = plen > 0 ? (tok_hi - tok_lo + per_tile - 1) / per_tile : 0;
   const int last_tok = prow_tiles ? tok_hi - tok_lo - (prow_tiles - 1) * per_tile : 0;
-  const int64_t pc_full = item_cost(ptiles, per_tile * p.group), pc_last = item_cost(ptiles, last_tok * p.group);
+  const int64_t pc_full = item_cost(p, ptiles, per_tile), pc_last = item_cost(p, ptiles, last_tok);
   const int64_t ptotal = prow_tiles ? ((prow_tiles - 1) * pc_full + pc_last) * p.hkv : 0;
   const int per_thread = (p.b + C::NTHREADS - 1) / C::NTHREADS;
   const int s_lo = min(tid * per_thread, p.b), s_hi = min(s_lo + per_thread, p.b);
   int64_t mine = 0;
-  for (int s = s_lo; s < s_hi; ++s) mine += seq_cost<C::ROWS>(p, s, per_tile) * p.hkv;
+  for (int s = s_lo; s < s_hi; ++s) mine += seq_cost(p, s, per_tile) * p.hkv;
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -312,7 +363,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     int64_t at = excl;
     int s = s_lo;
     for (; s < s_hi; ++s) {
-      const int64_t c = seq_cost<C::ROWS>(p, s, per_tile) * p.hkv;
+      const int64_t c = seq_cost(p, s, per_tile) * p.hkv;
       if (own_from < at + c) break;
       at += c;
     }
@@ -321,283 +372,47 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
   __syncthreads();
   const uint32_t tmem = B.tmem;
 
-  if (warp == NSW) {
-    // ------------------------------------------------------------ TMA producer
-    const int nch = TK / p.chunk;
-    uint32_t u = 0;  // units issued
-    bool ok = true;
-    prefetch_tensormap(&kmap);
-    for (int sg = 0; ok; ++sg) {
-      ok = warp_wait(&B.seg_full[sg % kSegs], (sg / kSegs) & 1);
-      if (!ok) break;
-      const Seg s = B.seg[sg % kSegs];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&B.seg_empty[sg % kSegs]);
-      if (s.part < 0) break;
-      const int ntile = s.ke - s.kb;
-      const int* table = s.part == 0 ? p.prefix_table : p.tables + s.seq * p.table_stride;
-      // plane index of this lane's chunk of key tile j (chunks past the limit, and blocks that
-      // do not exist, lie past the map and load as zeros)
-      auto page = [&](int j) {
-        const int p0 = j * TK + lane * p.chunk;
-        if (lane >= nch || j >= s.ke || p0 >= s.limit) return p.oob;
-        const int blk = __ldg(table + p0 / p.block_size);
-        if (blk < 0 || blk >= p.num_blocks) {
-          set_error(p.err, FOLD_DEVERR_BLOCK_TABLE);
-          return p.oob;
-        }
-        return blk * p.mul_b + s.head * p.mul_h;
-      };
-      int ids[2] = {0, 0};
-      int next = page(s.kb);
-      for (int pos = 0; ok && pos < 2 * ntile; ++pos) {
-        const bool is_v = pos != 0 && (pos == 2 * ntile - 1 || (pos & 1) == 0);
-        const int j = pos == 0 ? 0 : pos == 2 * ntile - 1 ? ntile - 1 : is_v ? pos / 2 - 1 : (pos + 1) / 2;
-        int id;
-        if (is_v) {
-          id = (j & 1) ? ids[1] : ids[0];
-        } else {
-          id = next;
-          if (j & 1) ids[1] = id;
-          else ids[0] = id;
-          next = page(s.kb + j + 1);  // looked up one tile ahead
-        }
-        const int c3 = (((s.kb + j) * TK + lane * p.chunk) % p.block_size) / 8;
-#pragma unroll
-        for (int w = 0; w < KU; ++w, ++u) {
-          const int slot = u % NU;
-          if (u >= NU) ok = warp_wait(&B.empty[slot], ((u / NU) - 1) & 1);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive_expect_tx(&B.full[slot], C::UNIT);
-          __syncwarp();
-          if (lane < nch)
-            tma_load_5d(smem + slot * C::UNIT + lane * p.chunk * (C::UC * 2), is_v ? &vmap : &kmap, &B.full[slot],
-                        w * C::NCG, c3, id);
-        }
-      }
-    }
-    if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
-    // copies in flight land before exit
-    for (uint32_t w = u > NU ? u - NU : 0; w < u; ++w) warp_wait(&B.full[w % NU], (w / NU) & 1);
-  } else if (warp == NSW + 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      constexpr uint32_t idesc_s = idesc_of(C::F16, TK, 0);
-      constexpr uint32_t idesc_o = idesc_of(C::F16, C::UC, 1);
-      const uint32_t base = smem_u32(smem), q_base = base + C::OFF_Q;
-      uint32_t u0 = 0, qu = 0;             // ring units and Q tiles of earlier segments
-      uint32_t pcnt[2] = {0, 0};           // P tiles consumed per S buffer
-      bool ok = true;
-      int sg = 0;
-      for (; ok; ++sg) {
-        ok = mbar_wait(&B.seg_full[sg % kSegs], (sg / kSegs) & 1);
-        if (!ok) break;
-        const Seg s = B.seg[sg % kSegs];
-        mbar_arrive(&B.seg_empty[sg % kSegs]);
-        if (s.part < 0) break;
-        const int ntile = s.ke - s.kb;
-        const bool wide = s.rows > 128;  // the slots are row halves; else they alternate key tiles
-        const int steps = wide ? 2 * ntile : ntile;
-        auto qk = [&](int i) {
-          const int b = i & 1, j = wide ? i >> 1 : i;
-          const uint32_t quse = qu + (wide ? b : 0), qslot = quse % QB;
-          if (wide ? i < 2 : i == 0) ok = ok && mbar_wait(&B.q_full[qslot], (quse / QB) & 1);
-          const uint32_t u = u0 + k_pos(j) * KU;
-          const uint32_t d = tmem + C::TMEM_S + b * TK;
-#pragma unroll
-          for (int w = 0; w < KU; ++w) {
-            const uint32_t slot = (u + w) % NU;
-            if (!wide || b == 0) ok = ok && mbar_wait(&B.full[slot], ((u + w) / NU) & 1);
-            if (!ok) return;
-            tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < C::UC / 16; ++kk) {
-              const uint32_t a = q_base + qslot * C::Q_TILE + (w * C::NCG + (kk >> 2)) * C::Q_CG + (kk & 3) * 32;
-              const uint32_t kb = base + slot * C::UNIT + (kk >> 2) * 1024 + (kk & 3) * 32;
-              tc_mma(d, smem_desc(a, 16, 1024, kSwizzle128), smem_desc(kb, 16, C::NCG * 1024, kSwizzle128), idesc_s,
-                     w > 0 || kk > 0);
-            }
-          }
-          tc_commit(&B.s_full[b]);
-          if (!wide || b == 1)
-            for (int w = 0; w < KU; ++w) tc_commit(&B.empty[(u + w) % NU]);
-          if (i + (wide ? 2 : 1) >= steps) tc_commit(&B.q_empty[qslot]);
-        };
-        qk(0);
-        if (ok && steps > 1) qk(1);
-        for (int i = 0; ok && i < steps; ++i) {
-          const int b = i & 1, j = wide ? i >> 1 : i;
-          ok = mbar_wait(&B.p_full[b], pcnt[b] & 1);
-          ++pcnt[b];
-          // the accumulators of the last segment have been read
-          if (ok && i == 0 && sg > 0) ok = mbar_wait(&B.o_free, (sg - 1) & 1);
-          const uint32_t u = u0 + v_pos(j, ntile) * KU;
-          const uint32_t a = tmem + C::TMEM_S + b * TK;
-          const uint32_t o = tmem + C::TMEM_O + (NWG == 2 ? b * HD : 0);
-          const bool first = NWG == 2 ? i < 2 : i == 0;
-#pragma unroll
-          for (int w = 0; w < KU; ++w) {
-            const uint32_t slot = (u + w) % NU;
-            if (!wide || b == 0) ok = ok && mbar_wait(&B.full[slot], ((u + w) / NU) & 1);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int ks = 0; ks < TK / 16; ++ks) {
-              const uint32_t v = base + slot * C::UNIT + ks * 2 * C::NCG * 1024;
-              tc_mma_ts(o + w * C::UC, a + ks * 8, smem_desc(v, 1024, C::NCG * 1024, kSwizzle128), idesc_o,
-                        !first || ks > 0);
-            }
-          }
-          if (!ok) break;
-          if (NWG == 1) tc_commit(&B.pv_done);
-          if (!wide || b == 1)
-            for (int w = 0; w < KU; ++w) tc_commit(&B.empty[(u + w) % NU]);
-          if (i + 2 < steps) qk(i + 2);
-        }
-        if (!ok) break;
-        tc_commit(&B.seg_done);
-        u0 += 2 * ntile * KU;
-        qu += wide ? 2 : 1;
-      }
-      if (!ok) {  // let what was issued finish before TMEM goes
-        set_error(p.err, FOLD_DEVERR_TIMEOUT);
-        tc_commit(&B.seg_done);
-        mbar_wait(&B.seg_done, sg & 1);
-      }
-    }
+  // Every role walks the segments in the scheduler's order.
+  auto next_seg = [&](int sg, Seg& s) {
+    if (!warp_wait(&B.seg_full[sg % kSegs], (sg / kSegs) & 1)) return false;
+    s = B.seg[sg % kSegs];
     __syncwarp();
-  } else if (warp == NSW + 2) {
-    // ------------------------------------------------------------ scheduler and Q loader
-    uint32_t qu = 0;
-    int sg = 0;
-    bool ok = true;
-    auto publish = [&](const Seg& s) {
-      if (sg >= kSegs) ok = warp_wait(&B.seg_empty[sg % kSegs], ((sg / kSegs) - 1) & 1);
-      if (!ok) return;
-      if (lane == 0) {
-        B.seg[sg % kSegs] = s;
-        mbar_arrive(&B.seg_full[sg % kSegs]);
-      }
-      __syncwarp();
-      ++sg;
-      if (s.part < 0) return;
-      for (int r0 = 0; r0 < s.rows; r0 += 128, ++qu) {
-        const uint32_t slot = qu % QB;
-        if (qu >= QB) ok = warp_wait(&B.q_empty[slot], ((qu / QB) - 1) & 1);
-        if (!ok) return;
-        const int nr = min(128, s.rows - r0);
-        const uint32_t dst = smem_u32(smem + C::OFF_Q + slot * C::Q_TILE);
-        for (int e = lane; e < nr * (HD / 8); e += 32) {
-          const int r = e / (HD / 8), c = e - r * (HD / 8);
-          const int x = (r0 + r) / p.group, g = r0 + r - x * p.group;
-          const T* src = static_cast<const T*>(p.q) + (s.tok0 + x) * p.q_st + (s.head * p.group + g) * p.q_sh + c * 8;
-          cp_async_16(dst + (c >> 3) * C::Q_CG + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, 16);
-        }
-        cp_async_wait_all();
-        fence_proxy_async();  // Q is read by the tensor cores
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B.q_full[slot]);
-      }
-    };
-    // one item: s without its tile range; at: its place on the line
-    auto item = [&](Seg s, int ntok, int64_t at) {
-      const int tiles = (s.limit + TK - 1) / TK, w = tile_cost(s.rows);
-      // key tiles of this item that lie before place x of the line
-      auto tiles_before = [&](int64_t x) {
-        const int64_t y = x - at - kItemCost + w / 2;
-        return y <= 0 ? 0 : static_cast<int>(min64(y / w, tiles));
-      };
-      s.kb = tiles_before(x0), s.ke = cta + 1 == ctas ? tiles : tiles_before(x1);
-      if (s.kb < s.ke) publish(s);
-      if (at >= x0) {  // the item starts here: note the CTAs that hold its tiles
-        int c0 = cta, cnt = 0;
-        if (tiles > 0) {
-          auto upto = [&](int c) { return c + 1 >= ctas ? tiles : tiles_before(cut(c + 1)); };
-          while (upto(c0) == 0) ++c0;
-          int c1 = static_cast<int>(min64(ctas - 1, (at + kItemCost + static_cast<int64_t>(tiles) * w) * ctas / total));
-          c1 = max(c1, c0);
-          while (c1 > c0 && tiles_before(cut(c1)) >= tiles) --c1;
-          cnt = c1 - c0 + 1;
-        }
-        for (int x = lane; x < ntok; x += 32)
-          p.plan[(static_cast<int64_t>(s.part) * p.n + s.tok0 + x) * p.hkv + s.head] = make_int4(c0, cnt, s.tok0, 0);
-      }
-    };
-    if (x0 < x1) {
-      Seg s{};
-      if (x0 < ptotal) {
-        const int64_t row_cost = pc_full * p.hkv;
-        int rt = static_cast<int>(min64(x0 / row_cost, prow_tiles - 1));
-        const int64_t in_row = x0 - rt * row_cost;
-        int h = static_cast<int>(min64(in_row / (rt + 1 < prow_tiles ? pc_full : pc_last), p.hkv - 1));
-        for (; ok && rt < prow_tiles; ++rt, h = 0) {
-          const int ntok = rt + 1 < prow_tiles ? per_tile : last_tok;
-          const int64_t c = rt + 1 < prow_tiles ? pc_full : pc_last;
-          for (; ok && h < p.hkv; ++h) {
-            const int64_t at = rt * row_cost + h * c;
-            if (at >= x1) break;
-            s.part = 0, s.seq = 0, s.head = h, s.tok0 = tok_lo + rt * per_tile, s.rows = ntok * p.group;
-            s.limit = plen, s.lim0 = plen, s.lim_step = 0;
-            item(s, ntok, at);
-          }
-          if (h < p.hkv) break;
-        }
-      }
-      if (x1 > ptotal) {
-        int64_t at = ptotal + B.start_base;
-        for (int q = B.start_seq; ok && q < p.b && at < x1; ++q) {
-          int first, last;
-          seq_rows(p, q, first, last);
-          const int m = capped(__ldg(p.own_lens + q), p.own_cap, p.err);
-          for (int t0 = first; ok && t0 < last && at < x1; t0 += per_tile) {
-            const int ntok = min(per_tile, last - t0);
-            s.part = 1, s.seq = q, s.tok0 = t0, s.rows = ntok * p.group, s.lim_step = p.causal ? 1 : 0;
-            own_limits(p, first, last, m, t0, ntok, s.limit, s.lim0);
-            const int64_t c = item_cost((s.limit + TK - 1) / TK, s.rows);
-            int h = 0;
-            if (at + c * p.hkv <= x0) h = p.hkv;  // wholly before this CTA's piece
-            else if (x0 > at) h = static_cast<int>((x0 - at) / c);
-            for (; ok && h < p.hkv && at + h * c < x1; ++h) {
-              s.head = h;
-              item(s, ntok, at + h * c);
-            }
-            at += c * p.hkv;
-          }
-        }
-      }
-    }
-    if (ok) {
-      Seg s{};
-      s.part = -1;
-      publish(s);
-    }
-    if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
-  } else if (warp < NSW) {
+    if (lane == 0) mbar_arrive(&B.seg_empty[sg % kSegs]);
+    return true;
+  };
+
+  // With two softmax warpgroups the launch's registers (168 a thread) are dealt out again: a softmax
+  // thread holds a row of S (128 values). 2 * 208 + 88 = 3 * 168.
+  if (warp < NSW) {
+    if constexpr (NWG == 2) regs_up<208>();
     // ------------------------------------------------------------ softmax warps
     const int wg = warp >> 2, row = (warp & 3) * 32 + lane;  // row of the slot = TMEM lane
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
     uint32_t scnt[2] = {0, 0};  // S tiles read per buffer
-    uint32_t u0 = 0, pv = 0;
+    uint32_t step0 = 0, tile0 = 0;  // steps and tiles of the CTA's earlier segments
+    uint32_t done = 0;          // segments this warpgroup had steps of
+    uint32_t joins = 0;         // segments whose two slots were joined
     bool ok = true;
     for (int sg = 0; ok; ++sg) {
-      ok = warp_wait(&B.seg_full[sg % kSegs], (sg / kSegs) & 1);
-      if (!ok) break;
-      const Seg s = B.seg[sg % kSegs];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&B.seg_empty[sg % kSegs]);
-      if (s.part < 0) break;
+      Seg s;
+      ok = next_seg(sg, s);
+      if (!ok || s.part < 0) break;
       const int ntile = s.ke - s.kb;
-      const bool wide = s.rows > 128;
-      const int r = row + (wide ? wg * 128 : 0);
-      const bool live = r < s.rows;
-      const int x = live ? r / p.group : 0;
+      const bool wide = s.ntok > p.half_toks;
+      const bool joined = NWG == 2 && !wide && ntile > 1;  // both slots hold every row's keys
+      // this warpgroup's first step of the segment: its row half, or its first tile
+      const int mine0 = NWG == 2 ? (wg ^ step0) & 1 : 0;
+      const int half = wide ? mine0 : 0;
+      const int tok_first = half * p.half_toks;  // first token of this warpgroup's rows
+      const bool live = row < min(s.ntok - tok_first, p.half_toks) * p.group;
+      const int xr = row / p.group, x = live ? tok_first + xr : 0;
       const int lim = live ? min(s.limit, s.lim0 + x * s.lim_step) : 0;
       const bool warp_live = __any_sync(0xffffffffu, live);
       const int warp_lim = __reduce_min_sync(0xffffffffu, live ? lim : 0x7fffffff);
       float m = -INFINITY, l = 0.f;
       bool empty_o = true;
-      for (int j = (NWG == 2 && !wide) ? wg : 0; j < ntile; j += (NWG == 2 && !wide) ? 2 : 1) {
-        const int b = NWG == 2 ? wg : j & 1;
+      for (int j = (NWG == 2 && !wide) ? mine0 : 0; j < ntile; j += (NWG == 2 && !wide) ? 2 : 1) {
+        const int b = NWG == 2 ? wg : (step0 + j) & 1;
         ok = warp_wait(&B.s_full[b], scnt[b] & 1);
         ++scnt[b];
         if (!ok) break;
@@ -629,7 +444,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             if (!empty_o) {
               // the accumulator holds the products up to the slot's last tile; with one
               // accumulator the last tile's may still be running
-              if (NWG == 1) ok = warp_wait(&B.pv_done, (pv + j - 1) & 1);
+              if (NWG == 1) ok = warp_wait(&B.pv_done, (tile0 + j - 1) & 1);
               if (!ok) break;
               tc_fence_after();
               const uint32_t oa = tmem + C::TMEM_O + (NWG == 2 ? wg * HD : 0) + lane_addr;
@@ -665,9 +480,9 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         // slots of the last page past the limit may hold anything (NaN included): their V rows
         // become zeros before the tensor cores read them
         const int vk = s.limit - key0;
-        if (vk < TK && vk % p.chunk != 0 && (!wide || wg == 0)) {
+        if (vk < TK && vk % p.chunk != 0 && (!wide || mine0 == 0)) {
           const int vend = (vk / p.chunk + 1) * p.chunk;
-          const uint32_t u = u0 + v_pos(j, ntile) * KU;
+          const uint32_t u = v_pos(tile0 + j) * KU;
 #pragma unroll
           for (int w = 0; w < KU; ++w) {
             ok = ok && warp_wait(&B.full[(u + w) % NU], ((u + w) / NU) & 1);
@@ -687,36 +502,39 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         if (lane == 0) mbar_arrive(&B.p_full[b]);
       }
       if (!ok) break;
-      u0 += 2 * ntile * KU;
-      pv += ntile;
+      tile0 += ntile, step0 += wide ? 2 * ntile : ntile;
+      if (NWG == 2 && !wide && ntile == 1 && mine0 == 1) continue;  // the other slot's segment
 
       // ---- the segment's partial: O / l and lse
-      ok = warp_wait(&B.seg_done, sg & 1);
+      ok = warp_wait(&B.seg_done[NWG == 2 ? wg : 0], done++ & 1);
       if (!ok) break;
       tc_fence_after();
-      const bool joined = NWG == 2 && !wide;  // both slots hold every row's keys
       float ws[2] = {1.f, 0.f};
       if (joined) {
+        if (joins > 0) ok = warp_wait(&B.stat_free, (joins - 1) & 1);
+        if (!ok) break;
         stats[wg * 128 + row] = make_float2(m, l);
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&B.stat_full);
-        ok = warp_wait(&B.stat_full, sg & 1);
+        ok = warp_wait(&B.stat_full, joins & 1);  // and both accumulators are complete
         if (!ok) break;
+        tc_fence_after();
         const float2 a = stats[row], c = stats[128 + row];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.stat_free);
+        ++joins;
         m = fmaxf(a.x, c.x);
         const float mz = m == -INFINITY ? 0.f : m;
         ws[0] = fast_exp2(a.x - mz), ws[1] = fast_exp2(c.x - mz);
         l = a.y * ws[0] + c.y * ws[1];
-      } else if (NWG == 2) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&B.stat_full);  // keeps the barrier's phase with the segments'
       }
       const bool some = l > 0.f;
       const float inv = some ? 1.f / l : 0.f;
       ws[0] *= inv, ws[1] *= inv;
-      const int tok = s.tok0 + x, hqi = s.head * p.group + r - x * p.group;
+      const int tok = s.tok0 + x, hqi = s.head * p.group + row - xr * p.group;
       const int64_t prim = (static_cast<int64_t>(s.part) * p.n + tok) * p.hq + hqi;
-      const int64_t cont = static_cast<int64_t>(cta) * C::ROWS + r;
+      const int64_t cont = static_cast<int64_t>(cta) * C::ROWS + half * 128 + row;
       float* od = s.kb == 0 ? p.o_prim + prim * HD : p.o_cont + cont * HD;
       if (live && (!joined || wg == 0))
         (s.kb == 0 ? p.lse_prim + prim : p.lse_cont + cont)[0] =
@@ -724,15 +542,14 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       if (warp_live) {
         // joined slots: each warpgroup writes half of the columns of both accumulators' sum
         const int c_lo = joined ? wg * (HD / 2) : 0, c_hi = joined ? c_lo + HD / 2 : HD;
-        const bool two = joined && ntile > 1;
-        const uint32_t oa = tmem + C::TMEM_O + ((NWG == 2 && wide) ? wg * HD : 0) + lane_addr;
+        const uint32_t oa = tmem + C::TMEM_O + ((NWG == 2 && !joined) ? wg * HD : 0) + lane_addr;
 #pragma unroll 1
         for (int c = c_lo; c < c_hi; c += 16) {
           float o[16];
           tmem_ld16(oa + c, o);
 #pragma unroll
           for (int k = 0; k < 16; ++k) o[k] = some ? o[k] * ws[0] : l;  // l: 0, or the NaN of the row
-          if (two) {
+          if (joined) {
             float o2[16];
             tmem_ld16(oa + HD + c, o2);
 #pragma unroll
@@ -747,9 +564,306 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&B.o_free);
+      if (lane == 0) {
+        // an accumulator is free when all warps that read it are through (joined: both groups')
+        if (joined) mbar_arrive(&B.o_free[0]), mbar_arrive(&B.o_free[1]);
+        else mbar_arrive_n(&B.o_free[NWG == 2 ? wg : 0], NSW / 4);
+      }
     }
     if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+  } else {
+    if constexpr (NWG == 2) regs_down<88>();
+    if (warp == NSW) {
+      // ------------------------------------------------------------ TMA producer
+      const int nch = TK / p.chunk;
+      uint32_t u = 0;  // ring position
+      bool ok = true;
+      prefetch_tensormap(&kmap);
+      prefetch_tensormap(&vmap);
+      // one K or V tile at this lane's chunk's place
+      auto load_tile = [&](const CUtensorMap* map, int c3, int id) {
+#pragma unroll
+        for (int w = 0; w < KU; ++w, ++u) {
+          const int slot = u % NU;
+          if (u >= NU) ok = warp_wait(&B.empty[slot], ((u / NU) - 1) & 1);
+          if (!ok) return;
+          if (lane == 0) mbar_arrive_expect_tx(&B.full[slot], C::UNIT);
+          __syncwarp();
+          if (lane < nch)
+            tma_load_5d(smem + slot * C::UNIT + lane * p.chunk * (C::UC * 2), map, &B.full[slot], w * C::NCG, c3, id);
+        }
+      };
+      bool owed = false;  // the V tile of the last K tile is still to come
+      int v_c3 = 0, v_id = 0;
+      for (int sg = 0; ok; ++sg) {
+        Seg s;
+        ok = next_seg(sg, s);
+        if (!ok || s.part < 0) break;
+        const int* table = s.part == 0 ? p.prefix_table : p.tables + s.seq * p.table_stride;
+        // plane index of this lane's chunk of key tile j (chunks past the limit, and blocks that
+        // do not exist, lie past the map and load as zeros)
+        auto page = [&](int j) {
+          const int p0 = j * TK + lane * p.chunk;
+          if (lane >= nch || j >= s.ke || p0 >= s.limit) return p.oob;
+          const int blk = __ldg(table + p0 / p.block_size);
+          if (blk < 0 || blk >= p.num_blocks) {
+            set_error(p.err, FOLD_DEVERR_BLOCK_TABLE);
+            return p.oob;
+          }
+          return blk * p.mul_b + s.head * p.mul_h;
+        };
+        int next = page(s.kb);
+        for (int j = s.kb; ok && j < s.ke; ++j) {
+          const int id = next, c3 = ((j * TK + lane * p.chunk) % p.block_size) / 8;
+          next = page(j + 1);  // looked up one tile ahead
+          load_tile(&kmap, c3, id);
+          if (ok && owed) load_tile(&vmap, v_c3, v_id);
+          owed = true, v_c3 = c3, v_id = id;
+        }
+      }
+      uint32_t gap = 0;
+      if (ok && owed) {
+        gap = u, u += KU;  // the last V keeps its place (v_pos); the K that would run ahead of it is left out
+        load_tile(&vmap, v_c3, v_id);
+      }
+      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+      // copies in flight land before exit
+      for (uint32_t w = u > NU ? u - NU : 0; w < u; ++w)
+        if (gap == 0 || w - gap >= KU) warp_wait(&B.full[w % NU], (w / NU) & 1);
+    } else if (warp == NSW + 1) {
+      // ------------------------------------------------------------ MMA issuer
+      // Steps over all segments, alternating the S buffers: QK of step g+2 is issued behind PV of
+      // step g, across segments' borders. The whole warp walks; one lane issues.
+      constexpr uint32_t idesc_s = idesc_of(C::F16, TK, 0);
+      constexpr uint32_t idesc_o = idesc_of(C::F16, C::UC, 1);
+      constexpr uint32_t hi_q = desc_hi(1024), hi_kv = desc_hi(C::NCG * 1024);
+      const uint32_t base = uniform(smem_u32(smem)), q_base = base + C::OFF_Q, tm = uniform(tmem);
+      struct Step {
+        uint32_t tile;  // of the CTA
+        bool valid, first, last, free_kv;
+      } st0, st1;
+      bool ok = true, more = true, wide = false;
+      int sg = 0, i = 0, steps = 0;   // next segment; next step of the current one
+      uint32_t tile0 = 0, tiles = 0;  // first tile of the current segment; tiles of those before the next
+      uint32_t qu = 0;                // Q tiles used before the current segment
+      uint32_t pcnt[2] = {0, 0}, ocnt[2] = {0, 0};
+      auto qk = [&](Step& st, const int b) {  // the next step, into S buffer b
+        st.valid = false;
+        if (!more) return;
+        if (i == steps) {
+          if (steps) qu += wide ? 2 : 1;
+          Seg s;
+          ok = next_seg(sg, s);
+          if (!ok) return;
+          ++sg;
+          if (s.part < 0) {
+            more = false;
+            return;
+          }
+          wide = s.ntok > p.half_toks;  // the steps of a tile are its row halves
+          tile0 = tiles, tiles += s.ke - s.kb;
+          steps = (s.ke - s.kb) * (wide ? 2 : 1), i = 0;
+        }
+        const int half = wide ? i & 1 : 0;
+        const uint32_t tile = tile0 + (wide ? i >> 1 : i);
+        const uint32_t quse = qu + half, qslot = quse % QB;
+        if (i == half) ok = warp_wait(&B.q_full[qslot], (quse / QB) & 1);
+        const uint32_t u = k_pos(tile) * KU;
+        const bool free_kv = !wide || half == 1;
+#pragma unroll
+        for (int w = 0; w < KU; ++w) {
+          const uint32_t slot = (u + w) % NU;
+          if (half == 0) ok = ok && warp_wait(&B.full[slot], ((u + w) / NU) & 1);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t a = uniform(desc_lo(q_base + qslot * C::Q_TILE + w * C::NCG * C::Q_CG, 16));
+          const uint32_t k = uniform(desc_lo(base + slot * C::UNIT, 16));
+          if (elect_one()) {
+#pragma unroll
+            for (int kk = 0; kk < C::UC / 16; ++kk)
+              mma_ss(tm + C::TMEM_S + b * TK, a + ((kk >> 2) * C::Q_CG + (kk & 3) * 32) / 16, hi_q,
+                     k + ((kk >> 2) * 1024 + (kk & 3) * 32) / 16, hi_kv, idesc_s, w > 0 || kk > 0);
+            if (w == KU - 1) tc_commit(&B.s_full[b]);
+            if (free_kv) tc_commit(&B.empty[slot]);
+            if (w == KU - 1 && i + (wide ? 2 : 1) >= steps) tc_commit(&B.q_empty[qslot]);
+          }
+          __syncwarp();
+        }
+        st = Step{tile, true, NWG == 2 ? i < 2 : i == 0, i + NWG >= steps, free_kv};
+        ++i;
+      };
+      auto pv = [&](Step& st, const int b) {
+        const int acc = NWG == 2 ? b : 0;
+        ok = warp_wait(&B.p_full[b], pcnt[b]++ & 1);
+        if (ok && st.first) {  // the accumulator's last segment has been read
+          if (ocnt[acc] > 0) ok = warp_wait(&B.o_free[acc], (ocnt[acc] - 1) & 1);
+          ++ocnt[acc];
+        }
+        const uint32_t u = v_pos(st.tile) * KU, fresh = st.first ? 1 : 0;
+#pragma unroll
+        for (int w = 0; w < KU; ++w) {
+          const uint32_t slot = (u + w) % NU;
+          ok = ok && warp_wait(&B.full[slot], ((u + w) / NU) & 1);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t v = uniform(desc_lo(base + slot * C::UNIT, 1024)), add = uniform(fresh ^ 1);
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < TK / 16; ++ks)
+              mma_ts(tm + C::TMEM_O + acc * HD + w * C::UC, tm + C::TMEM_S + b * TK + ks * 8,
+                     v + ks * 2 * C::NCG * 1024 / 16, hi_kv, idesc_o, ks > 0 ? 1 : add);
+            if (NWG == 1 && w == KU - 1) tc_commit(&B.pv_done);
+            if (st.free_kv) tc_commit(&B.empty[slot]);
+            if (w == KU - 1 && st.last) tc_commit(&B.seg_done[acc]);
+          }
+          __syncwarp();
+        }
+        qk(st, b);
+      };
+      qk(st0, 0);
+      if (ok) qk(st1, 1);
+      while (ok && st0.valid) {
+        pv(st0, 0);
+        if (!ok || !st1.valid) break;
+        pv(st1, 1);
+      }
+      if (!ok) {  // let what was issued finish before TMEM goes
+        if (elect_one()) {
+          set_error(p.err, FOLD_DEVERR_TIMEOUT);
+          tc_commit(&B.drained);
+        }
+        __syncwarp();
+        warp_wait(&B.drained, 0);
+      }
+    } else if (warp == NSW + 3) {
+      // ------------------------------------------------------------ Q loader
+      uint32_t qu = 0;
+      bool ok = true;
+      for (int sg = 0; ok; ++sg) {
+        Seg s;
+        ok = next_seg(sg, s);
+        if (!ok || s.part < 0) break;
+        for (int t0 = 0; ok && t0 < s.ntok; t0 += p.half_toks, ++qu) {
+          const uint32_t slot = qu % QB;
+          if (qu >= QB) ok = warp_wait(&B.q_empty[slot], ((qu / QB) - 1) & 1);
+          if (!ok) break;
+          const int nt = min(p.half_toks, s.ntok - t0);
+          unsigned char* dst = smem + C::OFF_Q + slot * C::Q_TILE;
+          if (nt > kFewToks) {
+            // a box of half_toks tokens (those past nt give rows that nobody reads)
+            if (lane == 0) {
+              mbar_arrive_expect_tx(&B.q_full[slot], HD / 64 * p.half_toks * p.group * 128);
+#pragma unroll
+              for (int c = 0; c < HD / 64; ++c)
+                tma_load_3d_plain(dst + c * C::Q_CG, &qmap, &B.q_full[slot], c * 64, s.head * p.group, s.tok0 + t0);
+            }
+            __syncwarp();
+          } else {
+            constexpr int CPR = HD / 8, RPI = 32 / CPR;  // 16-byte chunks of a row, rows a round
+            const int c = lane % CPR;
+            int r = lane / CPR, x = r / p.group, g = r - x * p.group;
+            const uint32_t d = smem_u32(dst) + (c >> 3) * C::Q_CG;
+            const T* src = static_cast<const T*>(p.q) + (s.tok0 + t0) * p.q_st + s.head * p.group * p.q_sh + c * 8;
+            for (; x < nt; r += RPI, g += RPI) {
+              while (g >= p.group) g -= p.group, ++x;
+              if (x < nt) cp_async_16(d + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + x * p.q_st + g * p.q_sh, 16);
+            }
+            cp_async_wait_all();
+            fence_proxy_async();  // Q is read by the tensor cores
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&B.q_full[slot]);
+          }
+        }
+      }
+      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+    } else if (warp == NSW + 2) {
+      // ------------------------------------------------------------ scheduler
+      int sg = 0;
+      bool ok = true;
+      auto publish = [&](const Seg& s) {
+        if (sg >= kSegs) ok = warp_wait(&B.seg_empty[sg % kSegs], ((sg / kSegs) - 1) & 1);
+        if (!ok) return;
+        if (lane == 0) {
+          B.seg[sg % kSegs] = s;
+          mbar_arrive(&B.seg_full[sg % kSegs]);
+        }
+        __syncwarp();
+        ++sg;
+      };
+      // one item: s without its tile range; at: its place on the line
+      auto item = [&](Seg s, int64_t at) {
+        const int tiles = (s.limit + TK - 1) / TK, w = tile_cost(p, s.ntok);
+        // key tiles of this item that lie before place x of the line
+        auto tiles_before = [&](int64_t x) {
+          const int64_t y = x - at - kItemCost + w / 2;
+          return y <= 0 ? 0 : static_cast<int>(min64(y / w, tiles));
+        };
+        s.kb = tiles_before(x0), s.ke = cta + 1 == ctas ? tiles : tiles_before(x1);
+        if (s.kb < s.ke) publish(s);
+        if (at >= x0) {  // the item starts here: note the CTAs that hold its tiles
+          int c0 = cta, cnt = 0;
+          if (tiles > 0) {
+            auto upto = [&](int c) { return c + 1 >= ctas ? tiles : tiles_before(cut(c + 1)); };
+            while (upto(c0) == 0) ++c0;
+            int c1 = static_cast<int>(min64(ctas - 1, (at + kItemCost + static_cast<int64_t>(tiles) * w) * ctas / total));
+            c1 = max(c1, c0);
+            while (c1 > c0 && tiles_before(cut(c1)) >= tiles) --c1;
+            cnt = c1 - c0 + 1;
+          }
+          for (int x = lane; x < s.ntok; x += 32)
+            p.plan[(static_cast<int64_t>(s.part) * p.n + s.tok0 + x) * p.hkv + s.head] = make_int4(c0, cnt, s.tok0, 0);
+        }
+      };
+      if (x0 < x1) {
+        Seg s{};
+        if (x0 < ptotal) {
+          const int64_t row_cost = pc_full * p.hkv;
+          int rt = static_cast<int>(min64(x0 / row_cost, prow_tiles - 1));
+          const int64_t in_row = x0 - rt * row_cost;
+          int h = static_cast<int>(min64(in_row / (rt + 1 < prow_tiles ? pc_full : pc_last), p.hkv - 1));
+          for (; ok && rt < prow_tiles; ++rt, h = 0) {
+            const int ntok = rt + 1 < prow_tiles ? per_tile : last_tok;
+            const int64_t c = rt + 1 < prow_tiles ? pc_full : pc_last;
+            for (; ok && h < p.hkv; ++h) {
+              const int64_t at = rt * row_cost + h * c;
+              if (at >= x1) break;
+              s.part = 0, s.seq = 0, s.head = h, s.tok0 = tok_lo + rt * per_tile, s.ntok = ntok;
+              s.limit = plen, s.lim0 = plen, s.lim_step = 0;
+              item(s, at);
+            }
+            if (h < p.hkv) break;
+          }
+        }
+        if (x1 > ptotal) {
+          int64_t at = ptotal + B.start_base;
+          for (int q = B.start_seq; ok && q < p.b && at < x1; ++q) {
+            int first, last;
+            seq_rows(p, q, first, last);
+            const int m = capped(__ldg(p.own_lens + q), p.own_cap, p.err);
+            for (int t0 = first; ok && t0 < last && at < x1; t0 += per_tile) {
+              const int ntok = min(per_tile, last - t0);
+              s.part = 1, s.seq = q, s.tok0 = t0, s.ntok = ntok, s.lim_step = p.causal ? 1 : 0;
+              own_limits(p, first, last, m, t0, ntok, s.limit, s.lim0);
+              const int64_t c = item_cost(p, (s.limit + TK - 1) / TK, ntok);
+              int h = 0;
+              if (at + c * p.hkv <= x0) h = p.hkv;  // wholly before this CTA's piece
+              else if (x0 > at) h = static_cast<int>((x0 - at) / c);
+              for (; ok && h < p.hkv && at + h * c < x1; ++h) {
+                s.head = h;
+                item(s, at + h * c);
+              }
+              at += c * p.hkv;
+            }
+          }
+        }
+      }
+      if (ok) {
+        Seg s{};
+        s.part = -1;
+        publish(s);
+      }
+      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+    }
   }
 
   tc_fence_before();
@@ -797,7 +911,7 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixParams p)
     const int4 plan = p.plan[tr * p.hkv + hk];
     if (plan.y < 1) continue;
     add(p.lse_prim[tr * p.hq + h], p.o_prim + (tr * p.hq + h) * HD);
-    const int r = (tok - plan.z) * p.group + g;
+    const int x = tok - plan.z, half = x / p.half_toks, r = half * 128 + (x - half * p.half_toks) * p.group + g;
     for (int c = plan.x + 1; c < plan.x + plan.y; ++c) {
       const int64_t at = static_cast<int64_t>(c) * ROWS + r;
       add(p.lse_cont[at], p.o_cont + at * HD);
@@ -837,12 +951,8 @@ int ctas_of_device() {
   return sms > 0 ? sms : 148;
 }
 
-// 5-D map of a K or V plane: 64 columns, 8 slots, 64-column groups, groups of 8 slots, and blocks
-// and heads as one index (in units of the smaller of their strides). A box of `chunk` slots lands
-// as [group of 8 slots][64-column group][8 rows of 128 bytes], 128-byte swizzled: consecutive
-// chunks stack to a tile whose 8-row groups have one stride, whatever the page size.
-int plane_map(const void* base, int hd, int box_cols, int block_size, int chunk, int64_t slot, int64_t unit,
-              int64_t count, bool f16, CUtensorMap* out) {
+int encode_map(const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+               bool f16, CUtensorMap* out) {
   static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult r;
@@ -852,13 +962,8 @@ int plane_map(const void* base, int hd, int box_cols, int block_size, int chunk,
                : nullptr;
   }();
   if (!encode) return fail(FOLD_ERR_TENSOR_MAP, "prefix read: cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t dims[5] = {64, 8, static_cast<cuuint64_t>(hd / 64), static_cast<cuuint64_t>(block_size / 8),
-                              static_cast<cuuint64_t>(count)};
-  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(slot) * 2, 128, static_cast<cuuint64_t>(slot) * 16,
-                                 static_cast<cuuint64_t>(unit) * 2};
-  const cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(box_cols / 64), static_cast<cuuint32_t>(chunk / 8), 1};
   const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
-  const CUresult r = encode(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+  const CUresult r = encode(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
                             const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -867,17 +972,48 @@ int plane_map(const void* base, int hd, int box_cols, int block_size, int chunk,
   return FOLD_OK;
 }
 
+// 3-D map of q: columns, heads, tokens; a box is one 64-column group of a half row tile's rows.
+int query_map(const PrefixParams& p, int hd, bool f16, CUtensorMap* out) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(p.hq), static_cast<cuuint64_t>(p.n)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.q_sh) * 2, static_cast<cuuint64_t>(p.q_st) * 2};
+  const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(p.half_toks)};
+  return encode_map(p.q, 3, dims, strides, box, f16, out);
+}
+
+// 5-D map of a K or V plane: 64 columns, 8 slots, 64-column groups, groups of 8 slots, and blocks
+// and heads as one index (in units of the smaller of their strides). A box of `chunk` slots lands
+// as [group of 8 slots][64-column group][8 rows of 128 bytes], 128-byte swizzled: consecutive
+// chunks stack to a tile whose 8-row groups have one stride, whatever the page size.
+int plane_map(const void* base, int hd, int box_cols, int block_size, int chunk, int64_t slot, int64_t unit,
+              int64_t count, bool f16, CUtensorMap* out) {
+  const cuuint64_t dims[5] = {64, 8, static_cast<cuuint64_t>(hd / 64), static_cast<cuuint64_t>(block_size / 8),
+                              static_cast<cuuint64_t>(count)};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(slot) * 2, 128, static_cast<cuuint64_t>(slot) * 16,
+                                 static_cast<cuuint64_t>(unit) * 2};
+  const cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(box_cols / 64), static_cast<cuuint32_t>(chunk / 8), 1};
+  return encode_map(base, 5, dims, strides, box, f16, out);
+}
+
 template <int HD, class T>
 int launch_prefix(const PrefixParams& p, const void* k, const void* v, int64_t slot, int64_t unit, cudaStream_t stream) {
   using C = Cfg<HD, T>;
-  CUtensorMap kmap, vmap;
+  CUtensorMap qmap, kmap, vmap;
+  if (int s = query_map(p, HD, C::F16, &qmap)) return s;
   const int64_t count = p.oob;
   if (int s = plane_map(k, HD, C::UC, p.block_size, p.chunk, slot, unit, count, C::F16, &kmap)) return s;
   if (int s = plane_map(v, HD, C::UC, p.block_size, p.chunk, slot, unit, count, C::F16, &vmap)) return s;
   static std::atomic<uint64_t> configured{0};
   if (int s = allow_smem(prefix_read_kernel<C>, C::SMEM, configured, "cudaFuncSetAttribute(prefix_read)")) return s;
+  if constexpr (C::NWG == 2) {
+    // the register shares the warps take must add up to what a block is launched with
+    static const int regs = [] {
+      cudaFuncAttributes a{};
+      return cudaFuncGetAttributes(&a, prefix_read_kernel<C>) == cudaSuccess ? a.numRegs : 0;
+    }();
+    if (regs != 168) return fail(FOLD_ERR_UNSUPPORTED, "prefix read: built with other register shares than launched");
+  }
   if (int s = launch_behind(prefix_read_kernel<C>, dim3(p.ctas), C::NTHREADS, C::SMEM, stream, "prefix_read_kernel",
-                            kmap, vmap, p))
+                            qmap, kmap, vmap, p))
     return s;
   const int64_t rows = static_cast<int64_t>(p.n) * p.hq;
   return launch_behind(prefix_merge_kernel<HD, T, C::ROWS>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream,
@@ -916,6 +1052,10 @@ int fold_prefix_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
       q_stride_head % 8 || o_stride_tok % 8 || o_stride_head % 8 || cache_stride_block % 8 || cache_stride_head % 8 ||
       cache_stride_slot % 8)
     return fail(FOLD_ERR_ALIGNMENT, "prefix read: rows of q, out and the cache must start on 16-byte boundaries");
+  if (n == 1) q_stride_tok = static_cast<int64_t>(hq) * hd;  // strides of a single row or head are free
+  if (hq == 1) q_stride_head = hd;
+  if (q_stride_tok < 1 || q_stride_head < 1 || q_stride_tok >= (int64_t(1) << 38) || q_stride_head >= (int64_t(1) << 38))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "prefix read: q's strides must be positive");
   if (cache_stride_slot < hd || cache_stride_slot >= (int64_t(1) << 35))
     return fail(FOLD_ERR_INVALID_ARGUMENT, "prefix read: bad cache strides");
   // blocks and heads as one index of the plane
@@ -957,7 +1097,7 @@ int fold_prefix_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   p.oob = static_cast<int>((num_blocks - 1) * mul_b + (hkv - 1) * mul_h + 1);
   p.causal = causal ? 1 : 0, p.scale_log2 = softmax_scale * kLog2e;
   p.out = out, p.o_st = o_stride_tok, p.o_sh = o_stride_head, p.lse = lse;
-  p.n = n, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.ctas = ctas, p.err = err;
+  p.n = n, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.half_toks = 128 / p.group, p.ctas = ctas, p.err = err;
   char* ws = static_cast<char*>(workspace);
   p.plan = reinterpret_cast<int4*>(ws + w.plan);
   p.o_prim = reinterpret_cast<float*>(ws + w.o_prim), p.lse_prim = reinterpret_cast<float*>(ws + w.lse_prim);

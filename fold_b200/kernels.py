@@ -476,7 +476,7 @@ def prefix_read(q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, bl
     if lse is not None and (lse.shape != (hq, n) or lse.dtype != torch.float32 or not lse.is_contiguous()):
         raise FoldError("prefix_read: lse must be contiguous float32 [Hq, n]")
     _check_err("prefix_read", err)
-    if q.stride(-1) != 1:
+    if q.stride(-1) != 1 or min(q.stride()) < 1:  # heads or rows that share memory are copied apart
         q = q.contiguous()
     if workspace is None:
         workspace = prefix_workspace(n, hq, hkv, d, q.device)
