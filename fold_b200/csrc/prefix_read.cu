@@ -95,12 +95,12 @@ struct Cfg {
   static constexpr int Q_CG = 128 * 128;  // one 64-column group of a Q tile
   static constexpr int Q_TILE = 128 * HD * 2;
   static constexpr int QB = HD == 256 ? 1 : 2;
-  static constexpr int MISC = 768 + 2048;  // barriers, segments, scan; row statistics
+  static constexpr int MISC = 1024 + 2048;  // barriers, segments, scan; row statistics
   static constexpr int FIT = (kSmemLimit - MISC - QB * Q_TILE) / UNIT;
   static constexpr int NU = FIT > 12 ? 12 : FIT;
   static constexpr int OFF_Q = NU * UNIT;
   static constexpr int OFF_BAR = OFF_Q + QB * Q_TILE;
-  static constexpr int OFF_STAT = OFF_BAR + 768;
+  static constexpr int OFF_STAT = OFF_BAR + 1024;
   static constexpr int SMEM = OFF_BAR + MISC;
   static constexpr int TMEM_S = 0, TMEM_O = 256, TMEM_COLS = 512;
   static constexpr bool F16 = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
@@ -110,7 +110,7 @@ struct Cfg {
 };
 
 // Cost units (a quarter of a key tile of a row tile of at most 128 rows).
-constexpr int kTileCost = 4, kWideTileCost = 8, kItemCost = 4;
+constexpr int kTileCost = 5, kWideTileCost = 8, kItemCost = 12, kFewItemCost = 6;
 
 struct Seg {
   int part;  // 0: prefix, 1: own keys, -1: no more work
@@ -122,6 +122,9 @@ struct Seg {
 };
 constexpr int kSegs = 4;
 
+// Segments of up to this many rows are read by the softmax warps themselves (FewRows).
+constexpr int kFewRows = 16;
+
 // Q of up to this many tokens is copied row by row, of more as one box of the half tile (a box always
 // moves all of its rows).
 constexpr int kFewToks = 8;
@@ -131,14 +134,14 @@ struct Bars {
   uint64_t s_full[2], p_full[2], pv_done;
   uint64_t q_full[2], q_empty[2];
   uint64_t seg_full[kSegs], seg_empty[kSegs];
-  uint64_t seg_done[2], o_free[2], stat_full, stat_free, drained;
+  uint64_t seg_done[2], o_free[2], stat_full, stat_free, drained, meet;
   uint32_t tmem;
-  int start_seq;
-  int64_t start_base;
-  int64_t scan[12];
+  int start_seq[2];
+  int64_t start_base[2];
+  int64_t scan[2][12];
   Seg seg[kSegs];
 };
-static_assert(sizeof(Bars) <= 768, "barriers fit their place");
+static_assert(sizeof(Bars) <= 1024, "barriers fit their place");
 
 // ---------------------------------------------------------------- the line of work
 __device__ __forceinline__ int capped(int len, int cap, int* err) {
@@ -166,23 +169,31 @@ __device__ __forceinline__ void own_limits(const PrefixParams& p, int first, int
   limit = p.causal ? max(min(m, lim0 + ntok - 1), 0) : m;
 }
 
-__device__ __forceinline__ int64_t item_cost(const PrefixParams& p, int tiles, int ntok) {
-  return kItemCost + static_cast<int64_t>(tiles) * tile_cost(p, ntok);
+// Division of non-negative values, in 32 bits where they fit.
+__device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
 }
 
-// Cost of all own items of sequence s and one KV head.
-__device__ __forceinline__ int64_t seq_cost(const PrefixParams& p, int s, int per_tile) {
+__device__ __forceinline__ int start_cost(const PrefixParams& p, int ntok) {
+  return ntok * p.group <= kFewRows ? kFewItemCost : kItemCost;
+}
+__device__ __forceinline__ int64_t item_cost(const PrefixParams& p, int tiles, int ntok) {
+  return tiles == 0 ? 2 : start_cost(p, ntok) + static_cast<int64_t>(tiles) * tile_cost(p, ntok);
+}
+
+// Cost of the own items of sequence s and one KV head: of many rows, and of few.
+template <class C>
+__device__ __forceinline__ void seq_cost(const PrefixParams& p, int s, int per_tile, int64_t (&cost)[2]) {
   int first, last;
   seq_rows(p, s, first, last);
   const int m = capped(__ldg(p.own_lens + s), p.own_cap, p.err);
-  int64_t c = 0;
+  cost[0] = cost[1] = 0;
   for (int t0 = first; t0 < last; t0 += per_tile) {
     const int nt = min(per_tile, last - t0);
     int limit, lim0;
     own_limits(p, first, last, m, t0, nt, limit, lim0);
-    c += item_cost(p, (limit + TK - 1) / TK, nt);
+    cost[nt * p.group <= kFewRows] += item_cost(p, (limit + TK - 1) / TK, nt);
   }
-  return c;
 }
 
 // ---------------------------------------------------------------- TMEM and MMA forms of this kernel
@@ -207,6 +218,12 @@ __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Eight floats to a 32-byte boundary, one whole sector.
+__device__ __forceinline__ void store8(float* dst, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -282,6 +299,12 @@ __device__ __forceinline__ uint32_t v_pos(uint32_t j) { return 2 * j + 2; }
 __device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
 }
+// The arrival of all n threads a barrier expects, once the MMAs issued so far have completed.
+template <int N>
+__device__ __forceinline__ void commit_for(uint64_t* bar) {
+  if constexpr (N > 1) mbar_arrive_n(bar, N - 1);
+  tc_commit(bar);
+}
 template <int N>
 __device__ __forceinline__ void regs_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -290,6 +313,267 @@ template <int N>
 __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
+
+// ---------------------------------------------------------------- segments of few rows
+// A row tile of at most FEW_ROWS rows (a decode step's, whose keys are read once for a handful of
+// rows) would leave most of the 128 lanes of S idle and pay for the way through the MMA warp. The
+// softmax warps take such a segment themselves with mma.sync: each warp owns 128 / NSW keys of every
+// tile and keeps rows x keys and rows x hd fragments in registers (S = Q K^T, its C fragments are the
+// A fragments of P V), with a maximum, sum and O of its own, so that no warp waits for another until
+// the segment's end, where the warps' partials are joined through the Q tile. Memory bound: the
+// ring's units are all in flight.
+template <class C>
+struct FewRows {
+  static constexpr int HD = C::HD, KW = TK / C::NSW;
+  using T = typename C::T;
+  const PrefixParams& p;
+  const Seg& s;
+  Bars& B;
+  unsigned char* smem;
+  float2* stats;
+  const int warp, lane, cta;
+  const uint32_t tile0, qu;
+  uint32_t meets;
+
+  // All softmax warps, with a bounded wait.
+  __device__ __forceinline__ bool meet() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&B.meet);
+    return warp_wait(&B.meet, meets++ & 1);
+  }
+  __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (C::F16) mma_f16(d, a[0], a[1], a[2], a[3], b0, b1);
+    else mma_bf16(d, a[0], a[1], a[2], a[3], b0, b1);
+  }
+
+  __device__ __forceinline__ bool run() {
+    constexpr int MT = kFewRows / 16;
+    const int ntile = s.ke - s.kb, rows = s.ntok * p.group;
+    const int g = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;  // fragment row, column; ldmatrix
+    const uint32_t qslot = qu % C::QB;
+    if (!warp_wait(&B.q_full[qslot], (qu / C::QB) & 1)) return false;
+    const uint32_t base = smem_u32(smem), qt = base + C::OFF_Q + qslot * C::Q_TILE;
+    auto q_frag = [&](int mt, int kk, uint32_t (&a)[4]) {
+      const int r = mt * 16 + (mi & 1) * 8 + mr, c = 2 * kk + (mi >> 1);
+      ldsm_x4(qt + (c >> 3) * C::Q_CG + r * 128 + (((c & 7) ^ mr) << 4), a[0], a[1], a[2], a[3]);
+    };
+    constexpr bool HOLD = MT == 1 && HD <= 128;  // Q stays in registers
+    uint32_t qf[HOLD ? HD / 16 : 1][4];
+    if constexpr (HOLD) {
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) q_frag(0, kk, qf[kk]);
+    }
+    float o[MT][HD / 8][4], m[MT][2], l[MT][2];
+    int lim[MT][2];
+    bool in[MT][2];
+    int low = 0x7fffffff;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = mt * 16 + e * 8 + g;
+        in[mt][e] = r < rows;
+        lim[mt][e] = in[mt][e] ? min(s.limit, s.lim0 + (r / p.group) * s.lim_step) : 0;
+        if (in[mt][e]) low = min(low, lim[mt][e]);
+        m[mt][e] = -INFINITY, l[mt][e] = 0.f;
+      }
+    low = __reduce_min_sync(0xffffffffu, low);  // keys that every row sees
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][c][e] = 0.f;
+
+    for (int j = 0; j < ntile; ++j) {
+      const int key0 = (s.kb + j) * TK;
+      const uint32_t ku = k_pos(tile0 + j) * C::KU, vu = v_pos(tile0 + j) * C::KU;
+#pragma unroll
+      for (int w = 0; w < C::KU; ++w)
+        if (!warp_wait(&B.full[(ku + w) % C::NU], ((ku + w) / C::NU) & 1)) return false;
+      constexpr int KG = KW / 16;  // groups of 16 keys
+      const int row0 = warp * KW;  // this warp's first key of the tile
+      const bool any = key0 + row0 < s.limit;
+      uint32_t pa[KG][MT][4];
+      if (any) {
+        float x[KG][MT][2][4];
+#pragma unroll
+        for (int i = 0; i < KG * MT * 8; ++i) (&x[0][0][0][0])[i] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+          const uint32_t unit = base + ((ku + kk * 16 / C::UC) % C::NU) * C::UNIT;
+          const int c = (2 * kk + (mi & 1)) % (C::UC / 8);
+          uint32_t a[MT][4];
+          if constexpr (!HOLD) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) q_frag(mt, kk, a[mt]);
+          }
+#pragma unroll
+          for (int kg = 0; kg < KG; ++kg) {
+            uint32_t b[4];
+            ldsm_x4(unit + (((row0 + kg * 16) >> 3) + (mi >> 1)) * C::NCG * 1024 + (c >> 3) * 1024 + mr * 128 +
+                        (((c & 7) ^ mr) << 4),
+                    b[0], b[1], b[2], b[3]);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma(x[kg][mt][0], HOLD ? qf[HOLD ? kk : 0] : a[mt], b[0], b[1]);
+              mma(x[kg][mt][1], HOLD ? qf[HOLD ? kk : 0] : a[mt], b[2], b[3]);
+            }
+          }
+        }
+        if (key0 + row0 + KW > low) {
+#pragma unroll
+          for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                if (key0 + row0 + kg * 16 + (e >> 2) * 8 + 2 * t4 + (e & 1) >= lim[mt][(e >> 1) & 1])
+                  x[kg][mt][e >> 2][e & 3] = -INFINITY;
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          float f[2] = {1.f, 1.f};
+          bool up = false;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+              for (int n = 0; n < 2; ++n) top = fmax3(top, x[kg][mt][n][2 * e], x[kg][mt][n][2 * e + 1]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * p.scale_log2;
+            const bool raise = in[mt][e] && (top > m[mt][e] + kRowRaise || (m[mt][e] == -INFINITY && top > m[mt][e]));
+            if (raise) f[e] = fast_exp2(m[mt][e] - top), m[mt][e] = top;
+            up |= raise;
+          }
+          if (__any_sync(0xffffffffu, up)) {
+            l[mt][0] *= f[0], l[mt][1] *= f[1];
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) o[mt][c][0] *= f[0], o[mt][c][1] *= f[0], o[mt][c][2] *= f[1], o[mt][c][3] *= f[1];
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float neg = m[mt][e] == -INFINITY ? 0.f : C::SHIFT - m[mt][e];
+#pragma unroll
+            for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const float a = fast_exp2(fmaf(x[kg][mt][n][2 * e], p.scale_log2, neg));
+                const float d = fast_exp2(fmaf(x[kg][mt][n][2 * e + 1], p.scale_log2, neg));
+                l[mt][e] += a + d;
+                pa[kg][mt][2 * n + e] = pack2<T>(a, d);
+              }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {  // K goes back before V is waited for: the ring need not hold both
+#pragma unroll
+        for (int w = 0; w < C::KU; ++w) mbar_arrive(&B.empty[(ku + w) % C::NU]);
+      }
+#pragma unroll
+      for (int w = 0; w < C::KU; ++w)
+        if (!warp_wait(&B.full[(vu + w) % C::NU], ((vu + w) / C::NU) & 1)) return false;
+      if (any) {
+        // slots past the limit may hold anything (NaN included): this warp's rows of them become zeros
+        const int seen = s.limit - key0 - row0;
+        if (seen < KW) {
+#pragma unroll
+          for (int w = 0; w < C::KU; ++w) {
+            unsigned char* vt = smem + ((vu + w) % C::NU) * C::UNIT;
+            for (int e = lane; e < (KW - seen) * C::NCG * 8; e += 32) {
+              const int r = row0 + seen + e / (C::NCG * 8), c = e % (C::NCG * 8);
+              *reinterpret_cast<uint4*>(vt + (r >> 3) * C::NCG * 1024 + (c >> 3) * 1024 + (r & 7) * 128 + (c & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_proxy_async();  // the unit is loaded again by TMA
+          __syncwarp();
+        }
+#pragma unroll
+        for (int c = 0; c < HD / 16; ++c) {
+          const uint32_t unit = base + ((vu + c * 16 / C::UC) % C::NU) * C::UNIT;
+          const int cc = (2 * c + (mi >> 1)) % (C::UC / 8);
+#pragma unroll
+          for (int kg = 0; kg < KG; ++kg) {
+            uint32_t b[4];
+            ldsm_x4_t(unit + (((row0 + kg * 16) >> 3) + (mi & 1)) * C::NCG * 1024 + (cc >> 3) * 1024 + mr * 128 +
+                          (((cc & 7) ^ mr) << 4),
+                      b[0], b[1], b[2], b[3]);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma(o[mt][2 * c], pa[kg][mt], b[0], b[1]);
+              mma(o[mt][2 * c + 1], pa[kg][mt], b[2], b[3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+#pragma unroll
+        for (int w = 0; w < C::KU; ++w) mbar_arrive(&B.empty[(vu + w) % C::NU]);
+      }
+    }
+
+    // ---- the warps' partials joined, eight rows at a time, in the Q tile's memory
+    float* scratch = reinterpret_cast<float*>(smem + C::OFF_Q + qslot * C::Q_TILE);  // [warp][8 rows][HD]
+#pragma unroll
+    for (int h = 0; h < 2 * MT; ++h) {
+      if (h * 8 >= rows) break;
+      const int mt = h >> 1, e = h & 1, nr = min(8, rows - h * 8);
+      if (!meet()) return false;  // Q, or the last eight rows, have been read
+      float ls = l[mt][e];
+      ls += __shfl_xor_sync(0xffffffffu, ls, 1);
+      ls += __shfl_xor_sync(0xffffffffu, ls, 2);
+      if (t4 == 0) stats[warp * 8 + g] = make_float2(m[mt][e], ls);
+      if (g < nr) {
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c)
+          *reinterpret_cast<float2*>(scratch + (warp * 8 + g) * HD + c * 8 + 2 * t4) =
+              make_float2(o[mt][c][2 * e], o[mt][c][2 * e + 1]);
+      }
+      if (!meet()) return false;
+      for (int r = warp; r < nr; r += C::NSW) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < C::NSW; ++w) top = fmaxf(top, stats[w * 8 + r].x);
+        const float mz = top == -INFINITY ? 0.f : top;
+        float f[C::NSW], sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < C::NSW; ++w) {
+          const float2 a = stats[w * 8 + r];
+          f[w] = fast_exp2(a.x - mz), sum += f[w] * a.y;
+        }
+        const bool some = sum > 0.f;
+        const float inv = some ? 1.f / sum : 0.f;
+        const int row = h * 8 + r, x = row / p.group;
+        const int64_t prim = (static_cast<int64_t>(s.part) * p.n + s.tok0 + x) * p.hq + s.head * p.group + row - x * p.group;
+        const int64_t cont = static_cast<int64_t>(cta) * C::ROWS + row;
+        float* od = s.kb == 0 ? p.o_prim + prim * HD : p.o_cont + cont * HD;
+        for (int c = lane * 4; c < HD; c += 128) {
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < C::NSW; ++w) {
+            const float4 v = *reinterpret_cast<const float4*>(scratch + (w * 8 + r) * HD + c);
+            acc.x += f[w] * v.x, acc.y += f[w] * v.y, acc.z += f[w] * v.z, acc.w += f[w] * v.w;
+          }
+          // no key: 0; a NaN sum reaches the output
+          *reinterpret_cast<float4*>(od + c) = some ? make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv)
+                                                    : make_float4(sum, sum, sum, sum);
+        }
+        if (lane == 0)
+          (s.kb == 0 ? p.lse_prim + prim : p.lse_cont + cont)[0] =
+              some ? (top - C::SHIFT + __log2f(sum)) * kLn2 : (sum == 0.f ? -INFINITY : sum);
+      }
+    }
+    fence_proxy_async();  // the Q tile may be loaded by TMA next
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&B.q_empty[qslot]);
+    return true;
+  }
+};
 
 // ---------------------------------------------------------------- the kernel
 template <class C>
@@ -306,15 +590,15 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
 
   if (warp == NSW) {
     if (lane == 0) {
-      for (int i = 0; i < NU; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], 1);
+      for (int i = 0; i < NU; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], NSW);
       for (int i = 0; i < 2; ++i) {
         mbar_init(&B.s_full[i], 1), mbar_init(&B.p_full[i], 4);
-        mbar_init(&B.q_full[i], 1), mbar_init(&B.q_empty[i], 1);
+        mbar_init(&B.q_full[i], 1), mbar_init(&B.q_empty[i], NSW);
         mbar_init(&B.seg_done[i], 1), mbar_init(&B.o_free[i], NSW);
       }
       for (int i = 0; i < kSegs; ++i) mbar_init(&B.seg_full[i], 1), mbar_init(&B.seg_empty[i], 3 + NSW);
       mbar_init(&B.pv_done, 1), mbar_init(&B.stat_full, NSW), mbar_init(&B.stat_free, NSW);
-      mbar_init(&B.drained, 1);
+      mbar_init(&B.drained, 1), mbar_init(&B.meet, NSW);
       fence_mbar_init();
     }
     __syncwarp();
@@ -324,55 +608,79 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
   }
   wait_for_producer();
 
-  // ---- the line: prefix items first, then every sequence's own items
+  // ---- the line: items of many rows, then items of few; of each the prefix's before the sequences'
   const int tok_lo = min(max(__ldg(p.qsl), 0), p.n), tok_hi = min(max(__ldg(p.qsl + p.b), tok_lo), p.n);
   const int plen = capped(__ldg(p.prefix_len), p.prefix_cap, p.err);
   const int ptiles = (plen + TK - 1) / TK;
   const int prow_tiles = plen > 0 ? (tok_hi - tok_lo + per_tile - 1) / per_tile : 0;
   const int last_tok = prow_tiles ? tok_hi - tok_lo - (prow_tiles - 1) * per_tile : 0;
   const int64_t pc_full = item_cost(p, ptiles, per_tile), pc_last = item_cost(p, ptiles, last_tok);
-  const int64_t ptotal = prow_tiles ? ((prow_tiles - 1) * pc_full + pc_last) * p.hkv : 0;
+  const bool last_few = last_tok * p.group <= kFewRows;  // only the last row tile can be of few rows
+  const int64_t pfull = prow_tiles ? (prow_tiles - 1) * pc_full * p.hkv : 0, plast = prow_tiles ? pc_last * p.hkv : 0;
   const int per_thread = (p.b + C::NTHREADS - 1) / C::NTHREADS;
   const int s_lo = min(tid * per_thread, p.b), s_hi = min(s_lo + per_thread, p.b);
-  int64_t mine = 0;
-  for (int s = s_lo; s < s_hi; ++s) mine += seq_cost(p, s, per_tile) * p.hkv;
-  int64_t incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
+  int64_t mine[2] = {0, 0}, incl[2];
+  for (int s = s_lo; s < s_hi; ++s) {
+    int64_t c[2];
+    seq_cost<C>(p, s, per_tile, c);
+    mine[0] += c[0] * p.hkv, mine[1] += c[1] * p.hkv;
   }
-  if (lane == 31) B.scan[warp] = incl;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    incl[k] = mine[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl[k], o);
+      if (lane >= o) incl[k] += y;
+    }
+    if (lane == 31) B.scan[k][warp] = incl[k];
+  }
   tc_fence_before();
   __syncthreads();  // barriers, TMEM address and warp sums are visible
   tc_fence_after();
-  int64_t before = 0, total = ptotal;
+  int64_t own_total[2] = {0, 0}, excl[2];
 #pragma unroll
-  for (int w = 0; w < C::NTHREADS / 32; ++w) {
-    if (w < warp) before += B.scan[w];
-    total += B.scan[w];
+  for (int k = 0; k < 2; ++k) {
+    excl[k] = incl[k] - mine[k];
+#pragma unroll
+    for (int w = 0; w < C::NTHREADS / 32; ++w) {
+      if (w < warp) excl[k] += B.scan[k][w];
+      own_total[k] += B.scan[k][w];
+    }
   }
+  // where on the line the prefix's and the sequences' items of either kind begin
+  const int64_t from_own[2] = {pfull + (last_few ? 0 : plast),
+                               pfull + plast + own_total[0]};
+  const int64_t from_last = last_few ? pfull + own_total[0] : pfull;
+  const int64_t total = from_own[1] + own_total[1];
   // no piece shorter than an item's start and one tile
   const int ctas = static_cast<int>(max64(1, min64(p.ctas, total / (kItemCost + kTileCost))));
-  auto cut = [&](int c) { return total * c / ctas; };
+  const int64_t each = quot(total, ctas);
+  const uint32_t rest = static_cast<uint32_t>(total - each * ctas);
+  auto cut = [&](int c) { return each * c + rest * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas); };
   const int cta = blockIdx.x;
   const int64_t x0 = cta < ctas ? cut(cta) : total, x1 = cta < ctas ? cut(cta + 1) : total;
-  const int64_t own_from = max64(x0 - ptotal, 0);  // where this CTA's own part starts
-  const int64_t excl = before + incl - mine;
-  if (mine > 0 && own_from >= excl && own_from < excl + mine) {
-    int64_t at = excl;
-    int s = s_lo;
-    for (; s < s_hi; ++s) {
-      const int64_t c = seq_cost(p, s, per_tile) * p.hkv;
-      if (own_from < at + c) break;
-      at += c;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int64_t own_x = max64(x0 - from_own[k], 0);  // where this CTA's piece of them starts
+    if (mine[k] > 0 && own_x >= excl[k] && own_x < excl[k] + mine[k]) {
+      int64_t at = excl[k];
+      int s = s_lo;
+      for (; s < s_hi; ++s) {
+        int64_t c[2];
+        seq_cost<C>(p, s, per_tile, c);
+        if (own_x < at + c[k] * p.hkv) break;
+        at += c[k] * p.hkv;
+      }
+      B.start_seq[k] = s, B.start_base[k] = at;
     }
-    B.start_seq = s, B.start_base = at;
   }
   __syncthreads();
   const uint32_t tmem = B.tmem;
+  release_dependents();  // the merge may be scheduled; it waits for this grid to complete
 
   // Every role walks the segments in the scheduler's order.
+  auto few_rows = [&](const Seg& s) { return s.ntok * p.group <= kFewRows; };
   auto next_seg = [&](int sg, Seg& s) {
     if (!warp_wait(&B.seg_full[sg % kSegs], (sg / kSegs) & 1)) return false;
     s = B.seg[sg % kSegs];
@@ -391,12 +699,19 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     uint32_t scnt[2] = {0, 0};  // S tiles read per buffer
     uint32_t step0 = 0, tile0 = 0;  // steps and tiles of the CTA's earlier segments
     uint32_t done = 0;          // segments this warpgroup had steps of
+    uint32_t qu = 0;            // Q tiles of earlier segments
+    int few_from = -1;          // the first segment of few rows
+    Seg few_seg{};
     uint32_t joins = 0;         // segments whose two slots were joined
     bool ok = true;
     for (int sg = 0; ok; ++sg) {
       Seg s;
       ok = next_seg(sg, s);
       if (!ok || s.part < 0) break;
+      if (few_rows(s)) {
+        few_from = sg, few_seg = s;
+        break;
+      }
       const int ntile = s.ke - s.kb;
       const bool wide = s.ntok > p.half_toks;
       const bool joined = NWG == 2 && !wide && ntile > 1;  // both slots hold every row's keys
@@ -502,7 +817,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         if (lane == 0) mbar_arrive(&B.p_full[b]);
       }
       if (!ok) break;
-      tile0 += ntile, step0 += wide ? 2 * ntile : ntile;
+      tile0 += ntile, step0 += wide ? 2 * ntile : ntile, qu += wide ? 2 : 1;
       if (NWG == 2 && !wide && ntile == 1 && mine0 == 1) continue;  // the other slot's segment
 
       // ---- the segment's partial: O / l and lse
@@ -544,21 +859,23 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         const int c_lo = joined ? wg * (HD / 2) : 0, c_hi = joined ? c_lo + HD / 2 : HD;
         const uint32_t oa = tmem + C::TMEM_O + ((NWG == 2 && !joined) ? wg * HD : 0) + lane_addr;
 #pragma unroll 1
-        for (int c = c_lo; c < c_hi; c += 16) {
-          float o[16];
-          tmem_ld16(oa + c, o);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = some ? o[k] * ws[0] : l;  // l: 0, or the NaN of the row
+        for (int c = c_lo; c < c_hi; c += 32) {
+          float o[32];
+          tmem_ld32(oa + c, o);
           if (joined) {
-            float o2[16];
-            tmem_ld16(oa + HD + c, o2);
+            float o2[32];
+            tmem_ld32(oa + HD + c, o2);
+            tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] += some ? o2[k] * ws[1] : 0.f;
+            for (int k = 0; k < 32; ++k) o[k] = some ? o[k] * ws[0] + o2[k] * ws[1] : l;
+          } else {
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = some ? o[k] * ws[0] : l;  // l: 0, or the NaN of the row
           }
           if (live) {
 #pragma unroll
-            for (int k = 0; k < 16; k += 4)
-              *reinterpret_cast<float4*>(od + c + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            for (int k = 0; k < 32; k += 8) store8(od + c + k, o + k);
           }
         }
       }
@@ -568,6 +885,21 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         // an accumulator is free when all warps that read it are through (joined: both groups')
         if (joined) mbar_arrive(&B.o_free[0]), mbar_arrive(&B.o_free[1]);
         else mbar_arrive_n(&B.o_free[NWG == 2 ? wg : 0], NSW / 4);
+      }
+    }
+    // ---- the segments of few rows, which come last
+    if (ok && few_from >= 0) {
+      // every warpgroup is through with the earlier segments, and their tiles with the ring
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.meet);
+      ok = warp_wait(&B.meet, 0);
+      uint32_t meets = 1;
+      Seg s = few_seg;
+      for (int sg = few_from; ok && s.part >= 0;) {
+        FewRows<C> f{p, s, B, smem, stats, warp, lane, cta, tile0, qu, meets};
+        ok = f.run();
+        meets = f.meets, tile0 += s.ke - s.kb, ++qu;
+        ok = ok && next_seg(++sg, s);
       }
     }
     if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
@@ -642,91 +974,130 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         uint32_t tile;  // of the CTA
         bool valid, first, last, free_kv;
       } st0, st1;
-      bool ok = true, more = true, wide = false;
+      // The next step, worked out while the softmax of an earlier one runs: what stands between a
+      // finished P and the next S is then the two batches of MMAs alone.
+      struct Next {
+        bool known;   // in the current segment
+        bool landed;  // its K tile is there
+        uint32_t qslot, tile, a, k[KU], slot[KU];
+        int half;
+      } nx;
+      bool ok = true, more = true, ended = false, wide = false;
       int sg = 0, i = 0, steps = 0;   // next segment; next step of the current one
       uint32_t tile0 = 0, tiles = 0;  // first tile of the current segment; tiles of those before the next
       uint32_t qu = 0;                // Q tiles used before the current segment
       uint32_t pcnt[2] = {0, 0}, ocnt[2] = {0, 0};
-      auto qk = [&](Step& st, const int b) {  // the next step, into S buffer b
-        st.valid = false;
-        if (!more) return;
-        if (i == steps) {
-          if (steps) qu += wide ? 2 : 1;
-          Seg s;
-          ok = next_seg(sg, s);
-          if (!ok) return;
-          ++sg;
-          if (s.part < 0) {
-            more = false;
-            return;
-          }
-          wide = s.ntok > p.half_toks;  // the steps of a tile are its row halves
-          tile0 = tiles, tiles += s.ke - s.kb;
-          steps = (s.ke - s.kb) * (wide ? 2 : 1), i = 0;
-        }
-        const int half = wide ? i & 1 : 0;
-        const uint32_t tile = tile0 + (wide ? i >> 1 : i);
-        const uint32_t quse = qu + half, qslot = quse % QB;
-        if (i == half) ok = warp_wait(&B.q_full[qslot], (quse / QB) & 1);
-        const uint32_t u = k_pos(tile) * KU;
-        const bool free_kv = !wide || half == 1;
+      auto k_barrier = [&](int w) { return &B.full[nx.slot[w]]; };
+      auto look_ahead = [&]() {
+        nx.known = more && i < steps;
+        if (!nx.known) return;
+        nx.half = wide ? i & 1 : 0;
+        nx.tile = tile0 + (wide ? i >> 1 : i);
+        nx.qslot = (qu + nx.half) % QB;
+        nx.a = uniform(desc_lo(q_base + nx.qslot * C::Q_TILE, 16));
+        const uint32_t u = k_pos(nx.tile) * KU;
+        nx.landed = true;
 #pragma unroll
         for (int w = 0; w < KU; ++w) {
-          const uint32_t slot = (u + w) % NU;
-          if (half == 0) ok = ok && warp_wait(&B.full[slot], ((u + w) / NU) & 1);
+          nx.slot[w] = (u + w) % NU;
+          nx.k[w] = uniform(desc_lo(base + nx.slot[w] * C::UNIT, 16));
+          if (nx.half == 0)
+            nx.landed = nx.landed && __all_sync(0xffffffffu, mbar_try_wait(k_barrier(w), ((u + w) / NU) & 1));
+        }
+      };
+      auto next_segment = [&]() {
+        if (steps) qu += wide ? 2 : 1;
+        Seg s;
+        ok = next_seg(sg, s);
+        if (!ok) return;
+        ++sg;
+        if (s.part < 0 || few_rows(s)) {  // all that follow are the softmax warps' own
+          more = false, ended = s.part < 0;
+          return;
+        }
+        wide = s.ntok > p.half_toks;  // the steps of a tile are its row halves
+        tile0 = tiles, tiles += s.ke - s.kb;
+        steps = (s.ke - s.kb) * (wide ? 2 : 1), i = 0;
+      };
+      auto qk = [&](Step& st, const int b) {  // the next step, into S buffer b
+        st.valid = false;
+        if (!nx.known) {
+          if (!more) return;
+          next_segment();
+          if (!ok || !more) return;
+          look_ahead();
+        }
+        if (i == nx.half) {  // the first use of this Q tile
+          ok = warp_wait(&B.q_full[nx.qslot], ((qu + nx.half) / QB) & 1);
+          if (!ok) return;
+        }
+        const bool free_kv = !wide || nx.half == 1;
+        const uint32_t u = k_pos(nx.tile) * KU;
+#pragma unroll
+        for (int w = 0; w < KU; ++w) {
+          if (!nx.landed) ok = ok && warp_wait(k_barrier(w), ((u + w) / NU) & 1);
           if (!ok) return;
           tc_fence_after();
-          const uint32_t a = uniform(desc_lo(q_base + qslot * C::Q_TILE + w * C::NCG * C::Q_CG, 16));
-          const uint32_t k = uniform(desc_lo(base + slot * C::UNIT, 16));
           if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < C::UC / 16; ++kk)
-              mma_ss(tm + C::TMEM_S + b * TK, a + ((kk >> 2) * C::Q_CG + (kk & 3) * 32) / 16, hi_q,
-                     k + ((kk >> 2) * 1024 + (kk & 3) * 32) / 16, hi_kv, idesc_s, w > 0 || kk > 0);
+              mma_ss(tm + C::TMEM_S + b * TK, nx.a + ((w * C::NCG + (kk >> 2)) * C::Q_CG + (kk & 3) * 32) / 16, hi_q,
+                     nx.k[w] + ((kk >> 2) * 1024 + (kk & 3) * 32) / 16, hi_kv, idesc_s, w > 0 || kk > 0);
             if (w == KU - 1) tc_commit(&B.s_full[b]);
-            if (free_kv) tc_commit(&B.empty[slot]);
-            if (w == KU - 1 && i + (wide ? 2 : 1) >= steps) tc_commit(&B.q_empty[qslot]);
+            if (free_kv) commit_for<NSW>(&B.empty[nx.slot[w]]);
+            if (w == KU - 1 && i + (wide ? 2 : 1) >= steps) commit_for<NSW>(&B.q_empty[nx.qslot]);
           }
           __syncwarp();
         }
-        st = Step{tile, true, NWG == 2 ? i < 2 : i == 0, i + NWG >= steps, free_kv};
+        st = Step{nx.tile, true, NWG == 2 ? i < 2 : i == 0, i + NWG >= steps, free_kv};
         ++i;
       };
       auto pv = [&](Step& st, const int b) {
         const int acc = NWG == 2 ? b : 0;
-        ok = warp_wait(&B.p_full[b], pcnt[b]++ & 1);
+        const uint32_t u = v_pos(st.tile) * KU;
+        uint32_t slot[KU], v[KU];
+#pragma unroll
+        for (int w = 0; w < KU; ++w) {
+          slot[w] = (u + w) % NU;
+          v[w] = uniform(desc_lo(base + slot[w] * C::UNIT, 1024));
+          ok = ok && warp_wait(&B.full[slot[w]], ((u + w) / NU) & 1);
+        }
         if (ok && st.first) {  // the accumulator's last segment has been read
           if (ocnt[acc] > 0) ok = warp_wait(&B.o_free[acc], (ocnt[acc] - 1) & 1);
           ++ocnt[acc];
         }
-        const uint32_t u = v_pos(st.tile) * KU, fresh = st.first ? 1 : 0;
+        const uint32_t add = uniform(st.first ? 0 : 1);
+        look_ahead();
+        ok = ok && warp_wait(&B.p_full[b], pcnt[b]++ & 1);
+        if (!ok) return;
+        tc_fence_after();
 #pragma unroll
         for (int w = 0; w < KU; ++w) {
-          const uint32_t slot = (u + w) % NU;
-          ok = ok && warp_wait(&B.full[slot], ((u + w) / NU) & 1);
-          if (!ok) return;
-          tc_fence_after();
-          const uint32_t v = uniform(desc_lo(base + slot * C::UNIT, 1024)), add = uniform(fresh ^ 1);
           if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < TK / 16; ++ks)
               mma_ts(tm + C::TMEM_O + acc * HD + w * C::UC, tm + C::TMEM_S + b * TK + ks * 8,
-                     v + ks * 2 * C::NCG * 1024 / 16, hi_kv, idesc_o, ks > 0 ? 1 : add);
+                     v[w] + ks * 2 * C::NCG * 1024 / 16, hi_kv, idesc_o, ks > 0 ? 1 : add);
             if (NWG == 1 && w == KU - 1) tc_commit(&B.pv_done);
-            if (st.free_kv) tc_commit(&B.empty[slot]);
+            if (st.free_kv) commit_for<NSW>(&B.empty[slot[w]]);
             if (w == KU - 1 && st.last) tc_commit(&B.seg_done[acc]);
           }
           __syncwarp();
         }
         qk(st, b);
       };
+      nx.known = false;
       qk(st0, 0);
-      if (ok) qk(st1, 1);
+      if (ok) {
+        look_ahead();
+        qk(st1, 1);
+      }
       while (ok && st0.valid) {
         pv(st0, 0);
         if (!ok || !st1.valid) break;
         pv(st1, 1);
       }
+      for (Seg s; ok && !ended; ended = s.part < 0) ok = next_seg(sg++, s);
       if (!ok) {  // let what was issued finish before TMEM goes
         if (elect_one()) {
           set_error(p.err, FOLD_DEVERR_TIMEOUT);
@@ -792,21 +1163,23 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       };
       // one item: s without its tile range; at: its place on the line
       auto item = [&](Seg s, int64_t at) {
-        const int tiles = (s.limit + TK - 1) / TK, w = tile_cost(p, s.ntok);
+        const int tiles = (s.limit + TK - 1) / TK, w = tile_cost(p, s.ntok), start = start_cost(p, s.ntok);
+        const int64_t end = at + item_cost(p, tiles, s.ntok);
         // key tiles of this item that lie before place x of the line
         auto tiles_before = [&](int64_t x) {
-          const int64_t y = x - at - kItemCost + w / 2;
-          return y <= 0 ? 0 : static_cast<int>(min64(y / w, tiles));
+          if (x >= end) return tiles;
+          const int64_t y = x - at - start + w / 2;
+          return y <= 0 ? 0 : static_cast<int>(min64(quot(y, w), tiles));
         };
-        s.kb = tiles_before(x0), s.ke = cta + 1 == ctas ? tiles : tiles_before(x1);
+        s.kb = at >= x0 ? 0 : tiles_before(x0), s.ke = tiles_before(x1);
         if (s.kb < s.ke) publish(s);
         if (at >= x0) {  // the item starts here: note the CTAs that hold its tiles
-          int c0 = cta, cnt = 0;
-          if (tiles > 0) {
-            auto upto = [&](int c) { return c + 1 >= ctas ? tiles : tiles_before(cut(c + 1)); };
-            while (upto(c0) == 0) ++c0;
-            int c1 = static_cast<int>(min64(ctas - 1, (at + kItemCost + static_cast<int64_t>(tiles) * w) * ctas / total));
-            c1 = max(c1, c0);
+          int c0 = cta, cnt = tiles > 0;
+          if (s.ke < tiles) {
+            int upto = s.ke;
+            while (upto == 0) ++c0, upto = tiles_before(cut(c0 + 1));
+            // a CTA at or past the item's end, then back
+            int c1 = max(static_cast<int>(min64(ctas - 1, quot(end, each) + 1)), c0);
             while (c1 > c0 && tiles_before(cut(c1)) >= tiles) --c1;
             cnt = c1 - c0 + 1;
           }
@@ -814,48 +1187,56 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             p.plan[(static_cast<int64_t>(s.part) * p.n + s.tok0 + x) * p.hkv + s.head] = make_int4(c0, cnt, s.tok0, 0);
         }
       };
-      if (x0 < x1) {
+      // items of row tiles [rt, rt_end) of the prefix, c each, the first at place `from`
+      auto walk_prefix = [&](int rt, int rt_end, int64_t c, int64_t from) {
+        const int64_t row_cost = c * p.hkv;
+        if (rt >= rt_end || x1 <= from || x0 >= from + (rt_end - rt) * row_cost) return;
         Seg s{};
-        if (x0 < ptotal) {
-          const int64_t row_cost = pc_full * p.hkv;
-          int rt = static_cast<int>(min64(x0 / row_cost, prow_tiles - 1));
-          const int64_t in_row = x0 - rt * row_cost;
-          int h = static_cast<int>(min64(in_row / (rt + 1 < prow_tiles ? pc_full : pc_last), p.hkv - 1));
-          for (; ok && rt < prow_tiles; ++rt, h = 0) {
-            const int ntok = rt + 1 < prow_tiles ? per_tile : last_tok;
-            const int64_t c = rt + 1 < prow_tiles ? pc_full : pc_last;
-            for (; ok && h < p.hkv; ++h) {
-              const int64_t at = rt * row_cost + h * c;
-              if (at >= x1) break;
-              s.part = 0, s.seq = 0, s.head = h, s.tok0 = tok_lo + rt * per_tile, s.ntok = ntok;
-              s.limit = plen, s.lim0 = plen, s.lim_step = 0;
-              item(s, at);
-            }
-            if (h < p.hkv) break;
+        s.limit = s.lim0 = plen;
+        const int64_t in = max64(x0 - from, 0);
+        const int skip = static_cast<int>(quot(in, row_cost));
+        int64_t at = from + skip * row_cost;
+        int h = static_cast<int>(quot(in - skip * row_cost, c));
+        for (rt += skip; ok && rt < rt_end && at < x1; ++rt, h = 0, at += row_cost) {
+          s.tok0 = tok_lo + rt * per_tile, s.ntok = min(per_tile, tok_hi - s.tok0);
+          for (; ok && h < p.hkv && at + h * c < x1; ++h) {
+            s.head = h;
+            item(s, at + h * c);
           }
         }
-        if (x1 > ptotal) {
-          int64_t at = ptotal + B.start_base;
-          for (int q = B.start_seq; ok && q < p.b && at < x1; ++q) {
-            int first, last;
-            seq_rows(p, q, first, last);
-            const int m = capped(__ldg(p.own_lens + q), p.own_cap, p.err);
-            for (int t0 = first; ok && t0 < last && at < x1; t0 += per_tile) {
-              const int ntok = min(per_tile, last - t0);
-              s.part = 1, s.seq = q, s.tok0 = t0, s.ntok = ntok, s.lim_step = p.causal ? 1 : 0;
-              own_limits(p, first, last, m, t0, ntok, s.limit, s.lim0);
-              const int64_t c = item_cost(p, (s.limit + TK - 1) / TK, ntok);
-              int h = 0;
-              if (at + c * p.hkv <= x0) h = p.hkv;  // wholly before this CTA's piece
-              else if (x0 > at) h = static_cast<int>((x0 - at) / c);
-              for (; ok && h < p.hkv && at + h * c < x1; ++h) {
-                s.head = h;
-                item(s, at + h * c);
-              }
-              at += c * p.hkv;
+      };
+      // the sequences' own items of many (0) or few (1) rows
+      auto walk_own = [&](int k) {
+        if (own_total[k] == 0 || x1 <= from_own[k] || x0 >= from_own[k] + own_total[k]) return;
+        Seg s{};
+        s.part = 1, s.lim_step = p.causal ? 1 : 0;
+        int64_t at = from_own[k] + B.start_base[k];
+        for (int q = B.start_seq[k]; ok && q < p.b && at < x1; ++q) {
+          int first, last;
+          seq_rows(p, q, first, last);
+          const int m = capped(__ldg(p.own_lens + q), p.own_cap, p.err);
+          for (int t0 = first; ok && t0 < last && at < x1; t0 += per_tile) {
+            s.seq = q, s.tok0 = t0, s.ntok = min(per_tile, last - t0);
+            if (few_rows(s) != (k == 1)) continue;
+            own_limits(p, first, last, m, t0, s.ntok, s.limit, s.lim0);
+            const int64_t c = item_cost(p, (s.limit + TK - 1) / TK, s.ntok);
+            int h = 0;
+            if (at + c * p.hkv <= x0) h = p.hkv;  // wholly before this CTA's piece
+            else if (x0 > at) h = static_cast<int>(quot(x0 - at, c));
+            for (; ok && h < p.hkv && at + h * c < x1; ++h) {
+              s.head = h;
+              item(s, at + h * c);
             }
+            at += c * p.hkv;
           }
         }
+      };
+      if (x0 < x1) {
+        walk_prefix(0, prow_tiles - 1, pc_full, 0);
+        if (!last_few) walk_prefix(prow_tiles - 1, prow_tiles, pc_last, from_last);
+        walk_own(0);
+        if (last_few && prow_tiles) walk_prefix(prow_tiles - 1, prow_tiles, pc_last, from_last);
+        walk_own(1);
       }
       if (ok) {
         Seg s{};
@@ -874,54 +1255,107 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
   }
 }
 
-// Joins the partials of one row: its prefix item's and its own item's. One warp per (token, head).
-template <int HD, class T, int ROWS>
-__global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t row = blockIdx.x * 4ll + (threadIdx.x >> 5);
+// Joins the partials of one row: its prefix item's and its own item's, one per CTA that held a part
+// of the item. WPR warps a row take every WPR-th partial each; a lane reads the lse of one.
+// Latency bound (a few partials of a row, from L2): four warps a row where there are few rows (the
+// partials are then many), one where there are enough rows to fill the SMs.
+template <int HD, class T, int WPR>
+__global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixParams p, int cont_rows) {
+  constexpr int V = HD / 32, RPB = 4 / WPR;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * RPB + warp / WPR;
   const int tok = static_cast<int>(row / p.hq), h = static_cast<int>(row - static_cast<int64_t>(tok) * p.hq);
-  if (tok >= p.n || tok < p.qsl[0] || tok >= p.qsl[p.b]) return;
+  const int hk = h / p.group, g = h - hk * p.group;
   wait_for_producer();
-  constexpr int V = HD / 32;
+  if (tok >= p.n || tok < p.qsl[0] || tok >= p.qsl[p.b]) return;  // with WPR 4 the whole block
+  const bool prefix = p.prefix_len[0] > 0 && p.prefix_cap > 0;
+  const int4 none = make_int4(0, 0, 0, 0);
+  // a read that gave up (FOLD_DEVERR_TIMEOUT) may have left a plan unwritten
+  auto sane = [&](int4 v) {
+    const bool fine = v.x >= 0 && v.y >= 0 && v.y <= p.ctas && v.x <= p.ctas - v.y && v.z >= 0 && v.z <= tok &&
+                      tok - v.z < (cont_rows / 128) * p.half_toks;
+    return fine ? v : none;
+  };
+  const int4 pp = prefix ? sane(p.plan[static_cast<int64_t>(tok) * p.hkv + hk]) : none;
+  const int4 po = sane(p.plan[(static_cast<int64_t>(p.n) + tok) * p.hkv + hk]);
+  const int cnt = pp.y + po.y;
   float acc[V], m = -INFINITY, z = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  auto add = [&](float lse, const float* o) {
-    if (lse == -INFINITY) return;
-    const float mn = fmaxf(m, lse), f = __expf(m - mn), w = __expf(lse - mn);
-    m = mn, z = z * f + w;
-    float x[V];
-    if constexpr (V == 2) {
-      const float2 a = reinterpret_cast<const float2*>(o)[lane];
-      x[0] = a.x, x[1] = a.y;
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; i += 4) {
-        const float4 a = reinterpret_cast<const float4*>(o)[lane * (V / 4) + i / 4];
-        x[i] = a.x, x[i + 1] = a.y, x[i + 2] = a.z, x[i + 3] = a.w;
+  for (int base = 0; sub + WPR * base < cnt; base += 32) {
+    const int i = sub + WPR * (base + lane);
+    const float* o = nullptr;
+    float lse = -INFINITY;
+    if (i < cnt) {
+      const bool own = i >= pp.y;
+      const int4 plan = own ? po : pp;
+      const int k = own ? i - pp.y : i;
+      if (k == 0) {
+        const int64_t at = (static_cast<int64_t>(own ? p.n : 0) + tok) * p.hq + h;
+        lse = p.lse_prim[at], o = p.o_prim + at * HD;
+      } else {
+        const int x = tok - plan.z, half = x / p.half_toks;
+        const int64_t at = static_cast<int64_t>(plan.x + k) * cont_rows + half * 128 + (x - half * p.half_toks) * p.group + g;
+        lse = p.lse_cont[at], o = p.o_cont + at * HD;
       }
     }
+    float top = lse;
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = acc[i] * f + w * x[i];
-  };
-  const int hk = h / p.group, g = h - hk * p.group;
-#pragma unroll 1
-  for (int part = (p.prefix_len[0] > 0 && p.prefix_cap > 0) ? 0 : 1; part < 2; ++part) {
-    const int64_t tr = static_cast<int64_t>(part) * p.n + tok;
-    const int4 plan = p.plan[tr * p.hkv + hk];
-    if (plan.y < 1) continue;
-    add(p.lse_prim[tr * p.hq + h], p.o_prim + (tr * p.hq + h) * HD);
-    const int x = tok - plan.z, half = x / p.half_toks, r = half * 128 + (x - half * p.half_toks) * p.group + g;
-    for (int c = plan.x + 1; c < plan.x + plan.y; ++c) {
-      const int64_t at = static_cast<int64_t>(c) * ROWS + r;
-      add(p.lse_cont[at], p.o_cont + at * HD);
+    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    top = fmaxf(top, m);
+    const float mz = top == -INFINITY ? 0.f : top;
+    const float w = i < cnt ? __expf(lse - mz) : 0.f, f = __expf(m - mz);
+    m = top;
+    float zs = w;
+#pragma unroll
+    for (int s = 16; s; s >>= 1) zs += __shfl_xor_sync(0xffffffffu, zs, s);
+    z = z * f + zs;
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] *= f;
+    const int nk = min(32, (cnt - sub + WPR - 1) / WPR - base);
+#pragma unroll 4
+    for (int k = 0; k < nk; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      const float* ok = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), k));
+      if constexpr (V == 2) {
+        const float2 a = reinterpret_cast<const float2*>(ok)[lane];
+        acc[0] += wk * a.x, acc[1] += wk * a.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+          const float4 a = reinterpret_cast<const float4*>(ok)[lane * (V / 4) + j / 4];
+          acc[j] += wk * a.x, acc[j + 1] += wk * a.y, acc[j + 2] += wk * a.z, acc[j + 3] += wk * a.w;
+        }
+      }
     }
   }
-  const float inv = z > 0.f ? 1.f / z : 0.f;
+  if constexpr (WPR > 1) {
+    __shared__ float sm[WPR], sz[WPR], so[WPR][HD];
+    if (lane == 0) sm[sub] = m, sz[sub] = z;
+#pragma unroll
+    for (int j = 0; j < V; ++j) so[sub][lane * V + j] = acc[j];
+    __syncthreads();
+    if (sub) return;
+    float top = sm[0];
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) top = fmaxf(top, sm[w]);
+    const float mz = top == -INFINITY ? 0.f : top;
+    m = top, z = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) acc[j] = 0.f;
+#pragma unroll
+    for (int w = 0; w < WPR; ++w) {
+      const float f = __expf(sm[w] - mz);
+      z += sz[w] * f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) acc[j] += f * so[w][lane * V + j];
+    }
+  }
+  const float inv = z > 0.f ? 1.f / z : (z == 0.f ? 0.f : z);  // a NaN reaches the output
   T* out = static_cast<T*>(p.out) + tok * p.o_st + h * p.o_sh + lane * V;
   uint32_t w[V / 2];
 #pragma unroll
-  for (int i = 0; i < V; i += 2) w[i / 2] = pack2<T>(z == z ? acc[i] * inv : z, z == z ? acc[i + 1] * inv : z);
+  for (int i = 0; i < V; i += 2) w[i / 2] = pack2<T>(acc[i] * inv, acc[i + 1] * inv);
   if constexpr (V == 2) *reinterpret_cast<uint32_t*>(out) = w[0];
   else if constexpr (V == 4) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
   else *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
@@ -1016,8 +1450,11 @@ int launch_prefix(const PrefixParams& p, const void* k, const void* v, int64_t s
                             qmap, kmap, vmap, p))
     return s;
   const int64_t rows = static_cast<int64_t>(p.n) * p.hq;
-  return launch_behind(prefix_merge_kernel<HD, T, C::ROWS>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream,
-                       "prefix_merge_kernel", p);
+  if (rows <= 4096)
+    return launch_behind(prefix_merge_kernel<HD, T, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, stream,
+                         "prefix_merge_kernel", p, C::ROWS);
+  return launch_behind(prefix_merge_kernel<HD, T, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream,
+                       "prefix_merge_kernel", p, C::ROWS);
 }
 
 }  // namespace

@@ -177,6 +177,19 @@ def test_many_sequences():
          seed=5).check()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_short_parts_between_long_ones(hd):
+    """Row tiles of every width behind one another in one launch: sequences of one token, of a few
+    and of hundreds, with many short parts between the long ones."""
+    rng = np.random.default_rng(hd)
+    nq, own = [], []
+    for i in range(120):
+        nq.append(int(rng.choice([1, 1, 1, 1, 2, 5, 9, 33, 40, 70, 130])))
+        own.append(int(rng.choice([0, 1, 60, 130, 400])) if i % 3 else 128 + nq[-1])
+    Case(nq, own, 300, 8, 2, hd, 16, seed=hd).check()
+    Case(nq, own, 0, 4, 4, hd, 32, "fp16", seed=hd).check(causal=False)
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_large_logits(hd, dtype):
