@@ -96,17 +96,26 @@ def load():
 _fns = {}
 
 
-def call(name: str, *args) -> None:
-    """Calls an entry point and raises FoldError on a non-zero status."""
+def entry(name: str):
+    """The entry point itself; its status is the caller's to check (raise_status)."""
     fn = _fns.get(name)
     if fn is None:
         fn = _fns[name] = getattr(load(), name)
-    status = fn(*args)
+    return fn
+
+
+def raise_status(name: str, status: int) -> None:
+    lib = load()
+    msg = lib.fold_last_error().decode(errors="replace")
+    kind = lib.fold_status_string(status).decode()
+    raise FoldError(f"{name}: {kind}: {msg}")
+
+
+def call(name: str, *args) -> None:
+    """Calls an entry point and raises FoldError on a non-zero status."""
+    status = entry(name)(*args)
     if status:
-        lib = load()
-        msg = lib.fold_last_error().decode(errors="replace")
-        kind = lib.fold_status_string(status).decode()
-        raise FoldError(f"{name}: {kind}: {msg}")
+        raise_status(name, status)
 
 
 def num_sms() -> int:

@@ -58,9 +58,12 @@ int check_cuda(cudaError_t e, const char* what) {
 int check_launch(const char* what) { return check_cuda(cudaGetLastError(), what); }
 
 int device_sm_count() {
+  static std::atomic<int> known[64];  // a device's count does not change
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

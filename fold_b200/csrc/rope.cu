@@ -10,7 +10,12 @@
 // Bound: HBM bytes, each row read once and written once; a token's table row is shared by all its
 // heads. So one thread owns one unit, two 16-byte chunks that hold whole pairs (chunk c of each
 // half; two neighbouring chunks when interleaved or passed through), of HU heads of one token: the
-// table values are loaded once for the HU heads, and 2 * HU 16-byte loads are in flight.
+// table values are loaded once for the HU heads, and 2 * HU 16-byte loads are in flight while the
+// position and then the table row are fetched. What counts besides is how many threads wait at once:
+// 64 registers and blocks of 128. At 8192 tokens of 32 + 8 heads of 128 (168 MB) HU 4 with blocks of
+// 256 took 40.5 us, HU 2 37.3, HU 2 with blocks of 128 35.5 us (4.7 TB/s; a device copy of as much
+// by torch takes 59 us); 16K tokens appended with their queries (403 MB) 93.5, 76.2 and 72.4 us
+// (5.6 TB/s). Streaming loads and stores, and the table before the rows, were slower.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -19,6 +24,8 @@
 
 namespace fold {
 namespace {
+
+constexpr int kRopeThreads = 128;
 
 struct RopeRows {  // rows [n, heads, hd] with the innermost dim contiguous
   const void* in;
@@ -101,7 +108,7 @@ __device__ __forceinline__ bool locate(const RopeParams& p, int t, int hh, const
 
 // One thread per (token, group of HU heads, unit); neighbouring threads walk a row's units.
 template <class T, bool INTER, int HU>
-__global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads, 8) rope_kernel(const RopeParams p) {
   constexpr int E = 16 / sizeof(T);
   if (p.q.heads == 0) release_dependents();  // no query is written: a read behind may load its own early
   const int units = p.hd / (2 * E), runits = p.table ? p.rot / (2 * E) : 0;
@@ -186,7 +193,7 @@ __global__ void __launch_bounds__(256) rope_kernel(const RopeParams p) {
 // Rows that 16-byte units do not cover (odd head or rotated sizes, unaligned strides): one thread
 // per pair, and per passed-through element, of one head.
 template <class T, bool INTER>
-__global__ void __launch_bounds__(256) rope_scalar_kernel(const RopeParams p) {
+__global__ void __launch_bounds__(kRopeThreads) rope_scalar_kernel(const RopeParams p) {
   if (p.q.heads == 0) release_dependents();
   const int rot = p.table ? p.rot : 0, half = rot >> 1, units = half + p.hd - rot;
   const int heads = p.q.heads + p.k.heads + p.v.heads, rotated = p.q.heads + p.k.heads;
@@ -235,7 +242,7 @@ int launch_rope(const RopeParams& p, cudaStream_t stream) {
           p.cs_slot % E == 0;
   int sms = device_sm_count();
   if (sms <= 0) sms = 148;
-  const int threads = 256;
+  const int threads = kRopeThreads;
   auto grid = [&](int64_t total, int per_sm) {
     const int64_t want = (total + threads - 1) / threads, cap = static_cast<int64_t>(sms) * per_sm;
     return static_cast<unsigned>(want < cap ? want : cap);
@@ -247,12 +254,13 @@ int launch_rope(const RopeParams& p, cudaStream_t stream) {
   }
   const int64_t units = static_cast<int64_t>(p.n) * heads * (p.hd / (2 * E));
   if (units <= static_cast<int64_t>(sms) * 1024) {
-    // too few units to fill the SMs' threads with four heads each: one head a thread is the
-    // shortest chain of loads
+    // too few units to fill the SMs' threads with two heads each: one head a thread is the shortest
+    // chain (1 to 256 tokens of 40 heads: 2.1-2.9 us, two heads 2.7-3.4 us; equal at 512 tokens,
+    // 4.0 us; from there two heads, 10.6 against 12.1 us at 2048)
     rope_kernel<T, INTER, 1><<<grid(units, 64), threads, 0, stream>>>(p);
   } else {
-    const int64_t total = static_cast<int64_t>(p.n) * ((heads + 3) / 4) * (p.hd / (2 * E));
-    rope_kernel<T, INTER, 4><<<grid(total, 64), threads, 0, stream>>>(p);
+    const int64_t total = static_cast<int64_t>(p.n) * ((heads + 1) / 2) * (p.hd / (2 * E));
+    rope_kernel<T, INTER, 2><<<grid(total, 64), threads, 0, stream>>>(p);
   }
   return check_launch("rope_kernel");
 }

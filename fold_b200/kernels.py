@@ -309,56 +309,72 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def _check_devices(what, first, *rest):
-    """All given tensors on one CUDA device."""
-    _require_cuda(first, *rest)
+    """All given tensors on one CUDA device; returns its index."""
     dev = first.get_device()
     for t in rest:
         if t is not None and t.get_device() != dev:
+            _require_cuda(first, *rest)
             raise FoldError(f"{what}: the tensors are on different devices")
+    if dev < 0:
+        _require_cuda(first)
+    return dev
 
 
-def _call_on(t, name, *args):
-    """Calls an entry point on t's device and that device's current stream (the last argument)."""
-    dev = t.get_device()
-    if dev == torch.cuda.current_device():
-        _lib.call(name, *args, _stream(t))
+def _call_on(dev, name, *args):
+    """Calls an entry point on device `dev` and that device's current stream (the last argument)."""
+    fn = _lib.entry(name)
+    if dev == _get_device():
+        status = fn(*args, _raw_stream(dev) if _raw_stream else torch.cuda.current_stream(dev).cuda_stream)
     else:
         with torch.cuda.device(dev):
-            _lib.call(name, *args, _stream(t))
+            status = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if status:
+        _lib.raise_status(name, status)
+
+
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _check_err(what, err):
-    if err is not None and (err.dtype != torch.int32 or err.numel() < 1):
+    if err.dtype != torch.int32 or err.numel() < 1:
         raise FoldError(f"{what}: err must be an int32 tensor of at least one element")
 
 
 def _check_table(what, table, d):
-    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous() or table.shape[0] < 1:
+    """(rows, rot_dim) of a rope table for heads of d."""
+    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous():
         raise FoldError(f"{what}: the rope table must be contiguous float32 [rows, rot_dim]")
-    rot = table.shape[1]
-    if rot < 2 or rot % 2 or rot > d:
+    rows, rot = table.shape
+    if rows < 1 or rot < 2 or rot % 2 or rot > d:
         raise FoldError(f"{what}: the table's rot_dim must be even and at most the head dimension")
+    return rows, rot
 
 
 def _check_index(what, name, t, n):
     if t.dim() != 1 or t.shape[0] != n:
         raise FoldError(f"{what}: {name} needs one entry per token")
+    if t.dtype == torch.int64 and t.is_contiguous():
+        return t
     if t.dtype not in (torch.int64, torch.int32):
         raise FoldError(f"{what}: {name} must be int64 or int32")
-    return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
+    return t.to(torch.int64).contiguous()
 
 
 def _rotary_out(what, x, out):
-    """(x, out) with contiguous heads; a new output when none is given."""
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    """(x, its strides, out, its strides) with contiguous heads; a new output when none is given."""
+    xs = x.stride()
+    if xs[2] != 1 and x.shape[2] > 1:
         if out is x:
             raise FoldError(f"{what}: the head dimension must be contiguous")
         x = x.contiguous()
+        xs = x.stride()
     if out is None:
-        return x, torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    if out.shape != x.shape or out.dtype != x.dtype or (out.stride(-1) != 1 and out.shape[-1] > 1):
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        return x, xs, out, out.stride()
+    os = out.stride()
+    if out.shape != x.shape or out.dtype != x.dtype or (os[2] != 1 and out.shape[2] > 1):
         raise FoldError(f"{what}: an output has its input's shape and type and a contiguous head dimension")
-    return x, out
+    return x, xs, out, os
 
 
 def rotary(q, k, positions, table, *, interleaved=False, inverse=False, q_out=None, k_out=None, err=None):
@@ -368,33 +384,40 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, q_out=No
     scaled frequencies. `inverse` applies the transposed rotation, which takes the outputs'
     gradients to the inputs'. Outputs are new tensors unless given; one may be its own input.
     A position outside the table is clamped and reported in err (int32 [1])."""
-    _check_devices("rotary", q, k, positions, table, q_out, k_out, err)
+    dev = _check_devices("rotary", q, k, positions, table, q_out, k_out, err)
     if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
         raise FoldError("rotary: q and k must be [n, heads, head_dim] with equal n and head_dim")
-    if q.dtype not in _DTYPES or (k is not None and k.dtype != q.dtype):
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None or (k is not None and k.dtype != q.dtype):
         raise FoldError("rotary: q and k must both be bfloat16, float16 or float32")
     n, hq, d = q.shape
-    _check_table("rotary", table, d)
-    _check_err("rotary", err)
+    rows, rot = _check_table("rotary", table, d)
     positions = _check_index("rotary", "positions", positions, n)
-    q, q_out = _rotary_out("rotary", q, q_out)
+    q, qs, q_out, qos = _rotary_out("rotary", q, q_out)
+    kp = kop = ep = None
     hk, ks, kos = 0, (0, 0), (0, 0)
     if k is not None:
-        k, k_out = _rotary_out("rotary", k, k_out)
-        hk, ks, kos = k.shape[1], k.stride(), k_out.stride()
-    _call_on(q, "fold_rotary", _p(q), q.stride(0), q.stride(1), _p(q_out), q_out.stride(0), q_out.stride(1), hq, _p(k),
-             ks[0], ks[1], _p(k_out), kos[0], kos[1], hk, _p(positions), _p(table), table.shape[0], table.shape[1], n,
-             d, _DTYPES[q.dtype], int(bool(interleaved)), int(bool(inverse)), _p(err))
+        k, ks, k_out, kos = _rotary_out("rotary", k, k_out)
+        hk, kp, kop = k.shape[1], k.data_ptr(), k_out.data_ptr()
+    if err is not None:
+        _check_err("rotary", err)
+        ep = err.data_ptr()
+    _call_on(dev, "fold_rotary", q.data_ptr(), qs[0], qs[1], q_out.data_ptr(), qos[0], qos[1], hq, kp, ks[0], ks[1],
+             kop, kos[0], kos[1], hk, positions.data_ptr(), table.data_ptr(), rows, rot, n, d, dtype,
+             1 if interleaved else 0, 1 if inverse else 0, ep)
     return q_out, k_out
 
 
 def _check_planes(what, k_cache, v_cache):
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or k_cache.stride() != v_cache.stride() \
-            or (k_cache.stride(-1) != 1 and k_cache.shape[-1] > 1):
+    """Strides of the K and V planes of a paged cache."""
+    st = k_cache.stride()
+    if len(st) != 4 or v_cache.shape != k_cache.shape or st != v_cache.stride() \
+            or (st[3] != 1 and k_cache.shape[3] > 1):
         raise FoldError(f"{what}: K and V planes must be [num_blocks, Hkv, block_size, head_dim] views with equal "
                         "strides and a contiguous head dimension")
     if v_cache.dtype != k_cache.dtype:
         raise FoldError(f"{what}: K and V planes must have one type")
+    return st
 
 
 def append_paged(k, v, positions, slots, k_cache, v_cache, table, *, interleaved=False, q=None, q_out=None, err=None):
@@ -405,45 +428,69 @@ def append_paged(k, v, positions, slots, k_cache, v_cache, table, *, interleaved
     same launch and returned (q_out, a new tensor unless given; it may be q). table None stores the
     keys as they are. The non-negative slots of a call must be distinct; a slot past the cache is
     skipped and reported in err."""
-    _check_devices("append_paged", k, v, positions, slots, k_cache, v_cache, table, q, q_out, err)
-    _check_planes("append_paged", k_cache, v_cache)
+    dev = _check_devices("append_paged", k, v, positions, slots, k_cache, v_cache, table, q, q_out, err)
+    cs = _check_planes("append_paged", k_cache, v_cache)
     nb, hkv, bs, d = k_cache.shape
-    if k.dim() != 3 or k.shape[1:] != (hkv, d) or v.shape != k.shape:
+    ks, vs = k.stride(), v.stride()
+    if len(ks) != 3 or k.shape[1] != hkv or k.shape[2] != d or v.shape != k.shape:
         raise FoldError("append_paged: K and V must be [n, Hkv, head_dim] matching the cache planes")
-    if k.dtype not in _DTYPES or v.dtype != k.dtype or k_cache.dtype != k.dtype:
+    dtype = _DTYPES.get(k.dtype)
+    if dtype is None or v.dtype != k.dtype or k_cache.dtype != k.dtype:
         raise FoldError("append_paged: K, V and the cache must all be bfloat16, float16 or float32")
     n = k.shape[0]
-    _check_err("append_paged", err)
-    if (k.stride(-1) != 1 or v.stride(-1) != 1) and d > 1:
+    if (ks[2] != 1 or vs[2] != 1) and d > 1:
         raise FoldError("append_paged: the head dimension of K and V must be contiguous")
     slots = _check_index("append_paged", "slots", slots, n)
+    rows = rot = hq = 0
+    pp = tp = qp = qop = ep = None
+    qs = qos = (0, 0)
     if table is not None:
-        _check_table("append_paged", table, d)
+        rows, rot = _check_table("append_paged", table, d)
         positions = _check_index("append_paged", "positions", positions, n)
-    hq, qs, qos = 0, (0, 0), (0, 0)
+        pp, tp = positions.data_ptr(), table.data_ptr()
     if q is not None:
         if table is None:
             raise FoldError("append_paged: queries are given only to be rotated (table is None)")
         if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d or q.dtype != k.dtype:
             raise FoldError("append_paged: q must be [n, Hq, head_dim] of the keys' type")
-        q, q_out = _rotary_out("append_paged", q, q_out)
-        hq, qs, qos = q.shape[1], q.stride(), q_out.stride()
-    rows, rot = (0, 0) if table is None else table.shape
-    _call_on(k, "fold_append_paged", _p(k), k.stride(0), k.stride(1), _p(v), v.stride(0), v.stride(1),
-             _p(positions) if table is not None else None, _p(slots), n, _p(k_cache), _p(v_cache), nb, bs,
-             k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), _p(table), rows, rot, hkv, d, _DTYPES[k.dtype],
-             int(bool(interleaved)), _p(q), qs[0], qs[1], _p(q_out) if q is not None else None, qos[0], qos[1], hq,
-             _p(err))
-    return q_out if q is not None else None
+        q, qs, q_out, qos = _rotary_out("append_paged", q, q_out)
+        hq, qp, qop = q.shape[1], q.data_ptr(), q_out.data_ptr()
+    else:
+        q_out = None
+    if err is not None:
+        _check_err("append_paged", err)
+        ep = err.data_ptr()
+    _call_on(dev, "fold_append_paged", k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], pp, slots.data_ptr(), n,
+             k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, cs[0], cs[1], cs[2], tp, rows, rot, hkv, d, dtype,
+             1 if interleaved else 0, qp, qs[0], qs[1], qop, qos[0], qos[1], hq, ep)
+    return q_out
+
+
+def _prefix_workspace_bytes(n, hq, hkv, d, dev):
+    if dev == _get_device():
+        size = _lib.prefix_read_workspace(n, hq, hkv, d)
+    else:
+        with torch.cuda.device(dev):
+            size = _lib.prefix_read_workspace(n, hq, hkv, d)
+    if size < 0:
+        raise FoldError(f"prefix_read: no kernel for n {n}, Hq {hq}, Hkv {hkv}, head_dim {d}")
+    return size
 
 
 def prefix_workspace(n, hq, hkv, d, device):
     """A workspace for prefix_read calls of up to these sizes (one per call that may overlap another)."""
-    with torch.cuda.device(device):
-        size = _lib.prefix_read_workspace(int(n), int(hq), int(hkv), int(d))
-    if size < 0:
-        raise FoldError(f"prefix_read: no kernel for n {n}, Hq {hq}, Hkv {hkv}, head_dim {d}")
-    return torch.empty(max(size, 16), device=device, dtype=torch.uint8)
+    dev = torch.device(device)
+    if dev.type != "cuda":
+        raise FoldError("FOLD kernels take CUDA tensors (there is no CPU path)")
+    size = _prefix_workspace_bytes(int(n), int(hq), int(hkv), int(d), _get_device() if dev.index is None else dev.index)
+    return torch.empty(size, device=dev, dtype=torch.uint8)
+
+
+def _check_ints(what, name, t, dim):
+    st = t.stride()
+    if t.dtype != torch.int32 or len(st) != dim or (st[-1] != 1 and t.shape[-1] > 1):
+        raise FoldError(f"{what}: {name} must be int32 with {dim} dimension(s), the last one contiguous")
+    return st
 
 
 def prefix_read(q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, block_tables, out, *, softmax_scale,
@@ -457,36 +504,45 @@ def prefix_read(q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, bl
     [num_blocks, Hkv, block_size, D] planes (paged_planes); lengths and tables are int32 on the
     device. Writes out [n, Hq, D] and, when given, lse [Hq, n] float32; a row without a key gets
     out 0 and lse -inf. `workspace` (prefix_workspace) is allocated per call when not given."""
-    _check_devices("prefix_read", q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, block_tables, out, lse,
-                   workspace, err)
-    if q.dim() != 3 or out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
+    dev = _check_devices("prefix_read", q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, block_tables, out,
+                         lse, workspace, err)
+    qs, os = q.stride(), out.stride()
+    if len(qs) != 3 or out.shape != q.shape or out.dtype != q.dtype or os[2] != 1:
         raise FoldError("prefix_read: q and out must be [n, Hq, head_dim] of one type, out's head dimension contiguous")
     n, hq, d = q.shape
-    _check_planes("prefix_read", k_cache, v_cache)
+    cs = _check_planes("prefix_read", k_cache, v_cache)
     nb, hkv, bs, dk = k_cache.shape
-    if q.dtype not in (torch.bfloat16, torch.float16) or k_cache.dtype != q.dtype or dk != d:
+    dtype = _DTYPES.get(q.dtype)
+    if dtype is None or dtype == 2 or k_cache.dtype != q.dtype or dk != d:
         raise FoldError("prefix_read: q and the cache must both be bfloat16 or float16 with one head dimension")
-    for name, t, dim in (("query_start_loc", qsl, 1), ("own_lens", own_lens, 1), ("prefix_len", prefix_len, 1),
-                         ("prefix_table", prefix_table, 1), ("block_tables", block_tables, 2)):
-        if t.dtype != torch.int32 or t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1):
-            raise FoldError(f"prefix_read: {name} must be int32 with {dim} dimension(s), the last one contiguous")
+    _check_ints("prefix_read", "query_start_loc", qsl, 1)
+    _check_ints("prefix_read", "own_lens", own_lens, 1)
+    _check_ints("prefix_read", "prefix_len", prefix_len, 1)
+    _check_ints("prefix_read", "prefix_table", prefix_table, 1)
+    bt = _check_ints("prefix_read", "block_tables", block_tables, 2)
     b = own_lens.shape[0]
     if qsl.shape[0] != b + 1 or block_tables.shape[0] != b or prefix_len.shape[0] != 1:
         raise FoldError("prefix_read: query_start_loc needs b + 1 entries, block_tables b rows and prefix_len one entry")
-    if lse is not None and (lse.shape != (hq, n) or lse.dtype != torch.float32 or not lse.is_contiguous()):
-        raise FoldError("prefix_read: lse must be contiguous float32 [Hq, n]")
-    _check_err("prefix_read", err)
-    if q.stride(-1) != 1 or min(q.stride()) < 1:  # heads or rows that share memory are copied apart
+    lp = ep = None
+    if lse is not None:
+        if lse.shape != (hq, n) or lse.dtype != torch.float32 or not lse.is_contiguous():
+            raise FoldError("prefix_read: lse must be contiguous float32 [Hq, n]")
+        lp = lse.data_ptr()
+    if err is not None:
+        _check_err("prefix_read", err)
+        ep = err.data_ptr()
+    if qs[2] != 1 or qs[0] < 1 or qs[1] < 1:  # heads or rows that share memory are copied apart
         q = q.contiguous()
+        qs = q.stride()
     if workspace is None:
-        workspace = prefix_workspace(n, hq, hkv, d, q.device)
+        workspace = q.new_empty(_prefix_workspace_bytes(n, hq, hkv, d, dev), dtype=torch.uint8)
     elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
         raise FoldError("prefix_read: workspace must be a contiguous uint8 tensor (prefix_workspace)")
-    _call_on(q, "fold_prefix_read", _p(q), q.stride(0), q.stride(1), _p(qsl), _p(own_lens), _p(prefix_len), b,
-             _p(k_cache), _p(v_cache), nb, bs, k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), _p(prefix_table),
-             prefix_table.shape[0], _p(block_tables), block_tables.stride(0), block_tables.shape[1], int(bool(causal)),
-             float(softmax_scale), _p(out), out.stride(0), out.stride(1), _p(lse), _p(workspace), workspace.numel(), n,
-             hq, hkv, d, _DTYPES[q.dtype], _p(err))
+    _call_on(dev, "fold_prefix_read", q.data_ptr(), qs[0], qs[1], qsl.data_ptr(), own_lens.data_ptr(),
+             prefix_len.data_ptr(), b, k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, cs[0], cs[1], cs[2],
+             prefix_table.data_ptr(), prefix_table.shape[0], block_tables.data_ptr(), bt[0], block_tables.shape[1],
+             1 if causal else 0, softmax_scale, out.data_ptr(), os[0], os[1], lp, workspace.data_ptr(),
+             workspace.numel(), n, hq, hkv, d, dtype, ep)
 
 
 def append(k, v, positions, slots, side, *, pos_lo=0, skip_foreign=False, err=None):
