@@ -970,40 +970,57 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       constexpr uint32_t idesc_o = idesc_of(C::F16, C::UC, 1);
       constexpr uint32_t hi_q = desc_hi(1024), hi_kv = desc_hi(C::NCG * 1024);
       const uint32_t base = uniform(smem_u32(smem)), q_base = base + C::OFF_Q, tm = uniform(tmem);
+      // Where a tile's units lie in the ring, walked (K0 K1 V0 K2 V1 ...) rather than divided out.
+      struct Place {
+        uint32_t slot, parity;
+        __device__ __forceinline__ void move(uint32_t n) {
+          slot += n;
+          if (slot >= NU) slot -= NU, parity ^= 1;
+        }
+        __device__ __forceinline__ Place unit(int w) const {
+          Place x = *this;
+          if (w) x.move(w);
+          return x;
+        }
+      };
       struct Step {
-        uint32_t tile;  // of the CTA
-        bool valid, first, last, free_kv;
+        Place v;
+        uint32_t v_lo[KU];
+        bool valid, first, last, new_tile, free_kv;
       } st0, st1;
       // The next step, worked out while the softmax of an earlier one runs: what stands between a
       // finished P and the next S is then the two batches of MMAs alone.
       struct Next {
         bool known;   // in the current segment
         bool landed;  // its K tile is there
-        uint32_t qslot, tile, a, k[KU], slot[KU];
+        Place k, v;
+        uint32_t a, k_lo[KU], v_lo[KU];
         int half;
       } nx;
       bool ok = true, more = true, ended = false, wide = false;
-      int sg = 0, i = 0, steps = 0;   // next segment; next step of the current one
-      uint32_t tile0 = 0, tiles = 0;  // first tile of the current segment; tiles of those before the next
-      uint32_t qu = 0;                // Q tiles used before the current segment
+      int sg = 0, i = 0, steps = 0;  // next segment; next step of the current one
+      uint32_t qu = 0;               // Q tiles used before the current segment
       uint32_t pcnt[2] = {0, 0}, ocnt[2] = {0, 0};
-      auto k_barrier = [&](int w) { return &B.full[nx.slot[w]]; };
+      Place k_at{0, 0}, v_at{2 * KU, 0};  // of the next tile
+      uint32_t k_step = KU;
       auto look_ahead = [&]() {
         nx.known = more && i < steps;
         if (!nx.known) return;
         nx.half = wide ? i & 1 : 0;
-        nx.tile = tile0 + (wide ? i >> 1 : i);
-        nx.qslot = (qu + nx.half) % QB;
-        nx.a = uniform(desc_lo(q_base + nx.qslot * C::Q_TILE, 16));
-        const uint32_t u = k_pos(nx.tile) * KU;
-        nx.landed = true;
+        if (nx.half == 0) {
+          nx.k = k_at, nx.v = v_at;
+          k_at.move(k_step), v_at.move(2 * KU);
+          k_step = 2 * KU;
+          nx.landed = true;
 #pragma unroll
-        for (int w = 0; w < KU; ++w) {
-          nx.slot[w] = (u + w) % NU;
-          nx.k[w] = uniform(desc_lo(base + nx.slot[w] * C::UNIT, 16));
-          if (nx.half == 0)
-            nx.landed = nx.landed && __all_sync(0xffffffffu, mbar_try_wait(k_barrier(w), ((u + w) / NU) & 1));
+          for (int w = 0; w < KU; ++w) {
+            const Place k = nx.k.unit(w), v = nx.v.unit(w);
+            nx.landed = nx.landed && mbar_try_wait(&B.full[k.slot], k.parity);
+            nx.k_lo[w] = uniform(desc_lo(base + k.slot * C::UNIT, 16));
+            nx.v_lo[w] = uniform(desc_lo(base + v.slot * C::UNIT, 1024));
+          }
         }
+        if (i <= nx.half || NWG == 2) nx.a = uniform(desc_lo(q_base + (qu + nx.half) % QB * C::Q_TILE, 16));
       };
       auto next_segment = [&]() {
         if (steps) qu += wide ? 2 : 1;
@@ -1016,9 +1033,9 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           return;
         }
         wide = s.ntok > p.half_toks;  // the steps of a tile are its row halves
-        tile0 = tiles, tiles += s.ke - s.kb;
         steps = (s.ke - s.kb) * (wide ? 2 : 1), i = 0;
       };
+      // The waits of one step end in one vote of the warp.
       auto qk = [&](Step& st, const int b) {  // the next step, into S buffer b
         st.valid = false;
         if (!nx.known) {
@@ -1027,63 +1044,68 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (!ok || !more) return;
           look_ahead();
         }
-        if (i == nx.half) {  // the first use of this Q tile
-          ok = warp_wait(&B.q_full[nx.qslot], ((qu + nx.half) / QB) & 1);
-          if (!ok) return;
-        }
-        const bool free_kv = !wide || nx.half == 1;
-        const uint32_t u = k_pos(nx.tile) * KU;
+        const bool q_first = i == nx.half;  // the first use of this Q tile
+        if (q_first || !nx.landed) {
+          if (q_first) ok = mbar_wait(&B.q_full[(qu + nx.half) % QB], ((qu + nx.half) / QB) & 1);
+          if (!nx.landed) {
 #pragma unroll
-        for (int w = 0; w < KU; ++w) {
-          if (!nx.landed) ok = ok && warp_wait(k_barrier(w), ((u + w) / NU) & 1);
-          if (!ok) return;
-          tc_fence_after();
-          if (elect_one()) {
+            for (int w = 0; w < KU; ++w) ok = ok && mbar_wait(&B.full[nx.k.unit(w).slot], nx.k.unit(w).parity);
+            nx.landed = true;
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        const bool free_kv = !wide || nx.half == 1;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int w = 0; w < KU; ++w) {
 #pragma unroll
             for (int kk = 0; kk < C::UC / 16; ++kk)
               mma_ss(tm + C::TMEM_S + b * TK, nx.a + ((w * C::NCG + (kk >> 2)) * C::Q_CG + (kk & 3) * 32) / 16, hi_q,
-                     nx.k[w] + ((kk >> 2) * 1024 + (kk & 3) * 32) / 16, hi_kv, idesc_s, w > 0 || kk > 0);
+                     nx.k_lo[w] + ((kk >> 2) * 1024 + (kk & 3) * 32) / 16, hi_kv, idesc_s, w > 0 || kk > 0);
             if (w == KU - 1) tc_commit(&B.s_full[b]);
-            if (free_kv) commit_for<NSW>(&B.empty[nx.slot[w]]);
-            if (w == KU - 1 && i + (wide ? 2 : 1) >= steps) commit_for<NSW>(&B.q_empty[nx.qslot]);
+            if (free_kv) commit_for<NSW>(&B.empty[nx.k.unit(w).slot]);
           }
-          __syncwarp();
+          if (i + (wide ? 2 : 1) >= steps) commit_for<NSW>(&B.q_empty[(qu + nx.half) % QB]);
         }
-        st = Step{nx.tile, true, NWG == 2 ? i < 2 : i == 0, i + NWG >= steps, free_kv};
+        __syncwarp();
+        st.v = nx.v;
+#pragma unroll
+        for (int w = 0; w < KU; ++w) st.v_lo[w] = nx.v_lo[w];
+        st.valid = true, st.first = NWG == 2 ? i < 2 : i == 0, st.last = i + NWG >= steps;
+        st.new_tile = nx.half == 0, st.free_kv = free_kv;
         ++i;
       };
       auto pv = [&](Step& st, const int b) {
         const int acc = NWG == 2 ? b : 0;
-        const uint32_t u = v_pos(st.tile) * KU;
-        uint32_t slot[KU], v[KU];
+        look_ahead();
+        if (st.new_tile) {
 #pragma unroll
-        for (int w = 0; w < KU; ++w) {
-          slot[w] = (u + w) % NU;
-          v[w] = uniform(desc_lo(base + slot[w] * C::UNIT, 1024));
-          ok = ok && warp_wait(&B.full[slot[w]], ((u + w) / NU) & 1);
+          for (int w = 0; w < KU; ++w) ok = ok && mbar_wait(&B.full[st.v.unit(w).slot], st.v.unit(w).parity);
         }
-        if (ok && st.first) {  // the accumulator's last segment has been read
-          if (ocnt[acc] > 0) ok = warp_wait(&B.o_free[acc], (ocnt[acc] - 1) & 1);
+        if (st.first) {  // the accumulator's last segment has been read
+          if (ocnt[acc] > 0) ok = ok && mbar_wait(&B.o_free[acc], (ocnt[acc] - 1) & 1);
           ++ocnt[acc];
         }
         const uint32_t add = uniform(st.first ? 0 : 1);
-        look_ahead();
-        ok = ok && warp_wait(&B.p_full[b], pcnt[b]++ & 1);
+        ok = ok && mbar_wait(&B.p_full[b], pcnt[b]++ & 1);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
         tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-        for (int w = 0; w < KU; ++w) {
-          if (elect_one()) {
+          for (int w = 0; w < KU; ++w) {
 #pragma unroll
             for (int ks = 0; ks < TK / 16; ++ks)
               mma_ts(tm + C::TMEM_O + acc * HD + w * C::UC, tm + C::TMEM_S + b * TK + ks * 8,
-                     v[w] + ks * 2 * C::NCG * 1024 / 16, hi_kv, idesc_o, ks > 0 ? 1 : add);
-            if (NWG == 1 && w == KU - 1) tc_commit(&B.pv_done);
-            if (st.free_kv) commit_for<NSW>(&B.empty[slot[w]]);
-            if (w == KU - 1 && st.last) tc_commit(&B.seg_done[acc]);
+                     st.v_lo[w] + ks * 2 * C::NCG * 1024 / 16, hi_kv, idesc_o, ks > 0 ? 1 : add);
+            if (st.free_kv) commit_for<NSW>(&B.empty[st.v.unit(w).slot]);
           }
-          __syncwarp();
+          if (NWG == 1) tc_commit(&B.pv_done);
+          if (st.last) tc_commit(&B.seg_done[acc]);
         }
+        __syncwarp();
         qk(st, b);
       };
       nx.known = false;
