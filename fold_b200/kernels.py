@@ -306,6 +306,7 @@ def merge_partials(o_wpart, lse_wpart, o_fpart, lse_fpart, out, qsl, seq_lens, *
 
 # Element types of the operators that take more than bf16 (fold_dtype in include/fold_b200.h).
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_INT32 = torch.int32
 
 
 def _check_devices(what, first, *rest):
@@ -410,12 +411,11 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, q_out=No
 
 def _check_planes(what, k_cache, v_cache):
     """Strides of the K and V planes of a paged cache."""
-    st = k_cache.stride()
-    if len(st) != 4 or v_cache.shape != k_cache.shape or st != v_cache.stride() \
-            or (st[3] != 1 and k_cache.shape[3] > 1):
+    st, shape = k_cache.stride(), k_cache.shape
+    if len(st) != 4 or v_cache.shape != shape or st != v_cache.stride() or (st[3] != 1 and shape[3] > 1):
         raise FoldError(f"{what}: K and V planes must be [num_blocks, Hkv, block_size, head_dim] views with equal "
                         "strides and a contiguous head dimension")
-    if v_cache.dtype != k_cache.dtype:
+    if v_cache.dtype is not k_cache.dtype:
         raise FoldError(f"{what}: K and V planes must have one type")
     return st
 
@@ -486,13 +486,6 @@ def prefix_workspace(n, hq, hkv, d, device):
     return torch.empty(size, device=dev, dtype=torch.uint8)
 
 
-def _check_ints(what, name, t, dim):
-    st = t.stride()
-    if t.dtype != torch.int32 or len(st) != dim or (st[-1] != 1 and t.shape[-1] > 1):
-        raise FoldError(f"{what}: {name} must be int32 with {dim} dimension(s), the last one contiguous")
-    return st
-
-
 def prefix_read(q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, block_tables, out, *, softmax_scale,
                 causal=True, lse=None, workspace=None, err=None):
     """Attention of a batch of sequences that share a prefix, the prefix read once for all of them.
@@ -506,26 +499,28 @@ def prefix_read(q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, bl
     out 0 and lse -inf. `workspace` (prefix_workspace) is allocated per call when not given."""
     dev = _check_devices("prefix_read", q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, block_tables, out,
                          lse, workspace, err)
-    qs, os = q.stride(), out.stride()
-    if len(qs) != 3 or out.shape != q.shape or out.dtype != q.dtype or os[2] != 1:
+    qs, os, shape = q.stride(), out.stride(), q.shape
+    dtype = q.dtype
+    if len(qs) != 3 or out.shape != shape or out.dtype is not dtype or os[2] != 1:
         raise FoldError("prefix_read: q and out must be [n, Hq, head_dim] of one type, out's head dimension contiguous")
-    n, hq, d = q.shape
+    n, hq, d = shape
     cs = _check_planes("prefix_read", k_cache, v_cache)
     nb, hkv, bs, dk = k_cache.shape
-    dtype = _DTYPES.get(q.dtype)
-    if dtype is None or dtype == 2 or k_cache.dtype != q.dtype or dk != d:
+    code = _DTYPES.get(dtype)
+    if code is None or code == 2 or k_cache.dtype is not dtype or dk != d:
         raise FoldError("prefix_read: q and the cache must both be bfloat16 or float16 with one head dimension")
-    _check_ints("prefix_read", "query_start_loc", qsl, 1)
-    _check_ints("prefix_read", "own_lens", own_lens, 1)
-    _check_ints("prefix_read", "prefix_len", prefix_len, 1)
-    _check_ints("prefix_read", "prefix_table", prefix_table, 1)
-    bt = _check_ints("prefix_read", "block_tables", block_tables, 2)
-    b = own_lens.shape[0]
-    if qsl.shape[0] != b + 1 or block_tables.shape[0] != b or prefix_len.shape[0] != 1:
-        raise FoldError("prefix_read: query_start_loc needs b + 1 entries, block_tables b rows and prefix_len one entry")
+    if not (qsl.dtype is own_lens.dtype is prefix_len.dtype is prefix_table.dtype is block_tables.dtype is _INT32):
+        raise FoldError("prefix_read: the lengths and tables must be int32")
+    if not (qsl.is_contiguous() and own_lens.is_contiguous() and prefix_table.is_contiguous()):
+        raise FoldError("prefix_read: query_start_loc, own_lens and prefix_table must be contiguous")
+    b, bt = own_lens.numel(), block_tables.stride()
+    if qsl.numel() != b + 1 or prefix_len.numel() != 1:
+        raise FoldError("prefix_read: query_start_loc needs b + 1 entries and prefix_len one")
+    if len(bt) != 2 or block_tables.shape[0] != b or (bt[1] != 1 and block_tables.shape[1] > 1):
+        raise FoldError("prefix_read: block_tables must be [b, blocks] with contiguous rows")
     lp = ep = None
     if lse is not None:
-        if lse.shape != (hq, n) or lse.dtype != torch.float32 or not lse.is_contiguous():
+        if lse.shape != (hq, n) or lse.dtype is not torch.float32 or not lse.is_contiguous():
             raise FoldError("prefix_read: lse must be contiguous float32 [Hq, n]")
         lp = lse.data_ptr()
     if err is not None:
@@ -535,14 +530,17 @@ def prefix_read(q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, bl
         q = q.contiguous()
         qs = q.stride()
     if workspace is None:
-        workspace = q.new_empty(_prefix_workspace_bytes(n, hq, hkv, d, dev), dtype=torch.uint8)
-    elif workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise FoldError("prefix_read: workspace must be a contiguous uint8 tensor (prefix_workspace)")
+        size = _prefix_workspace_bytes(n, hq, hkv, d, dev)
+        workspace = q.new_empty(size, dtype=torch.uint8)
+    else:
+        size = workspace.numel()
+        if workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+            raise FoldError("prefix_read: workspace must be a contiguous uint8 tensor (prefix_workspace)")
     _call_on(dev, "fold_prefix_read", q.data_ptr(), qs[0], qs[1], qsl.data_ptr(), own_lens.data_ptr(),
              prefix_len.data_ptr(), b, k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, cs[0], cs[1], cs[2],
-             prefix_table.data_ptr(), prefix_table.shape[0], block_tables.data_ptr(), bt[0], block_tables.shape[1],
-             1 if causal else 0, softmax_scale, out.data_ptr(), os[0], os[1], lp, workspace.data_ptr(),
-             workspace.numel(), n, hq, hkv, d, dtype, ep)
+             prefix_table.data_ptr(), prefix_table.numel(), block_tables.data_ptr(), bt[0], block_tables.shape[1],
+             1 if causal else 0, softmax_scale, out.data_ptr(), os[0], os[1], lp, workspace.data_ptr(), size, n, hq,
+             hkv, d, code, ep)
 
 
 def append(k, v, positions, slots, side, *, pos_lo=0, skip_foreign=False, err=None):
