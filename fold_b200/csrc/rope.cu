@@ -8,10 +8,11 @@
 // (2i, 2i+1); dims past rot pass through. Arithmetic is float32 with one rounding to the type.
 //
 // Bound: HBM bytes, each row read once and written once; a token's table row is shared by all its
-// heads. So one thread owns one unit, two 16-byte chunks that hold whole pairs (chunk c of each
+// heads. So one thread owns one unit, two chunks of W bytes that hold whole pairs (chunk c of each
 // half; two neighbouring chunks when interleaved or passed through), of HU heads of one token: the
-// table values are loaded once for the HU heads, and 2 * HU 16-byte loads are in flight while the
-// position and then the table row are fetched. What counts besides is how many threads wait at once:
+// table values are loaded once for the HU heads, and 2 * HU loads are in flight while the position
+// and then the table row are fetched. W is 16, or 8 or 4 where the halves or the rows start on such
+// boundaries only. What counts besides is how many threads wait at once:
 // 64 registers and blocks of 128. At 8192 tokens of 32 + 8 heads of 128 (168 MB) HU 4 with blocks of
 // 256 took 40.5 us, HU 2 37.3, HU 2 with blocks of 128 35.5 us (4.7 TB/s; a device copy of as much
 // by torch takes 59 us); 16K tokens appended with their queries (403 MB) 93.5, 76.2 and 72.4 us
@@ -64,11 +65,36 @@ __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x);
 template <>
 __device__ __forceinline__ float from_f32(float x) { return x; }
 
-template <class T>
+template <int W>
+struct Word;
+template <>
+struct Word<16> { using type = uint4; };
+template <>
+struct Word<8> { using type = uint2; };
+template <>
+struct Word<4> { using type = uint32_t; };
+// A chunk of W bytes.
+template <class T, int W>
 union Chunk {
-  uint4 raw;
-  T e[16 / sizeof(T)];
+  typename Word<W>::type raw;
+  T e[W / sizeof(T)];
 };
+// N consecutive floats of the table (N * 4 bytes aligned, or 16).
+template <int N>
+__device__ __forceinline__ void load_floats(const float* p, float* v) {
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 u = __ldg(reinterpret_cast<const float4*>(p + i));
+      v[i] = u.x, v[i + 1] = u.y, v[i + 2] = u.z, v[i + 3] = u.w;
+    }
+  } else if constexpr (N == 2) {
+    const float2 u = __ldg(reinterpret_cast<const float2*>(p));
+    v[0] = u.x, v[1] = u.y;
+  } else {
+    v[0] = __ldg(p);
+  }
+}
 
 // The table row of token t (a position outside the table is clamped and reported).
 __device__ __forceinline__ const float* table_row(const RopeParams& p, int t) {
@@ -107,9 +133,10 @@ __device__ __forceinline__ bool locate(const RopeParams& p, int t, int hh, const
 }
 
 // One thread per (token, group of HU heads, unit); neighbouring threads walk a row's units.
-template <class T, bool INTER, int HU>
+template <class T, bool INTER, int W, int HU>
 __global__ void __launch_bounds__(kRopeThreads, 8) rope_kernel(const RopeParams p) {
-  constexpr int E = 16 / sizeof(T);
+  constexpr int E = W / sizeof(T);
+  using word = typename Word<W>::type;
   if (p.q.heads == 0) release_dependents();  // no query is written: a read behind may load its own early
   const int units = p.hd / (2 * E), runits = p.table ? p.rot / (2 * E) : 0;
   const int heads = p.q.heads + p.k.heads + p.v.heads, groups = (heads + HU - 1) / HU;
@@ -134,7 +161,7 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_kernel(const RopeParams 
     else if (turn) a = 2 * c * E, b = a + E;
     else a = runits * 2 * E + 2 * (c - runits) * E, b = a + E;
 
-    Chunk<T> x[HU], y[HU];
+    Chunk<T, W> x[HU], y[HU];
     T* dst[HU];
     bool live[HU];
 #pragma unroll
@@ -143,32 +170,28 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_kernel(const RopeParams 
       const int hh = g * HU + j;
       live[j] = hh < heads && locate<T>(p, t, hh, src, dst[j]);
       if (live[j]) {
-        x[j].raw = *reinterpret_cast<const uint4*>(src + a);
-        y[j].raw = *reinterpret_cast<const uint4*>(src + b);
+        x[j].raw = *reinterpret_cast<const word*>(src + a);
+        y[j].raw = *reinterpret_cast<const word*>(src + b);
       }
     }
     float cs[E], sn[E];
     if (turn && g * HU < rotated) {
       const float* row = table_row(p, t);
-      const float4* tc = reinterpret_cast<const float4*>(row + c * E);
-      const float4* ts = reinterpret_cast<const float4*>(row + (p.rot >> 1) + c * E);
+      load_floats<E>(row + c * E, cs);
+      load_floats<E>(row + (p.rot >> 1) + c * E, sn);
 #pragma unroll
-      for (int i = 0; i < E / 4; ++i) {
-        const float4 u = __ldg(tc + i), w = __ldg(ts + i);
-        cs[4 * i] = u.x, cs[4 * i + 1] = u.y, cs[4 * i + 2] = u.z, cs[4 * i + 3] = u.w;
-        sn[4 * i] = p.sgn * w.x, sn[4 * i + 1] = p.sgn * w.y, sn[4 * i + 2] = p.sgn * w.z, sn[4 * i + 3] = p.sgn * w.w;
-      }
+      for (int i = 0; i < E; ++i) sn[i] *= p.sgn;
     }
 #pragma unroll
     for (int j = 0; j < HU; ++j) {
       if (!live[j]) continue;
       if (turn && g * HU + j < rotated) {
-        Chunk<T> ox, oy;
-        if constexpr (INTER) {  // pair i of the unit: elements 2i, 2i + 1 of the two chunks in a row
+        Chunk<T, W> ox, oy;
+        if constexpr (INTER && E > 1) {  // pair i of the unit: elements 2i, 2i + 1 of the two chunks in a row
 #pragma unroll
           for (int i = 0; i < E; ++i) {
-            const Chunk<T>& s = i < E / 2 ? x[j] : y[j];
-            Chunk<T>& o = i < E / 2 ? ox : oy;
+            const Chunk<T, W>& s = i < E / 2 ? x[j] : y[j];
+            Chunk<T, W>& o = i < E / 2 ? ox : oy;
             const int e = 2 * (i < E / 2 ? i : i - E / 2);
             const float lo = to_f32(s.e[e]), hi = to_f32(s.e[e + 1]);
             o.e[e] = from_f32<T>(lo * cs[i] - hi * sn[i]);
@@ -184,85 +207,97 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_kernel(const RopeParams 
         }
         x[j] = ox, y[j] = oy;
       }
-      *reinterpret_cast<uint4*>(dst[j] + a) = x[j].raw;
-      *reinterpret_cast<uint4*>(dst[j] + b) = y[j].raw;
+      *reinterpret_cast<word*>(dst[j] + a) = x[j].raw;
+      *reinterpret_cast<word*>(dst[j] + b) = y[j].raw;
     }
   }
 }
 
-// Rows that 16-byte units do not cover (odd head or rotated sizes, unaligned strides): one thread
-// per pair, and per passed-through element, of one head.
+// Rows that no such unit covers (an odd number of pairs in halves of 2-byte elements, rows off every
+// boundary): a warp per row, a lane per pair and per passed-through element.
 template <class T, bool INTER>
 __global__ void __launch_bounds__(kRopeThreads) rope_scalar_kernel(const RopeParams p) {
   if (p.q.heads == 0) release_dependents();
-  const int rot = p.table ? p.rot : 0, half = rot >> 1, units = half + p.hd - rot;
-  const int heads = p.q.heads + p.k.heads + p.v.heads, rotated = p.q.heads + p.k.heads;
-  const int64_t total = static_cast<int64_t>(p.n) * heads * units;
-  for (int64_t idx = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; idx < total;
-       idx += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    const int64_t row = idx / units;
-    const int c = static_cast<int>(idx - row * units);
-    const int t = static_cast<int>(row / heads), hh = static_cast<int>(row - static_cast<int64_t>(t) * heads);
+  const int rot = p.table ? p.rot : 0, half = rot >> 1;
+  const uint32_t heads = p.q.heads + p.k.heads + p.v.heads;
+  const int rotated = p.q.heads + p.k.heads, lane = threadIdx.x & 31;
+  const int64_t rows = static_cast<int64_t>(p.n) * heads, warps = static_cast<int64_t>(gridDim.x) * (kRopeThreads / 32);
+  for (int64_t row = blockIdx.x * static_cast<int64_t>(kRopeThreads / 32) + (threadIdx.x >> 5); row < rows; row += warps) {
+    const int t = (row >> 32) == 0 ? static_cast<int>(static_cast<uint32_t>(row) / heads) : static_cast<int>(row / heads);
+    const int hh = static_cast<int>(row - static_cast<int64_t>(t) * heads);
     const T* src;
     T* dst;
     if (!locate<T>(p, t, hh, src, dst)) continue;
-    if (c >= half) {  // passed through
-      dst[rot + c - half] = src[rot + c - half];
+    if (hh >= rotated || half == 0) {
+      for (int i = lane; i < p.hd; i += 32) dst[i] = src[i];
       continue;
     }
-    const int a = INTER ? 2 * c : c, b = INTER ? 2 * c + 1 : c + half;
-    T x = src[a], y = src[b];
-    if (hh < rotated) {
-      const float* tr = table_row(p, t);
-      const float lo = to_f32(x), hi = to_f32(y), cs = __ldg(tr + c), sn = p.sgn * __ldg(tr + half + c);
-      x = from_f32<T>(lo * cs - hi * sn), y = from_f32<T>(hi * cs + lo * sn);
+    const float* tr = table_row(p, t);
+    for (int c = lane; c < half; c += 32) {
+      const int a = INTER ? 2 * c : c, b = INTER ? 2 * c + 1 : c + half;
+      const float lo = to_f32(src[a]), hi = to_f32(src[b]), cs = __ldg(tr + c), sn = p.sgn * __ldg(tr + half + c);
+      dst[a] = from_f32<T>(lo * cs - hi * sn), dst[b] = from_f32<T>(hi * cs + lo * sn);
     }
-    dst[a] = x, dst[b] = y;
+    for (int i = rot + lane; i < p.hd; i += 32) dst[i] = src[i];
   }
 }
 
-// Whether every row of r starts on a 16-byte boundary (es: element size).
-bool rows_aligned(const RopeRows& r, int es, bool with_out) {
+// Whether every row of r starts on a boundary of `bytes` (es: element size).
+bool rows_aligned(const RopeRows& r, int es, int bytes, bool with_out) {
   if (r.heads == 0) return true;
-  const int e = 16 / es;
-  return aligned16(r.in) && r.in_st % e == 0 && r.in_sh % e == 0 &&
-         (!with_out || (aligned16(r.out) && r.out_st % e == 0 && r.out_sh % e == 0));
+  const int64_t e = bytes / es;
+  auto on = [&](const void* x) { return (reinterpret_cast<uintptr_t>(x) & (bytes - 1)) == 0; };
+  return on(r.in) && r.in_st % e == 0 && r.in_sh % e == 0 &&
+         (!with_out || (on(r.out) && r.out_st % e == 0 && r.out_sh % e == 0));
+}
+
+// Whether units of two chunks of W bytes cover the rows.
+template <class T, int W>
+bool units_fit(const RopeParams& p) {
+  constexpr int E = W / sizeof(T);
+  const bool to_cache = p.slots != nullptr;
+  bool fit = p.hd % (2 * E) == 0 && (!p.table || (p.rot % (2 * E) == 0 && aligned16(p.table))) &&
+             rows_aligned(p.q, sizeof(T), W, true) && rows_aligned(p.k, sizeof(T), W, !to_cache) &&
+             rows_aligned(p.v, sizeof(T), W, false);
+  if (to_cache)
+    fit = fit && (reinterpret_cast<uintptr_t>(p.k.out) & (W - 1)) == 0 &&
+          (reinterpret_cast<uintptr_t>(p.v.out) & (W - 1)) == 0 && p.cs_block % E == 0 && p.cs_head % E == 0 &&
+          p.cs_slot % E == 0;
+  return fit;
+}
+
+unsigned rope_grid(int64_t threads) {
+  int sms = device_sm_count();
+  if (sms <= 0) sms = 148;
+  const int64_t want = (threads + kRopeThreads - 1) / kRopeThreads, cap = static_cast<int64_t>(sms) * 64;
+  return static_cast<unsigned>(want < cap ? want : cap);
+}
+
+template <class T, bool INTER, int W>
+int launch_units(const RopeParams& p, cudaStream_t stream) {
+  constexpr int E = W / sizeof(T);
+  const int heads = p.q.heads + p.k.heads + p.v.heads, units = p.hd / (2 * E);
+  const int64_t all = static_cast<int64_t>(p.n) * heads * units;
+  // up to about 1000 units an SM one head a thread is the shortest chain (1 to 256 tokens of 40 heads:
+  // 2.1-2.9 us, two heads 2.7-3.4 us; equal at 512 tokens, 4.0 us); from there two heads, 10.6 against
+  // 12.1 us at 2048
+  if (all <= 148 * 1024)
+    rope_kernel<T, INTER, W, 1><<<rope_grid(all), kRopeThreads, 0, stream>>>(p);
+  else
+    rope_kernel<T, INTER, W, 2><<<rope_grid(static_cast<int64_t>(p.n) * ((heads + 1) / 2) * units), kRopeThreads, 0, stream>>>(p);
+  return check_launch("rope_kernel");
 }
 
 template <class T, bool INTER>
 int launch_rope(const RopeParams& p, cudaStream_t stream) {
-  constexpr int E = 16 / sizeof(T);
-  const int heads = p.q.heads + p.k.heads + p.v.heads;
-  const bool to_cache = p.slots != nullptr;
-  bool vec = p.hd % (2 * E) == 0 && (!p.table || (p.rot % (2 * E) == 0 && aligned16(p.table))) &&
-             rows_aligned(p.q, sizeof(T), true) && rows_aligned(p.k, sizeof(T), !to_cache) &&
-             rows_aligned(p.v, sizeof(T), false);
-  if (to_cache)
-    vec = vec && aligned16(p.k.out) && aligned16(p.v.out) && p.cs_block % E == 0 && p.cs_head % E == 0 &&
-          p.cs_slot % E == 0;
-  int sms = device_sm_count();
-  if (sms <= 0) sms = 148;
-  const int threads = kRopeThreads;
-  auto grid = [&](int64_t total, int per_sm) {
-    const int64_t want = (total + threads - 1) / threads, cap = static_cast<int64_t>(sms) * per_sm;
-    return static_cast<unsigned>(want < cap ? want : cap);
-  };
-  if (!vec) {
-    const int units = p.table ? p.hd - p.rot / 2 : p.hd;
-    rope_scalar_kernel<T, INTER><<<grid(static_cast<int64_t>(p.n) * heads * units, 64), threads, 0, stream>>>(p);
-    return check_launch("rope_scalar_kernel");
+  if (units_fit<T, 16>(p)) return launch_units<T, INTER, 16>(p, stream);
+  if (units_fit<T, 8>(p)) return launch_units<T, INTER, 8>(p, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (units_fit<T, 4>(p)) return launch_units<T, INTER, 4>(p, stream);
   }
-  const int64_t units = static_cast<int64_t>(p.n) * heads * (p.hd / (2 * E));
-  if (units <= static_cast<int64_t>(sms) * 1024) {
-    // too few units to fill the SMs' threads with two heads each: one head a thread is the shortest
-    // chain (1 to 256 tokens of 40 heads: 2.1-2.9 us, two heads 2.7-3.4 us; equal at 512 tokens,
-    // 4.0 us; from there two heads, 10.6 against 12.1 us at 2048)
-    rope_kernel<T, INTER, 1><<<grid(units, 64), threads, 0, stream>>>(p);
-  } else {
-    const int64_t total = static_cast<int64_t>(p.n) * ((heads + 1) / 2) * (p.hd / (2 * E));
-    rope_kernel<T, INTER, 2><<<grid(total, 64), threads, 0, stream>>>(p);
-  }
-  return check_launch("rope_kernel");
+  const int64_t rows = static_cast<int64_t>(p.n) * (p.q.heads + p.k.heads + p.v.heads);
+  rope_scalar_kernel<T, INTER><<<rope_grid(rows * 32), kRopeThreads, 0, stream>>>(p);
+  return check_launch("rope_scalar_kernel");
 }
 
 int dispatch_rope(const RopeParams& p, int dtype, int interleaved, cudaStream_t stream) {

@@ -343,19 +343,20 @@ def _check_err(what, err):
 
 def _check_table(what, table, d):
     """(rows, rot_dim) of a rope table for heads of d."""
-    if table.dtype != torch.float32 or table.dim() != 2 or not table.is_contiguous():
+    shape = table.shape
+    if table.dtype is not torch.float32 or len(shape) != 2 or not table.is_contiguous():
         raise FoldError(f"{what}: the rope table must be contiguous float32 [rows, rot_dim]")
-    rows, rot = table.shape
+    rows, rot = shape
     if rows < 1 or rot < 2 or rot % 2 or rot > d:
         raise FoldError(f"{what}: the table's rot_dim must be even and at most the head dimension")
     return rows, rot
 
 
 def _check_index(what, name, t, n):
-    if t.dim() != 1 or t.shape[0] != n:
-        raise FoldError(f"{what}: {name} needs one entry per token")
-    if t.dtype == torch.int64 and t.is_contiguous():
+    if t.dtype is torch.int64 and t.is_contiguous() and t.shape == (n,):
         return t
+    if t.shape != (n,):
+        raise FoldError(f"{what}: {name} needs one entry per token")
     if t.dtype not in (torch.int64, torch.int32):
         raise FoldError(f"{what}: {name} must be int64 or int32")
     return t.to(torch.int64).contiguous()
@@ -364,6 +365,9 @@ def _check_index(what, name, t, n):
 def _rotary_out(what, x, out):
     """(x, its strides, out, its strides) with contiguous heads; a new output when none is given."""
     xs = x.stride()
+    if out is None and xs[2] == 1:
+        out = torch.empty_like(x)
+        return x, xs, out, out.stride()
     if xs[2] != 1 and x.shape[2] > 1:
         if out is x:
             raise FoldError(f"{what}: the head dimension must be contiguous")
@@ -375,6 +379,8 @@ def _rotary_out(what, x, out):
     os = out.stride()
     if out.shape != x.shape or out.dtype != x.dtype or (os[2] != 1 and out.shape[2] > 1):
         raise FoldError(f"{what}: an output has its input's shape and type and a contiguous head dimension")
+    if (os[0] == 0 and out.shape[0] > 1) or (os[1] == 0 and out.shape[1] > 1):
+        raise FoldError(f"{what}: the rows of an output must not share memory")
     return x, xs, out, os
 
 
@@ -386,12 +392,16 @@ def rotary(q, k, positions, table, *, interleaved=False, inverse=False, q_out=No
     gradients to the inputs'. Outputs are new tensors unless given; one may be its own input.
     A position outside the table is clamped and reported in err (int32 [1])."""
     dev = _check_devices("rotary", q, k, positions, table, q_out, k_out, err)
-    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
-        raise FoldError("rotary: q and k must be [n, heads, head_dim] with equal n and head_dim")
-    dtype = _DTYPES.get(q.dtype)
-    if dtype is None or (k is not None and k.dtype != q.dtype):
+    shape, dtype = q.shape, _DTYPES.get(q.dtype)
+    if len(shape) != 3:
+        raise FoldError("rotary: q must be [n, heads, head_dim]")
+    n, hq, d = shape
+    if k is not None:
+        hk = k.shape
+        if len(hk) != 3 or hk[0] != n or hk[2] != d:
+            raise FoldError("rotary: q and k must be [n, heads, head_dim] with equal n and head_dim")
+    if dtype is None or (k is not None and k.dtype is not q.dtype):
         raise FoldError("rotary: q and k must both be bfloat16, float16 or float32")
-    n, hq, d = q.shape
     rows, rot = _check_table("rotary", table, d)
     positions = _check_index("rotary", "positions", positions, n)
     q, qs, q_out, qos = _rotary_out("rotary", q, q_out)
