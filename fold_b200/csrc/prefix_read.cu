@@ -125,9 +125,10 @@ constexpr int kSegs = 4;
 // Segments of up to this many rows are read by the softmax warps themselves (FewRows).
 constexpr int kFewRows = 16;
 
-// Q of up to this many tokens is copied row by row, of more as one box of the half tile (a box always
-// moves all of its rows).
-constexpr int kFewToks = 8;
+// Q of up to this many rows is copied row by row (cp.async), of more as one TMA box of the half tile,
+// which always moves all of its rows: 32 KB at head size 128, for 4 rows of a decode step half as much
+// again as a short sequence's keys. Row by row a warp copies two rows a round.
+constexpr int kFewQRows = 32;
 
 struct Bars {
   uint64_t full[12], empty[12];
@@ -1142,7 +1143,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (!ok) break;
           const int nt = min(p.half_toks, s.ntok - t0);
           unsigned char* dst = smem + C::OFF_Q + slot * C::Q_TILE;
-          if (nt > kFewToks) {
+          if (nt * p.group > kFewQRows) {
             // a box of half_toks tokens (those past nt give rows that nobody reads)
             if (lane == 0) {
               mbar_arrive_expect_tx(&B.q_full[slot], HD / 64 * p.half_toks * p.group * 128);

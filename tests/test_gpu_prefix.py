@@ -151,6 +151,44 @@ def test_ragged_rows(hd, hq, hkv, causal):
     Case(nq, own, 0, hq, hkv, hd, 16, seed=hd).check(causal)
 
 
+@pytest.mark.parametrize("hq,hkv", [(64, 2), (128, 1), (17, 1), (96, 2), (24, 1)])
+def test_wide_groups(hq, hkv):
+    """Groups of many heads: one token fills a row tile, or three fill half of one."""
+    Case([1, 3, 2, 9], [40, 3, 200, 9], 260, hq, hkv, 128, 16, seed=hq).check()
+    Case([1, 5], [1, 300], 0, hq, hkv, 64, 32, "fp16", seed=hq).check()
+
+
+def test_output_in_place_of_the_query():
+    c = Case([1, 4, 70], [30, 200, 70], 300, 8, 2, 128, 16)
+    want, _ = c.check()
+    kernels.prefix_read(*c.args(), c.q, softmax_scale=c.scale)
+    assert torch.equal(c.q, want)
+
+
+def test_broadcast_query_heads():
+    """A query whose heads share memory is read as if it were copied out."""
+    c = Case([1, 2], [30, 60], 100, 8, 2, 128, 16)
+    c.q = c.q[:, :1].expand(3, 8, 128)
+    out = torch.empty(3, 8, 128, device="cuda", dtype=torch.bfloat16)
+    kernels.prefix_read(*c.args(), out, softmax_scale=c.scale)
+    c.q = c.q.contiguous()
+    assert torch.equal(out, c.read()[0])
+
+
+def test_blocks_past_32_bits():
+    """Keys in blocks that lie past 2^32 elements of the cache."""
+    nb, hkv, bs, hd = 33000, 8, 64, 128
+    kv = torch.empty(nb, hkv, bs, 2 * hd, dtype=torch.bfloat16, device="cuda")
+    c = Case([1, 20], [100, 150], 200, 8, 8, 128, 64, seed=3)
+    used = c.kv.shape[0]
+    kv[-used:] = c.kv
+    c.k, c.v = kv[..., :hd], kv[..., hd:]
+    shift = nb - used
+    c.prefix_table += shift
+    c.tables += shift
+    c.check()
+
+
 def test_rows_that_see_nothing():
     c = Case([2, 1, 3], [0, 0, 1], 0, 4, 2, 128, 16)
     out, lse = c.check()
