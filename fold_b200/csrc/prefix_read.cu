@@ -796,13 +796,18 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         // slots of the last page past the limit may hold anything (NaN included): their V rows
         // become zeros before the tensor cores read them
         const int vk = s.limit - key0;
-        if (vk < TK && vk % p.chunk != 0 && (!wide || mine0 == 0)) {
+        const bool rest = vk < TK && vk % p.chunk != 0 && (!wide || mine0 == 0);
+        if (rest || (warp & 3) == 0) {  // V has landed when the MMA warp gets P
+          const uint32_t u = v_pos(tile0 + j) * KU;
+#pragma unroll
+          for (int w = 0; w < KU; ++w) ok = ok && warp_wait(&B.full[(u + w) % NU], ((u + w) / NU) & 1);
+          if (!ok) break;
+        }
+        if (rest) {
           const int vend = (vk / p.chunk + 1) * p.chunk;
           const uint32_t u = v_pos(tile0 + j) * KU;
 #pragma unroll
           for (int w = 0; w < KU; ++w) {
-            ok = ok && warp_wait(&B.full[(u + w) % NU], ((u + w) / NU) & 1);
-            if (!ok) break;
             unsigned char* vt = smem + ((u + w) % NU) * C::UNIT;
             for (int e = row; e < (vend - vk) * C::NCG * 8; e += 128) {
               const int vr = vk + e / (C::NCG * 8), c = e % (C::NCG * 8);
@@ -810,7 +815,6 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
                                         (c & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
           }
-          if (!ok) break;
           fence_proxy_async();
         }
         tc_fence_before();
@@ -971,8 +975,10 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       constexpr uint32_t idesc_o = idesc_of(C::F16, C::UC, 1);
       constexpr uint32_t hi_q = desc_hi(1024), hi_kv = desc_hi(C::NCG * 1024);
       const uint32_t base = uniform(smem_u32(smem)), q_base = base + C::OFF_Q, tm = uniform(tmem);
-      // Where a tile's units lie in the ring, walked (K0 K1 V0 K2 V1 ...) rather than divided out.
-      struct Place {
+      // The issue of MMAs lasts about as long as they run, so all else in a step comes where it hides
+      // behind the last ones issued: the next K behind PV, the next P behind QK. V is waited for by
+      // the softmax warps, before they hand over P.
+      struct Place {  // of a unit in the ring, walked (K0 K1 V0 K2 V1 ...) rather than divided out
         uint32_t slot, parity;
         __device__ __forceinline__ void move(uint32_t n) {
           slot += n;
@@ -986,110 +992,77 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       };
       struct Step {
         Place v;
-        uint32_t v_lo[KU];
-        bool valid, first, last, new_tile, free_kv;
+        uint32_t v_lo[KU], fresh;
+        bool valid, first, last, free_kv;
       } st0, st1;
-      // The next step, worked out while the softmax of an earlier one runs: what stands between a
-      // finished P and the next S is then the two batches of MMAs alone.
-      struct Next {
-        bool known;   // in the current segment
-        bool landed;  // its K tile is there
-        Place k, v;
-        uint32_t a, k_lo[KU], v_lo[KU];
-        int half;
-      } nx;
       bool ok = true, more = true, ended = false, wide = false;
       int sg = 0, i = 0, steps = 0;  // next segment; next step of the current one
       uint32_t qu = 0;               // Q tiles used before the current segment
       uint32_t pcnt[2] = {0, 0}, ocnt[2] = {0, 0};
-      Place k_at{0, 0}, v_at{2 * KU, 0};  // of the next tile
-      uint32_t k_step = KU;
-      auto look_ahead = [&]() {
-        nx.known = more && i < steps;
-        if (!nx.known) return;
-        nx.half = wide ? i & 1 : 0;
-        if (nx.half == 0) {
-          nx.k = k_at, nx.v = v_at;
-          k_at.move(k_step), v_at.move(2 * KU);
-          k_step = 2 * KU;
-          nx.landed = true;
-#pragma unroll
-          for (int w = 0; w < KU; ++w) {
-            const Place k = nx.k.unit(w), v = nx.v.unit(w);
-            nx.landed = nx.landed && mbar_try_wait(&B.full[k.slot], k.parity);
-            nx.k_lo[w] = uniform(desc_lo(base + k.slot * C::UNIT, 16));
-            nx.v_lo[w] = uniform(desc_lo(base + v.slot * C::UNIT, 1024));
-          }
-        }
-        if (i <= nx.half || NWG == 2) nx.a = uniform(desc_lo(q_base + (qu + nx.half) % QB * C::Q_TILE, 16));
-      };
-      auto next_segment = [&]() {
-        if (steps) qu += wide ? 2 : 1;
-        Seg s;
-        ok = next_seg(sg, s);
-        if (!ok) return;
-        ++sg;
-        if (s.part < 0 || few_rows(s)) {  // all that follow are the softmax warps' own
-          more = false, ended = s.part < 0;
-          return;
-        }
-        wide = s.ntok > p.half_toks;  // the steps of a tile are its row halves
-        steps = (s.ke - s.kb) * (wide ? 2 : 1), i = 0;
-      };
-      // The waits of one step end in one vote of the warp.
+      Place k_at{0, 0}, v_at{2 * KU, 0}, k_now{0, 0}, v_now{0, 0};  // of the next tile, of this one
+      uint32_t k_step = KU, k_lo[KU], v_lo[KU];
       auto qk = [&](Step& st, const int b) {  // the next step, into S buffer b
         st.valid = false;
-        if (!nx.known) {
+        if (i == steps) {
           if (!more) return;
-          next_segment();
-          if (!ok || !more) return;
-          look_ahead();
+          if (steps) qu += wide ? 2 : 1;
+          Seg s;
+          ok = next_seg(sg, s);
+          if (!ok) return;
+          ++sg;
+          if (s.part < 0 || few_rows(s)) {  // all that follow are the softmax warps' own
+            more = false, ended = s.part < 0, i = steps = 0;
+            return;
+          }
+          wide = s.ntok > p.half_toks;  // the steps of a tile are its row halves
+          steps = (s.ke - s.kb) * (wide ? 2 : 1), i = 0;
         }
-        const bool q_first = i == nx.half;  // the first use of this Q tile
-        if (q_first || !nx.landed) {
-          if (q_first) ok = mbar_wait(&B.q_full[(qu + nx.half) % QB], ((qu + nx.half) / QB) & 1);
-          if (!nx.landed) {
+        const int half = wide ? i & 1 : 0;
+        const uint32_t quse = qu + half, qslot = quse % QB;
+        const uint32_t a = uniform(desc_lo(q_base + qslot * C::Q_TILE, 16));
+        if (half == 0) {
+          k_now = k_at, v_now = v_at;
+          k_at.move(k_step), v_at.move(2 * KU);
+          k_step = 2 * KU;
 #pragma unroll
-            for (int w = 0; w < KU; ++w) ok = ok && mbar_wait(&B.full[nx.k.unit(w).slot], nx.k.unit(w).parity);
-            nx.landed = true;
+          for (int w = 0; w < KU; ++w) {
+            k_lo[w] = uniform(desc_lo(base + k_now.unit(w).slot * C::UNIT, 16));
+            ok = ok && mbar_wait(&B.full[k_now.unit(w).slot], k_now.unit(w).parity);
           }
         }
+        if (i == half) ok = ok && mbar_wait(&B.q_full[qslot], (quse / QB) & 1);  // the first use of this Q tile
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
-        const bool free_kv = !wide || nx.half == 1;
+        const bool free_kv = !wide || half == 1;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int w = 0; w < KU; ++w) {
 #pragma unroll
             for (int kk = 0; kk < C::UC / 16; ++kk)
-              mma_ss(tm + C::TMEM_S + b * TK, nx.a + ((w * C::NCG + (kk >> 2)) * C::Q_CG + (kk & 3) * 32) / 16, hi_q,
-                     nx.k_lo[w] + ((kk >> 2) * 1024 + (kk & 3) * 32) / 16, hi_kv, idesc_s, w > 0 || kk > 0);
+              mma_ss(tm + C::TMEM_S + b * TK, a + ((w * C::NCG + (kk >> 2)) * C::Q_CG + (kk & 3) * 32) / 16, hi_q,
+                     k_lo[w] + ((kk >> 2) * 1024 + (kk & 3) * 32) / 16, hi_kv, idesc_s, w > 0 || kk > 0);
             if (w == KU - 1) tc_commit(&B.s_full[b]);
-            if (free_kv) commit_for<NSW>(&B.empty[nx.k.unit(w).slot]);
+            if (free_kv) commit_for<NSW>(&B.empty[k_now.unit(w).slot]);
           }
-          if (i + (wide ? 2 : 1) >= steps) commit_for<NSW>(&B.q_empty[(qu + nx.half) % QB]);
+          if (i + (wide ? 2 : 1) >= steps) commit_for<NSW>(&B.q_empty[qslot]);
         }
         __syncwarp();
-        st.v = nx.v;
+        st.valid = true, st.first = NWG == 2 ? i < 2 : i == 0, st.last = i + NWG >= steps, st.free_kv = free_kv;
+        st.v = v_now, st.fresh = uniform(st.first ? 0 : 1);
 #pragma unroll
-        for (int w = 0; w < KU; ++w) st.v_lo[w] = nx.v_lo[w];
-        st.valid = true, st.first = NWG == 2 ? i < 2 : i == 0, st.last = i + NWG >= steps;
-        st.new_tile = nx.half == 0, st.free_kv = free_kv;
+        for (int w = 0; w < KU; ++w) {
+          if (half == 0) v_lo[w] = uniform(desc_lo(base + v_now.unit(w).slot * C::UNIT, 1024));
+          st.v_lo[w] = v_lo[w];
+        }
         ++i;
       };
       auto pv = [&](Step& st, const int b) {
         const int acc = NWG == 2 ? b : 0;
-        look_ahead();
-        if (st.new_tile) {
-#pragma unroll
-          for (int w = 0; w < KU; ++w) ok = ok && mbar_wait(&B.full[st.v.unit(w).slot], st.v.unit(w).parity);
-        }
         if (st.first) {  // the accumulator's last segment has been read
-          if (ocnt[acc] > 0) ok = ok && mbar_wait(&B.o_free[acc], (ocnt[acc] - 1) & 1);
+          if (ocnt[acc] > 0) ok = mbar_wait(&B.o_free[acc], (ocnt[acc] - 1) & 1);
           ++ocnt[acc];
         }
-        const uint32_t add = uniform(st.first ? 0 : 1);
         ok = ok && mbar_wait(&B.p_full[b], pcnt[b]++ & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) return;
@@ -1100,7 +1073,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
 #pragma unroll
             for (int ks = 0; ks < TK / 16; ++ks)
               mma_ts(tm + C::TMEM_O + acc * HD + w * C::UC, tm + C::TMEM_S + b * TK + ks * 8,
-                     st.v_lo[w] + ks * 2 * C::NCG * 1024 / 16, hi_kv, idesc_o, ks > 0 ? 1 : add);
+                     st.v_lo[w] + ks * 2 * C::NCG * 1024 / 16, hi_kv, idesc_o, ks > 0 ? 1 : st.fresh);
             if (st.free_kv) commit_for<NSW>(&B.empty[st.v.unit(w).slot]);
           }
           if (NWG == 1) tc_commit(&B.pv_done);
@@ -1109,12 +1082,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         __syncwarp();
         qk(st, b);
       };
-      nx.known = false;
       qk(st0, 0);
-      if (ok) {
-        look_ahead();
-        qk(st1, 1);
-      }
+      if (ok) qk(st1, 1);
       while (ok && st0.valid) {
         pv(st0, 0);
         if (!ok || !st1.valid) break;
