@@ -21,13 +21,32 @@
 //     maximum raised lazily, P = 2^(y - m) rounded to the input type and stored over S in TMEM,
 //     O in TMEM rescaled when a maximum rose; at a segment's end O / l and lse go to memory;
 //   TMA warp: K and V tiles, each lane one chunk of a page, into a ring of units;
-//   MMA warp: S = Q K^T and O += P V (P from TMEM), issued by one thread;
-//   scheduler warp: walks the items, publishes segments in a small ring, loads Q by cp.async.
+//   MMA warp: S = Q K^T and O += P V (P from TMEM), issued by one lane;
+//   scheduler warp: walks the items, publishes segments in a small ring;
+//   Q warp: the segments' queries, by TMA or row by row.
 // Two S buffers and two O accumulators ("slots") keep the tensor cores busy while a warpgroup is
-// in its softmax: above 128 rows the slots are the two halves of the row tile and share each K and
-// V tile; otherwise they take the key tiles in turn and are joined at the end of the segment. At
-// head size 256 one accumulator fills the columns that S leaves, so one warpgroup serves both S
-// buffers.
+// in its softmax: a wide row tile's slots are its two halves and share each K and V tile; otherwise
+// they take the key tiles in turn and are joined at the end of the segment. At head size 256 one
+// accumulator fills the columns that S leaves, so one warpgroup serves both S buffers. Segments of a
+// few rows go another way (FewRows) and come last on the line.
+//
+// Rounding. Logits, maxima, sums, O and the partials are float32; P is rounded once to the type of
+// V (the MMA takes operands of one type), the sums are of the unrounded P, the result is rounded
+// once. Against 64 bits that is 0.0023 (bf16) or 0.00029 (fp16) of the outputs' norm, where rounding
+// the outputs alone is 0.0017 and 0.00021.
+//
+// Measured (bf16, head size 128, 32 query and 8 KV heads, pages of 16; the whole call):
+//   256 sequences of one token, 32K shared and up to 256 own keys: 186 us (740 TFLOP/s; in the long
+//     run over the prefix 1160, 0.70 of the measured peak);
+//   3 sequences of 8 tokens, 128K shared: 106 us (5.1 TB/s, 0.78 of the measured copy rate; 6 TB/s
+//     behind the first 10 us);
+//   64 sequences of one token, 16K shared and up to 1024 own keys: 62 us, of which the start of the
+//     pipeline (lengths, line, first page, first tile) takes 8 and the merge 4.
+// What bounds the wide case: with the exponentials left out it takes as long, with most of the MMAs
+// left out 0.8 and without both 0.75 of the time: the K and V tiles' way from L2 into shared memory
+// and the MMAs share the SM's bandwidth, and the hand-over between softmax and MMA is a chain of
+// waits. Tried and dropped: exponentials by polynomial beside the special unit, P handed over in two
+// halves, the tile's maximum found beside the exponentials, a second MMA warp (one a slot).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
@@ -69,6 +88,7 @@ struct PrefixParams {
   int64_t o_st, o_sh;
   float* lse;
   int n, hq, hkv, group;
+  int item_cost;  // kItemCost, by head size
   int half_toks;  // tokens whose rows fill a half of a wide row tile: 128 / group
   int ctas;
   // workspace
@@ -86,7 +106,7 @@ struct Cfg {
   static constexpr int HD = HD_;
   static constexpr int NWG = HD == 256 ? 1 : 2;  // softmax warpgroups = O accumulators
   static constexpr int NSW = NWG * 4;
-  static constexpr int NTHREADS = (NSW + 4) * 32;  // + TMA, MMA, scheduler, one idle
+  static constexpr int NTHREADS = (NSW + 4) * 32;  // + TMA, MMA, scheduler, Q
   static constexpr int ROWS = NWG * 128;
   static constexpr int UC = HD < 128 ? HD : 128;  // columns of a unit
   static constexpr int KU = HD / UC;              // units of a K (or V) tile
@@ -109,8 +129,12 @@ struct Cfg {
   static_assert(NU >= 4 && SMEM <= kSmemLimit, "shared memory");
 };
 
-// Cost units (a quarter of a key tile of a row tile of at most 128 rows).
-constexpr int kTileCost = 5, kWideTileCost = 8, kItemCost = 12, kFewItemCost = 6;
+// Cost units of the line, from the CTAs' finishing times at decode, prompt and draft shapes: about
+// 0.3 us, an eighth of a key tile of a wide row tile. A tile of up to 128 rows takes 5, of few rows 4;
+// an item costs its Q, its first keys' way through the pipeline and its partial besides (at head size
+// 256, where one Q tile and one accumulator hold nothing ready, more).
+constexpr int kWideTileCost = 8, kTileCost = 5, kFewTileCost = 4;
+constexpr int kItemCost = 12, kItemCost256 = 20, kFewItemCost = 6;
 
 struct Seg {
   int part;  // 0: prefix, 1: own keys, -1: no more work
@@ -154,7 +178,7 @@ __device__ __forceinline__ int capped(int len, int cap, int* err) {
 }
 
 __device__ __forceinline__ int tile_cost(const PrefixParams& p, int ntok) {
-  return ntok > p.half_toks ? kWideTileCost : kTileCost;
+  return ntok * p.group <= kFewRows ? kFewTileCost : ntok > p.half_toks ? kWideTileCost : kTileCost;
 }
 
 // Query rows of sequence s, [first, last), kept inside [0, n] whatever qsl holds.
@@ -176,7 +200,7 @@ __device__ __forceinline__ int64_t quot(int64_t a, int64_t b) {
 }
 
 __device__ __forceinline__ int start_cost(const PrefixParams& p, int ntok) {
-  return ntok * p.group <= kFewRows ? kFewItemCost : kItemCost;
+  return ntok * p.group <= kFewRows ? kFewItemCost : p.item_cost;
 }
 __device__ __forceinline__ int64_t item_cost(const PrefixParams& p, int tiles, int ntok) {
   return tiles == 0 ? 2 : start_cost(p, ntok) + static_cast<int64_t>(tiles) * tile_cost(p, ntok);
@@ -316,13 +340,15 @@ __device__ __forceinline__ void regs_down() {
 }
 
 // ---------------------------------------------------------------- segments of few rows
-// A row tile of at most FEW_ROWS rows (a decode step's, whose keys are read once for a handful of
+// A row tile of at most kFewRows rows (a decode step's, whose keys are read once for a handful of
 // rows) would leave most of the 128 lanes of S idle and pay for the way through the MMA warp. The
 // softmax warps take such a segment themselves with mma.sync: each warp owns 128 / NSW keys of every
 // tile and keeps rows x keys and rows x hd fragments in registers (S = Q K^T, its C fragments are the
 // A fragments of P V), with a maximum, sum and O of its own, so that no warp waits for another until
 // the segment's end, where the warps' partials are joined through the Q tile. Memory bound: the
-// ring's units are all in flight.
+// ring's units are all in flight (one row over 200K keys: 137 us, 6.0 TB/s, as by the MMA warp's way;
+// 2048 short segments of 4 rows, 1 to 256 keys each: 58 us against 82). 17 to 32 rows took 2.5 us a
+// tile here against 1.7. The joining deferred behind the next segment's first tile was slower (65 us).
 template <class C>
 struct FewRows {
   static constexpr int HD = C::HD, KW = TK / C::NSW;
@@ -667,7 +693,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     if (mine[k] > 0 && own_x >= excl[k] && own_x < excl[k] + mine[k]) {
       int64_t at = excl[k];
       int s = s_lo;
-      for (; s < s_hi; ++s) {
+      for (; s + 1 < s_hi; ++s) {  // the thread's last one needs no look
         int64_t c[2];
         seq_cost<C>(p, s, per_tile, c);
         if (own_x < at + c[k] * p.hkv) break;
@@ -1249,8 +1275,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
 
 // Joins the partials of one row: its prefix item's and its own item's, one per CTA that held a part
 // of the item. WPR warps a row take every WPR-th partial each; a lane reads the lse of one.
-// Latency bound (a few partials of a row, from L2): four warps a row where there are few rows (the
-// partials are then many), one where there are enough rows to fill the SMs.
+// Latency bound (a few partials of a row, from L2).
 template <int HD, class T, int WPR>
 __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixParams p, int cont_rows) {
   constexpr int V = HD / 32, RPB = 4 / WPR;
@@ -1442,7 +1467,9 @@ int launch_prefix(const PrefixParams& p, const void* k, const void* v, int64_t s
                             qmap, kmap, vmap, p))
     return s;
   const int64_t rows = static_cast<int64_t>(p.n) * p.hq;
-  if (rows <= 4096)
+  // few rows have many partials each: four warps a row at 64 rows over 16K keys (27 us the whole call,
+  // one warp 31), 768 rows over 128K (101 against 105); one warp from 2048 rows on (62 against 64)
+  if (rows <= 1024)
     return launch_behind(prefix_merge_kernel<HD, T, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, stream,
                          "prefix_merge_kernel", p, C::ROWS);
   return launch_behind(prefix_merge_kernel<HD, T, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream,
@@ -1526,7 +1553,7 @@ int fold_prefix_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   p.oob = static_cast<int>((num_blocks - 1) * mul_b + (hkv - 1) * mul_h + 1);
   p.causal = causal ? 1 : 0, p.scale_log2 = softmax_scale * kLog2e;
   p.out = out, p.o_st = o_stride_tok, p.o_sh = o_stride_head, p.lse = lse;
-  p.n = n, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.half_toks = 128 / p.group, p.ctas = ctas, p.err = err;
+  p.n = n, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.half_toks = 128 / p.group, p.item_cost = hd == 256 ? kItemCost256 : kItemCost, p.ctas = ctas, p.err = err;
   char* ws = static_cast<char*>(workspace);
   p.plan = reinterpret_cast<int4*>(ws + w.plan);
   p.o_prim = reinterpret_cast<float*>(ws + w.o_prim), p.lse_prim = reinterpret_cast<float*>(ws + w.lse_prim);
