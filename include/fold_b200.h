@@ -105,8 +105,8 @@ int fold_far_query(const void* q, int64_t q_stride_tok, int64_t q_stride_head, v
  * the gradient of the inputs. rope_table: float32 [table_rows, rot_dim], row p holding
  * c cos(p f_i) then c sin(p f_i), c the attention factor of scaled frequencies (1 otherwise); a
  * position outside [0, table_rows) is clamped and sets FOLD_DEVERR_ROPE_RANGE. An output may be its
- * input; any other overlap of inputs and outputs is not allowed. Rows are read 16 bytes at a time
- * where rot_dim and hd are multiples of 32 bytes' elements and rows start on 16-byte boundaries,
+ * input; any other overlap of inputs and outputs is not allowed. Rows are read 16, 8 or 4 bytes at a
+ * time, the most that half of rot_dim, hd / 2, the row starts and strides are whole multiples of,
  * else element by element. hd at most 8192. */
 int fold_rotary(const void* q, int64_t q_stride_tok, int64_t q_stride_head, void* q_out, int64_t qo_stride_tok,
                 int64_t qo_stride_head, int hq, const void* k, int64_t k_stride_tok, int64_t k_stride_head,
