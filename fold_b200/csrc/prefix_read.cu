@@ -36,11 +36,11 @@
 // the outputs alone is 0.0017 and 0.00021.
 //
 // Measured (bf16, head size 128, 32 query and 8 KV heads, pages of 16; the whole call):
-//   256 sequences of one token, 32K shared and up to 256 own keys: 186 us (740 TFLOP/s; in the long
+//   256 sequences of one token, 32K shared and up to 256 own keys: 174 us (790 TFLOP/s; in the long
 //     run over the prefix 1160, 0.70 of the measured peak);
 //   3 sequences of 8 tokens, 128K shared: 106 us (5.1 TB/s, 0.78 of the measured copy rate; 6 TB/s
 //     behind the first 10 us);
-//   64 sequences of one token, 16K shared and up to 1024 own keys: 62 us, of which the start of the
+//   64 sequences of one token, 16K shared and up to 1024 own keys: 58 us, of which the start of the
 //     pipeline (lengths, line, first page, first tile) takes 8 and the merge 4.
 // What bounds the wide case: with the exponentials left out it takes as long, with most of the MMAs
 // left out 0.8 and without both 0.75 of the time: the K and V tiles' way from L2 into shared memory
@@ -130,11 +130,12 @@ struct Cfg {
 };
 
 // Cost units of the line, from the CTAs' finishing times at decode, prompt and draft shapes: about
-// 0.3 us, an eighth of a key tile of a wide row tile. A tile of up to 128 rows takes 5, of few rows 4;
+// 0.3 us, an eighth of a key tile of a wide row tile. A tile of up to 128 rows takes 6, of few rows 4;
 // an item costs its Q, its first keys' way through the pipeline and its partial besides (at head size
-// 256, where one Q tile and one accumulator hold nothing ready, more).
-constexpr int kWideTileCost = 8, kTileCost = 5, kFewTileCost = 4;
-constexpr int kItemCost = 12, kItemCost256 = 20, kFewItemCost = 6;
+// 256, where one Q tile and one accumulator hold nothing ready, more; of few rows, where two are under
+// way at a time, less: with 6 for 3 the 256 sequences over 32K keys took 184 us, with 2 183, with 3 174).
+constexpr int kWideTileCost = 8, kTileCost = 6, kFewTileCost = 4;
+constexpr int kItemCost = 12, kItemCost256 = 20, kFewItemCost = 3;
 
 struct Seg {
   int part;  // 0: prefix, 1: own keys, -1: no more work
@@ -146,6 +147,14 @@ struct Seg {
 };
 constexpr int kSegs = 4;
 
+// The line may be cut where the few rows begin if either side has this many CTAs.
+constexpr int kCutCtas = 16;
+// No piece is shorter, nor, by a rounded number of CTAs on a side of that cut, shorter than the
+// longest tile: then no CTA between an item's first and last is without a tile of it, and its
+// partials are those of consecutive CTAs. Eight sequences' own keys alone (64 items): 16.8 us, with
+// pieces of 18 units at least 18.7.
+constexpr int kMinPiece = 10;
+static_assert(kMinPiece * (kCutCtas - 1) / kCutCtas >= kWideTileCost, "a tile a piece");
 // Segments of up to this many rows are read by the softmax warps themselves (FewRows).
 constexpr int kFewRows = 16;
 
@@ -159,7 +168,7 @@ struct Bars {
   uint64_t s_full[2], p_full[2], pv_done;
   uint64_t q_full[2], q_empty[2];
   uint64_t seg_full[kSegs], seg_empty[kSegs];
-  uint64_t seg_done[2], o_free[2], stat_full, stat_free, drained, meet;
+  uint64_t seg_done[2], o_free[2], stat_full, stat_free, drained, meet, few_meet[2], few_turn;
   uint32_t tmem;
   int start_seq[2];
   int64_t start_base[2];
@@ -342,31 +351,34 @@ __device__ __forceinline__ void regs_down() {
 // ---------------------------------------------------------------- segments of few rows
 // A row tile of at most kFewRows rows (a decode step's, whose keys are read once for a handful of
 // rows) would leave most of the 128 lanes of S idle and pay for the way through the MMA warp. The
-// softmax warps take such a segment themselves with mma.sync: each warp owns 128 / NSW keys of every
-// tile and keeps rows x keys and rows x hd fragments in registers (S = Q K^T, its C fragments are the
-// A fragments of P V), with a maximum, sum and O of its own, so that no warp waits for another until
-// the segment's end, where the warps' partials are joined through the Q tile. Memory bound: the
-// ring's units are all in flight (one row over 200K keys: 137 us, 6.0 TB/s, as by the MMA warp's way;
-// 2048 short segments of 4 rows, 1 to 256 keys each: 58 us against 82). 17 to 32 rows took 2.5 us a
-// tile here against 1.7. The joining deferred behind the next segment's first tile was slower (65 us).
+// softmax warps take such segments themselves with mma.sync, a warpgroup every other one: each of its
+// four warps owns 32 keys of every tile and keeps rows x keys and rows x hd fragments in registers
+// (S = Q K^T, its C fragments are the A fragments of P V), with a maximum, sum and O of its own, so
+// that no warp waits for another until the segment's end, where the warps' partials are joined
+// through the Q tile. A short segment is a chain of latencies (Q, K, V, two meetings of the warps, the
+// partial), which the other group's segment fills: 2048 segments of 4 rows and 1 to 256 keys take 52 us,
+// by both groups together 58, by the MMA warp's way 82. Memory bound: the ring's units are all in
+// flight (one row over 200K keys: 137 us, 6.0 TB/s). 17 to 32 rows took 2.5 us a tile here against 1.7;
+// the joining deferred behind the next segment's first tile was slower.
 template <class C>
 struct FewRows {
-  static constexpr int HD = C::HD, KW = TK / C::NSW;
+  static constexpr int HD = C::HD, GW = 4, KW = TK / GW;  // warps of a group, keys of a tile a warp owns
   using T = typename C::T;
   const PrefixParams& p;
   const Seg& s;
   Bars& B;
   unsigned char* smem;
   float2* stats;
-  const int warp, lane, cta;
+  const int group, warp, lane, cta;  // warp: of the group
   const uint32_t tile0, qu;
-  uint32_t meets;
+  uint32_t meets;    // of this group's warps so far
+  const uint32_t index;  // of the segment among those of few rows
 
-  // All softmax warps, with a bounded wait.
+  // The group's warps, with a bounded wait.
   __device__ __forceinline__ bool meet() {
     __syncwarp();
-    if (lane == 0) mbar_arrive(&B.meet);
-    return warp_wait(&B.meet, meets++ & 1);
+    if (lane == 0) mbar_arrive(&B.few_meet[group]);
+    return warp_wait(&B.few_meet[group], meets++ & 1);
   }
   __device__ __forceinline__ static void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (C::F16) mma_f16(d, a[0], a[1], a[2], a[3], b0, b1);
@@ -378,6 +390,9 @@ struct FewRows {
     const int ntile = s.ke - s.kb, rows = s.ntok * p.group;
     const int g = lane >> 2, t4 = lane & 3, mi = lane >> 3, mr = lane & 7;  // fragment row, column; ldmatrix
     const uint32_t qslot = qu % C::QB;
+    // the other group has the last tile of the segment before: every earlier unit of the ring has
+    // landed, so that a wait for this segment's units cannot take an older phase for theirs
+    if (C::NWG == 2 && index > 0 && !warp_wait(&B.few_turn, (index - 1) & 1)) return false;
     if (!warp_wait(&B.q_full[qslot], (qu / C::QB) & 1)) return false;
     const uint32_t base = smem_u32(smem), qt = base + C::OFF_Q + qslot * C::Q_TILE;
     auto q_frag = [&](int mt, int kk, uint32_t (&a)[4]) {
@@ -498,11 +513,15 @@ struct FewRows {
       __syncwarp();
       if (lane == 0) {  // K goes back before V is waited for: the ring need not hold both
 #pragma unroll
-        for (int w = 0; w < C::KU; ++w) mbar_arrive(&B.empty[(ku + w) % C::NU]);
+        for (int w = 0; w < C::KU; ++w) mbar_arrive_n(&B.empty[(ku + w) % C::NU], C::NWG);
       }
 #pragma unroll
       for (int w = 0; w < C::KU; ++w)
         if (!warp_wait(&B.full[(vu + w) % C::NU], ((vu + w) / C::NU) & 1)) return false;
+      if (j + 1 == ntile) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.few_turn);
+      }
       if (any) {
         // slots past the limit may hold anything (NaN included): this warp's rows of them become zeros
         const int seen = s.limit - key0 - row0;
@@ -540,7 +559,7 @@ struct FewRows {
       __syncwarp();
       if (lane == 0) {
 #pragma unroll
-        for (int w = 0; w < C::KU; ++w) mbar_arrive(&B.empty[(vu + w) % C::NU]);
+        for (int w = 0; w < C::KU; ++w) mbar_arrive_n(&B.empty[(vu + w) % C::NU], C::NWG);
       }
     }
 
@@ -554,7 +573,7 @@ struct FewRows {
       float ls = l[mt][e];
       ls += __shfl_xor_sync(0xffffffffu, ls, 1);
       ls += __shfl_xor_sync(0xffffffffu, ls, 2);
-      if (t4 == 0) stats[warp * 8 + g] = make_float2(m[mt][e], ls);
+      if (t4 == 0) stats[(group * GW + warp) * 8 + g] = make_float2(m[mt][e], ls);
       if (g < nr) {
 #pragma unroll
         for (int c = 0; c < HD / 8; ++c)
@@ -562,15 +581,15 @@ struct FewRows {
               make_float2(o[mt][c][2 * e], o[mt][c][2 * e + 1]);
       }
       if (!meet()) return false;
-      for (int r = warp; r < nr; r += C::NSW) {
+      for (int r = warp; r < nr; r += GW) {
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < C::NSW; ++w) top = fmaxf(top, stats[w * 8 + r].x);
+        for (int w = 0; w < GW; ++w) top = fmaxf(top, stats[(group * GW + w) * 8 + r].x);
         const float mz = top == -INFINITY ? 0.f : top;
-        float f[C::NSW], sum = 0.f;
+        float f[GW], sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < C::NSW; ++w) {
-          const float2 a = stats[w * 8 + r];
+        for (int w = 0; w < GW; ++w) {
+          const float2 a = stats[(group * GW + w) * 8 + r];
           f[w] = fast_exp2(a.x - mz), sum += f[w] * a.y;
         }
         const bool some = sum > 0.f;
@@ -582,7 +601,7 @@ struct FewRows {
         for (int c = lane * 4; c < HD; c += 128) {
           float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int w = 0; w < C::NSW; ++w) {
+          for (int w = 0; w < GW; ++w) {
             const float4 v = *reinterpret_cast<const float4*>(scratch + (w * 8 + r) * HD + c);
             acc.x += f[w] * v.x, acc.y += f[w] * v.y, acc.z += f[w] * v.z, acc.w += f[w] * v.w;
           }
@@ -597,7 +616,7 @@ struct FewRows {
     }
     fence_proxy_async();  // the Q tile may be loaded by TMA next
     __syncwarp();
-    if (lane == 0) mbar_arrive(&B.q_empty[qslot]);
+    if (lane == 0) mbar_arrive_n(&B.q_empty[qslot], C::NWG);
     return true;
   }
 };
@@ -626,6 +645,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       for (int i = 0; i < kSegs; ++i) mbar_init(&B.seg_full[i], 1), mbar_init(&B.seg_empty[i], 3 + NSW);
       mbar_init(&B.pv_done, 1), mbar_init(&B.stat_full, NSW), mbar_init(&B.stat_free, NSW);
       mbar_init(&B.drained, 1), mbar_init(&B.meet, NSW);
+      mbar_init(&B.few_meet[0], 4), mbar_init(&B.few_meet[1], 4), mbar_init(&B.few_turn, 4);
       fence_mbar_init();
     }
     __syncwarp();
@@ -680,11 +700,23 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
                                pfull + plast + own_total[0]};
   const int64_t from_last = last_few ? pfull + own_total[0] : pfull;
   const int64_t total = from_own[1] + own_total[1];
-  // no piece shorter than an item's start and one tile
-  const int ctas = static_cast<int>(max64(1, min64(p.ctas, total / (kItemCost + kTileCost))));
-  const int64_t each = quot(total, ctas);
-  const uint32_t rest = static_cast<uint32_t>(total - each * ctas);
-  auto cut = [&](int c) { return each * c + rest * static_cast<uint32_t>(c) / static_cast<uint32_t>(ctas); };
+  const int ctas = static_cast<int>(max64(1, min64(p.ctas, total / kMinPiece)));
+  // CTAs 2i and 2i+1 run on neighbouring SMs, and one that reads few rows beside one with many slows
+  // both (the wide one's key tiles by a third, and the call waited for it: 183 us against 174 at 256
+  // sequences over 32K keys). So where both kinds have CTAs enough for it to cost little, the line is
+  // cut where the few rows begin, with an even number of CTAs before the cut.
+  const int64_t many = last_few ? from_last : from_own[1];
+  int before = (static_cast<int>(quot(many * ctas, max64(total, 1))) + 1) & ~1;
+  if (before < kCutCtas || ctas - before < kCutCtas) before = 0;
+  const int64_t cut_x = before ? many : 0;
+  const int64_t each[2] = {before ? quot(cut_x, before) : 0, quot(total - cut_x, ctas - before)};
+  const uint32_t rest[2] = {static_cast<uint32_t>(cut_x - each[0] * before),
+                            static_cast<uint32_t>(total - cut_x - each[1] * (ctas - before))};
+  auto cut = [&](int c) {  // where CTA c's piece begins
+    if (c < before) return each[0] * c + rest[0] * static_cast<uint32_t>(c) / static_cast<uint32_t>(before);
+    const uint32_t x = c - before;
+    return cut_x + each[1] * x + rest[1] * x / static_cast<uint32_t>(ctas - before);
+  };
   const int cta = blockIdx.x;
   const int64_t x0 = cta < ctas ? cut(cta) : total, x1 = cta < ctas ? cut(cta + 1) : total;
 #pragma unroll
@@ -924,12 +956,15 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&B.meet);
       ok = warp_wait(&B.meet, 0);
-      uint32_t meets = 1;
+      uint32_t meets = 0, index = 0;
       Seg s = few_seg;
-      for (int sg = few_from; ok && s.part >= 0;) {
-        FewRows<C> f{p, s, B, smem, stats, warp, lane, cta, tile0, qu, meets};
-        ok = f.run();
-        meets = f.meets, tile0 += s.ke - s.kb, ++qu;
+      for (int sg = few_from; ok && s.part >= 0; ++index) {
+        if (NWG == 1 || (index & 1) == static_cast<uint32_t>(wg)) {
+          FewRows<C> f{p, s, B, smem, stats, wg, warp & 3, lane, cta, tile0, qu, meets, index};
+          ok = f.run();
+          meets = f.meets;
+        }
+        tile0 += s.ke - s.kb, ++qu;
         ok = ok && next_seg(++sg, s);
       }
     }
@@ -1197,7 +1232,9 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             int upto = s.ke;
             while (upto == 0) ++c0, upto = tiles_before(cut(c0 + 1));
             // a CTA at or past the item's end, then back
-            int c1 = max(static_cast<int>(min64(ctas - 1, quot(end, each) + 1)), c0);
+            const int k = end > cut_x;
+            const int64_t past = (k ? before + quot(end - cut_x, each[1]) : quot(end, each[0])) + 1;
+            int c1 = max(static_cast<int>(min64(ctas - 1, past)), c0);
             while (c1 > c0 && tiles_before(cut(c1)) >= tiles) --c1;
             cnt = c1 - c0 + 1;
           }

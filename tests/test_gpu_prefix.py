@@ -215,6 +215,21 @@ def test_many_sequences():
          seed=5).check()
 
 
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("tiles", [1, 2, 5, 14, 30, 61, 100])
+def test_short_pieces_of_a_wide_prefix(tiles, hd):
+    """Few units in all: every piece is as short as pieces get, about one wide key tile."""
+    Case([1] * 40 + [24], [3] * 40 + [24], 128 * tiles - 5, 4, 1, hd, 16, seed=tiles).check()
+
+
+@pytest.mark.parametrize("prefix", [700, 2048, 3333])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_line_cut_where_few_rows_begin(hd, prefix):
+    """Many-row items of the prefix and few-row items of the sequences, both over dozens of CTAs."""
+    rng = np.random.default_rng(prefix)
+    Case([1] * 210, rng.integers(1, 200, 210).tolist(), prefix, 8, 2, hd, 16, seed=prefix).check()
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_many_short_parts_between_long_ones(hd):
     """Row tiles of every width behind one another in one launch: sequences of one token, of a few
