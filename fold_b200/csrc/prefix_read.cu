@@ -1539,8 +1539,11 @@ int fold_prefix_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   if (!(softmax_scale > 0.f) || softmax_scale > 1e30f)
     return fail(FOLD_ERR_INVALID_ARGUMENT, "prefix read: softmax_scale must be positive and finite");
   if (n == 0 || b == 0) return FOLD_OK;
-  if (!q || !qsl || !own_lens || !prefix_len || !k_cache || !v_cache || !prefix_table || !block_tables || !out)
+  if (!q || !qsl || !own_lens || !prefix_len || !k_cache || !v_cache || (prefix_table_len && !prefix_table) ||
+      (block_tables_len && !block_tables) || !out)  // a table of no blocks may be null
     return fail(FOLD_ERR_INVALID_ARGUMENT, "prefix read: null pointer");
+  if ((n > 1 && o_stride_tok == 0) || (hq > 1 && o_stride_head == 0))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "prefix read: the rows of out must not share memory");
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || q_stride_tok % 8 ||
       q_stride_head % 8 || o_stride_tok % 8 || o_stride_head % 8 || cache_stride_block % 8 || cache_stride_head % 8 ||
       cache_stride_slot % 8)
@@ -1590,7 +1593,8 @@ int fold_prefix_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   p.oob = static_cast<int>((num_blocks - 1) * mul_b + (hkv - 1) * mul_h + 1);
   p.causal = causal ? 1 : 0, p.scale_log2 = softmax_scale * kLog2e;
   p.out = out, p.o_st = o_stride_tok, p.o_sh = o_stride_head, p.lse = lse;
-  p.n = n, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.half_toks = 128 / p.group, p.item_cost = hd == 256 ? kItemCost256 : kItemCost, p.ctas = ctas, p.err = err;
+  p.n = n, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.half_toks = 128 / p.group;
+  p.item_cost = hd == 256 ? kItemCost256 : kItemCost, p.ctas = ctas, p.err = err;
   char* ws = static_cast<char*>(workspace);
   p.plan = reinterpret_cast<int4*>(ws + w.plan);
   p.o_prim = reinterpret_cast<float*>(ws + w.o_prim), p.lse_prim = reinterpret_cast<float*>(ws + w.lse_prim);

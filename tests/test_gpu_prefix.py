@@ -196,6 +196,14 @@ def test_rows_that_see_nothing():
     assert bool(torch.isfinite(lse[:, 5]).all())
 
 
+@pytest.mark.parametrize("own,prefix", [([40, 9], 0), ([0, 0], 300), ([0, 0], 0)])
+def test_tables_of_no_blocks(own, prefix):
+    c = Case([2, 1], own, prefix, 8, 2, 128, 16, table_pad=0)
+    c.prefix_table = c.prefix_table[:-(-prefix // 16)]
+    assert c.prefix_table.numel() == 0 or prefix
+    c.check(causal=False)
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_long_split(hd):
     """Few rows over many keys (split over the SMs and joined), and one long sequence among short."""

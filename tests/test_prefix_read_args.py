@@ -22,7 +22,7 @@ def call(**kw):
     dict(bs=0), dict(bs=8), dict(bs=24), dict(ptl=-1), dict(btl=-1), dict(hd=96), dict(hd=0), dict(dtype=2),
     dict(dtype=9), dict(hq=129 * 2), dict(q=8), dict(k=24), dict(v=8), dict(out=4), dict(qs=(512, 4)),
     dict(os=(508, 128)), dict(cs=(8192, 4096, 260)), dict(cs=(8192 + 8, 4096, 256)), dict(ws=None), dict(wb=16),
-    dict(ws=8), dict(nb=1 << 31)])
+    dict(ws=8), dict(nb=1 << 31), dict(os=(0, 128)), dict(os=(512, 0))])
 def test_refusals(bad):
     with pytest.raises(FoldError, match="prefix read"):
         call(**bad)
