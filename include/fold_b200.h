@@ -192,7 +192,8 @@ int fold_window_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
  * The prefix's position j < prefix_len[0] lies in block prefix_table[j / block_size]; own position
  * j in block block_tables[i * block_tables_stride + j / block_size], both at offset
  * j % block_size of the planes k_cache and v_cache ([num_blocks, hkv, block_size, hd] with the
- * given strides, as fold_window_read; the block stride a multiple of the head stride). The keys
+ * given strides, as fold_window_read; of the block and head strides one a multiple of the other). A
+ * table of length 0 may be NULL. The keys
  * already hold their rotation (fold_append_paged). Row r of sequence i sees the whole prefix and,
  * of its own m = own_lens[i] keys, all, or when `causal` the first m - (query rows of i) + r + 1
  * (bottom-right alignment). out [n, hq, hd] = the softmax-weighted values, lse [hq, n] (contiguous,
