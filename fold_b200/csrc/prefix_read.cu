@@ -118,6 +118,13 @@ struct Cfg {
   static constexpr int MISC = 1024 + 2048;  // barriers, segments, scan; row statistics
   static constexpr int FIT = (kSmemLimit - MISC - QB * Q_TILE) / UNIT;
   static constexpr int NU = FIT > 12 ? 12 : FIT;
+  // A wait for a unit goes by its phase's parity, so the unit NU places before it must be known to have
+  // landed: else the wait may take that one's older phase for its own. A softmax warp that holds S of
+  // tile j knows K up to j and V up to j - 2 landed (S of j is issued behind P V of j - 2), so of the
+  // places before V of j (units from (2j + 2) KU on) only those of V of j - 1 (from 2j KU on) are open.
+  // A ring of three tiles or more does not reach back to them; at head size 256 (5 units, KU 2) it
+  // does, and every softmax warp waits for V of every tile.
+  static constexpr bool ALL_WAIT_V = NU < 3 * KU;
   static constexpr int OFF_Q = NU * UNIT;
   static constexpr int OFF_BAR = OFF_Q + QB * Q_TILE;
   static constexpr int OFF_STAT = OFF_BAR + 1024;
@@ -855,7 +862,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         // become zeros before the tensor cores read them
         const int vk = s.limit - key0;
         const bool rest = vk < TK && vk % p.chunk != 0 && (!wide || mine0 == 0);
-        if (rest || (warp & 3) == 0) {  // V has landed when the MMA warp gets P
+        if (C::ALL_WAIT_V || rest || (warp & 3) == 0) {  // V has landed when the MMA warp gets P
           const uint32_t u = v_pos(tile0 + j) * KU;
 #pragma unroll
           for (int w = 0; w < KU; ++w) ok = ok && warp_wait(&B.full[(u + w) % NU], ((u + w) / NU) & 1);

@@ -251,6 +251,21 @@ def test_many_short_parts_between_long_ones(hd):
     Case(nq, own, 0, 4, 4, hd, 32, "fp16", seed=hd).check(causal=False)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_stale_slots_behind_every_long_segment(hd):
+    """Segments of many rows that each end inside a page of scattered small pages, tile counts of
+    one to seven in turn: the last tile's stale slots (NaN) are zeroed while tiles before it may
+    still be on their way through the ring. Every pass gives the same bits."""
+    rng = np.random.default_rng(hd)
+    nq = [20 + int(x) for x in rng.integers(0, 60, 96)]
+    own = [max(n, 128 * (i % 7) + 1 + int(rng.integers(0, 127))) for i, n in enumerate(nq)]
+    c = Case(nq, own, 0, 4, 4, hd, 16, seed=hd)
+    want, wl = c.check()
+    for _ in range(20):
+        out, lse = c.read()
+        assert torch.equal(out, want) and torch.equal(lse, wl)
+
+
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_large_logits(hd, dtype):
