@@ -47,19 +47,52 @@ def default_inv_freq(theta: float, rotary_dim: int, device=None) -> torch.Tensor
     return torch.from_numpy((1.0 / (theta ** (i / rotary_dim))).astype(np.float32)).to(device)
 
 
+# Keys of each rule, and keys that any of them may carry.
+_SCALING_KEYS = {
+    "default": set(),
+    "linear": set(),
+    "ntk": set(),
+    "llama3": {"low_freq_factor", "high_freq_factor"},
+    "yarn": {"beta_fast", "beta_slow", "truncate", "attention_factor", "mscale", "mscale_all_dim"},
+}
+_COMMON_KEYS = {"rope_type", "type", "factor", "rope_theta", "original_max_position_embeddings",
+                "max_position_embeddings", "partial_rotary_factor", "finetuned"}
+
+
+def _yarn_attention(given, s):
+    """YaRN's attention factor for contexts s times the trained one."""
+    if "attention_factor" in given:
+        return float(given["attention_factor"])
+    m, a = float(given.get("mscale", 0.0)), float(given.get("mscale_all_dim", 0.0))
+    if m and a:
+        return (0.1 * m * np.log(s) + 1.0) / (0.1 * a * np.log(s) + 1.0)
+    if a or m not in (0.0, 1.0):  # mscale 1 alone is the plain factor by every definition
+        raise ValueError("scaled_inv_freq: yarn takes mscale and mscale_all_dim together")
+    return 0.1 * np.log(s) + 1.0
+
+
 def scaled_inv_freq(theta: float, rotary_dim: int, scaling=None, device=None):
     """(frequencies float32 [rotary_dim / 2], attention factor) of a long-context rotary scaling, for
     rope_table(inv_freq, rows, device, factor). `scaling` is None (native) or a dict in the form
     model configurations give it:
 
+      {"rope_type": "default"}                 native
       {"rope_type": "linear", "factor": s}     positions interpolated: f / s
       {"rope_type": "ntk", "factor": s}        base stretched: theta * s^(d / (d - 2))
       {"rope_type": "llama3", "factor": s, "low_freq_factor": a, "high_freq_factor": b,
        "original_max_position_embeddings": L}  f / s below a turns in L, f above b, linear between
       {"rope_type": "yarn", "factor": s, "original_max_position_embeddings": L, "beta_fast": 32,
        "beta_slow": 1}                         f above beta_fast turns in L, f / s below beta_slow,
-                                               a linear ramp over the dims between; the attention
-                                               factor is 0.1 ln s + 1 unless "attention_factor"
+                                               a linear ramp over the dims between, its ends at whole
+                                               dims unless "truncate" is false; the attention factor is
+                                               "attention_factor" where given, else 0.1 ln s + 1, or
+                                               with "mscale" m and "mscale_all_dim" a
+                                               (0.1 m ln s + 1) / (0.1 a ln s + 1)
+
+    Keys that say nothing about the rotation's angles (the trained or the longest context beside a rule
+    that does not use it, the part of the head that is rotated) may be there, as may a "rope_theta"
+    equal to theta. Any other key, and one of mscale and mscale_all_dim alone (definitions of it
+    differ), is refused, since leaving it out would give other frequencies than the model's.
     """
     d = int(rotary_dim)
     if d < 2 or d % 2 or not theta > 0:
@@ -68,39 +101,55 @@ def scaled_inv_freq(theta: float, rotary_dim: int, scaling=None, device=None):
     f = 1.0 / (float(theta) ** (i / d))
     attention = 1.0
     if scaling is not None:
-        kind = scaling.get("rope_type", scaling.get("type"))
-        if kind not in ("linear", "ntk", "llama3", "yarn"):
+        kind = scaling.get("rope_type") or scaling.get("type")
+        if kind not in _SCALING_KEYS:
             raise ValueError(f"scaled_inv_freq: unknown rope_type {kind!r}")
-        s = float(scaling["factor"])
-        if not s >= 1.0:
-            raise ValueError("scaled_inv_freq: factor must be at least 1")
+        given = {k: v for k, v in scaling.items() if v is not None}
+        unknown = sorted(set(given) - _COMMON_KEYS - _SCALING_KEYS[kind])
+        if unknown:
+            raise ValueError(f"scaled_inv_freq: {kind} does not take {', '.join(unknown)}")
+        if float(given.get("rope_theta", theta)) != float(theta):
+            raise ValueError(f"scaled_inv_freq: theta {theta} is not the scaling's rope_theta {given['rope_theta']}")
+
+        def need(key):
+            if key not in given:
+                raise ValueError(f"scaled_inv_freq: {kind} needs {key}")
+            return float(given[key])
+
+        s = float(given.get("factor", 1.0)) if kind == "default" else need("factor")
+        if not 1.0 <= s < np.inf or (kind == "default" and s != 1.0):
+            raise ValueError("scaled_inv_freq: factor must be finite and at least 1, of default 1")
         if kind == "linear":
             f = f / s
         elif kind == "ntk":
             if d < 4:
                 raise ValueError("scaled_inv_freq: ntk needs a rotary_dim of at least 4")
             f = 1.0 / ((float(theta) * s ** (d / (d - 2))) ** (i / d))
-        else:
-            ctx = float(scaling["original_max_position_embeddings"])
+        elif kind != "default":
+            ctx = need("original_max_position_embeddings")
+            if not 0 < ctx < np.inf:
+                raise ValueError("scaled_inv_freq: original_max_position_embeddings must be positive")
             turns = ctx * f / (2.0 * np.pi)  # whole turns of each pair over the trained context
             if kind == "llama3":
-                lo, hi = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+                lo, hi = need("low_freq_factor"), need("high_freq_factor")
                 if not hi > lo > 0:
                     raise ValueError("scaled_inv_freq: llama3 needs high_freq_factor > low_freq_factor > 0")
                 keep = np.clip((turns - lo) / (hi - lo), 0.0, 1.0)
             else:
-                fast, slow = float(scaling.get("beta_fast", 32)), float(scaling.get("beta_slow", 1))
+                fast, slow = float(given.get("beta_fast", 32)), float(given.get("beta_slow", 1))
                 if not fast > slow > 0 or not theta > 1:
                     raise ValueError("scaled_inv_freq: yarn needs beta_fast > beta_slow > 0 and theta > 1")
 
                 def dim_of(n):  # the (real-valued) pair index that makes n turns
                     return d * np.log(ctx / (n * 2.0 * np.pi)) / (2.0 * np.log(float(theta)))
 
-                lo, hi = max(np.floor(dim_of(fast)), 0.0), min(np.ceil(dim_of(slow)), d - 1.0)
+                lo, hi = dim_of(fast), dim_of(slow)
+                if given.get("truncate", True):
+                    lo, hi = np.floor(lo), np.ceil(hi)
+                lo, hi = max(lo, 0.0), min(hi, d - 1.0)
                 ramp = (np.arange(d // 2) - lo) / max(hi - lo, 1e-3)
                 keep = 1.0 - np.clip(ramp, 0.0, 1.0)
-                attention = scaling.get("attention_factor")
-                attention = 0.1 * np.log(s) + 1.0 if attention is None else float(attention)
+                attention = _yarn_attention(given, s)
             f = f * keep + (f / s) * (1.0 - keep)
     return torch.from_numpy(f.astype(np.float32)).to(device), float(attention)
 

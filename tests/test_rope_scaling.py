@@ -82,6 +82,75 @@ def test_scaling_refusals(theta, d, cfg):
         rope.scaled_inv_freq(theta, d, cfg)
 
 
+def yarn(theta, d, s, L, lo, hi):
+    """YaRN's frequencies with the correction range [lo, hi] given."""
+    out = []
+    for i, x in enumerate(native(theta, d)):
+        r = min(max((i - lo) / (hi - lo), 0.0), 1.0)
+        out.append(x / s * r + x * (1 - r))
+    return out
+
+
+def test_yarn_correction_range_that_is_not_rounded():
+    L, s, d, theta = 4096, 32.0, 64, 150000.0
+    cfg = {"rope_type": "yarn", "factor": s, "original_max_position_embeddings": L, "beta_fast": 32.0,
+           "beta_slow": 1.0}
+    lo, hi = (d * math.log(L / (n * 2 * math.pi)) / (2 * math.log(theta)) for n in (32, 1))
+    assert lo != math.floor(lo) and hi != math.ceil(hi) and 0 < lo < hi < d - 1
+    close(rope.scaled_inv_freq(theta, d, {**cfg, "truncate": False})[0], yarn(theta, d, s, L, lo, hi))
+    rounded = yarn(theta, d, s, L, math.floor(lo), math.ceil(hi))
+    for extra in ({}, {"truncate": True}, {"truncate": None}):
+        close(rope.scaled_inv_freq(theta, d, {**cfg, **extra})[0], rounded)
+
+
+@pytest.mark.parametrize("s", [1.0, 4.0, 40.0])
+def test_yarn_attention_factor_of_mscale(s):
+    cfg = {"rope_type": "yarn", "factor": s, "original_max_position_embeddings": 4096}
+
+    def got(**extra):
+        return rope.scaled_inv_freq(10000.0, 64, {**cfg, **extra})[1]
+
+    def scale(m):
+        return 0.1 * m * math.log(s) + 1.0
+
+    assert got(mscale=1.0, mscale_all_dim=1.0) == 1.0
+    assert got(mscale=0.707, mscale_all_dim=0.707) == 1.0
+    assert got(mscale=1.0, mscale_all_dim=0.5) == pytest.approx(scale(1.0) / scale(0.5), abs=1e-15)
+    assert got(mscale=0.707, mscale_all_dim=1.0) == pytest.approx(scale(0.707) / scale(1.0), abs=1e-15)
+    assert got() == got(mscale=1.0) == got(mscale=1.0, mscale_all_dim=0) == pytest.approx(scale(1.0), abs=1e-15)
+    assert got(mscale=1.0, mscale_all_dim=0.5, attention_factor=1.25) == 1.25
+    for alone in (dict(mscale=0.707), dict(mscale_all_dim=0.5), dict(mscale=0.707, mscale_all_dim=0.0)):
+        with pytest.raises(ValueError, match="together"):
+            got(**alone)
+
+
+def test_default_is_native():
+    want = rope.scaled_inv_freq(10000.0, 64)
+    for cfg in ({"rope_type": "default"}, {"type": "default"}, {"rope_type": None, "type": "default"},
+                {"rope_type": "default", "rope_theta": 10000, "partial_rotary_factor": 0.5, "factor": None}):
+        f, c = rope.scaled_inv_freq(10000.0, 64, cfg)
+        assert torch.equal(f, want[0]) and c == 1.0
+
+
+@pytest.mark.parametrize("cfg,word", [
+    ({"rope_type": "linear"}, "factor"), ({"rope_type": "linear", "factor": float("inf")}, "factor"),
+    ({"rope_type": "default", "factor": 4.0}, "factor"), ({}, "rope_type"),
+    ({"rope_type": "yarn", "factor": 4.0}, "original_max_position_embeddings"),
+    ({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 0}, "original_max_position_embeddings"),
+    ({"rope_type": "llama3", "factor": 4.0, "low_freq_factor": 1, "high_freq_factor": 4},
+     "original_max_position_embeddings"),
+    ({"rope_type": "llama3", "factor": 4.0, "original_max_position_embeddings": 8192, "high_freq_factor": 4},
+     "low_freq_factor"),
+    ({"rope_type": "linear", "factor": 2.0, "alpha": 3.0}, "alpha"),
+    ({"rope_type": "linear", "factor": 2.0, "attention_factor": 1.1}, "attention_factor"),
+    ({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "attn_factor": 0.9}, "attn_factor"),
+    ({"rope_type": "default", "mrope_section": [16, 24, 24]}, "mrope_section"),
+    ({"rope_type": "linear", "factor": 2.0, "rope_theta": 500000.0}, "rope_theta")])
+def test_keys_that_are_missing_or_not_handled_are_refused(cfg, word):
+    with pytest.raises(ValueError, match=word):
+        rope.scaled_inv_freq(10000.0, 64, cfg)
+
+
 def test_table_carries_the_factor():
     f = rope.default_inv_freq(10000.0, 16)
     plain, scaled = rope.rope_table(f, 64, "cpu"), rope.rope_table(f, 64, "cpu", factor=1.25)
