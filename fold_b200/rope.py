@@ -174,7 +174,11 @@ def rope_table(inv_freq: torch.Tensor, rows: int, device, factor: float = 1.0) -
     """Shared device table with at least `rows` rows for these frequencies and this attention
     factor (scaled_inv_freq)."""
     device = torch.device(device)
-    key = (np.asarray(inv_freq.detach().cpu(), dtype=np.float32).tobytes(), str(device), float(factor))
+    if device.type == "cuda" and device.index is None:  # one table a device, whichever is current
+        device = torch.device("cuda", torch.cuda.current_device())
+    # the frequencies as the table is computed from them: float64 ones and their float32 rounding
+    # lie 4e-3 rad apart at position 131072
+    key = (np.asarray(inv_freq.detach().cpu(), dtype=np.float64).tobytes(), str(device), float(factor))
     with _tables_lock:
         t = _tables.get(key)
         if t is None or t.shape[0] < rows:

@@ -162,6 +162,39 @@ def test_table_carries_the_factor():
     assert np.abs(scaled.numpy()[:64] - 1.25 * want).max() <= 2 * F32
 
 
+@pytest.mark.parametrize("first", [torch.float32, torch.float64])
+def test_tables_of_float64_frequencies_and_of_their_rounding_are_apart(first):
+    f = torch.tensor([1.0, 10.0 ** -0.125, 10.0 ** -0.75 + (first is torch.float64) * 0.01], dtype=torch.float64)
+    both = [f.to(first), f.to(torch.float64 if first is torch.float32 else torch.float32)]
+    for x in both:  # in either order
+        t = rope.rope_table(x, 131073, "cpu")
+        ang = 131072.0 * x.double().numpy()
+        want = np.concatenate([np.cos(ang), np.sin(ang)])
+        # the angle rounds in float64 (2^-53 of 1.3e5), the entry to float32
+        assert np.abs(t[131072].numpy() - want).max() <= F32 + 2.0 ** -34
+    assert rope.rope_table(both[0], 100, "cpu") is not rope.rope_table(both[1], 100, "cpu")
+
+
+def test_table_of_a_device_without_index_follows_the_current_one(monkeypatch):
+    current, moved = [0], []
+
+    def to(self, device):
+        moved.append(torch.device(device))
+        return self.clone()
+
+    monkeypatch.setattr(torch.Tensor, "to", to)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(rope, "_tables", {})
+    f = rope.default_inv_freq(10000.0, 8)
+    moved.clear()
+    a = rope.rope_table(f, 16, "cuda")
+    current[0] = 1
+    b = rope.rope_table(f, 16, "cuda")
+    assert moved == [torch.device("cuda:0"), torch.device("cuda:1")] and a is not b
+    assert rope.rope_table(f, 16, "cuda:0") is a and rope.rope_table(f, 16, torch.device("cuda", 1)) is b
+    assert rope.rope_table(f, 16, "cuda") is b
+
+
 def call_rotary(**kw):
     a = dict(q=16, hq=2, k=16, hk=1, pos=16, table=16, rows=8, rot=16, n=3, hd=32, dtype=0)
     a.update(kw)
