@@ -177,6 +177,7 @@ def test_tables_of_float64_frequencies_and_of_their_rounding_are_apart(first):
 
 def test_table_of_a_device_without_index_follows_the_current_one(monkeypatch):
     current, moved = [0], []
+    f = rope.default_inv_freq(10000.0, 8)
 
     def to(self, device):
         moved.append(torch.device(device))
@@ -185,8 +186,6 @@ def test_table_of_a_device_without_index_follows_the_current_one(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "to", to)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
     monkeypatch.setattr(rope, "_tables", {})
-    f = rope.default_inv_freq(10000.0, 8)
-    moved.clear()
     a = rope.rope_table(f, 16, "cuda")
     current[0] = 1
     b = rope.rope_table(f, 16, "cuda")
