@@ -1425,6 +1425,9 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixParams p,
 }
 
 // ---------------------------------------------------------------- host
+// The places of a workspace, counted from its first 32-byte boundary: partials are stored 32 bytes at a
+// time (store8), callers give 16-byte boundaries.
+constexpr int kBaseAlign = 32;
 struct Layout {
   int64_t plan, o_prim, lse_prim, o_cont, lse_cont, bytes;
 };
@@ -1437,7 +1440,7 @@ Layout layout(int64_t n, int hq, int hkv, int hd, int ctas) {
   w.lse_prim = w.o_prim + up(2 * n * hq * hd * 4);
   w.o_cont = w.lse_prim + up(2 * n * hq * 4);
   w.lse_cont = w.o_cont + up(ctas * rows * hd * 4);
-  w.bytes = w.lse_cont + up(ctas * rows * 4);
+  w.bytes = w.lse_cont + up(ctas * rows * 4) + kBaseAlign - 16;
   return w;
 }
 
@@ -1602,7 +1605,7 @@ int fold_prefix_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   p.out = out, p.o_st = o_stride_tok, p.o_sh = o_stride_head, p.lse = lse;
   p.n = n, p.hq = hq, p.hkv = hkv, p.group = hq / hkv, p.half_toks = 128 / p.group;
   p.item_cost = hd == 256 ? kItemCost256 : kItemCost, p.ctas = ctas, p.err = err;
-  char* ws = static_cast<char*>(workspace);
+  char* ws = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(workspace) + kBaseAlign - 1) & ~uintptr_t(kBaseAlign - 1));
   p.plan = reinterpret_cast<int4*>(ws + w.plan);
   p.o_prim = reinterpret_cast<float*>(ws + w.o_prim), p.lse_prim = reinterpret_cast<float*>(ws + w.lse_prim);
   p.o_cont = reinterpret_cast<float*>(ws + w.o_cont), p.lse_cont = reinterpret_cast<float*>(ws + w.lse_cont);

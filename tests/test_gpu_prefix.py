@@ -189,6 +189,22 @@ def test_blocks_past_32_bits():
     c.check()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_workspace_on_any_16_byte_boundary(hd):
+    """A workspace cut out of a larger buffer, at every 16-byte boundary of a sector, for segments of
+    few and of many rows; nothing beside it is written."""
+    c = Case([1, 30, 3], [70, 300, 3], 500, 8, 2, hd, 16, seed=hd)
+    want, wl = c.check()
+    size = kernels.prefix_workspace(34, 8, 2, hd, "cuda").numel()
+    arena = torch.empty(size + 256, device="cuda", dtype=torch.uint8)
+    assert arena.data_ptr() % 32 == 0
+    for at in (0, 16, 32, 48, 112):
+        arena.fill_(171)
+        out, lse = c.read(workspace=arena[at:at + size])
+        assert torch.equal(out, want) and torch.equal(lse, wl)
+        assert bool((arena[:at] == 171).all()) and bool((arena[at + size:] == 171).all())
+
+
 def test_rows_that_see_nothing():
     c = Case([2, 1, 3], [0, 0, 1], 0, 4, 2, 128, 16)
     out, lse = c.check()
