@@ -96,12 +96,12 @@ __device__ __forceinline__ void load_floats(const float* p, float* v) {
   }
 }
 
-// The table row of token t (a position outside the table is clamped and reported).
-__device__ __forceinline__ const float* table_row(const RopeParams& p, int t) {
+// The table row of token t (a position outside the table is clamped and, where asked, reported).
+__device__ __forceinline__ const float* table_row(const RopeParams& p, int t, bool report) {
   if (!p.table) return nullptr;
   int64_t pos = __ldg(p.positions + t);
   if (pos < 0 || pos >= p.table_rows) {
-    set_error(p.err, FOLD_DEVERR_ROPE_RANGE);
+    if (report) set_error(p.err, FOLD_DEVERR_ROPE_RANGE);
     pos = pos < 0 ? 0 : p.table_rows - 1;
   }
   return p.table + pos * p.rot;
@@ -163,12 +163,13 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_kernel(const RopeParams 
 
     Chunk<T, W> x[HU], y[HU];
     T* dst[HU];
-    bool live[HU];
+    bool live[HU], any = false;  // any: a head of these is turned and written
 #pragma unroll
     for (int j = 0; j < HU; ++j) {
       const T* src = nullptr;
       const int hh = g * HU + j;
       live[j] = hh < heads && locate<T>(p, t, hh, src, dst[j]);
+      any |= live[j] && hh < rotated;
       if (live[j]) {
         x[j].raw = *reinterpret_cast<const word*>(src + a);
         y[j].raw = *reinterpret_cast<const word*>(src + b);
@@ -176,7 +177,8 @@ __global__ void __launch_bounds__(kRopeThreads, 8) rope_kernel(const RopeParams 
     }
     float cs[E], sn[E];
     if (turn && g * HU < rotated) {
-      const float* row = table_row(p, t);
+      // the row is fetched beside the slot, whatever that says; a skipped token's position is no error
+      const float* row = table_row(p, t, any);
       load_floats<E>(row + c * E, cs);
       load_floats<E>(row + (p.rot >> 1) + c * E, sn);
 #pragma unroll
@@ -232,7 +234,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_scalar_kernel(const RopePar
       for (int i = lane; i < p.hd; i += 32) dst[i] = src[i];
       continue;
     }
-    const float* tr = table_row(p, t);
+    const float* tr = table_row(p, t, true);
     for (int c = lane; c < half; c += 32) {
       const int a = INTER ? 2 * c : c, b = INTER ? 2 * c + 1 : c + half;
       const float lo = to_f32(src[a]), hi = to_f32(src[b]), cs = __ldg(tr + c), sn = p.sgn * __ldg(tr + half + c);

@@ -186,6 +186,33 @@ def test_append_paged_without_rotation_and_out_of_range():
     assert torch.equal(kv, want)
 
 
+@pytest.mark.parametrize("n,hq,hkv,hd,rot", [
+    (4, 0, 2, 128, 128), (4, 0, 1, 64, 32), (4, 0, 2, 80, 36), (4, 0, 2, 64, 30), (3000, 0, 8, 128, 128),
+    (4, 3, 2, 128, 128), (3000, 3, 2, 64, 64), (4, 3, 2, 64, 30)])
+def test_positions_of_skipped_tokens(n, hq, hkv, hd, rot):
+    """A skipped token's position matters to its query alone: padding rows may hold any position, in
+    kernels of wide units (one head a thread, and two) and of a warp a row."""
+    x = inputs(n, hq + 2 * hkv, hd, torch.bfloat16, n)
+    q, k, v = x[:, :hq] if hq else None, x[:, hq:hq + hkv], x[:, hq + hkv:]
+    f = rope.default_inv_freq(10000.0, rot)
+    table = rope.rope_table(f, 50, "cuda")[:50]
+    kv, kc, vc = cache(-(-n // 16), hkv, 16, hd, torch.bfloat16, "heads_first")
+    slots = torch.arange(n, device="cuda")
+    slots[1::2] = -1
+    pos = torch.arange(n, device="cuda") % 50
+    good = pos.clone()
+    pos[1::4], pos[3::4], good[1::4], good[3::4] = -1, 50, 0, 49  # as they are clamped
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    want = kv.clone()
+    qw = kernels.append_paged(k, v, good, slots, want[..., :hd], want[..., hd:], table, q=q, err=err)
+    assert int(err) == 0
+    qo = kernels.append_paged(k, v, pos, slots, kc, vc, table, q=q, err=err)
+    assert int(err) == (DEVERR_ROPE_RANGE if hq else 0)
+    assert torch.equal(kv, want)
+    if hq:
+        assert torch.equal(qo, qw)
+
+
 def test_append_paged_offsets_past_32_bits():
     """A cache whose last slots lie past 2^32 elements."""
     nb, hkv, bs, hd = 33000, 8, 64, 128  # 4.3e9 elements, 8.7 GB
