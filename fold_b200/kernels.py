@@ -367,7 +367,11 @@ def _rotary_out(what, x, out):
     xs = x.stride()
     if out is None and xs[2] == 1:
         out = torch.empty_like(x)
-        return x, xs, out, out.stride()
+        os = out.stride()
+        if os[2] != 1:  # rows of x that overlap at a stride of one element: empty_like orders the dims anew
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            os = out.stride()
+        return x, xs, out, os
     if xs[2] != 1 and x.shape[2] > 1:
         if out is x:
             raise FoldError(f"{what}: the head dimension must be contiguous")

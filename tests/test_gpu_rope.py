@@ -94,6 +94,16 @@ def test_rotary_in_place_and_strided(interleaved):
     assert torch.equal(rest, big)
 
 
+@pytest.mark.parametrize("stride", [(128, 1, 1), (1, 1, 1), (0, 128, 1), (256, 0, 1)])
+def test_rotary_of_rows_that_share_memory(stride):
+    table = rope.rope_table(rope.default_inv_freq(10000.0, 128), 300, "cuda")
+    x = inputs(200, 2, 128, torch.bfloat16, 6).as_strided((200, 2, 128), stride)
+    pos = torch.arange(200, device="cuda")
+    got = kernels.rotary(x, x, pos, table)
+    want, _ = kernels.rotary(x.contiguous(), None, pos, table)
+    assert torch.equal(got[0], want) and torch.equal(got[1], want)
+
+
 def test_rotary_inverse_is_the_gradient():
     """The inverse call against differences of a weighted sum of the outputs, and against the
     transpose of the formula."""

@@ -235,6 +235,20 @@ def test_append_of_nothing_is_a_no_op():
     call_append(n=0)
 
 
+@pytest.mark.parametrize("size,stride", [
+    ((200, 2, 128), (128, 1, 1)), ((5, 3, 16), (1, 1, 1)), ((7, 4, 8), (1, 7, 1)), ((4, 2, 8), (0, 0, 1)),
+    ((4, 6, 32), (0, 32, 1)), ((4, 6, 32), (192, 0, 1)), ((4, 6, 32), (32, 128, 1)), ((4, 6, 32), (192, 32, 1)),
+    ((1, 1, 32), (1, 1, 1)), ((3, 2, 8), (16, 1, 2)), ((6, 1, 8), (8, 1, 1)), ((1, 6, 8), (1, 1, 1))])
+def test_a_new_output_has_rows_of_its_own(size, stride):
+    """Whatever the strides of the input: each row of the output is contiguous and no two share memory."""
+    x = torch.zeros(40000).as_strided(size, stride)
+    got, xs, out, os = kernels._rotary_out("rotary", x, None)
+    assert torch.equal(got, x) and xs == got.stride() and xs[2] == 1
+    assert out.shape == x.shape and os == out.stride() and os[2] == 1
+    places = torch.arange(out.untyped_storage().nbytes() // 4).as_strided(size, os, out.storage_offset())
+    assert places.unique().numel() == places.numel()
+
+
 def test_wrappers_take_cuda_tensors_only():
     x = torch.zeros(2, 1, 32)
     t = rope.rope_table(rope.default_inv_freq(1e4, 32), 8, "cpu")
