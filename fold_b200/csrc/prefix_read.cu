@@ -1552,7 +1552,8 @@ int fold_prefix_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   if (!q || !qsl || !own_lens || !prefix_len || !k_cache || !v_cache || (prefix_table_len && !prefix_table) ||
       (block_tables_len && !block_tables) || !out)  // a table of no blocks may be null
     return fail(FOLD_ERR_INVALID_ARGUMENT, "prefix read: null pointer");
-  if ((n > 1 && o_stride_tok == 0) || (hq > 1 && o_stride_head == 0))
+  auto overlap = [&](int64_t stride) { return stride < hd && stride > -hd; };  // of rows that are neighbours
+  if ((n > 1 && overlap(o_stride_tok)) || (hq > 1 && overlap(o_stride_head)))
     return fail(FOLD_ERR_INVALID_ARGUMENT, "prefix read: the rows of out must not share memory");
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || q_stride_tok % 8 ||
       q_stride_head % 8 || o_stride_tok % 8 || o_stride_head % 8 || cache_stride_block % 8 || cache_stride_head % 8 ||

@@ -20,6 +20,9 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <initializer_list>
+#include <utility>
+
 #include "common.cuh"
 #include "host_common.h"
 
@@ -322,6 +325,14 @@ int check_rope(const float* table, int64_t table_rows, int rot_dim, int n, int h
   return FOLD_OK;
 }
 
+// Whether rows of hd elements at these strides (of dims of `size` each) cannot be told apart in memory:
+// two neighbours of some dim overlap.
+bool neighbours_overlap(int hd, std::initializer_list<std::pair<int64_t, int64_t>> dims) {
+  for (const auto& [size, stride] : dims)
+    if (size > 1 && stride < hd && stride > -hd) return true;
+  return false;
+}
+
 }  // namespace
 }  // namespace fold
 
@@ -338,6 +349,9 @@ int fold_rotary(const void* q, int64_t q_stride_tok, int64_t q_stride_head, void
   if (n == 0 || hq + hk == 0) return FOLD_OK;
   if (!positions || !rope_table || (hq && (!q || !q_out)) || (hk && (!k || !k_out)))
     return fail(FOLD_ERR_INVALID_ARGUMENT, "rotary: null pointer");
+  if ((hq && neighbours_overlap(hd, {{n, qo_stride_tok}, {hq, qo_stride_head}})) ||
+      (hk && neighbours_overlap(hd, {{n, ko_stride_tok}, {hk, ko_stride_head}})))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "rotary: the rows of an output must not share memory");
   RopeParams p{};
   p.q = RopeRows{q, q_out, q_stride_tok, q_stride_head, qo_stride_tok, qo_stride_head, hq};
   p.k = RopeRows{k, k_out, k_stride_tok, k_stride_head, ko_stride_tok, ko_stride_head, hk};
@@ -364,6 +378,13 @@ int fold_append_paged(const void* k, int64_t k_stride_tok, int64_t k_stride_head
   if (!k || !v || !slots || !k_cache || !v_cache || (rope_table && !positions) || (hq && (!q || !q_out)))
     return fail(FOLD_ERR_INVALID_ARGUMENT, "paged append: null pointer");
   if (hq && !rope_table) return fail(FOLD_ERR_INVALID_ARGUMENT, "paged append: queries are given only to be rotated");
+  if (hq && neighbours_overlap(hd, {{n, qo_stride_tok}, {hq, qo_stride_head}}))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "paged append: the rows of an output must not share memory");
+  const int64_t apart = static_cast<const char*>(v_cache) - static_cast<const char*>(k_cache);
+  const int64_t row_bytes = static_cast<int64_t>(hd) * (dtype == FOLD_FP32 ? 4 : 2);
+  if (neighbours_overlap(hd, {{num_blocks, cache_stride_block}, {hkv, cache_stride_head}, {block_size, cache_stride_slot}}) ||
+      (apart < row_bytes && apart > -row_bytes))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "paged append: the slots of the cache's planes must not share memory");
   RopeParams p{};
   p.q = RopeRows{q, q_out, q_stride_tok, q_stride_head, qo_stride_tok, qo_stride_head, hq};
   p.k = RopeRows{k, k_cache, k_stride_tok, k_stride_head, 0, 0, hkv};

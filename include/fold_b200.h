@@ -105,9 +105,9 @@ int fold_far_query(const void* q, int64_t q_stride_tok, int64_t q_stride_head, v
  * the gradient of the inputs. rope_table: float32 [table_rows, rot_dim], row p holding
  * c cos(p f_i) then c sin(p f_i), c the attention factor of scaled frequencies (1 otherwise); a
  * position outside [0, table_rows) is clamped and sets FOLD_DEVERR_ROPE_RANGE. An output may be its
- * input; any other overlap of inputs and outputs is not allowed. Rows are read 16, 8 or 4 bytes at a
- * time, the most that half of rot_dim, hd / 2, the row starts and strides are whole multiples of,
- * else element by element. hd at most 8192. */
+ * input; any other overlap of inputs and outputs, or of an output's rows, is not allowed. Rows are
+ * read 16, 8 or 4 bytes at a time, the most that half of rot_dim, hd / 2, the row starts and strides
+ * are whole multiples of, else element by element. hd at most 8192. */
 int fold_rotary(const void* q, int64_t q_stride_tok, int64_t q_stride_head, void* q_out, int64_t qo_stride_tok,
                 int64_t qo_stride_head, int hq, const void* k, int64_t k_stride_tok, int64_t k_stride_head,
                 void* k_out, int64_t ko_stride_tok, int64_t ko_stride_head, int hk, const int64_t* positions,
@@ -118,9 +118,9 @@ int fold_rotary(const void* q, int64_t q_stride_tok, int64_t q_stride_head, void
  * cache update behind it (fold/attention.py:245-246,256) by one launch. k, v [n, hkv, hd] of type
  * `dtype`; token i goes to slot slots[i] = block * block_size + offset of the planes k_cache and
  * v_cache ([num_blocks, hkv, block_size, hd], same type, given strides in elements, innermost dim
- * contiguous, both planes share them), k rotated as by fold_rotary, v as it is. A token with a
- * negative slot is skipped; one at or past num_blocks * block_size is skipped and sets
- * FOLD_DEVERR_APPEND_RANGE. The non-negative slots of one call are distinct (of two tokens with
+ * contiguous, both planes share them, no two slots share memory), k rotated as by fold_rotary, v as
+ * it is. A token with a negative slot is skipped (its position then matters to its query alone); one
+ * at or past num_blocks * block_size is skipped and sets FOLD_DEVERR_APPEND_RANGE. The non-negative slots of one call are distinct (of two tokens with
  * one slot, which one's 16-byte pieces remain is not defined). rope_table NULL: keys are stored as
  * they are, positions are not read. With hq > 0 the queries q [n, hq, hd] of the same tokens are
  * rotated into q_out too (whatever their slots), in the same launch; q_out may be q. */

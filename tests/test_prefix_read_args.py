@@ -28,6 +28,12 @@ def test_refusals(bad):
         call(**bad)
 
 
+@pytest.mark.parametrize("strides", [(0, 128), (512, 0), (512, 120), (64, 128), (512, -8)])
+def test_output_rows_that_share_memory_are_refused(strides):
+    with pytest.raises(FoldError, match="share memory"):
+        call(os=strides)
+
+
 def test_of_nothing_is_a_no_op():
     call(n=0)
     call(b=0)

@@ -231,6 +231,28 @@ def test_append_refusals(bad):
         call_append(**bad)
 
 
+def append_strides(kc=64, vc=4096, nb=2, bs=16, cs=(512, 512, 32), hkv=1, hd=32, dtype=0, qo=(64, 32), hq=0):
+    _lib.call("fold_append_paged", 16, 32, 32, 16, 32, 32, 16, 16, 3, kc, vc, nb, bs, *cs, 16, 8, 16, hkv, hd, dtype, 0,
+              16, 64, 32, 16, *qo, hq, None, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(cs=(0, 512, 32)), dict(cs=(512, 0, 32), hkv=2), dict(cs=(512, 512, 0)), dict(cs=(31, 512, 32)),
+    dict(cs=(1024, 512, 16), hkv=2), dict(cs=(-16, 512, 32)), dict(vc=64), dict(vc=64 + 62), dict(vc=64 - 62),
+    dict(vc=64 + 126, dtype=2), dict(hq=2, qo=(64, 0)), dict(hq=2, qo=(1, 32))])
+def test_append_refuses_slots_and_rows_that_share_memory(bad):
+    with pytest.raises(FoldError, match="share memory"):
+        append_strides(**bad)
+
+
+@pytest.mark.parametrize("which", ["q", "k"])
+@pytest.mark.parametrize("strides", [(0, 32), (64, 0), (64, 31), (1, 32), (64, -8)])
+def test_rotary_refuses_output_rows_that_share_memory(which, strides):
+    a, b = (strides, (64, 32)) if which == "q" else ((64, 32), strides)
+    with pytest.raises(FoldError, match="share memory"):
+        _lib.call("fold_rotary", 16, 64, 32, 16, *a, 2, 16, 64, 32, 16, *b, 2, 16, 16, 8, 16, 3, 32, 0, 0, 0, None, None)
+
+
 def test_append_of_nothing_is_a_no_op():
     call_append(n=0)
 
