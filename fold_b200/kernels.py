@@ -353,6 +353,8 @@ def _check_table(what, table, d):
 
 
 def _check_index(what, name, t, n):
+    if t is None:
+        raise FoldError(f"{what}: {name} are needed")
     if t.dtype is torch.int64 and t.is_contiguous() and t.shape == (n,):
         return t
     if t.shape != (n,):

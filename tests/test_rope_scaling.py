@@ -271,6 +271,19 @@ def test_a_new_output_has_rows_of_its_own(size, stride):
     assert places.unique().numel() == places.numel()
 
 
+def test_positions_that_are_missing_are_refused(monkeypatch):
+    """A rotation without positions is an argument error (the check of the device is put aside)."""
+    monkeypatch.setattr(kernels, "_check_devices", lambda *a: 0)
+    x, kv, i = torch.zeros(2, 1, 32), torch.zeros(1, 1, 16, 64), torch.zeros(2, dtype=torch.int64)
+    t = rope.rope_table(rope.default_inv_freq(1e4, 32), 8, "cpu")
+    with pytest.raises(FoldError, match="positions"):
+        kernels.rotary(x, None, None, t)
+    with pytest.raises(FoldError, match="positions"):
+        kernels.append_paged(x, x, None, i, kv[..., :32], kv[..., 32:], t)
+    with pytest.raises(FoldError, match="slots"):
+        kernels.append_paged(x, x, i, None, kv[..., :32], kv[..., 32:], t)
+
+
 def test_wrappers_take_cuda_tensors_only():
     x = torch.zeros(2, 1, 32)
     t = rope.rope_table(rope.default_inv_freq(1e4, 32), 8, "cpu")
