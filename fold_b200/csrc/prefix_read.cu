@@ -1207,6 +1207,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         }
       }
       if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+      // copies in flight land before exit (a read that gives up may leave the last tiles unread)
+      for (uint32_t w = qu > QB ? qu - QB : 0; w < qu; ++w) warp_wait(&B.q_full[w % QB], (w / QB) & 1);
     } else if (warp == NSW + 2) {
       // ------------------------------------------------------------ scheduler
       int sg = 0;
