@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import argparse
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -27,6 +28,20 @@ NVCC_FLAGS = [
     "--expt-relaxed-constexpr",
     "-cudart", "static",
 ]
+
+# Registers a thread that kernels must be built with, by source and a pattern of their (mangled)
+# names: the shares that setmaxnreg deals out add up to what a block is launched with, and a block
+# that asks for more waits for good.
+REGISTERS = {"prefix_read": [(r"prefix_read_kernelI.*CfgILi(64|128)E", 168)]}
+
+
+def check_registers(source: str, log: str) -> None:
+    """Raises RuntimeError unless ptxas's report (-Xptxas -v) of `source` shows REGISTERS' counts."""
+    used = re.findall(r"Compiling entry function '(\w+)'.*?Used (\d+) registers", log, re.S)
+    for pattern, want in REGISTERS.get(source, []):
+        found = [int(n) for name, n in used if re.search(pattern, name)]
+        if not found or any(n != want for n in found):
+            raise RuntimeError(f"{source}: kernels {pattern} use {found or 'unknown'} registers, must use {want}")
 
 
 def nvcc() -> str:
@@ -60,8 +75,8 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     out_dir.mkdir(exist_ok=True)
     objs = []
     procs = []
-    extra = ["-Xptxas", "-v"] if ptxas_verbose else []
     for src in sources():
+        extra = ["-Xptxas", "-v"] if ptxas_verbose or src.stem in REGISTERS else []
         obj = out_dir / (src.stem + ".o")
         cmd = [nvcc(), *NVCC_FLAGS, *extra, "-I", str(INCLUDE), "-c", str(src), "-o", str(obj)]
         if verbose:
@@ -75,6 +90,8 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
             print(out, file=sys.stderr)
         if p.returncode:
             failed.append(src.name)
+        else:
+            check_registers(src.stem, out)
     if failed:
         raise RuntimeError(f"nvcc failed for {failed}")
     tmp = LIB.with_suffix(".so.tmp")

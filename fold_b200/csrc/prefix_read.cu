@@ -154,6 +154,11 @@ struct Seg {
 };
 constexpr int kSegs = 4;
 
+// Registers a thread of a block with two softmax warpgroups: at launch (384 threads; the build checks
+// it), then of the softmax warps and of the others.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "a share that is not there is waited for");
+
 // The line may be cut where the few rows begin if either side has this many CTAs.
 constexpr int kCutCtas = 16;
 // No piece is shorter, nor, by a rounded number of CTAs on a side of that cut, shorter than the
@@ -755,10 +760,10 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     return true;
   };
 
-  // With two softmax warpgroups the launch's registers (168 a thread) are dealt out again: a softmax
-  // thread holds a row of S (128 values). 2 * 208 + 88 = 3 * 168.
+  // With two softmax warpgroups the launch's registers are dealt out again: a softmax thread holds a row
+  // of S (128 values).
   if (warp < NSW) {
-    if constexpr (NWG == 2) regs_up<208>();
+    if constexpr (NWG == 2) regs_up<kSoftmaxRegs>();
     // ------------------------------------------------------------ softmax warps
     const int wg = warp >> 2, row = (warp & 3) * 32 + lane;  // row of the slot = TMEM lane
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -977,7 +982,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     }
     if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
   } else {
-    if constexpr (NWG == 2) regs_down<88>();
+    if constexpr (NWG == 2) regs_down<kOtherRegs>();
     if (warp == NSW) {
       // ------------------------------------------------------------ TMA producer
       const int nch = TK / p.chunk;
@@ -1510,7 +1515,7 @@ int launch_prefix(const PrefixParams& p, const void* k, const void* v, int64_t s
       cudaFuncAttributes a{};
       return cudaFuncGetAttributes(&a, prefix_read_kernel<C>) == cudaSuccess ? a.numRegs : 0;
     }();
-    if (regs != 168) return fail(FOLD_ERR_UNSUPPORTED, "prefix read: built with other register shares than launched");
+    if (regs != kLaunchRegs) return fail(FOLD_ERR_UNSUPPORTED, "prefix read: built with other register shares than launched");
   }
   if (int s = launch_behind(prefix_read_kernel<C>, dim3(p.ctas), C::NTHREADS, C::SMEM, stream, "prefix_read_kernel",
                             qmap, kmap, vmap, p))
