@@ -1521,9 +1521,10 @@ int launch_prefix(const PrefixParams& p, const void* k, const void* v, int64_t s
                             qmap, kmap, vmap, p))
     return s;
   const int64_t rows = static_cast<int64_t>(p.n) * p.hq;
-  // few rows have many partials each: four warps a row at 64 rows over 16K keys (27 us the whole call,
-  // one warp 31), 768 rows over 128K (101 against 105); one warp from 2048 rows on (62 against 64)
-  if (rows <= 1024)
+  // few rows have many partials each, which four warps share: with four and with one warp a row the whole
+  // call took 31.1 and 34.3 us at 256 rows over 16K keys, 68.5 and 71.5 at 1024 over 64K, 89.0 and 92.2 at
+  // 1152 over 64K, 43.1 and 43.8 at 1536 over 16K, 46.6 and 46.0 at 2048, 71.9 and 66.2 at 4096
+  if (rows <= 1536)
     return launch_behind(prefix_merge_kernel<HD, T, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, stream,
                          "prefix_merge_kernel", p, C::ROWS);
   return launch_behind(prefix_merge_kernel<HD, T, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream,
