@@ -33,12 +33,18 @@
 // Rounding. Logits, maxima, sums, O and the partials are float32; P is rounded once to the type of
 // V (the MMA takes operands of one type), the sums are of the unrounded P, the result is rounded
 // once. Against 64 bits that is 0.0023 (bf16) or 0.00029 (fp16) of the outputs' norm, where rounding
-// the outputs alone is 0.0017 and 0.00021.
+// the outputs alone is 0.0017 and 0.00021. In bf16, P as a high and a low part (two MMAs a tile)
+// brings 0.0023 to 0.0017 and costs a quarter: 256 sequences over 32K keys 220 us for 174, 64 over 16K
+// 71 for 58, prompts at head size 256 455 for 365. With value channels of eight times the size the
+// largest error is 0.0013 for 0.0007 where a row's weights lie on many of 128K keys, and that of the
+// result's own rounding (0.06) where they lie on few. So P stays one bf16; for more, keep the cache in
+// fp16.
 //
-// Measured (bf16, head size 128, 32 query and 8 KV heads, pages of 16; the whole call):
-//   256 sequences of one token, 32K shared and up to 256 own keys: 174 us (790 TFLOP/s; in the long
-//     run over the prefix 1160, 0.70 of the measured peak);
-//   3 sequences of 8 tokens, 128K shared: 106 us (5.1 TB/s, 0.78 of the measured copy rate; 6 TB/s
+// Measured (bf16, head size 128, 32 query and 8 KV heads, pages of 16; the GPU's time of a captured
+// call, the best of 15 samples of ten):
+//   256 sequences of one token, 32K shared and up to 256 own keys: 175 us (788 TFLOP/s; in the long
+//     run over the prefix 1160, 0.70 of the measured peak; 188 us at the clocks of a long run);
+//   3 sequences of 8 tokens, 128K shared: 107 us (5.0 TB/s, 0.77 of the measured copy rate; 6 TB/s
 //     behind the first 10 us);
 //   64 sequences of one token, 16K shared and up to 1024 own keys: 58 us, of which the start of the
 //     pipeline (lengths, line, first page, first tile) takes 8 and the merge 4.
@@ -139,8 +145,11 @@ struct Cfg {
 // Cost units of the line, from the CTAs' finishing times at decode, prompt and draft shapes: about
 // 0.3 us, an eighth of a key tile of a wide row tile. A tile of up to 128 rows takes 6, of few rows 4;
 // an item costs its Q, its first keys' way through the pipeline and its partial besides (at head size
-// 256, where one Q tile and one accumulator hold nothing ready, more; of few rows, where two are under
+// 256, where one Q tile and one accumulator hold nothing ready, more: prompts of 90 to 700 tokens behind
+// 8K keys took 416 us with 12, 391 with 16, 354 with 20, 364 with 24; of few rows, where two are under
 // way at a time, less: with 6 for 3 the 256 sequences over 32K keys took 184 us, with 2 183, with 3 174).
+// Head size 64 takes the same 12 as 128: drafted blocks 29.3, 29.6, 29.7, 30.3 us with 8, 12, 18, 24, those
+// prompts 259, 249, 246, 248, 96 single rows over 3000 keys 33.3, 31.4, 31.0, 31.2.
 constexpr int kWideTileCost = 8, kTileCost = 6, kFewTileCost = 4;
 constexpr int kItemCost = 12, kItemCost256 = 20, kFewItemCost = 3;
 
@@ -829,7 +838,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             l *= f, m = mn;
             if (!empty_o) {
               // the accumulator holds the products up to the slot's last tile; with one
-              // accumulator the last tile's may still be running
+              // accumulator the last tile's may still be running (those before it are complete with S
+              // of this tile, so the parity can stand for the last tile's phase only)
               if (NWG == 1) ok = warp_wait(&B.pv_done, (tile0 + j - 1) & 1);
               if (!ok) break;
               tc_fence_after();

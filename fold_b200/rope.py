@@ -172,7 +172,8 @@ _tables_lock = threading.Lock()
 
 def rope_table(inv_freq: torch.Tensor, rows: int, device, factor: float = 1.0) -> torch.Tensor:
     """Shared device table with at least `rows` rows for these frequencies and this attention
-    factor (scaled_inv_freq)."""
+    factor (scaled_inv_freq). A call that asks for more rows makes a new table: a captured graph's
+    owner keeps the one it was captured with."""
     device = torch.device(device)
     if device.type == "cuda" and device.index is None:  # one table a device, whichever is current
         device = torch.device("cuda", torch.cuda.current_device())
