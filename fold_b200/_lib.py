@@ -50,6 +50,17 @@ SIGNATURES = {
                          _i64, _i32, _i32, _f32, _vp, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp,
                          _vp],
     "fold_prefix_read_workspace": [_i32, _i32, _i32, _i32],
+    "fold_prompt_read": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _f32, _vp,
+                         _i64, _i64, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp],
+    "fold_prompt_read_grad": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+                              _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64,
+                              _i64, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _vp],
+    "fold_prompt_read_grad_workspace": [_i32, _i32, _i32, _i32],
+    "fold_grow_pages": [_vp, _i32, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp],
+    "fold_free_pages": [_vp, _i32, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i32, _i32, _vp, _vp],
+    "fold_fork_pages": [_vp, _i32, _vp, _i64, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i64,
+                        _i64, _i64, _vp, _i64, _vp, _vp],
+    "fold_fork_pages_workspace": [_i32],
     "fold_step_read": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _i64, _i64, _vp, _vp,
                        _vp, _vp, _vp, _i64, _i32, _i64, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp,
                        _i32, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _f32, _vp, _vp],
@@ -68,7 +79,8 @@ SIGNATURES = {
                                    _i32, _f32, _f32, _vp, _vp],
 }
 _RESTYPES = {"fold_status_string": ctypes.c_char_p, "fold_last_error": ctypes.c_char_p,
-             "fold_prefix_read_workspace": _i64}
+             "fold_prefix_read_workspace": _i64, "fold_prompt_read_grad_workspace": _i64,
+             "fold_fork_pages_workspace": _i64}
 
 _lock = threading.Lock()
 _lib = None
@@ -132,3 +144,7 @@ def far_read_kernel_for(hd: int, n: int, hq: int, hkv: int) -> int:
 
 def prefix_read_workspace(n: int, hq: int, hkv: int, hd: int) -> int:
     return int(load().fold_prefix_read_workspace(n, hq, hkv, hd))
+
+
+def prompt_read_grad_workspace(n: int, hq: int, hkv: int, hd: int) -> int:
+    return int(load().fold_prompt_read_grad_workspace(n, hq, hkv, hd))

@@ -11,6 +11,10 @@ DEVERR_ROPE_RANGE = 2
 DEVERR_TIMEOUT = 4
 DEVERR_CAPACITY = 8
 DEVERR_BLOCK_TABLE = 16
+DEVERR_PAGES = 32
+DEVERR_SHARED = 64
+DEVERR_ROW = 128
+DEVERR_REFS = 256
 
 DEVERR_NAMES = {
     DEVERR_APPEND_RANGE: "append/gather position outside the side cache",
@@ -18,6 +22,10 @@ DEVERR_NAMES = {
     DEVERR_TIMEOUT: "a pipeline wait of the far read gave up",
     DEVERR_CAPACITY: "far_len exceeds the side cache capacity",
     DEVERR_BLOCK_TABLE: "a window-read block-table entry outside the paged cache",
+    DEVERR_PAGES: "no free page was left for a row",
+    DEVERR_SHARED: "a row's partly filled last page is held by another row too",
+    DEVERR_ROW: "a row outside the tables, named twice, or forked to while in use",
+    DEVERR_REFS: "a page was given back that no row holds",
 }
 
 

@@ -7,6 +7,7 @@ lengths on the device (graph-capturable) and raise FoldError when the library re
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -557,6 +558,221 @@ def prefix_read(q, qsl, own_lens, prefix_len, k_cache, v_cache, prefix_table, bl
              prefix_table.data_ptr(), prefix_table.numel(), block_tables.data_ptr(), bt[0], block_tables.shape[1],
              1 if causal else 0, softmax_scale, out.data_ptr(), os[0], os[1], lp, workspace.data_ptr(), size, n, hq,
              hkv, d, code, ep)
+
+
+def _prompt_rows(what, name, x, n, heads, d, dtype):
+    """x and its strides; rows that are not contiguous or whose memory is shared or unaligned are copied."""
+    if x.dtype is not dtype or x.shape != (n, heads, d):
+        raise FoldError(f"{what}: {name} must be [n, heads, head_dim] of one type, n and head_dim")
+    st = x.stride()
+    if st[2] != 1 or st[0] < 1 or st[1] < 1 or st[0] % 8 or st[1] % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        st = x.stride()
+    return x, st
+
+
+def _prompt_out(what, name, x, n, heads, d, dtype):
+    """Strides of a given output."""
+    if x.dtype is not dtype or x.shape != (n, heads, d) or (x.stride(2) != 1 and d > 1):
+        raise FoldError(f"{what}: {name} must be [n, heads, head_dim] of its input's type, the head dimension contiguous")
+    return x.stride()
+
+
+def _prompt_shape(what, q, k, qsl, lse):
+    """(n, hq, hkv, d, type code, b) of packed prompts."""
+    shape, ks = q.shape, k.shape
+    code = _DTYPES.get(q.dtype)
+    if code is None or code == 2:
+        raise FoldError(f"{what}: q, k and v must be bfloat16 or float16")
+    if len(shape) != 3 or len(ks) != 3:
+        raise FoldError(f"{what}: q, k and v must be [n, heads, head_dim]")
+    n, hq, d = shape
+    if qsl.dtype is not _INT32 or qsl.dim() != 1 or qsl.shape[0] < 1 or not qsl.is_contiguous():
+        raise FoldError(f"{what}: query_start_loc must be contiguous int32 [b + 1]")
+    if lse is not None and (lse.shape != (hq, n) or lse.dtype is not torch.float32 or not lse.is_contiguous()):
+        raise FoldError(f"{what}: lse must be contiguous float32 [Hq, n]")
+    return n, hq, ks[1], d, code, qsl.shape[0] - 1
+
+
+def _ptr(what, t, check):
+    if t is None:
+        return None
+    check(what, t)
+    return t.data_ptr()
+
+
+def prompt_read(q, k, v, qsl, out, *, softmax_scale, causal=True, window_size=(-1, -1), lse=None, err=None):
+    """Attention over whole prompts packed one behind the other.
+
+    q [n, Hq, D], k and v [n, Hkv, D], bf16 or fp16 (RoPE'd), D a multiple of 8 up to 256: rows
+    [qsl[i], qsl[i + 1]) belong to sequence i (qsl int32 [b + 1] on the device). Row r of a sequence sees
+    its keys [r - left, r + right] of window_size (left, right) (-1: unbounded), up to its own when
+    causal. Writes out [n, Hq, D] (which may be q) and, when given, lse [Hq, n] float32; rows outside the
+    sequences are left alone. Keys and values go to a paged cache by append_paged; prompt_read_grad is the
+    gradient."""
+    dev = _check_devices("prompt_read", q, k, v, qsl, out, lse, err)
+    n, hq, hkv, d, code, b = _prompt_shape("prompt_read", q, k, qsl, lse)
+    os = _prompt_out("prompt_read", "out", out, n, hq, d, q.dtype)
+    q, qs = _prompt_rows("prompt_read", "q", q, n, hq, d, out.dtype)
+    k, ks = _prompt_rows("prompt_read", "k", k, n, hkv, d, out.dtype)
+    v, vs = _prompt_rows("prompt_read", "v", v, n, hkv, d, out.dtype)
+    left, right = window_size
+    _call_on(dev, "fold_prompt_read", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
+             vs[1], qsl.data_ptr(), b, 1 if causal else 0, left, right, softmax_scale, out.data_ptr(), os[0], os[1],
+             None if lse is None else lse.data_ptr(), n, hq, hkv, d, code, _ptr("prompt_read", err, _check_err))
+
+
+def prompt_grad_workspace(n, hq, hkv, d, device):
+    """A workspace for prompt_read_grad calls of up to these sizes (one per call that may overlap another)."""
+    dev = torch.device(device)
+    if dev.type != "cuda":
+        raise FoldError("FOLD kernels take CUDA tensors (there is no CPU path)")
+    size = _lib.prompt_read_grad_workspace(int(n), int(hq), int(hkv), int(d))
+    if size < 0:
+        raise FoldError(f"prompt_read_grad: no kernel for n {n}, Hq {hq}, Hkv {hkv}, head_dim {d}")
+    return torch.empty(size, device=dev, dtype=torch.uint8)
+
+
+def prompt_read_grad(dout, q, k, v, out, lse, qsl, *, softmax_scale, causal=True, window_size=(-1, -1), dlse=None,
+                     dq=None, dk=None, dv=None, workspace=None, err=None):
+    """Gradient of prompt_read: (dq, dk, dv) from dout [n, Hq, D] (and dlse [Hq, n] float32 of lse), the
+    inputs q, k, v, qsl and options of the forward call, and its results out and lse. The gradients of a key
+    or value are summed over the query heads of its group. They are new tensors unless given; rows outside
+    the sequences are zero in new ones, left alone in given ones. rotary(dq, dk, ..., inverse=True) takes
+    them on to the projections. Equal calls give equal bits. `workspace` (prompt_grad_workspace) is
+    allocated per call when not given."""
+    what = "prompt_read_grad"
+    dev = _check_devices(what, q, dout, k, v, out, lse, qsl, dlse, dq, dk, dv, workspace, err)
+    if lse is None:
+        raise FoldError("prompt_read_grad: lse of the forward call is needed")
+    n, hq, hkv, d, code, b = _prompt_shape(what, q, k, qsl, lse)
+    dtype = q.dtype
+    q, qs = _prompt_rows(what, "q", q, n, hq, d, dtype)
+    k, ks = _prompt_rows(what, "k", k, n, hkv, d, dtype)
+    v, vs = _prompt_rows(what, "v", v, n, hkv, d, dtype)
+    out, os = _prompt_rows(what, "out", out, n, hq, d, dtype)
+    dout, dos = _prompt_rows(what, "dout", dout, n, hq, d, dtype)
+    if dlse is not None and (dlse.shape != (hq, n) or dlse.dtype is not torch.float32 or not dlse.is_contiguous()):
+        raise FoldError("prompt_read_grad: dlse must be contiguous float32 [Hq, n]")
+    given = (dq is not None) + (dk is not None) + (dv is not None)
+    if given not in (0, 3):
+        raise FoldError("prompt_read_grad: all of dq, dk and dv are given, or none")
+    if not given:
+        make = torch.empty if b else torch.zeros
+        dq = make((n, hq, d), dtype=dtype, device=q.device)
+        dk = make((n, hkv, d), dtype=dtype, device=q.device)
+        dv = make((n, hkv, d), dtype=dtype, device=q.device)
+    dqs, dks, dvs = (_prompt_out(what, name, x, n, h, d, dtype)
+                     for name, x, h in (("dq", dq, hq), ("dk", dk, hkv), ("dv", dv, hkv)))
+    if n == 0 or b == 0:
+        return dq, dk, dv
+    if workspace is None:
+        size = _lib.prompt_read_grad_workspace(n, hq, hkv, d)
+        workspace = q.new_empty(max(size, 0), dtype=torch.uint8)
+    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise FoldError("prompt_read_grad: workspace must be a contiguous uint8 tensor (prompt_grad_workspace)")
+    left, right = window_size
+    _call_on(dev, "fold_prompt_read_grad", dout.data_ptr(), dos[0], dos[1], q.data_ptr(), qs[0], qs[1], k.data_ptr(),
+             ks[0], ks[1], v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0], os[1], lse.data_ptr(),
+             None if dlse is None else dlse.data_ptr(), qsl.data_ptr(), b, 1 if causal else 0, left, right,
+             softmax_scale, dq.data_ptr(), dqs[0], dqs[1], dk.data_ptr(), dks[0], dks[1], dv.data_ptr(), dvs[0],
+             dvs[1], 0 if given else 1, workspace.data_ptr(), workspace.numel(), n, hq, hkv, d, code,
+             _ptr(what, err, _check_err))
+    return dq, dk, dv
+
+
+def _check_pool(what, refs, block_tables, lens, rows, block_size):
+    """C-ABI arguments of a page pool."""
+    bt = block_tables.stride()
+    if not (refs.dtype is block_tables.dtype is lens.dtype is _INT32):
+        raise FoldError(f"{what}: refs, block_tables and lens must be int32")
+    if refs.dim() != 1 or lens.dim() != 1 or not refs.is_contiguous() or not lens.is_contiguous():
+        raise FoldError(f"{what}: refs [pages] and lens [rows] must be contiguous")
+    if len(bt) != 2 or block_tables.shape[0] != lens.shape[0] or (bt[1] != 1 and block_tables.shape[1] > 1):
+        raise FoldError(f"{what}: block_tables must be [rows, blocks] with contiguous rows, lens [rows]")
+    for t in rows:
+        if t is not None and (t.dtype is not _INT32 or t.dim() != 1 or not t.is_contiguous()):
+            raise FoldError(f"{what}: rows and lengths must be contiguous int32 vectors")
+    if block_size < 1:
+        raise FoldError(f"{what}: block_size must be positive")
+    return (refs.data_ptr(), refs.shape[0], block_tables.data_ptr(), bt[0], block_tables.shape[1], lens.data_ptr(),
+            lens.shape[0])
+
+
+def grow_pages(refs, block_tables, lens, qsl, n, *, block_size, rows=None, positions=None, slots=None, err=None):
+    """Pages of a paged cache for new tokens; returns (positions, slots), int64 [n], of append_paged.
+
+    refs int32 [pages] counts the rows that hold a page (0: free), lens int32 [rows] the tokens of each row of
+    block_tables int32 [rows, blocks]; all are changed in place, on the device. Sequence i gets the tokens
+    [qsl[i], qsl[i + 1]) of the n, in row rows[i] (None: row i; negative: skipped). The lowest-numbered free
+    pages are taken, in the sequences' order. Tokens outside the sequences, and those of a sequence that could
+    not grow, have slot -1; why is reported in err (int32 [1]): no free page, a table too short, a row outside
+    the tables or named twice, a partly filled last page that another row holds too (fork_pages the row)."""
+    dev = _check_devices("grow_pages", refs, block_tables, lens, qsl, rows, positions, slots, err)
+    pool = _check_pool("grow_pages", refs, block_tables, lens, (qsl, rows), block_size)
+    m = qsl.shape[0] - 1
+    if m < 0 or (rows is not None and rows.shape[0] != m):
+        raise FoldError("grow_pages: query_start_loc needs one entry more than there are sequences")
+    n = int(n)
+    if n < 0:
+        raise FoldError("grow_pages: n must not be negative")
+    if positions is None:
+        positions = refs.new_empty(n, dtype=torch.int64)
+    if slots is None:
+        slots = refs.new_empty(n, dtype=torch.int64)
+    for t in (positions, slots):
+        if t.dtype is not torch.int64 or t.shape != (n,) or not t.is_contiguous():
+            raise FoldError("grow_pages: positions and slots must be contiguous int64 [n]")
+    _call_on(dev, "fold_grow_pages", *pool, None if rows is None else rows.data_ptr(), qsl.data_ptr(), m, n, block_size,
+             positions.data_ptr(), slots.data_ptr(), _ptr("grow_pages", err, _check_err))
+    return positions, slots
+
+
+def free_pages(refs, block_tables, lens, rows=None, *, block_size, keep=None, err=None):
+    """Cuts rows (int32 [m]; None: all; a negative one is skipped) of a page pool (grow_pages) down to keep tokens
+    (int32 [m]; None: none): drafted tokens that were not accepted, sequences that are done. Pages that their
+    last row leaves become free."""
+    dev = _check_devices("free_pages", refs, block_tables, lens, rows, keep, err)
+    pool = _check_pool("free_pages", refs, block_tables, lens, (rows, keep), block_size)
+    m = lens.shape[0] if rows is None else rows.shape[0]
+    if keep is not None and keep.shape[0] != m:
+        raise FoldError("free_pages: keep needs one entry per row")
+    _call_on(dev, "fold_free_pages", *pool, None if rows is None else rows.data_ptr(),
+             None if keep is None else keep.data_ptr(), m, block_size, _ptr("free_pages", err, _check_err))
+
+
+def fork_pages(refs, block_tables, lens, src, dst, caches, *, workspace=None, err=None):
+    """Row dst[i] of a page pool (grow_pages) becomes a copy of row src[i] (int32 [m]; a negative row skips the
+    pair): full pages are shared, the tokens of a partly filled last page are copied to a fresh one in every
+    cache of the list `caches` (the layers' [pages, Hkv, block_size, width] tensors or planes, all of one
+    shape, type and strides). The rows dst must be empty (free_pages) and distinct; such that are not, and
+    children that find no free page, are reported in err."""
+    dev = _check_devices("fork_pages", refs, block_tables, lens, src, dst, workspace, err, *caches)
+    if not caches or caches[0].dim() != 4:
+        raise FoldError("fork_pages: caches is a list of [pages, Hkv, block_size, width] tensors")
+    first = caches[0]
+    shape, st, dtype = first.shape, first.stride(), first.dtype
+    for c in caches:
+        if c.shape != shape or c.stride() != st or c.dtype is not dtype:
+            raise FoldError("fork_pages: the caches must have one shape, type and strides")
+    if st[3] != 1 and shape[3] > 1:
+        raise FoldError("fork_pages: the last dimension of the caches must be contiguous")
+    if shape[0] < refs.shape[0] or min(shape) < 1:
+        raise FoldError("fork_pages: the caches hold fewer pages than refs counts")
+    pool = _check_pool("fork_pages", refs, block_tables, lens, (src, dst), shape[2])
+    m = src.shape[0]
+    if dst.shape[0] != m:
+        raise FoldError("fork_pages: src and dst need one entry per pair")
+    size = 16 * (m + 1)
+    if workspace is None:
+        workspace = refs.new_empty(size, dtype=torch.uint8)
+    elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise FoldError("fork_pages: workspace must be a contiguous uint8 tensor of 16 * (m + 1) bytes")
+    es = first.element_size()
+    ptrs = (ctypes.c_int64 * len(caches))(*[c.data_ptr() for c in caches])
+    _call_on(dev, "fold_fork_pages", *pool, src.data_ptr(), dst.data_ptr(), m, ptrs, len(caches), shape[1], shape[2],
+             shape[3] * es, st[0] * es, st[1] * es, st[2] * es, workspace.data_ptr(), workspace.numel(),
+             _ptr("fork_pages", err, _check_err))
 
 
 def append(k, v, positions, slots, side, *, pos_lo=0, skip_foreign=False, err=None):

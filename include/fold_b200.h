@@ -47,6 +47,10 @@ enum fold_dtype { FOLD_BF16 = 0, FOLD_FP16 = 1, FOLD_FP32 = 2 };
 #define FOLD_DEVERR_TIMEOUT 4      /* a pipeline wait of the far read, or a wait for a peer, gave up */
 #define FOLD_DEVERR_CAPACITY 8     /* far_len exceeds the side cache's capacity */
 #define FOLD_DEVERR_BLOCK_TABLE 16 /* a window-read block-table entry lies outside the paged cache */
+#define FOLD_DEVERR_PAGES 32       /* no free page was left for a row */
+#define FOLD_DEVERR_SHARED 64      /* a row's partly filled last page is held by another row too */
+#define FOLD_DEVERR_ROW 128        /* a row outside the tables, named twice, or forked to while in use */
+#define FOLD_DEVERR_REFS 256       /* a page was given back that no row holds */
 
 const char* fold_status_string(int status);
 const char* fold_last_error(void);
@@ -218,6 +222,81 @@ int fold_prefix_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
 /* Bytes of workspace fold_prefix_read takes for these sizes on the current device (-1: sizes it
  * does not take). */
 int64_t fold_prefix_read_workspace(int n, int hq, int hkv, int hd);
+
+/* Attention over whole prompts; no reference counterpart (the reference leaves a prompt's attention to
+ * vLLM and starts from its cache). Sequence i (of b) has the rows [qsl[i], qsl[i+1]) of q [n, hq, hd]
+ * and of k and v [n, hkv, hd] (qsl ascending, read on the device; rows outside [qsl[0], qsl[b]) are not
+ * read and their outputs are left as they were). Row r of a sequence of len rows sees its keys j with
+ * r - window_left <= j <= r + window_right (a negative bound is unbounded) and j <= r when `causal`.
+ * out [n, hq, hd] = the softmax-weighted values, lse [hq, n] (contiguous, may be NULL) the natural log
+ * of the sum of exp(softmax_scale * q.k). Keys and values of other sequences may hold anything; a value
+ * row that some rows of its sequence see must be finite even for rows that do not. dtype FOLD_BF16 or
+ * FOLD_FP16; hd a multiple of 8 up to 256 (64 and 128 take the tensor-memory kernels); every row on a
+ * 16-byte boundary; out must not overlap k or v, and q only as q itself. b and n are what a captured
+ * call is fixed to. err (may be NULL) takes FOLD_DEVERR_TIMEOUT. */
+int fold_prompt_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,
+                     int64_t k_stride_head, const void* v, int64_t v_stride_tok, int64_t v_stride_head, const int* qsl,
+                     int b, int causal, int window_left, int window_right, float softmax_scale, void* out,
+                     int64_t o_stride_tok, int64_t o_stride_head, float* lse, int n, int hq, int hkv, int hd, int dtype,
+                     int* err, void* stream);
+
+/* Gradient of fold_prompt_read: from dout [n, hq, hd] (and dlse [hq, n] of lse, may be NULL), its inputs
+ * and its results out and lse, the gradients dq [n, hq, hd], dk and dv [n, hkv, hd], those of a key or
+ * value summed over the heads of its group. Rows outside the sequences get zeros when `zero_rest`, else
+ * they are left as they were. No sum depends on the order in which blocks run: equal calls give equal
+ * bits. The gradients must not overlap the inputs. workspace: fold_prompt_read_grad_workspace bytes of
+ * device memory, 16-byte aligned, not shared by calls that may overlap; nothing in it outlives the call. */
+int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_stride_head, const void* q,
+                          int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,
+                          int64_t k_stride_head, const void* v, int64_t v_stride_tok, int64_t v_stride_head,
+                          const void* out, int64_t o_stride_tok, int64_t o_stride_head, const float* lse,
+                          const float* dlse, const int* qsl, int b, int causal, int window_left, int window_right,
+                          float softmax_scale, void* dq, int64_t dq_stride_tok, int64_t dq_stride_head, void* dk,
+                          int64_t dk_stride_tok, int64_t dk_stride_head, void* dv, int64_t dv_stride_tok,
+                          int64_t dv_stride_head, int zero_rest, void* workspace, int64_t workspace_bytes, int n,
+                          int hq, int hkv, int hd, int dtype, int* err, void* stream);
+
+/* Bytes of workspace fold_prompt_read_grad takes (-1: sizes it does not take). */
+int64_t fold_prompt_read_grad_workspace(int n, int hq, int hkv, int hd);
+
+/* Pages of a paged cache, kept on the device; no reference counterpart (vLLM's host keeps them).
+ * refs [num_pages] counts the rows that hold a page (0: free); row r of block_tables (num_rows rows of
+ * block_tables_len entries) holds lens[r] tokens in its first ceil(lens[r] / block_size) entries; entries
+ * behind those hold nothing and may be written. A call takes the lowest-numbered free pages. Everything
+ * is read and written on the device in the stream's order (calls on one pool do not overlap). At most
+ * 16384 sequences a call.
+ *
+ * fold_grow_pages: sequence i (of m) gets qsl[i+1] - qsl[i] more tokens in row rows[i] (rows NULL: row i;
+ * a negative row is skipped). lens grows; positions[t] and slots[t] (int64, n of them) are the position
+ * of token t in its sequence and block * block_size + offset, as fold_append_paged takes them; tokens
+ * outside the sequences, or of a sequence that did not grow, have slot -1. A sequence does not grow, and
+ * sets a bit of err, when its table cannot hold the tokens (FOLD_DEVERR_CAPACITY), its partly filled last
+ * page is held by another row too (FOLD_DEVERR_SHARED: fork the row to write behind it), its row lies
+ * outside the tables or was named before (FOLD_DEVERR_ROW), or, in the sequences' order, from the first
+ * on that found too few free pages, when it needs one (FOLD_DEVERR_PAGES). */
+int fold_grow_pages(int* refs, int num_pages, int* block_tables, int64_t block_tables_stride, int block_tables_len,
+                    int* lens, int num_rows, const int* rows, const int* qsl, int m, int n, int block_size,
+                    void* positions, void* slots, int* err, void* stream);
+
+/* Cuts rows[i] (NULL: row i) down to keep[i] tokens (NULL: none); pages that are left by their last row
+ * become free. A row named twice is cut to the smaller length, and gives each page back once. */
+int fold_free_pages(int* refs, int num_pages, int* block_tables, int64_t block_tables_stride, int block_tables_len,
+                    int* lens, int num_rows, const int* rows, const int* keep, int m, int block_size, int* err,
+                    void* stream);
+
+/* Row dst[i] becomes a copy of row src[i] as it was before the call: the full pages are shared, the tokens
+ * of a partly filled last page are copied to a fresh one in each of the caches, [num_pages, heads,
+ * block_size] rows of row_bytes at the given strides (bytes), all alike (caches: host array of device
+ * addresses). A negative row skips the pair. dst must be empty, else, or named before, it is left alone
+ * (FOLD_DEVERR_ROW); a child that finds no free page stays empty (FOLD_DEVERR_PAGES). workspace:
+ * fold_fork_pages_workspace bytes of device memory, 16-byte aligned, not shared by calls that overlap. */
+int fold_fork_pages(int* refs, int num_pages, int* block_tables, int64_t block_tables_stride, int block_tables_len,
+                    int* lens, int num_rows, const int* src, const int* dst, int m, const int64_t* caches, int num_caches,
+                    int heads, int block_size, int row_bytes, int64_t cache_stride_block, int64_t cache_stride_head,
+                    int64_t cache_stride_slot, void* workspace, int64_t workspace_bytes, int* err, void* stream);
+
+/* Bytes of workspace fold_fork_pages takes for m pairs (-1: too many). */
+int64_t fold_fork_pages_workspace(int m);
 
 /* Far-memory read of an fp8 side cache (fold_append_fp8): the work of fold_far_read with the keys
  * and values dequantised by k_scale, v_scale (float [hkv], device): K and V of the side cache are
