@@ -96,6 +96,28 @@ int side_tensor_map(const void* side, int pages, int hkv, int hd, int box_rows, 
   return FOLD_OK;
 }
 
+int tiled_map(const char* what, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+              const cuuint32_t* box, bool f16, CUtensorMap* out) {
+  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &r);
+    return e == cudaSuccess && r == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn)
+               : nullptr;
+  }();
+  const std::string w(what);
+  if (!encode) return fail(FOLD_ERR_TENSOR_MAP, w + ": cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+  const CUresult r = encode(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
+                            const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(FOLD_ERR_TENSOR_MAP, w + ": cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
+  return FOLD_OK;
+}
+
 int fp8_side_tensor_map(const void* side8, int pages, int hkv, CUtensorMap* out) {
   int dev = 0;
   if (int s = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return s;

@@ -34,6 +34,11 @@ int side_tensor_map_uncached(const void* side, int pages, int hkv, int hd, int b
 // 128 bytes, box 128 x 128, 128-byte swizzle (cached like side_tensor_map).
 int fp8_side_tensor_map(const void* side8, int pages, int hkv, CUtensorMap* out);
 
+// A map of a 16-bit tensor (bf16 or f16): dims and box in elements, strides in bytes, 128-byte swizzle, zeros
+// outside. `what` opens the messages.
+int tiled_map(const char* what, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+              const cuuint32_t* box, bool f16, CUtensorMap* out);
+
 int device_sm_count();
 
 // Raises a kernel's dynamic shared-memory limit to `bytes` on the current device. The attribute

@@ -55,7 +55,6 @@
 // halves, the tile's maximum found beside the exponentials, a second MMA warp (one a slot).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cudaTypedefs.h>
 
 #include <type_traits>
 
@@ -251,85 +250,18 @@ __device__ __forceinline__ void seq_cost(const PrefixParams& p, int s, int per_t
   }
 }
 
-// ---------------------------------------------------------------- TMEM and MMA forms of this kernel
-__device__ __forceinline__ void tmem_ld32(uint32_t a, float* v) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(a)
-      : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// ---------------------------------------------------------------- loads, stores and conversions of this kernel
 // Eight floats to a 32-byte boundary, one whole sector.
 __device__ __forceinline__ void store8(float* dst, const float* v) {
   asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "f"(v[0]), "f"(v[1]), "f"(v[2]),
                "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
                : "memory");
 }
-// One lane of a converged warp.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r != 0;
-}
-// A value that is the same in all lanes, as the compiler can see. The MMA instructions take their
-// operands from uniform registers: issued from one lane's own values each of them first moves five
-// (a step's 16 MMAs then took 1830 cycles of that lane, and bounded the kernel).
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-// Low words of shared-memory matrix descriptors; the high words are constants of the layout.
-__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4) << 16; }
-constexpr uint32_t desc_hi(uint32_t sbo) { return (sbo >> 4) | 1u << 14 | kSwizzle128 << 29; }
-// D[tmem] (+)= A[smem] x B[smem] and D[tmem] (+)= A[tmem] x B[smem].
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
-                                       uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, {%7, %7, %7, %7}, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(0u)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
-                                       uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
-      "setp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, {%6, %6, %6, %6}, p;\n\t}" ::"r"(d),
-      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(0u)
-      : "memory");
-}
-// Instruction descriptor of kind::f16 for bf16 or f16 operands, f32 accumulation, M = 128.
-constexpr uint32_t idesc_of(bool f16, int n, int b_mn) {
-  const uint32_t fmt = f16 ? 0u : 1u;
-  return (1u << 4) | (fmt << 7) | (fmt << 10) | (static_cast<uint32_t>(b_mn) << 16) |
-         (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
-}
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int c2, int c3, int c4) {
   asm volatile(
       "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(c2), "r"(c3), "r"(c4)
-      : "memory");
-}
-__device__ __forceinline__ void tma_load_3d_plain(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
-                                                  int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
 template <class T>
@@ -342,32 +274,11 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
   return pack_f16_sat(lo, hi);
 }
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
-}
 
 // Ring position (in tiles' K or V) of K and V of the CTA's tile j, counted over all its segments:
 // K runs one tile ahead, K0 K1 V0 K2 V1 ..., the order in which the MMAs first need them.
 __device__ __forceinline__ uint32_t k_pos(uint32_t j) { return j == 0 ? 0 : 2 * j - 1; }
 __device__ __forceinline__ uint32_t v_pos(uint32_t j) { return 2 * j + 2; }
-
-__device__ __forceinline__ void mbar_arrive_n(uint64_t* bar, uint32_t n) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(n) : "memory");
-}
-// The arrival of all n threads a barrier expects, once the MMAs issued so far have completed.
-template <int N>
-__device__ __forceinline__ void commit_for(uint64_t* bar) {
-  if constexpr (N > 1) mbar_arrive_n(bar, N - 1);
-  tc_commit(bar);
-}
-template <int N>
-__device__ __forceinline__ void regs_up() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void regs_down() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
 
 // ---------------------------------------------------------------- segments of few rows
 // A row tile of at most kFewRows rows (a decode step's, whose keys are read once for a handful of
@@ -1466,33 +1377,12 @@ int ctas_of_device() {
   return sms > 0 ? sms : 148;
 }
 
-int encode_map(const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
-               bool f16, CUtensorMap* out) {
-  static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
-    void* fn = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    const cudaError_t e = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &r);
-    return e == cudaSuccess && r == cudaDriverEntryPointSuccess
-               ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn)
-               : nullptr;
-  }();
-  if (!encode) return fail(FOLD_ERR_TENSOR_MAP, "prefix read: cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
-  const CUresult r = encode(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank,
-                            const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return fail(FOLD_ERR_TENSOR_MAP, "prefix read: cuTensorMapEncodeTiled failed with CUresult " + std::to_string(r));
-  return FOLD_OK;
-}
-
 // 3-D map of q: columns, heads, tokens; a box is one 64-column group of a half row tile's rows.
 int query_map(const PrefixParams& p, int hd, bool f16, CUtensorMap* out) {
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(p.hq), static_cast<cuuint64_t>(p.n)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.q_sh) * 2, static_cast<cuuint64_t>(p.q_st) * 2};
   const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(p.group), static_cast<cuuint32_t>(p.half_toks)};
-  return encode_map(p.q, 3, dims, strides, box, f16, out);
+  return tiled_map("prefix read", p.q, 3, dims, strides, box, f16, out);
 }
 
 // 5-D map of a K or V plane: 64 columns, 8 slots, 64-column groups, groups of 8 slots, and blocks
@@ -1506,7 +1396,7 @@ int plane_map(const void* base, int hd, int box_cols, int block_size, int chunk,
   const cuuint64_t strides[4] = {static_cast<cuuint64_t>(slot) * 2, 128, static_cast<cuuint64_t>(slot) * 16,
                                  static_cast<cuuint64_t>(unit) * 2};
   const cuuint32_t box[5] = {64, 8, static_cast<cuuint32_t>(box_cols / 64), static_cast<cuuint32_t>(chunk / 8), 1};
-  return encode_map(base, 5, dims, strides, box, f16, out);
+  return tiled_map("prefix read", base, 5, dims, strides, box, f16, out);
 }
 
 template <int HD, class T>

@@ -96,6 +96,33 @@ __device__ __forceinline__ void mma_t(float (&d)[4], const uint32_t (&a)[4], uin
   else mma_f16(d, a[0], a[1], a[2], a[3], b0, b1);
 }
 
+// ---------------------------------------------------------------- blocks that take tiles as they come
+// The grid has a block a tile; one that is through asks for the number of a block that has not started yet, and
+// that block never does: long and short tiles even out, and a tile's start overlaps the end of the one before.
+__device__ __forceinline__ void ask_next_block(void* answer, uint64_t* bar) {
+  fence_proxy_async_smem();  // the last answer has been read
+  mbar_arrive_expect_tx(bar, 16);
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// The number that was answered, or -1: all blocks have started.
+__device__ __forceinline__ int next_block(const void* answer) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "ld.shared.b128 a, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, a;\n\t}"
+      : "=&r"(got), "=&r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return got ? static_cast<int>(x) : -1;
+}
+
 // ---------------------------------------------------------------- tiles of 16-bit rows in shared memory
 // 64 rows of DP columns, padded by 16 bytes so that eight rows' chunks of 16 bytes hit all banks.
 template <int DP>
@@ -178,5 +205,7 @@ int prompt_shape(const char* what, const int* qsl, int b, int n, int hq, int hkv
 // An operand's pointer, alignment and strides; `written`: its rows must not share memory.
 int prompt_rows(const char* what, const char* name, const void* ptr, int64_t tok, int64_t head, int n, int heads,
                 int hd, bool written, prompt::Rows* out);
+// Map of an operand: columns, heads, rows; a box is 64 columns of `rows` rows of one head.
+int prompt_map(const char* what, const prompt::Rows& x, int heads, int n, int hd, int rows, bool f16, CUtensorMap* out);
 
 }  // namespace fold

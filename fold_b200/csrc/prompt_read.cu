@@ -5,6 +5,7 @@
 // o_r = sum_j e^(x_rj - lse_r) v_j and lse_r = log sum_j e^(x_rj). One pass over the keys keeps a running
 // maximum m and sum l of each row and rescales what was summed when the maximum rises.
 #include "prompt.cuh"
+#include "tcgen05.cuh"
 
 namespace fold {
 namespace {
@@ -24,7 +25,7 @@ __global__ void __launch_bounds__(128) prompt_read_mma_kernel(const ReadParams p
   using Sm = SmemTile<DP>;
   // weights in fp16 are held 2^10 up: small ones of many keys stay above its smallest step
   constexpr float kShift = std::is_same<T, __half>::value ? 10.f : 0.f;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const uint32_t sq = smem_u32(smem), sk = sq + Sm::BYTES, sv = sk + 2 * Sm::BYTES;
   wait_for_producer();
@@ -120,10 +121,461 @@ int launch_mma(const ReadParams& p, cudaStream_t stream) {
                        "prompt_read_mma_kernel", p);
 }
 
+// ---------------------------------------------------------------- tcgen05, head sizes 64 and 128
+// A CTA takes two tiles of 128 rows that read the same keys: two heads of a group, or, where a group has an
+// odd number of heads, 256 rows of one. Warps with fixed roles:
+//   two softmax warpgroups, one a tile: a thread owns a row; S from tensor memory, mask, maximum, P = 2^(y - m)
+//     rounded to the type of V and stored over S; O in tensor memory rescaled when a maximum rose; at the end
+//     O / l and lse go out;
+//   K and V by TMA into a ring, Q by TMA, the MMAs (S = Q K^T and O += P V, P from tensor memory), and a
+//   scheduler that asks for the next tile.
+// While one tile is in its softmax the tensor cores work for the other: P V of its last keys, then S of its next.
+template <int HD_, class T_>
+struct ReadCfg {
+  using T = T_;
+  static constexpr int HD = HD_, NTHREADS = 384, NSW = 8;
+  static constexpr int NCG = HD / 64;              // groups of 64 columns: a row of one is a swizzled 128 bytes
+  static constexpr int CG = 128 * 128;             // bytes of a group of a 128-row tile
+  static constexpr int UNIT = NCG * CG;            // a Q, K or V tile
+  static constexpr int QB = HD == 64 ? 2 : 1;      // Q tiles a warpgroup: at 64 the next one loads early
+  static constexpr int MISC = 1024;
+  static constexpr int FIT = (232448 - MISC - 2 * QB * UNIT) / UNIT;
+  static constexpr int NU = FIT > 8 ? 8 : FIT;     // K and V tiles in the ring
+  static constexpr int OFF_Q = NU * UNIT, OFF_BAR = OFF_Q + 2 * QB * UNIT, SMEM = OFF_BAR + MISC;
+  static constexpr int TMEM_S = 0, TMEM_O = 256;
+  static constexpr bool F16 = std::is_same<T, __half>::value;
+  // fp16 holds P up by 2^7, so that small weights stay above its smallest step; it stays below 2^15
+  static constexpr float SHIFT = F16 ? 7.f : 0.f;
+  static_assert(SMEM <= 232448 && NU >= 5, "shared memory");
+};
+
+// A row's maximum only moves when a logit passes it by more than this (log2 units).
+constexpr float kRowRaise = 8.f;
+
+// Registers a thread: at launch (the build checks it), then of the softmax warps and of the others.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "a share that is not there is waited for");
+
+struct ReadItem {
+  int first, len, hk;       // -1 len: no more
+  int row0[2], head[2], kb[2], ke[2];
+};
+constexpr int kItems = 3;
+
+struct ReadBars {
+  uint64_t full[8], empty[8];
+  uint64_t s_full[2], p_full[2], done[2], o_free[2];
+  uint64_t q_full[4], q_empty[4];
+  uint64_t item_full[kItems], item_empty[kItems], asked, drained;
+  uint4 answer;
+  uint32_t tmem;
+  ReadItem item[kItems];
+};
+static_assert(sizeof(ReadBars) <= 1024, "barriers fit their place");
+
+template <class C>
+__global__ void __launch_bounds__(C::NTHREADS, 1)
+    prompt_read_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                          const __grid_constant__ CUtensorMap vmap, const ReadParams p, const int pair_heads) {
+  using namespace tc;
+  using T = typename C::T;
+  constexpr int HD = C::HD, NU = C::NU, NSW = C::NSW, QB = C::QB;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  ReadBars& B = *reinterpret_cast<ReadBars*>(smem + C::OFF_BAR);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == NSW) {
+    if (lane == 0) {
+      for (int i = 0; i < NU; ++i) mbar_init(&B.full[i], 1), mbar_init(&B.empty[i], 1);
+      for (int i = 0; i < 2; ++i)
+        mbar_init(&B.s_full[i], 1), mbar_init(&B.p_full[i], 4), mbar_init(&B.done[i], 1), mbar_init(&B.o_free[i], 4);
+      for (int i = 0; i < 2 * QB; ++i) mbar_init(&B.q_full[i], 1), mbar_init(&B.q_empty[i], 1);
+      for (int i = 0; i < kItems; ++i) mbar_init(&B.item_full[i], 1), mbar_init(&B.item_empty[i], 3 + NSW);
+      mbar_init(&B.asked, 1), mbar_init(&B.drained, 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+  } else if (warp == NSW + 1) {
+    tmem_alloc(&B.tmem, 512);
+    tmem_relinquish();
+  }
+  wait_for_producer();
+  tc_fence_before();
+  __syncthreads();  // barriers and the address of tensor memory are visible
+  tc_fence_after();
+  const uint32_t tmem = B.tmem;
+  // Every role walks the items in the scheduler's order.
+  auto next_item = [&](int i, ReadItem& it) {
+    if (!warp_wait(&B.item_full[i % kItems], (i / kItems) & 1)) return false;
+    it = B.item[i % kItems];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&B.item_empty[i % kItems]);
+    return true;
+  };
+
+  if (warp < NSW) {
+    regs_up<kSoftmaxRegs>();
+    // ------------------------------------------------------------ softmax
+    const int wg = warp >> 2, row = (warp & 3) * 32 + lane;  // lane of tensor memory
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t sa = tmem + C::TMEM_S + wg * 128 + lane_addr, oa = tmem + C::TMEM_O + wg * HD + lane_addr;
+    uint32_t steps = 0, items = 0, tile0 = 0;  // of this warpgroup; tile0: key tiles of the CTA's earlier items
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      ReadItem it;
+      ok = next_item(i, it);
+      if (!ok || it.len < 0) break;
+      const int kb = min(it.kb[0], it.kb[1]), ke = max(it.ke[0], it.ke[1]);
+      const int r = it.row0[wg] + row;
+      const bool live = r < it.len;
+      int lo, hi;
+      keys_of(p.s, it.len, min(r, it.len - 1), min(r, it.len - 1) + 1, lo, hi);
+      const int warp_lo = __reduce_max_sync(0xffffffffu, lo), warp_hi = __reduce_min_sync(0xffffffffu, hi);
+      float m = -INFINITY, l = 0.f;
+      for (int j = it.kb[wg]; j < it.ke[wg]; ++j) {
+        ok = warp_wait(&B.s_full[wg], steps++ & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const int key0 = j * 128;
+        float v[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld32(sa + c, v + c);
+        tmem_wait_ld();
+        if (key0 < warp_lo || key0 + 128 > warp_hi) {
+          const int a = lo - key0;
+          const uint32_t seen = static_cast<uint32_t>(hi - lo);
+#pragma unroll
+          for (int c = 0; c < 128; ++c) v[c] = static_cast<uint32_t>(c - a) < seen ? v[c] : -INFINITY;
+        }
+        float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+        for (int c = 4; c < 128; c += 8) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = c + 4 + k < 128 ? fmax3(mx[k], v[c + k], v[c + 4 + k]) : fmaxf(mx[k], v[c + k]);
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.s.scale_log2;
+        const bool raise = top > m + kRowRaise || (m == -INFINITY && top > m);
+        if (__any_sync(0xffffffffu, raise)) {
+          const float mn = raise ? top : m;
+          const float f = raise ? fast_exp2(m - mn) : 1.f;  // 0 for the first keys
+          l *= f, m = mn;
+          if (j > it.kb[wg]) {  // the accumulator holds the products up to the last tile: S of this one came behind
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              float o[16];
+              tmem_ld16(oa + c, o);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) o[k] *= f;
+              tmem_st16(oa + c, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
+        }
+        const float neg = m == -INFINITY ? 0.f : C::SHIFT - m;
+        float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float a = v[c + 2 * k], d = v[c + 2 * k + 1];
+            ffma2(a, d, p.s.scale_log2, neg, neg);
+            a = fast_exp2(a), d = fast_exp2(d);
+            fadd2(l0, l1, l0, l1, a, d);
+            w[k] = pack_pair<T>(a, d);  // one rounding of P to the type of V
+          }
+          tmem_st16(sa + c / 2, w);
+        }
+        l += l0 + l1;
+        tmem_wait_st();
+        // values behind the sequence's end belong to others (NaN included): zeros before the tensor cores
+        // read them. The warpgroup whose P V comes first sees to it.
+        const int vk = it.len - key0;
+        if (vk < 128 && (wg == 0 || j < it.kb[0] || j >= it.ke[0])) {
+          const uint32_t u = 2 * (tile0 + j - kb) + 1;
+          ok = warp_wait(&B.full[u % NU], (u / NU) & 1);
+          if (!ok) break;
+          unsigned char* vt = smem + (u % NU) * C::UNIT;
+          for (int e = row; e < (128 - vk) * C::NCG * 8; e += 128) {
+            const int x = e / (C::NCG * 8), c = e % (C::NCG * 8);
+            *reinterpret_cast<uint4*>(vt + (c >> 3) * C::CG + (vk + x) * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.p_full[wg]);
+      }
+      tile0 += ke - kb;
+      if (!ok) break;
+      if (it.kb[wg] >= it.ke[wg]) continue;  // no tile for this warpgroup
+      ok = warp_wait(&B.done[wg], items++ & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const bool some = l > 0.f;
+      const float inv = some ? 1.f / l : 0.f;
+      T* out = static_cast<T*>(p.out.ptr) + static_cast<int64_t>(it.first + r) * p.out.tok + it.head[wg] * p.out.head;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        float o[32];
+        tmem_ld32(oa + c, o);
+        tmem_wait_ld();
+        if (live) {
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k)  // no key: l is 0; a NaN sum reaches the output
+            w[k] = some ? pack_pair<T>(o[2 * k] * inv, o[2 * k + 1] * inv) : pack_pair<T>(l, l);
+#pragma unroll
+          for (int k = 0; k < 16; k += 4)
+            *reinterpret_cast<uint4*>(out + c + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+        }
+      }
+      if (live && p.lse)
+        p.lse[static_cast<int64_t>(it.head[wg]) * p.s.n + it.first + r] =
+            some ? (m - C::SHIFT + __log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&B.o_free[wg]);
+    }
+    if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+  } else {
+    regs_down<kOtherRegs>();
+    if (warp == NSW) {
+      // ------------------------------------------------------------ K and V
+      uint32_t u = 0;
+      bool ok = true;
+      prefetch_tensormap(&kmap);
+      prefetch_tensormap(&vmap);
+      auto load = [&](const CUtensorMap* map, int hk, int row) {
+        const uint32_t slot = u % NU;
+        if (u >= NU) ok = warp_wait(&B.empty[slot], (u / NU - 1) & 1);
+        if (!ok) return;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&B.full[slot], C::UNIT);
+#pragma unroll
+          for (int c = 0; c < C::NCG; ++c)
+            tma_load_3d_plain(smem + slot * C::UNIT + c * C::CG, map, &B.full[slot], c * 64, hk, row);
+        }
+        __syncwarp();
+        ++u;
+      };
+      for (int i = 0; ok; ++i) {
+        ReadItem it;
+        ok = next_item(i, it);
+        if (!ok || it.len < 0) break;
+        const int kb = min(it.kb[0], it.kb[1]), ke = max(it.ke[0], it.ke[1]);
+        for (int j = kb; ok && j < ke; ++j) {
+          load(&kmap, it.hk, it.first + j * 128);
+          if (ok) load(&vmap, it.hk, it.first + j * 128);
+        }
+      }
+      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+      for (uint32_t w = u > NU ? u - NU : 0; w < u; ++w) warp_wait(&B.full[w % NU], (w / NU) & 1);  // copies land before exit
+    } else if (warp == NSW + 1) {
+      // ------------------------------------------------------------ MMAs
+      constexpr uint32_t idesc_s = idesc_of(C::F16, 128, 0), idesc_o = idesc_of(C::F16, HD, 1), hi = desc_hi(1024);
+      const uint32_t base = uniform(smem_u32(smem)), tm = uniform(tmem);
+      struct Step {
+        uint32_t v_lo, v_slot, v_parity, fresh;
+        bool valid, last, free_v;
+      } st[2];
+      st[0].valid = st[1].valid = false;
+      uint32_t qcnt[2] = {0, 0}, pcnt[2] = {0, 0}, ocnt[2] = {0, 0}, tile0 = 0;
+      bool ok = true;
+      auto pv = [&](int s) {  // O += P V of the tile whose S this warpgroup got last
+        Step& x = st[s];
+        if (!x.fresh) {  // the first of a tile of rows: the accumulator has been read
+          if (ocnt[s] > 0) ok = mbar_wait(&B.o_free[s], (ocnt[s] - 1) & 1);
+          ++ocnt[s];
+        }
+        ok = ok && mbar_wait(&B.full[x.v_slot], x.v_parity);
+        ok = ok && mbar_wait(&B.p_full[s], pcnt[s]++ & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        x.valid = false;
+        if (!ok) return;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            mma_ts(tm + C::TMEM_O + s * HD, tm + C::TMEM_S + s * 128 + k * 8, x.v_lo + k * 128, hi, idesc_o, k > 0 ? 1 : x.fresh);
+          if (x.free_v) tc_commit(&B.empty[x.v_slot]);
+          if (x.last) tc_commit(&B.done[s]);
+        }
+        __syncwarp();
+      };
+      for (int i = 0; ok; ++i) {
+        ReadItem it;
+        ok = next_item(i, it);
+        if (!ok || it.len < 0) break;
+        const int kb = min(it.kb[0], it.kb[1]), ke = max(it.ke[0], it.ke[1]);
+        for (int j = kb; ok && j < ke; ++j) {
+          const uint32_t u = 2 * (tile0 + j - kb), ks = u % NU, vs = (u + 1) % NU;
+          const uint32_t k_lo = uniform(desc_lo(base + ks * C::UNIT, 16)), v_lo = uniform(desc_lo(base + vs * C::UNIT, C::CG));
+          const bool in[2] = {j >= it.kb[0] && j < it.ke[0], j >= it.kb[1] && j < it.ke[1]};
+          bool got_k = false;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (!in[s]) {
+              if (st[s].valid) pv(s);  // its values' place in the ring is needed
+              if (!ok) break;
+              continue;
+            }
+            if (st[s].valid) pv(s);
+            if (!ok) break;
+            const uint32_t slot = s * QB + qcnt[s] % QB, qp = (qcnt[s] / QB) & 1;
+            if (j == it.kb[s]) {
+              // a new Q tile that is still on its way must not hold up the other warpgroup's last products
+              if (s == 0 && st[1].valid && !__all_sync(0xffffffffu, mbar_try_wait(&B.q_full[slot], qp))) pv(1);
+              ok = ok && mbar_wait(&B.q_full[slot], qp);
+            }
+            if (!got_k) ok = ok && mbar_wait(&B.full[ks], (u / NU) & 1);
+            got_k = true;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t q_lo = uniform(desc_lo(base + C::OFF_Q + slot * C::UNIT, 16));
+            const bool last_q = j + 1 == it.ke[s], last_k = s == 1 || !in[1];
+            if (elect_one()) {
+#pragma unroll
+              for (int k = 0; k < HD / 16; ++k) {
+                const uint32_t off = ((k >> 2) * C::CG + (k & 3) * 32) / 16;
+                mma_ss(tm + C::TMEM_S + s * 128, q_lo + off, hi, k_lo + off, hi, idesc_s, k > 0);
+              }
+              tc_commit(&B.s_full[s]);
+              if (last_k) tc_commit(&B.empty[ks]);
+              if (last_q) tc_commit(&B.q_empty[slot]);
+            }
+            __syncwarp();
+            st[s] = Step{v_lo, vs, ((u + 1) / NU) & 1, uniform(j > it.kb[s] ? 1u : 0u), true, last_q, last_k};
+            if (last_q) ++qcnt[s];
+          }
+        }
+        tile0 += ke - kb;
+      }
+      if (ok && st[0].valid) pv(0);
+      if (ok && st[1].valid) pv(1);
+      if (!ok) {  // let what was issued finish before tensor memory goes
+        if (elect_one()) {
+          set_error(p.err, FOLD_DEVERR_TIMEOUT);
+          tc_commit(&B.drained);
+        }
+        __syncwarp();
+        warp_wait(&B.drained, 0);
+      }
+    } else if (warp == NSW + 3) {
+      // ------------------------------------------------------------ Q
+      uint32_t cnt[2] = {0, 0};
+      bool ok = true;
+      prefetch_tensormap(&qmap);
+      for (int i = 0; ok; ++i) {
+        ReadItem it;
+        ok = next_item(i, it);
+        if (!ok || it.len < 0) break;
+        for (int s = 0; s < 2; ++s) {
+          if (it.kb[s] >= it.ke[s]) continue;
+          const uint32_t slot = s * QB + cnt[s] % QB, use = cnt[s] / QB;
+          if (use > 0) ok = warp_wait(&B.q_empty[slot], (use - 1) & 1);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&B.q_full[slot], C::UNIT);
+#pragma unroll
+            for (int c = 0; c < C::NCG; ++c)
+              tma_load_3d_plain(smem + C::OFF_Q + slot * C::UNIT + c * C::CG, &qmap, &B.q_full[slot], c * 64, it.head[s],
+                                it.first + it.row0[s]);
+          }
+          __syncwarp();
+          ++cnt[s];
+        }
+      }
+      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+      for (int s = 0; s < 2; ++s)  // copies land before exit
+        for (uint32_t w = cnt[s] > QB ? cnt[s] - QB : 0; w < cnt[s]; ++w) warp_wait(&B.q_full[s * QB + w % QB], (w / QB) & 1);
+    } else {
+      // ------------------------------------------------------------ scheduler
+      const int units = pair_heads ? p.s.hq / 2 : p.s.hq;
+      const int numbers = gridDim.x / units;
+      uint32_t asked = 0;
+      int out = 0;
+      bool ok = true;
+      auto publish = [&](const ReadItem& it) {
+        if (out >= kItems) ok = warp_wait(&B.item_empty[out % kItems], (out / kItems - 1) & 1);
+        if (!ok) return;
+        if (lane == 0) {
+          B.item[out % kItems] = it;
+          mbar_arrive(&B.item_full[out % kItems]);
+        }
+        __syncwarp();
+        ++out;
+      };
+      for (int id = blockIdx.x; ok && id >= 0;) {
+        if (lane == 0) ask_next_block(&B.answer, &B.asked);
+        __syncwarp();
+        // the last rows see most keys: first; heads of one tile follow one another, their keys stay near
+        const int x = numbers - 1 - id / units, unit = id % units;
+        Tile t;
+        const bool live = pair_heads ? find_tile<128>(p.s, x, t) : find_tile<256>(p.s, x, t);
+        if (live) {
+          ReadItem it;
+          it.first = t.first, it.len = t.len;
+          it.hk = (pair_heads ? 2 * unit : unit) / p.s.group;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            it.row0[s] = t.row0 + (pair_heads ? 0 : s * 128), it.head[s] = pair_heads ? 2 * unit + s : unit;
+            int lo = 0, hi = 0;
+            if (it.row0[s] < t.len) keys_of(p.s, t.len, it.row0[s], min(it.row0[s] + 128, t.len), lo, hi);
+            it.kb[s] = lo / 128, it.ke[s] = (hi + 127) / 128;
+            if (it.row0[s] >= t.len) it.kb[s] = it.ke[s] = it.ke[0];  // no rows (only the second may have none)
+          }
+          publish(it);
+        }
+        ok = warp_wait(&B.asked, asked++ & 1) && ok;  // (an answer lands before exit, too)
+        if (!ok) break;
+        id = next_block(&B.answer);
+        __syncwarp();
+      }
+      if (ok) {
+        ReadItem it{};
+        it.len = -1;
+        publish(it);
+      }
+      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == NSW + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int HD, class T>
+int launch_tc(const ReadParams& p, cudaStream_t stream) {
+  using C = ReadCfg<HD, T>;
+  const char* what = "prompt read";
+  CUtensorMap qmap, kmap, vmap;
+  if (int s = prompt_map(what, p.q, p.s.hq, p.s.n, HD, 128, C::F16, &qmap)) return s;
+  if (int s = prompt_map(what, p.k, p.s.hkv, p.s.n, HD, 128, C::F16, &kmap)) return s;
+  if (int s = prompt_map(what, p.v, p.s.hkv, p.s.n, HD, 128, C::F16, &vmap)) return s;
+  static std::atomic<uint64_t> configured{0};
+  if (int s = allow_smem(prompt_read_tc_kernel<C>, C::SMEM, configured, "cudaFuncSetAttribute(prompt_read)")) return s;
+  // the register shares the warps take must add up to what a block is launched with
+  static const int regs = [] {
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, prompt_read_tc_kernel<C>) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs != kLaunchRegs) return fail(FOLD_ERR_UNSUPPORTED, "prompt read: built with other register shares than launched");
+  const int pair = p.s.group % 2 == 0;
+  const int64_t blocks = static_cast<int64_t>(tile_numbers(p.s.n, p.s.b, pair ? 128 : 256)) * (pair ? p.s.hq / 2 : p.s.hq);
+  if (blocks > 0x7fffffff) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read: too many rows");
+  return launch_behind(prompt_read_tc_kernel<C>, dim3(static_cast<unsigned>(blocks)), C::NTHREADS, C::SMEM, stream,
+                       "prompt_read_tc_kernel", qmap, kmap, vmap, p, pair);
+}
+
 template <class T>
 int launch_read(const ReadParams& p, cudaStream_t stream) {
   const int hd = p.s.hd;
-  if (hd <= 64) return launch_mma<64, T>(p, stream);
+  if (hd == 64) return launch_tc<64, T>(p, stream);
+  if (hd == 128) return launch_tc<128, T>(p, stream);
+  if (hd < 64) return launch_mma<64, T>(p, stream);
   if (hd <= 96) return launch_mma<96, T>(p, stream);
   if (hd <= 128) return launch_mma<128, T>(p, stream);
   if (hd <= 192) return launch_mma<192, T>(p, stream);
@@ -148,6 +600,13 @@ int prompt_shape(const char* what, const int* qsl, int b, int n, int hq, int hkv
   p->left = bound(window_left), p->right = causal ? 0 : bound(window_right);
   p->scale = softmax_scale, p->scale_log2 = softmax_scale * kLog2e;
   return FOLD_OK;
+}
+
+int prompt_map(const char* what, const prompt::Rows& x, int heads, int n, int hd, int rows, bool f16, CUtensorMap* out) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(hd), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(n)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(x.head) * 2, static_cast<cuuint64_t>(x.tok) * 2};
+  const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(rows)};
+  return tiled_map(what, x.ptr, 3, dims, strides, box, f16, out);
 }
 
 int prompt_rows(const char* what, const char* name, const void* ptr, int64_t tok, int64_t head, int n, int heads,
