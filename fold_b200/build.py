@@ -33,7 +33,8 @@ NVCC_FLAGS = [
 # names: the shares that setmaxnreg deals out add up to what a block is launched with, and a block
 # that asks for more waits for good.
 REGISTERS = {"prefix_read": [(r"prefix_read_kernelI.*CfgILi(64|128)E", 168)],
-             "prompt_read": [(r"prompt_read_tc_kernelI", 168)]}
+             "prompt_read": [(r"prompt_read_tc_kernelI", 168)],
+             "prompt_grad": [(r"prompt_grad_tc_kernelI", 168)]}
 
 
 def check_registers(source: str, log: str) -> None:

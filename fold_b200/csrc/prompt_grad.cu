@@ -10,6 +10,7 @@
 // in memory would take five, but no sum depends on the order in which blocks run, and nothing of the
 // size of P is written.
 #include "prompt.cuh"
+#include "tcgen05.cuh"
 
 namespace fold {
 namespace {
@@ -20,7 +21,9 @@ struct GradParams {
   Rows q, k, v, out, dout, dq, dk, dv;
   const float* lse;   // [hq, n]
   const float* dlse;  // [hq, n] or null
-  float2* row;        // workspace [hq, n]: lse log2(e) - shift, delta 2^-shift (see Shift)
+  float2* row;        // workspace [hq, n]: shift - lse log2(e), -delta 2^-shift (see Shift)
+  float* part;        // workspace [splits][dk, dv][n, hkv, hd]: sums over some of a group's heads (splits > 1)
+  int splits;
   int zero_rest;      // rows outside the sequences get gradients of zero
   int* err;
 };
@@ -72,8 +75,20 @@ __global__ void __launch_bounds__(128) prompt_delta_kernel(const GradParams p) {
     const float lse = p.lse[at];
     if (p.dlse) sum -= p.dlse[at];
     // a row without a key (lse -inf) has weights of zero
-    p.row[at] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e - Shift<T>::kUp, sum * Shift<T>::kDown);
+    p.row[at] = make_float2(lse == -INFINITY ? -INFINITY : Shift<T>::kUp - lse * kLog2e, -sum * Shift<T>::kDown);
   }
+}
+
+// Whether row r sees one key, which then is its own: the weight is 1 whatever the logit, and dS is the
+// gradient of lse alone. (From dP and delta, rounded apart, it would be a remainder where the result is 0.)
+__device__ __forceinline__ bool lone(const Shape& s, int len, int r) {
+  int lo, hi;
+  keys_of(s, len, r, r + 1, lo, hi);
+  return hi - lo == 1;
+}
+template <class T>
+__device__ __forceinline__ float lone_ds(const GradParams& p, int h, int at, float weight) {
+  return p.dlse ? weight * p.dlse[static_cast<int64_t>(h) * p.s.n + at] * Shift<T>::kDown : 0.f;
 }
 
 // Columns a CTA sums gradients of: all, or halves above 128, whose accumulators would not fit the registers.
@@ -112,7 +127,7 @@ __device__ __forceinline__ void keys_mma(const GradParams& p, const Tile& t, int
       if (threadIdx.x < 64)
         rows[threadIdx.x] = j * 64 + threadIdx.x < t.len
                                 ? p.row[static_cast<int64_t>(h) * p.s.n + t.first + j * 64 + threadIdx.x]
-                                : make_float2(INFINITY, 0.f);
+                                : make_float2(-INFINITY, 0.f);
       cp_wait<0>();
       __syncthreads();
       float x[8][4], d[8][4];
@@ -129,8 +144,9 @@ __device__ __forceinline__ void keys_mma(const GradParams& p, const Tile& t, int
           const int r = i * 8 + 2 * t4 + (e & 1), row = j * 64 + r, key = key0 + (e >> 1) * 8;
           const float2 rr = rows[r];
           const bool in = row < t.len && key >= row - p.s.left && key <= row + p.s.right && key < t.len;
-          pv[e] = in ? fast_exp2(fmaf(x[i][e], p.s.scale_log2, -rr.x)) : 0.f;
-          sv4[e] = in ? pv[e] * fmaf(d[i][e], Shift<T>::kDown, -rr.y) : 0.f;
+          pv[e] = in ? fast_exp2(fmaf(x[i][e], p.s.scale_log2, rr.x)) : 0.f;
+          sv4[e] = in ? pv[e] * fmaf(d[i][e], Shift<T>::kDown, rr.y) : 0.f;
+          if (row == key && in && lone(p.s, t.len, row)) sv4[e] = lone_ds<T>(p, h, t.first + row, pv[e]);
         }
         pa[i >> 1][(i & 1) * 2] = pack_pair<T>(pv[0], pv[1]);
         pa[i >> 1][(i & 1) * 2 + 1] = pack_pair<T>(pv[2], pv[3]);
@@ -183,7 +199,7 @@ __device__ __forceinline__ void rows_mma(const GradParams& p, const Tile& t, int
     const int r = t.row0 + warp * 16 + e * 8 + g;
     keys_of(p.s, t.len, r, r + 1, klo[e], khi[e]);
     if (r >= t.len) khi[e] = 0;
-    rr[e] = r < t.len ? p.row[static_cast<int64_t>(h) * p.s.n + t.first + r] : make_float2(INFINITY, 0.f);
+    rr[e] = r < t.len ? p.row[static_cast<int64_t>(h) * p.s.n + t.first + r] : make_float2(-INFINITY, 0.f);
   }
   for (int j = kb; j < ke; ++j) {
     __syncthreads();
@@ -205,9 +221,9 @@ __device__ __forceinline__ void rows_mma(const GradParams& p, const Tile& t, int
       for (int e = 0; e < 4; ++e) {
         const int key = j * 64 + i * 8 + 2 * t4 + (e & 1);
         const bool in = key >= klo[e >> 1] && key < khi[e >> 1];
-        s4[e] = in ? fast_exp2(fmaf(x[i][e], p.s.scale_log2, -rr[e >> 1].x)) *
-                         fmaf(d[i][e], Shift<T>::kDown, -rr[e >> 1].y)
-                   : 0.f;
+        const float w = in ? fast_exp2(fmaf(x[i][e], p.s.scale_log2, rr[e >> 1].x)) : 0.f;
+        s4[e] = in ? w * fmaf(d[i][e], Shift<T>::kDown, rr[e >> 1].y) : 0.f;
+        if (in && khi[e >> 1] - klo[e >> 1] == 1) s4[e] = lone_ds<T>(p, h, t.first + key, w);
       }
       da[i >> 1][(i & 1) * 2] = pack_pair<T>(s4[0], s4[1]);
       da[i >> 1][(i & 1) * 2 + 1] = pack_pair<T>(s4[2], s4[3]);
@@ -231,7 +247,7 @@ __device__ __forceinline__ void rows_mma(const GradParams& p, const Tile& t, int
 // Blocks y < hkv: keys' gradients (more work each, so first); the others: a query head's.
 template <int DP, class T>
 __global__ void __launch_bounds__(128) prompt_grad_mma_kernel(const GradParams p) {
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   wait_for_producer();
   Tile t;
   const bool keys = static_cast<int>(blockIdx.y) < p.s.hkv;
@@ -250,6 +266,580 @@ int launch_mma(const GradParams& p, cudaStream_t stream) {
                        128, smem, stream, "prompt_grad_mma_kernel", p);
 }
 
+// ---------------------------------------------------------------- tcgen05, head sizes 64 and 128
+// A block takes an item: 128 keys of one KV head with the rows of some of its group's heads (dk, dv), or 128
+// rows of one head with their keys (dq). Both are the same work: two resident tiles r0, r1 and a stream of
+// tiles a, b,
+//     S = r0 a^T,  dP = r1 b^T,  dS = P (dP - delta),  acc1 += dS a,  and for keys  acc0 += P b
+// with (r0, r1, a, b) = (K, V, Q, dO) or (Q, dO, K, V): lanes of tensor memory are the resident rows. S and
+// dP have one place of 128 columns each, X and Y, which change places every tile: once dP is read, S of the
+// next tile goes over it, and dP of the next tile goes over what P and dS of this one were written to.
+// Order of the products: acc0 of this tile (P came while dP was computed), S of the next, acc1 of this, dP of
+// the next; the exponentials of a tile run beside acc1 and dP.
+//
+// dS is held as two numbers of the type, its rounding and what that leaves, so that dq and dk are nearly those
+// of a dS in 32 bits; P of dv is rounded once.
+template <int HD_, class T_>
+struct GradCfg {
+  using T = T_;
+  static constexpr int HD = HD_, NTHREADS = 384, NSW = 8;
+  static constexpr int NCG = HD / 64, CG = 128 * 128, UNIT = NCG * CG;
+  static constexpr int NA = HD == 64 ? 4 : 3, NB = HD == 64 ? 4 : 2;  // a is needed longer: by S, then by acc1
+  static constexpr int MISC = 1024 + 2048;
+  static constexpr int OFF_B = NA * UNIT, OFF_R = OFF_B + NB * UNIT, OFF_BAR = OFF_R + 2 * UNIT, OFF_STAT = OFF_BAR + 1024;
+  static constexpr int SMEM = OFF_BAR + MISC;
+  static constexpr int TMEM_ACC1 = 256, TMEM_ACC0 = 384;
+  static constexpr bool F16 = std::is_same<T, __half>::value;
+  static_assert(SMEM <= 232448, "shared memory");
+};
+
+// Registers a thread: at launch (the build checks it), then of the softmax warps and of the others.
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(2 * kSoftmaxRegs + kOtherRegs <= 3 * kLaunchRegs, "a share that is not there is waited for");
+
+struct GradItem {
+  int keys;               // 1: gradients of keys, 0: of rows, -1: no more
+  int first, len, row0;   // the resident tile's first row in its sequence
+  int head, h0, nh;       // resident head; heads of the stream
+  int jb, je;             // tiles of the stream, of each head
+  int split;
+};
+constexpr int kItems = 3;
+
+struct GradBars {
+  uint64_t a_full[4], a_empty[4], b_full[4], b_empty[4];
+  uint64_t r_full[2], r_empty[2];
+  uint64_t s_full, dp_full, p_full, dp_read, acc0_done, ds_full, acc_done, drained;
+  uint64_t st_full[2], st_empty[2];
+  uint64_t item_full[kItems], item_empty[kItems], asked;
+  uint4 answer;
+  uint32_t tmem;
+  GradItem item[kItems];
+};
+static_assert(sizeof(GradBars) <= 1024, "barriers fit their place");
+
+template <class C>
+__global__ void __launch_bounds__(C::NTHREADS, 1)
+    prompt_grad_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap domap,
+                          const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                          const GradParams p, const int key_items) {
+  using namespace tc;
+  using T = typename C::T;
+  constexpr int HD = C::HD, NSW = C::NSW, NA = C::NA, NB = C::NB;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  GradBars& B = *reinterpret_cast<GradBars*>(smem + C::OFF_BAR);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == NSW) {
+    if (lane == 0) {
+      for (int i = 0; i < NA; ++i) mbar_init(&B.a_full[i], 1), mbar_init(&B.a_empty[i], 1);
+      for (int i = 0; i < NB; ++i) mbar_init(&B.b_full[i], 1), mbar_init(&B.b_empty[i], 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&B.r_full[i], 1), mbar_init(&B.r_empty[i], 1);
+        mbar_init(&B.st_full[i], 1), mbar_init(&B.st_empty[i], NSW);
+      }
+      mbar_init(&B.s_full, 1), mbar_init(&B.dp_full, 1), mbar_init(&B.acc0_done, 1), mbar_init(&B.acc_done, 1);
+      mbar_init(&B.p_full, NSW), mbar_init(&B.dp_read, NSW), mbar_init(&B.ds_full, NSW);
+      for (int i = 0; i < kItems; ++i) mbar_init(&B.item_full[i], 1), mbar_init(&B.item_empty[i], 3 + NSW);
+      mbar_init(&B.asked, 1), mbar_init(&B.drained, 1);
+      fence_mbar_init();
+    }
+    __syncwarp();
+  } else if (warp == NSW + 1) {
+    tmem_alloc(&B.tmem, 512);
+    tmem_relinquish();
+  }
+  wait_for_producer();
+  tc_fence_before();
+  __syncthreads();  // barriers and the address of tensor memory are visible
+  tc_fence_after();
+  const uint32_t tmem = B.tmem;
+  // Every role walks the items in the scheduler's order.
+  auto next_item = [&](int i, GradItem& it) {
+    if (!warp_wait(&B.item_full[i % kItems], (i / kItems) & 1)) return false;
+    it = B.item[i % kItems];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&B.item_empty[i % kItems]);
+    return true;
+  };
+
+  if (warp < NSW) {
+    regs_up<kSoftmaxRegs>();
+    // ------------------------------------------------------------ softmax
+    // a warp: 32 lanes (resident rows) and the half of a tile's columns that its warpgroup has
+    const int wg = warp >> 2, res = (warp & 3) * 32 + lane;
+    const uint32_t mine = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + wg * 64;
+    const float* stat = reinterpret_cast<const float*>(smem + C::OFF_STAT);
+    uint32_t g = 0, gk = 0;  // tiles so far; of keys' items
+    bool ok = true;
+    for (int i = 0; ok; ++i) {
+      GradItem it;
+      ok = next_item(i, it);
+      if (!ok || it.keys < 0) break;
+      const bool keys = it.keys == 1;
+      const int r = min(it.row0 + res, it.len - 1);
+      const bool live = it.row0 + res < it.len;
+      int lo, hi;
+      if (keys) rows_of(p.s, it.len, r, r + 1, lo, hi);
+      else keys_of(p.s, it.len, r, r + 1, lo, hi);
+      const int warp_lo = __reduce_max_sync(0xffffffffu, lo), warp_hi = __reduce_min_sync(0xffffffffu, hi);
+      const bool own = lone(p.s, it.len, r);
+      float2 rr = make_float2(0.f, 0.f);
+      if (!keys) rr = p.row[static_cast<int64_t>(it.head) * p.s.n + it.first + r];
+      const int per = it.je - it.jb;
+      for (int t = 0; t < it.nh * per; ++t, ++g) {
+        const int h = keys ? it.h0 + t / per : it.head, col0 = (it.jb + t % per) * 128;  // stream row of column 0
+        const uint32_t x = mine + (g & 1) * 128, y = mine + ((g & 1) ^ 1) * 128;
+        ok = warp_wait(&B.s_full, g & 1);
+        if (!ok) break;
+        tc_fence_after();
+        float v[64];
+        tmem_ld32(x, v), tmem_ld32(x + 32, v + 32);
+        tmem_wait_ld();
+        const float* nl = stat + (gk & 1) * 256 + wg * 64;
+        if (keys) {
+          ok = warp_wait(&B.st_full[gk & 1], (gk >> 1) & 1);
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(nl + c);
+            ffma2(v[c], v[c + 1], p.s.scale_log2, a.x, a.y);
+            ffma2(v[c + 2], v[c + 3], p.s.scale_log2, a.z, a.w);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) ffma2(v[c], v[c + 1], p.s.scale_log2, rr.x, rr.x);
+        }
+#pragma unroll
+        for (int c = 0; c < 64; ++c) v[c] = fast_exp2(v[c]);
+        const bool masked = col0 < warp_lo || col0 + 128 > warp_hi;
+        const int from = lo - col0 - wg * 64;
+        const uint32_t seen = static_cast<uint32_t>(hi - lo);
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) v[c] = static_cast<uint32_t>(c - from) < seen ? v[c] : 0.f;
+        }
+        // rows behind the sequence's end belong to others (NaN included): zeros before the tensor cores read
+        // them beside weights of zero
+        const int left = it.len - col0;
+        if (left < 128) {
+          ok = warp_wait(&B.b_full[g % NB], (g / NB) & 1);
+          if (!ok) break;
+          unsigned char *ta = smem + (g % NA) * C::UNIT, *tb = smem + C::OFF_B + (g % NB) * C::UNIT;
+          for (int e = tid; e < (128 - left) * C::NCG * 8; e += NSW * 32) {
+            const int at = left + e / (C::NCG * 8), c = e % (C::NCG * 8);
+            const int off = (c >> 3) * C::CG + at * 128 + (c & 7) * 16;
+            *reinterpret_cast<uint4*>(ta + off) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(tb + off) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async();
+        }
+        if (keys) {
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) w[k] = pack_pair<T>(v[c + 2 * k], v[c + 2 * k + 1]);
+            tmem_st16(x + c / 2, w);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B.p_full);
+        }
+        ok = warp_wait(&B.dp_full, g & 1);
+        if (!ok) break;
+        tc_fence_after();
+        float d[64];
+        tmem_ld32(y, d), tmem_ld32(y + 32, d + 32);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.dp_read);
+        if (keys) {
+#pragma unroll
+          for (int c = 0; c < 64; c += 4) {
+            const float4 a = *reinterpret_cast<const float4*>(nl + 128 + c);
+            ffma2(d[c], d[c + 1], Shift<T>::kDown, a.x, a.y);
+            ffma2(d[c + 2], d[c + 3], Shift<T>::kDown, a.z, a.w);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B.st_empty[gk & 1]);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) ffma2(d[c], d[c + 1], Shift<T>::kDown, rr.y, rr.y);
+        }
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) d[c] = static_cast<uint32_t>(c - from) < seen ? d[c] : 0.f;
+        }
+#pragma unroll
+        for (int c = 0; c < 64; ++c) d[c] *= v[c];
+        if (masked && __any_sync(0xffffffffu, own)) {
+          const int self = r - col0 - wg * 64;
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (own && c == self) d[c] = lone_ds<T>(p, h, it.first + r, v[c]);
+        }
+        uint32_t low[32];
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            w[k] = pack_pair<T>(d[c + 2 * k], d[c + 2 * k + 1]);
+            const float2 f = unpack_pair<T>(w[k]);
+            low[c / 2 + k] = pack_pair<T>(d[c + 2 * k] - f.x, d[c + 2 * k + 1] - f.y);
+          }
+          tmem_st16(x + 32 + c / 2, w);
+        }
+        if (keys) {  // P has been read
+          ok = warp_wait(&B.acc0_done, gk & 1);
+          if (!ok) break;
+          tc_fence_after();
+          ++gk;
+        }
+        tmem_st16(x, low), tmem_st16(x + 16, low + 16);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&B.ds_full);
+      }
+      if (!ok) break;
+      ok = warp_wait(&B.acc_done, i & 1);
+      if (!ok) break;
+      tc_fence_after();
+      // keys: a warpgroup each of dv and dk; rows: half of dq's columns each
+      const uint32_t acc = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) +
+                           (keys ? (wg == 0 ? C::TMEM_ACC0 : C::TMEM_ACC1) : C::TMEM_ACC1 + wg * (HD / 2));
+      const float f = keys && wg == 0 ? Shift<T>::kDown : p.s.scale;
+      const Rows& to = keys ? (wg == 0 ? p.dv : p.dk) : p.dq;
+      const int64_t at = it.first + r;
+      T* out = static_cast<T*>(to.ptr) + at * to.tok + it.head * to.head + (keys ? 0 : wg * (HD / 2));
+      float* part = p.part + ((static_cast<int64_t>(2 * it.split + 1 - wg) * p.s.n + at) * p.s.hkv + it.head) * HD;
+      const bool partial = keys && p.splits > 1;
+#pragma unroll 1
+      for (int c = 0; c < (keys ? HD : HD / 2); c += 32) {
+        float o[32];
+        tmem_ld32(acc + c, o);
+        tmem_wait_ld();
+        if (!live) continue;
+        if (partial) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            *reinterpret_cast<float4*>(part + c + k) = make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; k += 8)
+            *reinterpret_cast<uint4*>(out + c + k) =
+                make_uint4(pack_pair<T>(o[k] * f, o[k + 1] * f), pack_pair<T>(o[k + 2] * f, o[k + 3] * f),
+                           pack_pair<T>(o[k + 4] * f, o[k + 5] * f), pack_pair<T>(o[k + 6] * f, o[k + 7] * f));
+        }
+      }
+      tc_fence_before();  // the next item's products come behind its first tile's P or dS
+    }
+    if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+  } else {
+    regs_down<kOtherRegs>();
+    if (warp == NSW) {
+      // ------------------------------------------------------------ loads
+      uint32_t g = 0, items = 0;
+      bool ok = true;
+      if (lane == 0) prefetch_tensormap(&qmap), prefetch_tensormap(&domap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
+      auto load = [&](const CUtensorMap* map, int offset, uint64_t* full, int head, int row) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(full, C::UNIT);
+#pragma unroll
+          for (int c = 0; c < C::NCG; ++c) tma_load_3d_plain(smem + offset + c * C::CG, map, full, c * 64, head, row);
+        }
+        __syncwarp();
+      };
+      for (int i = 0; ok; ++i) {
+        GradItem it;
+        ok = next_item(i, it);
+        if (!ok || it.keys < 0) break;
+        const bool keys = it.keys == 1;
+        const int per = it.je - it.jb;
+        for (int t = 0; ok && t < it.nh * per; ++t, ++g) {
+          const int row = it.first + (it.jb + t % per) * 128, head = it.h0 + t / per;
+          if (t == 0) {
+            if (i > 0) ok = warp_wait(&B.r_empty[0], (i - 1) & 1);
+            if (!ok) break;
+            load(keys ? &kmap : &qmap, C::OFF_R, &B.r_full[0], it.head, it.first + it.row0);
+          }
+          if (g >= NA) ok = warp_wait(&B.a_empty[g % NA], (g / NA - 1) & 1);
+          if (!ok) break;
+          load(keys ? &qmap : &kmap, (g % NA) * C::UNIT, &B.a_full[g % NA], head, row);
+          if (t == 0) {
+            if (i > 0) ok = warp_wait(&B.r_empty[1], (i - 1) & 1);
+            if (!ok) break;
+            load(keys ? &vmap : &domap, C::OFF_R + C::UNIT, &B.r_full[1], it.head, it.first + it.row0);
+            items = i + 1;
+          }
+          if (g >= NB) ok = warp_wait(&B.b_empty[g % NB], (g / NB - 1) & 1);
+          if (!ok) break;
+          load(keys ? &domap : &vmap, C::OFF_B + (g % NB) * C::UNIT, &B.b_full[g % NB], head, row);
+        }
+      }
+      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+      // copies land before exit
+      for (uint32_t w = g > NA ? g - NA : 0; w < g; ++w) warp_wait(&B.a_full[w % NA], (w / NA) & 1);
+      for (uint32_t w = g > NB ? g - NB : 0; w < g; ++w) warp_wait(&B.b_full[w % NB], (w / NB) & 1);
+      if (items > 0) warp_wait(&B.r_full[0], (items - 1) & 1), warp_wait(&B.r_full[1], (items - 1) & 1);
+    } else if (warp == NSW + 1) {
+      // ------------------------------------------------------------ MMAs
+      constexpr uint32_t idesc_s = idesc_of(C::F16, 128, 0), idesc_o = idesc_of(C::F16, HD, 1), hi = desc_hi(1024);
+      const uint32_t base = uniform(smem_u32(smem)), tm = uniform(tmem);
+      GradItem it;
+      int item = 0, t = 0, per = 1, total = 0;  // next item; place in the current one
+      bool ok = true;
+      struct Tile1 {
+        bool valid, keys, first, last;
+      } now{}, next{};
+      uint32_t gk = 0;  // tiles of keys' items
+      auto advance = [&](Tile1& x) {  // the tile behind
+        if (t == total) {
+          x.valid = false;
+          ok = next_item(item, it);
+          if (!ok || it.keys < 0) return;
+          ++item, t = 0, per = it.je - it.jb, total = it.nh * per;
+        }
+        x = Tile1{true, it.keys == 1, t == 0, t + 1 == total};
+        ++t;
+      };
+      // S or dP of tile n (the CTA's), resident tile w, into column `to`
+      auto product_ss = [&](const Tile1& x, int w, uint32_t n, uint32_t to) {
+        const uint32_t slot = w == 0 ? n % NA : n % NB, use = w == 0 ? n / NA : n / NB;
+        if (x.first) ok = mbar_wait(&B.r_full[w], (item - 1) & 1);
+        ok = ok && mbar_wait(w == 0 ? &B.a_full[slot] : &B.b_full[slot], use & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t a_lo = uniform(desc_lo(base + C::OFF_R + w * C::UNIT, 16));
+        const uint32_t b_lo = uniform(desc_lo(base + (w == 0 ? 0 : C::OFF_B) + slot * C::UNIT, 16));
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t off = ((k >> 2) * C::CG + (k & 3) * 32) / 16;
+            mma_ss(tm + to, a_lo + off, hi, b_lo + off, hi, idesc_s, k > 0);
+          }
+          tc_commit(w == 0 ? &B.s_full : &B.dp_full);
+          if (x.last) tc_commit(&B.r_empty[w]);
+        }
+        __syncwarp();
+      };
+      advance(now);
+      uint32_t g = 0;
+      if (ok && now.valid) product_ss(now, 0, 0, 0);
+      if (ok && now.valid) product_ss(now, 1, 0, 128);
+      while (ok && now.valid) {
+        const uint32_t x = (g & 1) * 128, y = x ^ 128;
+        const uint32_t a_lo = uniform(desc_lo(base + (g % NA) * C::UNIT, C::CG));
+        const uint32_t b_lo = uniform(desc_lo(base + C::OFF_B + (g % NB) * C::UNIT, C::CG));
+        const uint32_t more = uniform(now.first ? 0u : 1u);
+        advance(next);
+        if (!ok) break;
+        if (now.keys) {
+          ok = warp_wait(&B.p_full, gk++ & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              mma_ts(tm + C::TMEM_ACC0, tm + x + (k >> 2) * 64 + (k & 3) * 8, b_lo + k * 128, hi, idesc_o, k > 0 ? 1 : more);
+            tc_commit(&B.acc0_done);
+          }
+          __syncwarp();
+        }
+        ok = warp_wait(&B.dp_read, g & 1);
+        if (ok && next.valid) product_ss(next, 0, g + 1, y);
+        ok = ok && warp_wait(&B.ds_full, g & 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k)  // the roundings, then what they left
+            mma_ts(tm + C::TMEM_ACC1, tm + x + (k < 8 ? 32 : 0) + ((k >> 2) & 1) * 64 + (k & 3) * 8, a_lo + (k & 7) * 128, hi, idesc_o,
+                   k > 0 ? 1 : more);
+          tc_commit(&B.a_empty[g % NA]);
+          tc_commit(&B.b_empty[g % NB]);
+          if (now.last) tc_commit(&B.acc_done);
+        }
+        __syncwarp();
+        if (next.valid) product_ss(next, 1, g + 1, x);
+        now = next, ++g;
+      }
+      if (!ok) {  // let what was issued finish before tensor memory goes
+        if (elect_one()) {
+          set_error(p.err, FOLD_DEVERR_TIMEOUT);
+          tc_commit(&B.drained);
+        }
+        __syncwarp();
+        warp_wait(&B.drained, 0);
+      }
+    } else if (warp == NSW + 3) {
+      // ------------------------------------------------------------ lse and delta of streamed rows
+      float* stat = reinterpret_cast<float*>(smem + C::OFF_STAT);
+      uint32_t gk = 0;
+      bool ok = true;
+      for (int i = 0; ok; ++i) {
+        GradItem it;
+        ok = next_item(i, it);
+        if (!ok || it.keys < 0) break;
+        if (it.keys == 0) continue;
+        const int per = it.je - it.jb;
+        for (int t = 0; t < it.nh * per; ++t, ++gk) {
+          const int r0 = (it.jb + t % per) * 128;
+          const float2* src = p.row + static_cast<int64_t>(it.h0 + t / per) * p.s.n + it.first + r0;
+          float2 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[k] = r0 + k * 32 + lane < it.len ? src[k * 32 + lane] : make_float2(-INFINITY, 0.f);
+          if (gk >= 2) ok = warp_wait(&B.st_empty[gk & 1], (gk / 2 - 1) & 1);
+          if (!ok) break;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            stat[(gk & 1) * 256 + k * 32 + lane] = v[k].x, stat[(gk & 1) * 256 + 128 + k * 32 + lane] = v[k].y;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&B.st_full[gk & 1]);
+        }
+      }
+      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+    } else {
+      // ------------------------------------------------------------ scheduler
+      const int key_heads = p.s.hkv * p.splits, numbers = key_items / key_heads;
+      uint32_t asked = 0;
+      int out = 0;
+      bool ok = true;
+      auto publish = [&](const GradItem& it) {
+        if (out >= kItems) ok = warp_wait(&B.item_empty[out % kItems], (out / kItems - 1) & 1);
+        if (!ok) return;
+        if (lane == 0) {
+          B.item[out % kItems] = it;
+          mbar_arrive(&B.item_full[out % kItems]);
+        }
+        __syncwarp();
+        ++out;
+      };
+      for (int id = blockIdx.x; ok && id >= 0;) {
+        if (lane == 0) ask_next_block(&B.answer, &B.asked);
+        __syncwarp();
+        // the longest first: the first keys are seen by most rows, the last rows see most keys
+        const bool keys = id < key_items;
+        const int k = keys ? id : id - key_items, heads = keys ? key_heads : p.s.hq;
+        const int x = keys ? k / heads : numbers - 1 - k / heads, h = k % heads;
+        Tile t;
+        if (find_tile<128>(p.s, x, t)) {
+          GradItem it;
+          int lo, hi;
+          it.keys = keys, it.first = t.first, it.len = t.len, it.row0 = t.row0;
+          if (keys) {
+            it.head = h / p.splits, it.split = h % p.splits;
+            it.nh = p.s.group / p.splits, it.h0 = it.head * p.s.group + it.split * it.nh;
+            rows_of(p.s, t.len, t.row0, min(t.row0 + 128, t.len), lo, hi);
+          } else {
+            it.head = h, it.split = 0, it.h0 = h / p.s.group, it.nh = 1;
+            keys_of(p.s, t.len, t.row0, min(t.row0 + 128, t.len), lo, hi);
+          }
+          it.jb = lo / 128, it.je = (hi + 127) / 128;
+          publish(it);
+        }
+        ok = warp_wait(&B.asked, asked++ & 1) && ok;  // (an answer lands before exit, too)
+        if (!ok) break;
+        id = next_block(&B.answer);
+        __syncwarp();
+      }
+      if (ok) {
+        GradItem it{};
+        it.keys = -1;
+        publish(it);
+      }
+      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == NSW + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// dk and dv from the sums over some heads each, added in their order. Memory bound.
+template <class T>
+__global__ void __launch_bounds__(256) prompt_grad_join_kernel(const GradParams p) {
+  const int64_t x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;  // four elements of dk and of dv
+  const int per = p.s.hd / 4, c = static_cast<int>(x % per) * 4;
+  const int64_t row = x / per, t = row / p.s.hkv;
+  wait_for_producer();
+  if (t >= p.s.n || t < __ldg(p.s.qsl) || t >= __ldg(p.s.qsl + p.s.b)) return;
+  const int h = static_cast<int>(row - t * p.s.hkv);
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+      const float4 a = *reinterpret_cast<const float4*>(p.part + (static_cast<int64_t>(2 * s + w) * p.s.n * p.s.hkv + row) * p.s.hd + c);
+      sum.x += a.x, sum.y += a.y, sum.z += a.z, sum.w += a.w;
+    }
+    const Rows& to = w == 0 ? p.dk : p.dv;
+    *reinterpret_cast<uint2*>(static_cast<T*>(to.ptr) + t * to.tok + h * to.head + c) =
+        make_uint2(pack_pair<T>(sum.x, sum.y), pack_pair<T>(sum.z, sum.w));
+  }
+}
+
+// Into how many the heads of a group are split for the gradients of keys: enough that the device's blocks have
+// three items each, or every head by itself.
+int key_splits(int n, int hkv, int group) {
+  const int want = 3 * 148;
+  const int64_t items = (static_cast<int64_t>(n) + 127) / 128 * hkv;
+  for (int s = 1; s < group; ++s)
+    if (group % s == 0 && items * s >= want) return s;
+  return group;
+}
+// Bytes of the partial sums of a call, and of the largest call of up to n rows.
+int64_t part_bytes(int64_t n, int splits, int hkv, int hd) { return splits > 1 ? splits * 2 * n * hkv * hd * 4 : 0; }
+int64_t most_part_bytes(int n, int hkv, int group, int hd) {
+  int64_t most = 0;
+  for (int s = 2, below = 1; s <= group; ++s) {
+    if (group % s) continue;
+    // the next smaller split is not enough for this many tiles of 128 rows
+    const int64_t rows = ((3 * 148 + hkv * below - 1) / (hkv * below) - 1) * int64_t(128);
+    const int64_t x = part_bytes(rows < n ? rows : n, s, hkv, hd);
+    most = x > most ? x : most, below = s;
+  }
+  return most;
+}
+bool tensor_memory_size(int hd) { return hd == 64 || hd == 128; }
+
+template <int HD, class T>
+int launch_tc(const GradParams& p, cudaStream_t stream) {
+  using C = GradCfg<HD, T>;
+  const char* what = "prompt read grad";
+  CUtensorMap qmap, domap, kmap, vmap;
+  if (int s = prompt_map(what, p.q, p.s.hq, p.s.n, HD, 128, C::F16, &qmap)) return s;
+  if (int s = prompt_map(what, p.dout, p.s.hq, p.s.n, HD, 128, C::F16, &domap)) return s;
+  if (int s = prompt_map(what, p.k, p.s.hkv, p.s.n, HD, 128, C::F16, &kmap)) return s;
+  if (int s = prompt_map(what, p.v, p.s.hkv, p.s.n, HD, 128, C::F16, &vmap)) return s;
+  static std::atomic<uint64_t> configured{0};
+  if (int s = allow_smem(prompt_grad_tc_kernel<C>, C::SMEM, configured, "cudaFuncSetAttribute(prompt_grad)")) return s;
+  // the register shares the warps take must add up to what a block is launched with
+  static const int regs = [] {
+    cudaFuncAttributes a{};
+    return cudaFuncGetAttributes(&a, prompt_grad_tc_kernel<C>) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs != kLaunchRegs) return fail(FOLD_ERR_UNSUPPORTED, "prompt read grad: built with other register shares than launched");
+  const int64_t numbers = tile_numbers(p.s.n, p.s.b, 128), key_items = numbers * p.s.hkv * p.splits;
+  const int64_t blocks = key_items + numbers * p.s.hq;
+  if (blocks > 0x7fffffff) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: too many rows");
+  if (int s = launch_behind(prompt_grad_tc_kernel<C>, dim3(static_cast<unsigned>(blocks)), C::NTHREADS, C::SMEM, stream,
+                            "prompt_grad_tc_kernel", qmap, domap, kmap, vmap, p, static_cast<int>(key_items)))
+    return s;
+  if (p.splits == 1) return FOLD_OK;
+  const int64_t quads = static_cast<int64_t>(p.s.n) * p.s.hkv * (HD / 4);
+  if (quads > (int64_t(0x7fffffff) << 8)) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: too many rows");
+  return launch_behind(prompt_grad_join_kernel<T>, dim3(static_cast<unsigned>((quads + 255) / 256)), 256, 0, stream,
+                       "prompt_grad_join_kernel", p);
+}
+
 template <class T>
 int launch_grad(const GradParams& p, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(p.s.n) * p.s.hq;
@@ -257,7 +847,9 @@ int launch_grad(const GradParams& p, cudaStream_t stream) {
                             "prompt_delta_kernel", p))
     return s;
   const int hd = p.s.hd;
-  if (hd <= 64) return launch_mma<64, T>(p, stream);
+  if (hd == 64) return launch_tc<64, T>(p, stream);
+  if (hd == 128) return launch_tc<128, T>(p, stream);
+  if (hd < 64) return launch_mma<64, T>(p, stream);
   if (hd <= 96) return launch_mma<96, T>(p, stream);
   if (hd <= 128) return launch_mma<128, T>(p, stream);
   if (hd <= 192) return launch_mma<192, T>(p, stream);
@@ -271,7 +863,8 @@ extern "C" {
 
 int64_t fold_prompt_read_grad_workspace(int n, int hq, int hkv, int hd) {
   if (n < 0 || hq < 1 || hkv < 1 || hq % hkv || hq > 65535 || hd < 8 || hd > 256 || hd % 8) return -1;
-  return static_cast<int64_t>(n) * hq * 8 + 16;
+  const int64_t rows = (static_cast<int64_t>(n) * hq * 8 + 15) / 16 * 16;
+  return rows + 16 + (fold::tensor_memory_size(hd) ? fold::most_part_bytes(n, hkv, hq / hkv, hd) : 0);
 }
 
 int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_stride_head, const void* q,
@@ -300,10 +893,12 @@ int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_st
     if (int s = prompt_rows(what, r.name, r.ptr, r.tok, r.head, n, r.heads, hd, r.written, r.to)) return s;
   if (!lse) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: null pointer");
   if (static_cast<int64_t>(n) * hq > (int64_t(1) << 32)) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: too many rows");
-  if (!workspace || workspace_bytes < fold_prompt_read_grad_workspace(n, hq, hkv, hd))
+  p.splits = tensor_memory_size(hd) ? key_splits(n, hkv, p.s.group) : 1;
+  if (!workspace || workspace_bytes < (static_cast<int64_t>(n) * hq * 8 + 15) / 16 * 16 + part_bytes(n, p.splits, hkv, hd))
     return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: the workspace holds fold_prompt_read_grad_workspace bytes");
   if (!aligned16(workspace)) return fail(FOLD_ERR_ALIGNMENT, "prompt read grad: the workspace must be 16-byte aligned");
   p.lse = lse, p.dlse = dlse, p.row = static_cast<float2*>(workspace), p.zero_rest = zero_rest, p.err = err;
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (static_cast<int64_t>(n) * hq * 8 + 15) / 16 * 16);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == FOLD_BF16 ? launch_grad<__nv_bfloat16>(p, st) : launch_grad<__half>(p, st);
 }

@@ -174,6 +174,17 @@ def test_grad_of_lse(hd):
     check_grad(c, dlse=dlse)
 
 
+@pytest.mark.parametrize("hd", [64, 80, 128])
+@pytest.mark.parametrize("lens,window", [([1, 1, 1], (-1, -1)), ([300, 2], (0, 0))])
+def test_rows_of_one_key(lens, window, hd):
+    """A weight of 1 whatever the logit: queries and keys have no gradient but that of lse."""
+    c = Prompts(lens, 4, 2, hd, "fp16", seed=hd)
+    out, lse = read(c, True, window)
+    dq, dk, dv = grad(c, out, lse, True, window)
+    assert not bool(dq.any()) and not bool(dk.any()) and bool(dv.any())
+    check_grad(c, True, window, dlse=torch.randn(4, c.n, device="cuda", generator=torch.Generator("cuda").manual_seed(2)))
+
+
 def test_grad_long():
     check_grad(Prompts([1500, 700], 4, 1, 128, seed=6))
     check_grad(Prompts([1500, 700], 4, 1, 64, seed=6), True, (300, -1))
