@@ -234,6 +234,22 @@ __device__ __forceinline__ void fadd2(float& d0, float& d1, float a0, float a1, 
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
 
+// a0 *= b0 and a1 *= b1, and a0 -= b0 and a1 -= b1, as one packed two-lane FP32 instruction each.
+__device__ __forceinline__ void fmul2(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fsub2(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 x, y, m;\n\t"
+      "mov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tmov.b64 m, {%4, %4};\n\t"
+      "fma.rn.f32x2 x, y, m, x;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1), "f"(-1.f));
+}
+
 // 2^x through the SFU (x = -inf gives 0).
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;

@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           for (int c = 0; c < 64; ++c) d[c] = static_cast<uint32_t>(c - from) < seen ? d[c] : 0.f;
         }
 #pragma unroll
-        for (int c = 0; c < 64; ++c) d[c] *= v[c];
+        for (int c = 0; c < 64; c += 2) fmul2(d[c], d[c + 1], v[c], v[c + 1]);
         if (masked && __any_sync(0xffffffffu, own)) {
           const int self = r - col0 - wg * 64;
 #pragma unroll
@@ -488,7 +488,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           for (int k = 0; k < 16; ++k) {
             w[k] = pack_pair<T>(d[c + 2 * k], d[c + 2 * k + 1]);
             const float2 f = unpack_pair<T>(w[k]);
-            low[c / 2 + k] = pack_pair<T>(d[c + 2 * k] - f.x, d[c + 2 * k + 1] - f.y);
+            fsub2(d[c + 2 * k], d[c + 2 * k + 1], f.x, f.y);
+            low[c / 2 + k] = pack_pair<T>(d[c + 2 * k], d[c + 2 * k + 1]);
           }
           tmem_st16(x + 32 + c / 2, w);
         }
@@ -616,11 +617,12 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         tc_fence_after();
         const uint32_t a_lo = uniform(desc_lo(base + C::OFF_R + w * C::UNIT, 16));
         const uint32_t b_lo = uniform(desc_lo(base + (w == 0 ? 0 : C::OFF_B) + slot * C::UNIT, 16));
+        const uint32_t at = uniform(tm + to);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < HD / 16; ++k) {
             const uint32_t off = ((k >> 2) * C::CG + (k & 3) * 32) / 16;
-            mma_ss(tm + to, a_lo + off, hi, b_lo + off, hi, idesc_s, k > 0);
+            mma_ss(at, a_lo + off, hi, b_lo + off, hi, idesc_s, k > 0);
           }
           tc_commit(w == 0 ? &B.s_full : &B.dp_full);
           if (x.last) tc_commit(&B.r_empty[w]);
@@ -635,7 +637,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         const uint32_t x = (g & 1) * 128, y = x ^ 128;
         const uint32_t a_lo = uniform(desc_lo(base + (g % NA) * C::UNIT, C::CG));
         const uint32_t b_lo = uniform(desc_lo(base + C::OFF_B + (g % NB) * C::UNIT, C::CG));
-        const uint32_t more = uniform(now.first ? 0u : 1u);
+        const uint32_t more = uniform(now.first ? 0u : 1u), xa = uniform(tm + x);
         advance(next);
         if (!ok) break;
         if (now.keys) {
@@ -645,7 +647,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              mma_ts(tm + C::TMEM_ACC0, tm + x + (k >> 2) * 64 + (k & 3) * 8, b_lo + k * 128, hi, idesc_o, k > 0 ? 1 : more);
+              mma_ts(tm + C::TMEM_ACC0, xa + (k >> 2) * 64 + (k & 3) * 8, b_lo + k * 128, hi, idesc_o, k > 0 ? 1 : more);
             tc_commit(&B.acc0_done);
           }
           __syncwarp();
@@ -658,7 +660,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 16; ++k)  // the roundings, then what they left
-            mma_ts(tm + C::TMEM_ACC1, tm + x + (k < 8 ? 32 : 0) + ((k >> 2) & 1) * 64 + (k & 3) * 8, a_lo + (k & 7) * 128, hi, idesc_o,
+            mma_ts(tm + C::TMEM_ACC1, xa + (k < 8 ? 32 : 0) + ((k >> 2) & 1) * 64 + (k & 3) * 8, a_lo + (k & 7) * 128, hi, idesc_o,
                    k > 0 ? 1 : more);
           tc_commit(&B.a_empty[g % NA]);
           tc_commit(&B.b_empty[g % NB]);

@@ -392,10 +392,11 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         x.valid = false;
         if (!ok) return;
         tc_fence_after();
+        const uint32_t o = uniform(tm + C::TMEM_O + s * HD), pa = uniform(tm + C::TMEM_S + s * 128), v_lo = uniform(x.v_lo);
+        const uint32_t more = uniform(x.fresh);
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            mma_ts(tm + C::TMEM_O + s * HD, tm + C::TMEM_S + s * 128 + k * 8, x.v_lo + k * 128, hi, idesc_o, k > 0 ? 1 : x.fresh);
+          for (int k = 0; k < 8; ++k) mma_ts(o, pa + k * 8, v_lo + k * 128, hi, idesc_o, k > 0 ? 1 : more);
           if (x.free_v) tc_commit(&B.empty[x.v_slot]);
           if (x.last) tc_commit(&B.done[s]);
         }
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         const int kb = min(it.kb[0], it.kb[1]), ke = max(it.ke[0], it.ke[1]);
         for (int j = kb; ok && j < ke; ++j) {
           const uint32_t u = 2 * (tile0 + j - kb), ks = u % NU, vs = (u + 1) % NU;
-          const uint32_t k_lo = uniform(desc_lo(base + ks * C::UNIT, 16)), v_lo = uniform(desc_lo(base + vs * C::UNIT, C::CG));
+          const uint32_t k_lo = uniform(desc_lo(base + ks * C::UNIT, 16)), v_lo = desc_lo(base + vs * C::UNIT, C::CG);
           const bool in[2] = {j >= it.kb[0] && j < it.ke[0], j >= it.kb[1] && j < it.ke[1]};
           bool got_k = false;
 #pragma unroll
@@ -432,19 +433,20 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             if (!ok) break;
             tc_fence_after();
             const uint32_t q_lo = uniform(desc_lo(base + C::OFF_Q + slot * C::UNIT, 16));
+            const uint32_t at = uniform(tm + C::TMEM_S + s * 128);
             const bool last_q = j + 1 == it.ke[s], last_k = s == 1 || !in[1];
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < HD / 16; ++k) {
                 const uint32_t off = ((k >> 2) * C::CG + (k & 3) * 32) / 16;
-                mma_ss(tm + C::TMEM_S + s * 128, q_lo + off, hi, k_lo + off, hi, idesc_s, k > 0);
+                mma_ss(at, q_lo + off, hi, k_lo + off, hi, idesc_s, k > 0);
               }
               tc_commit(&B.s_full[s]);
               if (last_k) tc_commit(&B.empty[ks]);
               if (last_q) tc_commit(&B.q_empty[slot]);
             }
             __syncwarp();
-            st[s] = Step{v_lo, vs, ((u + 1) / NU) & 1, uniform(j > it.kb[s] ? 1u : 0u), true, last_q, last_k};
+            st[s] = Step{v_lo, vs, ((u + 1) / NU) & 1, j > it.kb[s] ? 1u : 0u, true, last_q, last_k};
             if (last_q) ++qcnt[s];
           }
         }
