@@ -274,15 +274,17 @@ int launch_mma(const GradParams& p, cudaStream_t stream) {
 // with (r0, r1, a, b) = (K, V, Q, dO) or (Q, dO, K, V): lanes of tensor memory are the resident rows. S and
 // dP have one place of 128 columns each, X and Y, which change places every tile: once dP is read, S of the
 // next tile goes over it, and dP of the next tile goes over what P and dS of this one were written to.
-// Order of the products: acc0 of this tile (P came while dP was computed), S of the next, acc1 of this, dP of
-// the next; the exponentials of a tile run beside acc1 and dP.
+// Order of the products: S of the next tile, acc0 of this one, acc1, dP of the next; dS runs beside S and acc0,
+// the exponentials of the next tile beside acc1 and dP.
 //
-// dS is held as two numbers of the type, its rounding and what that leaves, so that dq and dk are nearly those
-// of a dS in 32 bits; P of dv is rounded once.
+// P of dv is rounded once to the type. dS of a row that sees few keys is held as two numbers of the type, its
+// rounding and what that leaves: such rows have the largest gradients, and delta, from the rounded out, is least
+// exact for them (two_parts). Of other rows it is rounded once.
 template <int HD_, class T_>
 struct GradCfg {
   using T = T_;
   static constexpr int HD = HD_, NTHREADS = 384, NSW = 8;
+  static constexpr int NWG = NSW / 4, CW = 128 / NWG;  // softmax warpgroups; columns of a tile that each has
   static constexpr int NCG = HD / 64, CG = 128 * 128, UNIT = NCG * CG;
   static constexpr int NA = HD == 64 ? 4 : 3, NB = HD == 64 ? 4 : 2;  // a is needed longer: by S, then by acc1
   static constexpr int MISC = 1024 + 2048;
@@ -307,9 +309,11 @@ struct GradItem {
 constexpr int kItems = 3;
 
 struct GradBars {
-  uint64_t a_full[4], a_empty[4], b_full[4], b_empty[4];
-  uint64_t r_full[2], r_empty[2];
-  uint64_t s_full, dp_full, p_full, dp_read, acc0_done, ds_full, acc_done, drained;
+  uint64_t a_full[4], b_full[4], r_full[2];
+  // S may run a tile ahead of a softmax warp that has not looked yet; dP of a tile also tells the loads that the
+  // tile before is through (a commit takes the MMA warp some 200 cycles, so there is one for both)
+  uint64_t s_full[2], dp_full[4];
+  uint64_t p_full, dp_read, acc0_done, ds_full[2], acc_done, drained;
   uint64_t st_full[2], st_empty[2];
   uint64_t item_full[kItems], item_empty[kItems], asked;
   uint4 answer;
@@ -317,6 +321,34 @@ struct GradBars {
   GradItem item[kItems];
 };
 static_assert(sizeof(GradBars) <= 1024, "barriers fit their place");
+
+// Whether dS of the tile of rows from row0 on is held in two parts: where its last row sees up to 512 keys, or
+// 1024 if the rows before it see as many (behind a window, or without causality: gradients do not fall off there).
+__device__ __forceinline__ bool two_parts(const Shape& p, int len, int row0) {
+  const int r = min(row0 + 127, len - 1);
+  int lo, hi;
+  keys_of(p, len, r, r + 1, lo, hi);
+  const bool grows = p.right == 0 && p.left >= r;
+  return hi - lo <= (grows ? 512 : 1024);
+}
+
+// Columns of tensor memory that hold S (then P and dS) and dP of a tile. Keys' items change the two about, since
+// their two accumulators fill the rest; rows' items, with one, have a third place, so that S of the next tile need
+// not wait until dP of this one is read. The place of acc0 is only ever the spare one of a key's item.
+struct Places {
+  uint32_t s, d, spare;
+  bool keys;
+  __device__ __forceinline__ void start(bool k) { s = 0, d = 128, spare = 384, keys = k; }
+  // Moves to the next tile; true: its S lies where dP of this one was.
+  __device__ __forceinline__ bool step(bool next_keys) {
+    const bool over = next_keys ? spare == 384 : keys;
+    const uint32_t x = s;
+    if (over) s = d, d = x;
+    else s = spare, spare = x;
+    keys = next_keys;
+    return over;
+  }
+};
 
 template <class C>
 __global__ void __launch_bounds__(C::NTHREADS, 1)
@@ -331,14 +363,15 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (warp == NSW) {
     if (lane == 0) {
-      for (int i = 0; i < NA; ++i) mbar_init(&B.a_full[i], 1), mbar_init(&B.a_empty[i], 1);
-      for (int i = 0; i < NB; ++i) mbar_init(&B.b_full[i], 1), mbar_init(&B.b_empty[i], 1);
+      for (int i = 0; i < NA; ++i) mbar_init(&B.a_full[i], 1);
+      for (int i = 0; i < NB; ++i) mbar_init(&B.b_full[i], 1);
+      for (int i = 0; i < 4; ++i) mbar_init(&B.dp_full[i], 1);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&B.r_full[i], 1), mbar_init(&B.r_empty[i], 1);
+        mbar_init(&B.r_full[i], 1), mbar_init(&B.s_full[i], 1), mbar_init(&B.ds_full[i], NSW / 2);
         mbar_init(&B.st_full[i], 1), mbar_init(&B.st_empty[i], NSW);
       }
-      mbar_init(&B.s_full, 1), mbar_init(&B.dp_full, 1), mbar_init(&B.acc0_done, 1), mbar_init(&B.acc_done, 1);
-      mbar_init(&B.p_full, NSW), mbar_init(&B.dp_read, NSW), mbar_init(&B.ds_full, NSW);
+      mbar_init(&B.acc0_done, 1), mbar_init(&B.acc_done, 1);
+      mbar_init(&B.p_full, NSW), mbar_init(&B.dp_read, NSW);
       for (int i = 0; i < kItems; ++i) mbar_init(&B.item_full[i], 1), mbar_init(&B.item_empty[i], 3 + NSW);
       mbar_init(&B.asked, 1), mbar_init(&B.drained, 1);
       fence_mbar_init();
@@ -365,11 +398,14 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
   if (warp < NSW) {
     regs_up<kSoftmaxRegs>();
     // ------------------------------------------------------------ softmax
-    // a warp: 32 lanes (resident rows) and the half of a tile's columns that its warpgroup has
+    // a warp: 32 lanes (resident rows) and the half of a tile's columns that its warpgroup has. The half's 64
+    // columns of S take P and, when that has been read, the low part of dS in the first 32, dS in the others.
+    constexpr int CW = C::CW;
     const int wg = warp >> 2, res = (warp & 3) * 32 + lane;
-    const uint32_t mine = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + wg * 64;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), mine = lanes + wg * CW;
     const float* stat = reinterpret_cast<const float*>(smem + C::OFF_STAT);
-    uint32_t g = 0, gk = 0;  // tiles so far; of keys' items
+    uint32_t g = 0, gk = 0, g0 = 0;  // tiles so far; of keys' items; of those in two parts
+    Places at{};
     bool ok = true;
     for (int i = 0; ok; ++i) {
       GradItem it;
@@ -387,36 +423,40 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       if (!keys) rr = p.row[static_cast<int64_t>(it.head) * p.s.n + it.first + r];
       const int per = it.je - it.jb;
       for (int t = 0; t < it.nh * per; ++t, ++g) {
-        const int h = keys ? it.h0 + t / per : it.head, col0 = (it.jb + t % per) * 128;  // stream row of column 0
-        const uint32_t x = mine + (g & 1) * 128, y = mine + ((g & 1) ^ 1) * 128;
-        ok = warp_wait(&B.s_full, g & 1);
+        const int col0 = (it.jb + t % per) * 128;  // stream row of column 0
+        const bool two = two_parts(p.s, it.len, keys ? col0 : it.row0);
+        if (g == 0) at.start(keys);
+        else at.step(keys);
+        const uint32_t x = mine + at.s, y = mine + at.d;
+        ok = warp_wait(&B.s_full[g & 1], (g >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
-        float v[64];
-        tmem_ld32(x, v), tmem_ld32(x + 32, v + 32);
+        float v[CW];
+#pragma unroll
+        for (int c = 0; c < CW; c += 32) tmem_ld32(x + c, v + c);
         tmem_wait_ld();
-        const float* nl = stat + (gk & 1) * 256 + wg * 64;
+        const float* nl = stat + (gk & 1) * 256 + wg * CW;
         if (keys) {
           ok = warp_wait(&B.st_full[gk & 1], (gk >> 1) & 1);
           if (!ok) break;
 #pragma unroll
-          for (int c = 0; c < 64; c += 4) {
+          for (int c = 0; c < CW; c += 4) {
             const float4 a = *reinterpret_cast<const float4*>(nl + c);
             ffma2(v[c], v[c + 1], p.s.scale_log2, a.x, a.y);
             ffma2(v[c + 2], v[c + 3], p.s.scale_log2, a.z, a.w);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < 64; c += 2) ffma2(v[c], v[c + 1], p.s.scale_log2, rr.x, rr.x);
+          for (int c = 0; c < CW; c += 2) ffma2(v[c], v[c + 1], p.s.scale_log2, rr.x, rr.x);
         }
 #pragma unroll
-        for (int c = 0; c < 64; ++c) v[c] = fast_exp2(v[c]);
+        for (int c = 0; c < CW; ++c) v[c] = fast_exp2(v[c]);
         const bool masked = col0 < warp_lo || col0 + 128 > warp_hi;
-        const int from = lo - col0 - wg * 64;
+        const int from = lo - col0 - wg * CW;
         const uint32_t seen = static_cast<uint32_t>(hi - lo);
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c) v[c] = static_cast<uint32_t>(c - from) < seen ? v[c] : 0.f;
+          for (int c = 0; c < CW; ++c) v[c] = static_cast<uint32_t>(c - from) < seen ? v[c] : 0.f;
         }
         // rows behind the sequence's end belong to others (NaN included): zeros before the tensor cores read
         // them beside weights of zero
@@ -435,7 +475,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         }
         if (keys) {
 #pragma unroll
-          for (int c = 0; c < 64; c += 32) {
+          for (int c = 0; c < CW; c += 32) {
             uint32_t w[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) w[k] = pack_pair<T>(v[c + 2 * k], v[c + 2 * k + 1]);
@@ -446,18 +486,19 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&B.p_full);
         }
-        ok = warp_wait(&B.dp_full, g & 1);
+        ok = warp_wait(&B.dp_full[g & 3], (g >> 2) & 1);
         if (!ok) break;
         tc_fence_after();
-        float d[64];
-        tmem_ld32(y, d), tmem_ld32(y + 32, d + 32);
+        float d[CW];
+#pragma unroll
+        for (int c = 0; c < CW; c += 32) tmem_ld32(y + c, d + c);
         tmem_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&B.dp_read);
         if (keys) {
 #pragma unroll
-          for (int c = 0; c < 64; c += 4) {
+          for (int c = 0; c < CW; c += 4) {
             const float4 a = *reinterpret_cast<const float4*>(nl + 128 + c);
             ffma2(d[c], d[c + 1], Shift<T>::kDown, a.x, a.y);
             ffma2(d[c + 2], d[c + 3], Shift<T>::kDown, a.z, a.w);
@@ -466,76 +507,87 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (lane == 0) mbar_arrive(&B.st_empty[gk & 1]);
         } else {
 #pragma unroll
-          for (int c = 0; c < 64; c += 2) ffma2(d[c], d[c + 1], Shift<T>::kDown, rr.y, rr.y);
+          for (int c = 0; c < CW; c += 2) ffma2(d[c], d[c + 1], Shift<T>::kDown, rr.y, rr.y);
         }
         if (masked) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c) d[c] = static_cast<uint32_t>(c - from) < seen ? d[c] : 0.f;
+          for (int c = 0; c < CW; ++c) d[c] = static_cast<uint32_t>(c - from) < seen ? d[c] : 0.f;
         }
 #pragma unroll
-        for (int c = 0; c < 64; c += 2) fmul2(d[c], d[c + 1], v[c], v[c + 1]);
+        for (int c = 0; c < CW; c += 2) fmul2(d[c], d[c + 1], v[c], v[c + 1]);
         if (masked && __any_sync(0xffffffffu, own)) {
-          const int self = r - col0 - wg * 64;
+          const int self = r - col0 - wg * CW, h = keys ? it.h0 + t / per : it.head;
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
+          for (int c = 0; c < CW; ++c)
             if (own && c == self) d[c] = lone_ds<T>(p, h, it.first + r, v[c]);
         }
-        uint32_t low[32];
 #pragma unroll
-        for (int c = 0; c < 64; c += 32) {
+        for (int c = 0; c < CW; c += 32) {
           uint32_t w[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            w[k] = pack_pair<T>(d[c + 2 * k], d[c + 2 * k + 1]);
-            const float2 f = unpack_pair<T>(w[k]);
-            fsub2(d[c + 2 * k], d[c + 2 * k + 1], f.x, f.y);
-            low[c / 2 + k] = pack_pair<T>(d[c + 2 * k], d[c + 2 * k + 1]);
+          for (int k = 0; k < 16; ++k) w[k] = pack_pair<T>(d[c + 2 * k], d[c + 2 * k + 1]);
+          tmem_st16(x + CW / 2 + c / 2, w);
+          if (two) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const float2 f = unpack_pair<T>(w[k]);
+              fsub2(d[c + 2 * k], d[c + 2 * k + 1], f.x, f.y);
+            }
           }
-          tmem_st16(x + 32 + c / 2, w);
         }
-        if (keys) {  // P has been read
-          ok = warp_wait(&B.acc0_done, gk & 1);
-          if (!ok) break;
-          tc_fence_after();
-          ++gk;
+        if (two) {
+          if (keys) {  // P has been read
+            ok = warp_wait(&B.acc0_done, g0++ & 1);
+            if (!ok) break;
+            tc_fence_after();
+          }
+#pragma unroll
+          for (int c = 0; c < CW; c += 32) {
+            uint32_t w[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) w[k] = pack_pair<T>(d[c + 2 * k], d[c + 2 * k + 1]);
+            tmem_st16(x + c / 2, w);
+          }
         }
-        tmem_st16(x, low), tmem_st16(x + 16, low + 16);
+        if (keys) ++gk;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&B.ds_full);
+        if (lane == 0) mbar_arrive(&B.ds_full[wg * CW / 64]);
       }
       if (!ok) break;
       ok = warp_wait(&B.acc_done, i & 1);
       if (!ok) break;
       tc_fence_after();
-      // keys: a warpgroup each of dv and dk; rows: half of dq's columns each
-      const uint32_t acc = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) +
-                           (keys ? (wg == 0 ? C::TMEM_ACC0 : C::TMEM_ACC1) : C::TMEM_ACC1 + wg * (HD / 2));
-      const float f = keys && wg == 0 ? Shift<T>::kDown : p.s.scale;
-      const Rows& to = keys ? (wg == 0 ? p.dv : p.dk) : p.dq;
-      const int64_t at = it.first + r;
-      T* out = static_cast<T*>(to.ptr) + at * to.tok + it.head * to.head + (keys ? 0 : wg * (HD / 2));
-      float* part = p.part + ((static_cast<int64_t>(2 * it.split + 1 - wg) * p.s.n + at) * p.s.hkv + it.head) * HD;
+      // keys: half of the warpgroups for dv, half for dk; rows: dq's columns shared out
+      const bool dv = keys && wg < C::NWG / 2;
+      const int cols = keys ? HD * 2 / C::NWG : HD / C::NWG, c0 = (keys ? wg % (C::NWG / 2) : wg) * cols;
+      const uint32_t acc = lanes + (dv ? C::TMEM_ACC0 : C::TMEM_ACC1) + c0;
+      const float f = dv ? Shift<T>::kDown : p.s.scale;
+      const Rows& to = dv ? p.dv : keys ? p.dk : p.dq;
+      const int64_t row = it.first + r;
+      T* out = static_cast<T*>(to.ptr) + row * to.tok + it.head * to.head + c0;
+      float* part = p.part + ((static_cast<int64_t>(2 * it.split + dv) * p.s.n + row) * p.s.hkv + it.head) * HD + c0;
       const bool partial = keys && p.splits > 1;
 #pragma unroll 1
-      for (int c = 0; c < (keys ? HD : HD / 2); c += 32) {
-        float o[32];
-        tmem_ld32(acc + c, o);
-        tmem_wait_ld();
+      for (int c = 0; c < cols; c += 16) {
+        float o[16];
+        __syncwarp();
+        tmem_ld16(acc + c, o);
         if (!live) continue;
         if (partial) {
 #pragma unroll
-          for (int k = 0; k < 32; k += 4)
+          for (int k = 0; k < 16; k += 4)
             *reinterpret_cast<float4*>(part + c + k) = make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f);
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; k += 8)
+          for (int k = 0; k < 16; k += 8)
             *reinterpret_cast<uint4*>(out + c + k) =
                 make_uint4(pack_pair<T>(o[k] * f, o[k + 1] * f), pack_pair<T>(o[k + 2] * f, o[k + 3] * f),
                            pack_pair<T>(o[k + 4] * f, o[k + 5] * f), pack_pair<T>(o[k + 6] * f, o[k + 7] * f));
         }
       }
+      __syncwarp();
       tc_fence_before();  // the next item's products come behind its first tile's P or dS
     }
     if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
@@ -546,6 +598,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       uint32_t g = 0, items = 0;
       bool ok = true;
       if (lane == 0) prefetch_tensormap(&qmap), prefetch_tensormap(&domap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
+      // dP of tile n, and with it all products of the tiles before
+      auto through = [&](uint32_t n) { return warp_wait(&B.dp_full[n & 3], (n >> 2) & 1); };
       auto load = [&](const CUtensorMap* map, int offset, uint64_t* full, int head, int row) {
         if (lane == 0) {
           mbar_arrive_expect_tx(full, C::UNIT);
@@ -563,20 +617,18 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         for (int t = 0; ok && t < it.nh * per; ++t, ++g) {
           const int row = it.first + (it.jb + t % per) * 128, head = it.h0 + t / per;
           if (t == 0) {
-            if (i > 0) ok = warp_wait(&B.r_empty[0], (i - 1) & 1);
+            if (i > 0) ok = through(g - 1);
             if (!ok) break;
             load(keys ? &kmap : &qmap, C::OFF_R, &B.r_full[0], it.head, it.first + it.row0);
           }
-          if (g >= NA) ok = warp_wait(&B.a_empty[g % NA], (g / NA - 1) & 1);
+          if (g >= NA) ok = through(g - NA + 1);
           if (!ok) break;
           load(keys ? &qmap : &kmap, (g % NA) * C::UNIT, &B.a_full[g % NA], head, row);
           if (t == 0) {
-            if (i > 0) ok = warp_wait(&B.r_empty[1], (i - 1) & 1);
-            if (!ok) break;
             load(keys ? &vmap : &domap, C::OFF_R + C::UNIT, &B.r_full[1], it.head, it.first + it.row0);
             items = i + 1;
           }
-          if (g >= NB) ok = warp_wait(&B.b_empty[g % NB], (g / NB - 1) & 1);
+          if (g >= NB) ok = through(g - NB + 1);
           if (!ok) break;
           load(keys ? &domap : &vmap, C::OFF_B + (g % NB) * C::UNIT, &B.b_full[g % NB], head, row);
         }
@@ -591,55 +643,86 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       constexpr uint32_t idesc_s = idesc_of(C::F16, 128, 0), idesc_o = idesc_of(C::F16, HD, 1), hi = desc_hi(1024);
       const uint32_t base = uniform(smem_u32(smem)), tm = uniform(tmem);
       GradItem it;
-      int item = 0, t = 0, per = 1, total = 0;  // next item; place in the current one
+      int items = 0, j = 0, heads = 0;  // items so far; the next tile's place in the current one, heads left
+      uint32_t n = 0;                   // tiles so far
       bool ok = true;
-      struct Tile1 {
-        bool valid, keys, first, last;
-      } now{}, next{};
-      uint32_t gk = 0;  // tiles of keys' items
-      auto advance = [&](Tile1& x) {  // the tile behind
-        if (t == total) {
+      struct Step {
+        bool valid, keys, first, last, two;
+        uint32_t item;         // parity
+        uint32_t s, d, a, b;   // columns of S and dP; a's and b's shared memory, 16-byte units
+        uint32_t over, afresh; // S lies where dP of the tile before was; acc0 of a key's item may lie in its place
+      } now{}, next{}, then{};
+      Places at{};
+      bool was_keys[2] = {false, false};  // of the two tiles before
+      auto advance = [&](Step& x) {  // the tile behind the last one
+        if (heads == 0) {
           x.valid = false;
-          ok = next_item(item, it);
+          ok = next_item(items, it);
           if (!ok || it.keys < 0) return;
-          ++item, t = 0, per = it.je - it.jb, total = it.nh * per;
+          ++items, j = it.jb, heads = it.nh;
         }
-        x = Tile1{true, it.keys == 1, t == 0, t + 1 == total};
-        ++t;
+        x.valid = true, x.keys = it.keys == 1, x.item = (items - 1) & 1;
+        x.first = heads == it.nh && j == it.jb;
+        x.two = two_parts(p.s, it.len, x.keys ? j * 128 : it.row0);
+        if (++j == it.je) j = it.jb, --heads;
+        x.last = heads == 0;
+        if (n == 0) at.start(x.keys), x.over = 0;
+        else x.over = at.step(x.keys);
+        x.afresh = was_keys[1];
+        was_keys[1] = was_keys[0], was_keys[0] = x.keys;
+        x.s = uniform(tm + at.s), x.d = uniform(tm + at.d);
+        x.a = uniform((base + (n % NA) * C::UNIT) >> 4), x.b = uniform((base + C::OFF_B + (n % NB) * C::UNIT) >> 4);
+        ++n;
       };
-      // S or dP of tile n (the CTA's), resident tile w, into column `to`
-      auto product_ss = [&](const Tile1& x, int w, uint32_t n, uint32_t to) {
-        const uint32_t slot = w == 0 ? n % NA : n % NB, use = w == 0 ? n / NA : n / NB;
-        if (x.first) ok = mbar_wait(&B.r_full[w], (item - 1) & 1);
+      constexpr uint32_t kmajor = 1u << 16, mnmajor = static_cast<uint32_t>(C::CG >> 4) << 16;  // leading offsets
+      const uint32_t r0 = uniform(desc_lo(base + C::OFF_R, 16)), r1 = uniform(desc_lo(base + C::OFF_R + C::UNIT, 16));
+      auto landed = [&](const Step& x, int w, uint32_t g) {  // the operands of S (w 0) or dP (1)
+        const uint32_t slot = w == 0 ? g % NA : g % NB, use = w == 0 ? g / NA : g / NB;
+        if (x.first) ok = ok && mbar_wait(&B.r_full[w], x.item);
         ok = ok && mbar_wait(w == 0 ? &B.a_full[slot] : &B.b_full[slot], use & 1);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t a_lo = uniform(desc_lo(base + C::OFF_R + w * C::UNIT, 16));
-        const uint32_t b_lo = uniform(desc_lo(base + (w == 0 ? 0 : C::OFF_B) + slot * C::UNIT, 16));
-        const uint32_t at = uniform(tm + to);
-        if (elect_one()) {
+      };
+      auto product = [&](uint32_t to, uint32_t r, uint32_t x) {  // by one lane
 #pragma unroll
-          for (int k = 0; k < HD / 16; ++k) {
-            const uint32_t off = ((k >> 2) * C::CG + (k & 3) * 32) / 16;
-            mma_ss(at, a_lo + off, hi, b_lo + off, hi, idesc_s, k > 0);
-          }
-          tc_commit(w == 0 ? &B.s_full : &B.dp_full);
-          if (x.last) tc_commit(&B.r_empty[w]);
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t off = ((k >> 2) * C::CG + (k & 3) * 32) / 16;
+          mma_ss(to, r + off, hi, x + kmajor + off, hi, idesc_s, k > 0);
+        }
+      };
+      uint32_t gk = 0, g = 0;
+      advance(now);
+      if (ok && now.valid) {
+        landed(now, 0, 0);
+        tc_fence_after();
+        if (ok && elect_one()) {
+          product(now.s, r0, now.a);
+          tc_commit(&B.s_full[0]);
         }
         __syncwarp();
-      };
-      advance(now);
-      uint32_t g = 0;
-      if (ok && now.valid) product_ss(now, 0, 0, 0);
-      if (ok && now.valid) product_ss(now, 1, 0, 128);
+        if (ok) landed(now, 1, 0);
+        tc_fence_after();
+        if (ok && elect_one()) {
+          product(now.d, r1, now.b);
+          tc_commit(&B.dp_full[0]);
+        }
+        __syncwarp();
+        if (ok) advance(next);
+        if (ok && next.valid) landed(next, 0, 1);
+      }
       while (ok && now.valid) {
-        const uint32_t x = (g & 1) * 128, y = x ^ 128;
-        const uint32_t a_lo = uniform(desc_lo(base + (g % NA) * C::UNIT, C::CG));
-        const uint32_t b_lo = uniform(desc_lo(base + C::OFF_B + (g % NB) * C::UNIT, C::CG));
-        const uint32_t more = uniform(now.first ? 0u : 1u), xa = uniform(tm + x);
-        advance(next);
-        if (!ok) break;
+        const uint32_t more = uniform(now.first ? 0u : 1u), xa = uniform(now.s), am = uniform(now.a + mnmajor), bm = uniform(now.b + mnmajor);
+        if (next.valid) {
+          // S of the next tile first: the softmax warps come to it when they are through with dS
+          const uint32_t s_at = uniform(next.s), xb = uniform(next.a);
+          if (next.over || next.afresh) ok = warp_wait(&B.dp_read, g & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            product(s_at, r0, xb);
+            tc_commit(&B.s_full[(g + 1) & 1]);
+          }
+          __syncwarp();
+        }
         if (now.keys) {
           ok = warp_wait(&B.p_full, gk++ & 1);
           if (!ok) break;
@@ -647,28 +730,45 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              mma_ts(tm + C::TMEM_ACC0, xa + (k >> 2) * 64 + (k & 3) * 8, b_lo + k * 128, hi, idesc_o, k > 0 ? 1 : more);
-            tc_commit(&B.acc0_done);
+              mma_ts(tm + C::TMEM_ACC0, xa + (k * 16 / C::CW) * C::CW + k * 16 % C::CW / 2, bm + k * 128, hi, idesc_o, k > 0 ? 1 : more);
+            if (now.two) tc_commit(&B.acc0_done);
           }
           __syncwarp();
         }
-        ok = warp_wait(&B.dp_read, g & 1);
-        if (ok && next.valid) product_ss(next, 0, g + 1, y);
-        ok = ok && warp_wait(&B.ds_full, g & 1);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < 16; ++k)  // the roundings, then what they left
-            mma_ts(tm + C::TMEM_ACC1, xa + (k < 8 ? 32 : 0) + ((k >> 2) & 1) * 64 + (k & 3) * 8, a_lo + (k & 7) * 128, hi, idesc_o,
-                   k > 0 ? 1 : more);
-          tc_commit(&B.a_empty[g % NA]);
-          tc_commit(&B.b_empty[g % NB]);
-          if (now.last) tc_commit(&B.acc_done);
+        // what the next steps need, while dS is on its way
+        if (next.valid) {
+          advance(then);
+          landed(next, 1, g + 1);
         }
-        __syncwarp();
-        if (next.valid) product_ss(next, 1, g + 1, x);
-        now = next, ++g;
+        const uint32_t d_at = uniform(next.d), xd = uniform(next.b);
+#pragma unroll
+        for (int half = 0; ok && half < 2; ++half) {
+          ok = warp_wait(&B.ds_full[half], g & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = half * 4; k < half * 4 + 4; ++k)
+              mma_ts(tm + C::TMEM_ACC1, xa + (k * 16 / C::CW) * C::CW + k * 16 % C::CW / 2 + C::CW / 2, am + k * 128, hi, idesc_o, k > 0 ? 1 : more);
+            if (now.two) {  // what the roundings left
+#pragma unroll
+              for (int k = half * 4; k < half * 4 + 4; ++k)
+                mma_ts(tm + C::TMEM_ACC1, xa + (k * 16 / C::CW) * C::CW + k * 16 % C::CW / 2, am + k * 128, hi, idesc_o, 1);
+            }
+            if (half == 1) {
+              if (now.last) tc_commit(&B.acc_done);
+              if (next.valid) {
+                product(d_at, r1, xd);
+                tc_commit(&B.dp_full[(g + 1) & 3]);
+              }
+            }
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        now = next, next = then, then.valid = false;
+        ++g;
+        if (now.valid && next.valid) landed(next, 0, g + 1);
       }
       if (!ok) {  // let what was issued finish before tensor memory goes
         if (elect_one()) {

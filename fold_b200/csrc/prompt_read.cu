@@ -316,6 +316,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         float o[32];
+        __syncwarp();
         tmem_ld32(oa + c, o);
         tmem_wait_ld();
         if (live) {
