@@ -648,12 +648,13 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       bool ok = true;
       struct Step {
         bool valid, keys, first, last, two;
-        uint32_t item;         // parity
-        uint32_t s, d, a, b;   // columns of S and dP; a's and b's shared memory, 16-byte units
-        uint32_t over, afresh; // S lies where dP of the tile before was; acc0 of a key's item may lie in its place
-      } now{}, next{}, then{};
+        uint32_t item;              // parity
+        uint32_t s, d, aslot, bslot;
+        bool early;                 // S may come before dP of the tile before has been read
+      } now{}, next{};
       Places at{};
       bool was_keys[2] = {false, false};  // of the two tiles before
+      uint32_t aslot = 0, bslot = 0;
       auto advance = [&](Step& x) {  // the tile behind the last one
         if (heads == 0) {
           x.valid = false;
@@ -666,22 +667,30 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         x.two = two_parts(p.s, it.len, x.keys ? j * 128 : it.row0);
         if (++j == it.je) j = it.jb, --heads;
         x.last = heads == 0;
-        if (n == 0) at.start(x.keys), x.over = 0;
-        else x.over = at.step(x.keys);
-        x.afresh = was_keys[1];
+        bool over = false;
+        if (n == 0) at.start(x.keys);
+        else over = at.step(x.keys);
+        // (the spare place of the first rows behind a key's item may still be read as its acc0)
+        x.early = !over && !was_keys[1];
         was_keys[1] = was_keys[0], was_keys[0] = x.keys;
-        x.s = uniform(tm + at.s), x.d = uniform(tm + at.d);
-        x.a = uniform((base + (n % NA) * C::UNIT) >> 4), x.b = uniform((base + C::OFF_B + (n % NB) * C::UNIT) >> 4);
+        x.s = at.s, x.d = at.d, x.aslot = aslot, x.bslot = bslot;
+        if (++aslot == NA) aslot = 0;
+        if (++bslot == NB) bslot = 0;
         ++n;
       };
       constexpr uint32_t kmajor = 1u << 16, mnmajor = static_cast<uint32_t>(C::CG >> 4) << 16;  // leading offsets
       const uint32_t r0 = uniform(desc_lo(base + C::OFF_R, 16)), r1 = uniform(desc_lo(base + C::OFF_R + C::UNIT, 16));
-      auto landed = [&](const Step& x, int w, uint32_t g) {  // the operands of S (w 0) or dP (1)
-        const uint32_t slot = w == 0 ? g % NA : g % NB, use = w == 0 ? g / NA : g / NB;
+      uint32_t aphase = 0, bphase = 0;  // parities of the rings, a bit a slot
+      auto landed = [&](const Step& x, int w) {  // the operands of S (w 0) or dP (1)
+        const uint32_t slot = w == 0 ? x.aslot : x.bslot;
+        uint32_t& phase = w == 0 ? aphase : bphase;
         if (x.first) ok = ok && mbar_wait(&B.r_full[w], x.item);
-        ok = ok && mbar_wait(w == 0 ? &B.a_full[slot] : &B.b_full[slot], use & 1);
+        ok = ok && mbar_wait(w == 0 ? &B.a_full[slot] : &B.b_full[slot], phase >> slot & 1);
+        phase ^= 1u << slot;
         ok = __all_sync(0xffffffffu, ok);
       };
+      auto a_at = [&](const Step& x) { return (base + x.aslot * C::UNIT) >> 4; };
+      auto b_at = [&](const Step& x) { return (base + C::OFF_B + x.bslot * C::UNIT) >> 4; };
       auto product = [&](uint32_t to, uint32_t r, uint32_t x) {  // by one lane
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
@@ -692,33 +701,39 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       uint32_t gk = 0, g = 0;
       advance(now);
       if (ok && now.valid) {
-        landed(now, 0, 0);
+        const uint32_t s_at = uniform(tm + now.s), d_at = uniform(tm + now.d), xa = uniform(a_at(now)), xb = uniform(b_at(now));
+        landed(now, 0);
         tc_fence_after();
         if (ok && elect_one()) {
-          product(now.s, r0, now.a);
+          product(s_at, r0, xa);
           tc_commit(&B.s_full[0]);
         }
         __syncwarp();
-        if (ok) landed(now, 1, 0);
+        if (ok) landed(now, 1);
         tc_fence_after();
         if (ok && elect_one()) {
-          product(now.d, r1, now.b);
+          product(d_at, r1, xb);
           tc_commit(&B.dp_full[0]);
         }
         __syncwarp();
-        if (ok) advance(next);
-        if (ok && next.valid) landed(next, 0, 1);
       }
       while (ok && now.valid) {
-        const uint32_t more = uniform(now.first ? 0u : 1u), xa = uniform(now.s), am = uniform(now.a + mnmajor), bm = uniform(now.b + mnmajor);
+        // The issue of MMAs lasts about as long as they run, so all else comes where it hides behind the last
+        // ones issued, dP's.
+        const uint32_t more = uniform(now.first ? 0u : 1u), x = uniform(tm + now.s);
+        const uint32_t am = uniform(a_at(now) + mnmajor), bm = uniform(b_at(now) + mnmajor);
+        advance(next);
+        const uint32_t s_at = uniform(tm + next.s), d_at = uniform(tm + next.d);
+        const uint32_t xa = uniform(a_at(next)), xb = uniform(b_at(next));
+        if (!ok) break;
         if (next.valid) {
           // S of the next tile first: the softmax warps come to it when they are through with dS
-          const uint32_t s_at = uniform(next.s), xb = uniform(next.a);
-          if (next.over || next.afresh) ok = warp_wait(&B.dp_read, g & 1);
+          landed(next, 0);
+          if (ok && !next.early) ok = warp_wait(&B.dp_read, g & 1);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            product(s_at, r0, xb);
+            product(s_at, r0, xa);
             tc_commit(&B.s_full[(g + 1) & 1]);
           }
           __syncwarp();
@@ -730,17 +745,12 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              mma_ts(tm + C::TMEM_ACC0, xa + (k * 16 / C::CW) * C::CW + k * 16 % C::CW / 2, bm + k * 128, hi, idesc_o, k > 0 ? 1 : more);
+              mma_ts(tm + C::TMEM_ACC0, x + (k * 16 / C::CW) * C::CW + k * 16 % C::CW / 2, bm + k * 128, hi, idesc_o, k > 0 ? 1 : more);
             if (now.two) tc_commit(&B.acc0_done);
           }
           __syncwarp();
         }
-        // what the next steps need, while dS is on its way
-        if (next.valid) {
-          advance(then);
-          landed(next, 1, g + 1);
-        }
-        const uint32_t d_at = uniform(next.d), xd = uniform(next.b);
+        if (next.valid) landed(next, 1);
 #pragma unroll
         for (int half = 0; ok && half < 2; ++half) {
           ok = warp_wait(&B.ds_full[half], g & 1);
@@ -749,16 +759,16 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (elect_one()) {
 #pragma unroll
             for (int k = half * 4; k < half * 4 + 4; ++k)
-              mma_ts(tm + C::TMEM_ACC1, xa + (k * 16 / C::CW) * C::CW + k * 16 % C::CW / 2 + C::CW / 2, am + k * 128, hi, idesc_o, k > 0 ? 1 : more);
+              mma_ts(tm + C::TMEM_ACC1, x + (k * 16 / C::CW) * C::CW + k * 16 % C::CW / 2 + C::CW / 2, am + k * 128, hi, idesc_o, k > 0 ? 1 : more);
             if (now.two) {  // what the roundings left
 #pragma unroll
               for (int k = half * 4; k < half * 4 + 4; ++k)
-                mma_ts(tm + C::TMEM_ACC1, xa + (k * 16 / C::CW) * C::CW + k * 16 % C::CW / 2, am + k * 128, hi, idesc_o, 1);
+                mma_ts(tm + C::TMEM_ACC1, x + (k * 16 / C::CW) * C::CW + k * 16 % C::CW / 2, am + k * 128, hi, idesc_o, 1);
             }
             if (half == 1) {
               if (now.last) tc_commit(&B.acc_done);
               if (next.valid) {
-                product(d_at, r1, xd);
+                product(d_at, r1, xb);
                 tc_commit(&B.dp_full[(g + 1) & 3]);
               }
             }
@@ -766,9 +776,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           __syncwarp();
         }
         if (!ok) break;
-        now = next, next = then, then.valid = false;
-        ++g;
-        if (now.valid && next.valid) landed(next, 0, g + 1);
+        now = next, ++g;
       }
       if (!ok) {  // let what was issued finish before tensor memory goes
         if (elect_one()) {
