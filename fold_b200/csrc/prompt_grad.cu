@@ -313,7 +313,7 @@ struct GradBars {
   // S may run a tile ahead of a softmax warp that has not looked yet; dP of a tile also tells the loads that the
   // tile before is through (a commit takes the MMA warp some 200 cycles, so there is one for both)
   uint64_t s_full[2], dp_full[4];
-  uint64_t p_full, dp_read, acc0_done, ds_full[2], acc_done, drained;
+  uint64_t p_full[2], dp_read, acc0_done, ds_full[2], acc_done, drained;
   uint64_t st_full[2], st_empty[2];
   uint64_t item_full[kItems], item_empty[kItems], asked;
   uint4 answer;
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         mbar_init(&B.st_full[i], 1), mbar_init(&B.st_empty[i], NSW);
       }
       mbar_init(&B.acc0_done, 1), mbar_init(&B.acc_done, 1);
-      mbar_init(&B.p_full, NSW), mbar_init(&B.dp_read, NSW);
+      mbar_init(&B.p_full[0], NSW), mbar_init(&B.p_full[1], NSW), mbar_init(&B.dp_read, NSW);
       for (int i = 0; i < kItems; ++i) mbar_init(&B.item_full[i], 1), mbar_init(&B.item_empty[i], 3 + NSW);
       mbar_init(&B.asked, 1), mbar_init(&B.drained, 1);
       fence_mbar_init();
@@ -421,10 +421,10 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       const bool own = lone(p.s, it.len, r);
       float2 rr = make_float2(0.f, 0.f);
       if (!keys) rr = p.row[static_cast<int64_t>(it.head) * p.s.n + it.first + r];
-      const int per = it.je - it.jb;
-      for (int t = 0; t < it.nh * per; ++t, ++g) {
-        const int col0 = (it.jb + t % per) * 128;  // stream row of column 0
-        const bool two = two_parts(p.s, it.len, keys ? col0 : it.row0);
+      bool two = !keys && two_parts(p.s, it.len, it.row0);
+      for (int h = 0, j = it.jb; h < it.nh; ++g) {
+        const int col0 = j * 128;  // stream row of column 0
+        if (keys) two = two_parts(p.s, it.len, col0);
         if (g == 0) at.start(keys);
         else at.step(keys);
         const uint32_t x = mine + at.s, y = mine + at.d;
@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&B.p_full);
+          if (lane == 0) mbar_arrive(&B.p_full[gk & 1]);
         }
         ok = warp_wait(&B.dp_full[g & 3], (g >> 2) & 1);
         if (!ok) break;
@@ -516,10 +516,10 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
 #pragma unroll
         for (int c = 0; c < CW; c += 2) fmul2(d[c], d[c + 1], v[c], v[c + 1]);
         if (masked && __any_sync(0xffffffffu, own)) {
-          const int self = r - col0 - wg * CW, h = keys ? it.h0 + t / per : it.head;
+          const int self = r - col0 - wg * CW, head = keys ? it.h0 + h : it.head;
 #pragma unroll
           for (int c = 0; c < CW; ++c)
-            if (own && c == self) d[c] = lone_ds<T>(p, h, it.first + r, v[c]);
+            if (own && c == self) d[c] = lone_ds<T>(p, head, it.first + r, v[c]);
         }
 #pragma unroll
         for (int c = 0; c < CW; c += 32) {
@@ -554,6 +554,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&B.ds_full[wg * CW / 64]);
+        if (++j == it.je) j = it.jb, ++h;
       }
       if (!ok) break;
       ok = warp_wait(&B.acc_done, i & 1);
@@ -613,10 +614,11 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         ok = next_item(i, it);
         if (!ok || it.keys < 0) break;
         const bool keys = it.keys == 1;
-        const int per = it.je - it.jb;
-        for (int t = 0; ok && t < it.nh * per; ++t, ++g) {
-          const int row = it.first + (it.jb + t % per) * 128, head = it.h0 + t / per;
-          if (t == 0) {
+        for (int h = 0, j = it.jb; ok && h < it.nh; ++g) {
+          const int row = it.first + j * 128, head = it.h0 + h;
+          const bool first = h == 0 && j == it.jb;
+          if (++j == it.je) j = it.jb, ++h;
+          if (first) {
             if (i > 0) ok = through(g - 1);
             if (!ok) break;
             load(keys ? &kmap : &qmap, C::OFF_R, &B.r_full[0], it.head, it.first + it.row0);
@@ -624,7 +626,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (g >= NA) ok = through(g - NA + 1);
           if (!ok) break;
           load(keys ? &qmap : &kmap, (g % NA) * C::UNIT, &B.a_full[g % NA], head, row);
-          if (t == 0) {
+          if (first) {
             load(keys ? &vmap : &domap, C::OFF_R + C::UNIT, &B.r_full[1], it.head, it.first + it.row0);
             items = i + 1;
           }
@@ -739,7 +741,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           __syncwarp();
         }
         if (now.keys) {
-          ok = warp_wait(&B.p_full, gk++ & 1);
+          ok = warp_wait(&B.p_full[gk & 1], gk >> 1 & 1);
+          ++gk;
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -796,10 +799,10 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         ok = next_item(i, it);
         if (!ok || it.keys < 0) break;
         if (it.keys == 0) continue;
-        const int per = it.je - it.jb;
-        for (int t = 0; t < it.nh * per; ++t, ++gk) {
-          const int r0 = (it.jb + t % per) * 128;
-          const float2* src = p.row + static_cast<int64_t>(it.h0 + t / per) * p.s.n + it.first + r0;
+        for (int h = 0, j = it.jb; h < it.nh; ++gk) {
+          const int r0 = j * 128;
+          const float2* src = p.row + static_cast<int64_t>(it.h0 + h) * p.s.n + it.first + r0;
+          if (++j == it.je) j = it.jb, ++h;
           float2 v[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
