@@ -266,7 +266,8 @@ int launch_mma(const GradParams& p, cudaStream_t stream) {
                        128, smem, stream, "prompt_grad_mma_kernel", p);
 }
 
-// ---------------------------------------------------------------- tcgen05, head sizes 64 and 128
+// ---------------------------------------------------------------- tcgen05, head sizes up to 128
+// Heads of other sizes than 64 and 128 are loaded with zeros behind them (outside of the maps).
 // A block takes an item: 128 keys of one KV head with the rows of some of its group's heads (dk, dv), or 128
 // rows of one head with their keys (dq). Both are the same work: two resident tiles r0, r1 and a stream of
 // tiles a, b,
@@ -568,7 +569,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       const Rows& to = dv ? p.dv : keys ? p.dk : p.dq;
       const int64_t row = it.first + r;
       T* out = static_cast<T*>(to.ptr) + row * to.tok + it.head * to.head + c0;
-      float* part = p.part + ((static_cast<int64_t>(2 * it.split + dv) * p.s.n + row) * p.s.hkv + it.head) * HD + c0;
+      float* part = p.part + ((static_cast<int64_t>(2 * it.split + dv) * p.s.n + row) * p.s.hkv + it.head) * p.s.hd + c0;
       const bool partial = keys && p.splits > 1;
 #pragma unroll 1
       for (int c = 0; c < cols; c += 16) {
@@ -579,12 +580,13 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         if (partial) {
 #pragma unroll
           for (int k = 0; k < 16; k += 4)
-            *reinterpret_cast<float4*>(part + c + k) = make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f);
+            if (c0 + c + k < p.s.hd)
+              *reinterpret_cast<float4*>(part + c + k) = make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f);
         } else {
 #pragma unroll
           for (int k = 0; k < 16; k += 8)
-            *reinterpret_cast<uint4*>(out + c + k) =
-                make_uint4(pack_pair<T>(o[k] * f, o[k + 1] * f), pack_pair<T>(o[k + 2] * f, o[k + 3] * f),
+            if (c0 + c + k < p.s.hd)
+              *reinterpret_cast<uint4*>(out + c + k) = make_uint4(pack_pair<T>(o[k] * f, o[k + 1] * f), pack_pair<T>(o[k + 2] * f, o[k + 3] * f),
                            pack_pair<T>(o[k + 4] * f, o[k + 5] * f), pack_pair<T>(o[k + 6] * f, o[k + 7] * f));
         }
       }
@@ -921,17 +923,17 @@ int64_t most_part_bytes(int n, int hkv, int group, int hd) {
   }
   return most;
 }
-bool tensor_memory_size(int hd) { return hd == 64 || hd == 128; }
+bool tensor_memory_size(int hd) { return hd <= 128; }
 
 template <int HD, class T>
 int launch_tc(const GradParams& p, cudaStream_t stream) {
   using C = GradCfg<HD, T>;
   const char* what = "prompt read grad";
   CUtensorMap qmap, domap, kmap, vmap;
-  if (int s = prompt_map(what, p.q, p.s.hq, p.s.n, HD, 128, C::F16, &qmap)) return s;
-  if (int s = prompt_map(what, p.dout, p.s.hq, p.s.n, HD, 128, C::F16, &domap)) return s;
-  if (int s = prompt_map(what, p.k, p.s.hkv, p.s.n, HD, 128, C::F16, &kmap)) return s;
-  if (int s = prompt_map(what, p.v, p.s.hkv, p.s.n, HD, 128, C::F16, &vmap)) return s;
+  if (int s = prompt_map(what, p.q, p.s.hq, p.s.n, p.s.hd, 128, C::F16, &qmap)) return s;
+  if (int s = prompt_map(what, p.dout, p.s.hq, p.s.n, p.s.hd, 128, C::F16, &domap)) return s;
+  if (int s = prompt_map(what, p.k, p.s.hkv, p.s.n, p.s.hd, 128, C::F16, &kmap)) return s;
+  if (int s = prompt_map(what, p.v, p.s.hkv, p.s.n, p.s.hd, 128, C::F16, &vmap)) return s;
   static std::atomic<uint64_t> configured{0};
   if (int s = allow_smem(prompt_grad_tc_kernel<C>, C::SMEM, configured, "cudaFuncSetAttribute(prompt_grad)")) return s;
   // the register shares the warps take must add up to what a block is launched with
@@ -947,7 +949,7 @@ int launch_tc(const GradParams& p, cudaStream_t stream) {
                             "prompt_grad_tc_kernel", qmap, domap, kmap, vmap, p, static_cast<int>(key_items)))
     return s;
   if (p.splits == 1) return FOLD_OK;
-  const int64_t quads = static_cast<int64_t>(p.s.n) * p.s.hkv * (HD / 4);
+  const int64_t quads = static_cast<int64_t>(p.s.n) * p.s.hkv * (p.s.hd / 4);
   if (quads > (int64_t(0x7fffffff) << 8)) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: too many rows");
   return launch_behind(prompt_grad_join_kernel<T>, dim3(static_cast<unsigned>((quads + 255) / 256)), 256, 0, stream,
                        "prompt_grad_join_kernel", p);
@@ -960,11 +962,8 @@ int launch_grad(const GradParams& p, cudaStream_t stream) {
                             "prompt_delta_kernel", p))
     return s;
   const int hd = p.s.hd;
-  if (hd == 64) return launch_tc<64, T>(p, stream);
-  if (hd == 128) return launch_tc<128, T>(p, stream);
-  if (hd < 64) return launch_mma<64, T>(p, stream);
-  if (hd <= 96) return launch_mma<96, T>(p, stream);
-  if (hd <= 128) return launch_mma<128, T>(p, stream);
+  if (hd <= 64) return launch_tc<64, T>(p, stream);
+  if (hd <= 128) return launch_tc<128, T>(p, stream);
   if (hd <= 192) return launch_mma<192, T>(p, stream);
   return launch_mma<256, T>(p, stream);
 }

@@ -18,7 +18,7 @@ struct ReadParams {
   int* err;
 };
 
-// ---------------------------------------------------------------- mma.sync, any head size up to 256
+// ---------------------------------------------------------------- mma.sync, head sizes from 136 to 256
 // A CTA of four warps takes 64 rows of one head, a warp 16 of them; keys in tiles of 64, two stages.
 template <int DP, class T>
 __global__ void __launch_bounds__(128) prompt_read_mma_kernel(const ReadParams p) {
@@ -121,7 +121,8 @@ int launch_mma(const ReadParams& p, cudaStream_t stream) {
                        "prompt_read_mma_kernel", p);
 }
 
-// ---------------------------------------------------------------- tcgen05, head sizes 64 and 128
+// ---------------------------------------------------------------- tcgen05, head sizes up to 128
+// Heads of other sizes than 64 and 128 are loaded with zeros behind them (outside of the maps).
 // A CTA takes two tiles of 128 rows that read the same keys: two heads of a group, or, where a group has an
 // odd number of heads, 256 rows of one. Warps with fixed roles:
 //   two softmax warpgroups, one a tile: a thread owns a row; S from tensor memory, mask, maximum, P = 2^(y - m)
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       const float inv = some ? 1.f / l : 0.f;
       T* out = static_cast<T*>(p.out.ptr) + static_cast<int64_t>(it.first + r) * p.out.tok + it.head[wg] * p.out.head;
 #pragma unroll 1
-      for (int c = 0; c < HD; c += 32) {
+      for (int c = 0; c < p.s.hd; c += 32) {
         float o[32];
         __syncwarp();
         tmem_ld32(oa + c, o);
@@ -326,7 +327,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             w[k] = some ? pack_pair<T>(o[2 * k] * inv, o[2 * k + 1] * inv) : pack_pair<T>(l, l);
 #pragma unroll
           for (int k = 0; k < 16; k += 4)
-            *reinterpret_cast<uint4*>(out + c + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+            if (c + 2 * k < p.s.hd)
+              *reinterpret_cast<uint4*>(out + c + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
         }
       }
       if (live && p.lse)
@@ -555,9 +557,9 @@ int launch_tc(const ReadParams& p, cudaStream_t stream) {
   using C = ReadCfg<HD, T>;
   const char* what = "prompt read";
   CUtensorMap qmap, kmap, vmap;
-  if (int s = prompt_map(what, p.q, p.s.hq, p.s.n, HD, 128, C::F16, &qmap)) return s;
-  if (int s = prompt_map(what, p.k, p.s.hkv, p.s.n, HD, 128, C::F16, &kmap)) return s;
-  if (int s = prompt_map(what, p.v, p.s.hkv, p.s.n, HD, 128, C::F16, &vmap)) return s;
+  if (int s = prompt_map(what, p.q, p.s.hq, p.s.n, p.s.hd, 128, C::F16, &qmap)) return s;
+  if (int s = prompt_map(what, p.k, p.s.hkv, p.s.n, p.s.hd, 128, C::F16, &kmap)) return s;
+  if (int s = prompt_map(what, p.v, p.s.hkv, p.s.n, p.s.hd, 128, C::F16, &vmap)) return s;
   static std::atomic<uint64_t> configured{0};
   if (int s = allow_smem(prompt_read_tc_kernel<C>, C::SMEM, configured, "cudaFuncSetAttribute(prompt_read)")) return s;
   // the register shares the warps take must add up to what a block is launched with
@@ -576,11 +578,8 @@ int launch_tc(const ReadParams& p, cudaStream_t stream) {
 template <class T>
 int launch_read(const ReadParams& p, cudaStream_t stream) {
   const int hd = p.s.hd;
-  if (hd == 64) return launch_tc<64, T>(p, stream);
-  if (hd == 128) return launch_tc<128, T>(p, stream);
-  if (hd < 64) return launch_mma<64, T>(p, stream);
-  if (hd <= 96) return launch_mma<96, T>(p, stream);
-  if (hd <= 128) return launch_mma<128, T>(p, stream);
+  if (hd <= 64) return launch_tc<64, T>(p, stream);
+  if (hd <= 128) return launch_tc<128, T>(p, stream);
   if (hd <= 192) return launch_mma<192, T>(p, stream);
   return launch_mma<256, T>(p, stream);
 }

@@ -231,7 +231,7 @@ int64_t fold_prefix_read_workspace(int n, int hq, int hkv, int hd);
  * out [n, hq, hd] = the softmax-weighted values, lse [hq, n] (contiguous, may be NULL) the natural log
  * of the sum of exp(softmax_scale * q.k). Keys and values of other sequences may hold anything; a value
  * row that some rows of its sequence see must be finite even for rows that do not. dtype FOLD_BF16 or
- * FOLD_FP16; hd a multiple of 8 up to 256 (64 and 128 take the tensor-memory kernels); every row on a
+ * FOLD_FP16; hd a multiple of 8 up to 256 (up to 128 on the tensor-memory kernels); every row on a
  * 16-byte boundary; out must not overlap k or v, and q only as q itself. b and n are what a captured
  * call is fixed to. err (may be NULL) takes FOLD_DEVERR_TIMEOUT. */
 int fold_prompt_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,
