@@ -124,17 +124,17 @@ __device__ __forceinline__ int next_block(const void* answer) {
 }
 
 // ---------------------------------------------------------------- tiles of 16-bit rows in shared memory
-// 64 rows of DP columns, padded by 16 bytes so that eight rows' chunks of 16 bytes hit all banks.
+// Rows of DP columns, padded by 16 bytes so that eight rows' chunks of 16 bytes hit all banks.
 template <int DP>
 struct SmemTile {
-  static constexpr int ROW = DP * 2 + 16, BYTES = 64 * ROW;
+  static constexpr int ROW = DP * 2 + 16, BYTES = 64 * ROW;  // of 64 rows
 };
 
-// Copies rows [r0, r0 + 64) of a sequence (rows from `len` on and columns from hd on become zeros).
-template <int DP, int NT>
+// Copies rows [r0, r0 + R) of a sequence (rows from `len` on and columns from hd on become zeros).
+template <int DP, int NT, int R = 64>
 __device__ __forceinline__ void stage_rows(uint32_t dst, const Rows& x, int first, int len, int r0, int head, int hd) {
   const char* base = static_cast<const char*>(x.ptr) + head * x.head * 2;
-  for (int e = threadIdx.x; e < 64 * (DP / 8); e += NT) {
+  for (int e = threadIdx.x; e < R * (DP / 8); e += NT) {
     const int r = e / (DP / 8), c = e - r * (DP / 8);
     const bool in = r0 + r < len && c * 8 < hd;
     const char* src = in ? base + (static_cast<int64_t>(first + r0 + r) * x.tok + c * 8) * 2 : static_cast<const char*>(x.ptr);

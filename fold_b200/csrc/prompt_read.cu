@@ -19,25 +19,25 @@ struct ReadParams {
 };
 
 // ---------------------------------------------------------------- mma.sync, head sizes from 136 to 256
-// A CTA of four warps takes 64 rows of one head, a warp 16 of them; keys in tiles of 64, two stages.
+// A CTA of eight warps takes 128 rows of one head, a warp 16 of them; keys in tiles of 64, two stages.
 template <int DP, class T>
-__global__ void __launch_bounds__(128) prompt_read_mma_kernel(const ReadParams p) {
+__global__ void __launch_bounds__(256) prompt_read_mma_kernel(const ReadParams p) {
   using Sm = SmemTile<DP>;
   // weights in fp16 are held 2^10 up: small ones of many keys stay above its smallest step
   constexpr float kShift = std::is_same<T, __half>::value ? 10.f : 0.f;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const uint32_t sq = smem_u32(smem), sk = sq + Sm::BYTES, sv = sk + 2 * Sm::BYTES;
+  const uint32_t sq = smem_u32(smem), sk = sq + 2 * Sm::BYTES, sv = sk + 2 * Sm::BYTES;
   wait_for_producer();
   Tile t;
-  if (!find_tile<64>(p.s, gridDim.x - 1 - blockIdx.x, t)) return;  // the last rows see most keys: first
+  if (!find_tile<128>(p.s, gridDim.x - 1 - blockIdx.x, t)) return;  // the last rows see most keys: first
   const int h = blockIdx.y, hk = h / p.s.group, hd = p.s.hd;
   int lo, hi;
-  keys_of(p.s, t.len, t.row0, min(t.row0 + 64, t.len), lo, hi);
+  keys_of(p.s, t.len, t.row0, min(t.row0 + 128, t.len), lo, hi);
   const int kb = lo / 64, ke = (hi + 63) / 64;
-  stage_rows<DP, 128>(sq, p.q, t.first, t.len, t.row0, h, hd);
-  stage_rows<DP, 128>(sk, p.k, t.first, t.len, kb * 64, hk, hd);
-  stage_rows<DP, 128>(sv, p.v, t.first, t.len, kb * 64, hk, hd);
+  stage_rows<DP, 256, 128>(sq, p.q, t.first, t.len, t.row0, h, hd);
+  stage_rows<DP, 256>(sk, p.k, t.first, t.len, kb * 64, hk, hd);
+  stage_rows<DP, 256>(sv, p.v, t.first, t.len, kb * 64, hk, hd);
   cp_commit();
   float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -53,8 +53,8 @@ __global__ void __launch_bounds__(128) prompt_read_mma_kernel(const ReadParams p
   for (int j = kb; j < ke; ++j) {
     const int st = (j - kb) & 1;
     if (j + 1 < ke) {
-      stage_rows<DP, 128>(sk + (st ^ 1) * Sm::BYTES, p.k, t.first, t.len, (j + 1) * 64, hk, hd);
-      stage_rows<DP, 128>(sv + (st ^ 1) * Sm::BYTES, p.v, t.first, t.len, (j + 1) * 64, hk, hd);
+      stage_rows<DP, 256>(sk + (st ^ 1) * Sm::BYTES, p.k, t.first, t.len, (j + 1) * 64, hk, hd);
+      stage_rows<DP, 256>(sv + (st ^ 1) * Sm::BYTES, p.v, t.first, t.len, (j + 1) * 64, hk, hd);
     }
     cp_commit();
     cp_wait<1>();
@@ -114,10 +114,10 @@ __global__ void __launch_bounds__(128) prompt_read_mma_kernel(const ReadParams p
 
 template <int DP, class T>
 int launch_mma(const ReadParams& p, cudaStream_t stream) {
-  constexpr int smem = 5 * SmemTile<DP>::BYTES;
+  constexpr int smem = 6 * SmemTile<DP>::BYTES;
   static std::atomic<uint64_t> configured{0};
   if (int s = allow_smem(prompt_read_mma_kernel<DP, T>, smem, configured, "cudaFuncSetAttribute(prompt_read)")) return s;
-  return launch_behind(prompt_read_mma_kernel<DP, T>, dim3(tile_numbers(p.s.n, p.s.b, 64), p.s.hq), 128, smem, stream,
+  return launch_behind(prompt_read_mma_kernel<DP, T>, dim3(tile_numbers(p.s.n, p.s.b, 128), p.s.hq), 256, smem, stream,
                        "prompt_read_mma_kernel", p);
 }
 
