@@ -657,15 +657,15 @@ def prompt_read_grad(dout, q, k, v, out, lse, qsl, *, softmax_scale, causal=True
     given = (dq is not None) + (dk is not None) + (dv is not None)
     if given not in (0, 3):
         raise FoldError("prompt_read_grad: all of dq, dk and dv are given, or none")
-    if not given:
-        make = torch.empty if b else torch.zeros
-        dq = make((n, hq, d), dtype=dtype, device=q.device)
-        dk = make((n, hkv, d), dtype=dtype, device=q.device)
-        dv = make((n, hkv, d), dtype=dtype, device=q.device)
-    dqs, dks, dvs = (_prompt_out(what, name, x, n, h, d, dtype)
-                     for name, x, h in (("dq", dq, hq), ("dk", dk, hkv), ("dv", dv, hkv)))
+    if given:
+        dqs = _prompt_out(what, "dq", dq, n, hq, d, dtype)
+        dks, dvs = (_prompt_out(what, name, x, n, hkv, d, dtype) for name, x in (("dk", dk), ("dv", dv)))
+    else:
+        dq, dk, dv = q.new_empty((n, hq, d)), q.new_empty((n, hkv, d)), q.new_empty((n, hkv, d))
+        dqs, dks = (hq * d, d), (hkv * d, d)
+        dvs = dks
     if n == 0 or b == 0:
-        return dq, dk, dv
+        return (dq, dk, dv) if given else (dq.zero_(), dk.zero_(), dv.zero_())
     if workspace is None:
         size = _lib.prompt_read_grad_workspace(n, hq, hkv, d)
         workspace = q.new_empty(max(size, 0), dtype=torch.uint8)
