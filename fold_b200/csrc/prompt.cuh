@@ -90,6 +90,22 @@ __device__ __forceinline__ float2 unpack_pair(uint32_t x) {
   else return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
+// Sixteen elements of a row: one sector where rows lie on 32 bytes (`wide`), else two halves; `cols`: how many of them
+// the row has (16 or 8). A warp that stores a row a lane moves a line a cycle, so fewer, wider stores.
+__device__ __forceinline__ void store_row16(void* dst, const uint32_t* w, bool wide, int cols) {
+  if (wide && cols >= 16) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+                 "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    if (cols >= 8) static_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    if (cols >= 16) static_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+__device__ __forceinline__ bool rows_on_32(const Rows& x) {
+  return ((reinterpret_cast<uintptr_t>(x.ptr) | static_cast<uintptr_t>(x.tok) * 2 | static_cast<uintptr_t>(x.head) * 2) & 31u) == 0;
+}
+
 template <class T>
 __device__ __forceinline__ void mma_t(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __nv_bfloat16>::value) mma_bf16(d, a[0], a[1], a[2], a[3], b0, b1);

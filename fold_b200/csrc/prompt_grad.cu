@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       const int64_t row = it.first + r;
       T* out = static_cast<T*>(to.ptr) + row * to.tok + it.head * to.head + c0;
       float* part = p.part + ((static_cast<int64_t>(2 * it.split + dv) * p.s.n + row) * p.s.hkv + it.head) * p.s.hd + c0;
-      const bool partial = keys && p.splits > 1;
+      const bool partial = keys && p.splits > 1, wide = rows_on_32(to);
 #pragma unroll 1
       for (int c = 0; c < cols; c += 16) {
         float o[16];
@@ -603,11 +603,10 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             if (c0 + c + k < p.s.hd)
               *reinterpret_cast<float4*>(part + c + k) = make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f);
         } else {
+          uint32_t w[8];
 #pragma unroll
-          for (int k = 0; k < 16; k += 8)
-            if (c0 + c + k < p.s.hd)
-              *reinterpret_cast<uint4*>(out + c + k) = make_uint4(pack_pair<T>(o[k] * f, o[k + 1] * f), pack_pair<T>(o[k + 2] * f, o[k + 3] * f),
-                           pack_pair<T>(o[k + 4] * f, o[k + 5] * f), pack_pair<T>(o[k + 6] * f, o[k + 7] * f));
+          for (int k = 0; k < 8; ++k) w[k] = pack_pair<T>(o[2 * k] * f, o[2 * k + 1] * f);
+          store_row16(out + c, w, wide, p.s.hd - c0 - c);
         }
       }
       __syncwarp();

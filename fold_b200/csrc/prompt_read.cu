@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       ok = warp_wait(&B.done[wg], items++ & 1);
       if (!ok) break;
       tc_fence_after();
-      const bool some = l > 0.f;
+      const bool some = l > 0.f, wide = rows_on_32(p.out);
       const float inv = some ? 1.f / l : 0.f;
       T* out = static_cast<T*>(p.out.ptr) + static_cast<int64_t>(it.first + r) * p.out.tok + it.head[wg] * p.out.head;
 #pragma unroll 1
@@ -325,10 +325,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
 #pragma unroll
           for (int k = 0; k < 16; ++k)  // no key: l is 0; a NaN sum reaches the output
             w[k] = some ? pack_pair<T>(o[2 * k] * inv, o[2 * k + 1] * inv) : pack_pair<T>(l, l);
-#pragma unroll
-          for (int k = 0; k < 16; k += 4)
-            if (c + 2 * k < p.s.hd)
-              *reinterpret_cast<uint4*>(out + c + 2 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+          store_row16(out + c, w, wide, p.s.hd - c);
+          store_row16(out + c + 16, w + 8, wide, p.s.hd - c - 16);
         }
       }
       if (live && p.lse)
