@@ -133,6 +133,32 @@ struct GrowParams {
   int64_t* slots;
 };
 
+// Calls of up to this many tokens need one launch. A block of 1024 threads takes about a microsecond for each 1024
+// of them: 20000 tokens of 250 sequences took 31 us in one block.
+constexpr int kFewTokens = 1024;
+
+// Position and slot of token t, from those of its sequence's first token (at: the sequences' first tokens).
+__device__ __forceinline__ void grow_token(const GrowParams& p, const int* at, int t) {
+  const Pool& pool = p.pool;
+  const int i = p.m > 0 && t >= at[0] ? owner(at, p.m, t) : -1;
+  const int first = i < 0 ? 0 : at[i];
+  if (i >= 0 && t < min(max(p.qsl[i + 1], first), p.n)) {
+    if (t == first) return;  // written already
+    if (p.slots[first] >= 0) {
+      const int64_t pos = p.positions[first] + (t - first);
+      const int r = p.table_rows ? p.table_rows[i] : i;
+      // (a row that grew: its table has an entry for each of its tokens)
+      if (r >= 0 && r < pool.rows && pos < pool.capacity()) {
+        const int x = static_cast<int>(pos);
+        p.positions[t] = pos;
+        p.slots[t] = static_cast<int64_t>(*pool.entry(r, x / pool.bs)) * pool.bs + x % pool.bs;
+        return;
+      }
+    }
+  }
+  p.positions[t] = 0, p.slots[t] = -1;
+}
+
 __global__ void __launch_bounds__(kThreads) grow_pages_kernel(const GrowParams p) {
   extern __shared__ int dyn[];
   __shared__ int scratch[32];
@@ -208,22 +234,30 @@ __global__ void __launch_bounds__(kThreads) grow_pages_kernel(const GrowParams p
   }
   if (bad) set_error(pool.err, bad);
   __syncthreads();
-  const int lo = min(max(p.qsl[0], 0), p.n), hi = min(max(p.qsl[m], 0), p.n);
+  // position and slot of each sequence's first token; the others from those (grow_tokens)
+  for (int i = tid; i < m; i += kThreads) {
+    int first, last;
+    tokens(i, first, last);
+    if (first == last) continue;
+    const int x = old[i];
+    p.positions[first] = row[i] < 0 ? 0 : x;
+    p.slots[first] = row[i] < 0 ? -1 : static_cast<int64_t>(*pool.entry(row[i], x / pool.bs)) * pool.bs + x % pool.bs;
+  }
+  if (p.n > kFewTokens) return;
+  __syncthreads();
   for (int i = tid; i < m; i += kThreads) at[i] = min(max(p.qsl[i], 0), p.n);
   __syncthreads();
-  for (int t = tid; t < p.n; t += kThreads) {
-    int64_t pos = 0, slot = -1;
-    if (t >= lo && t < hi) {
-      const int i = owner(at, m, t);
-      if (row[i] >= 0) {
-        pos = old[i] + (t - at[i]);
-        const int x = static_cast<int>(pos);
-        // an entry within capacity(): written above or read before
-        slot = x < pool.lens[row[i]] ? static_cast<int64_t>(*pool.entry(row[i], x / pool.bs)) * pool.bs + x % pool.bs : -1;
-      }
-    }
-    p.positions[t] = pos, p.slots[t] = slot;
-  }
+  for (int t = tid; t < p.n; t += kThreads) grow_token(p, at, t);
+}
+
+// The tokens of a large call, 256 a block.
+__global__ void __launch_bounds__(256) grow_tokens_kernel(const GrowParams p) {
+  extern __shared__ int dyn[];
+  wait_for_producer();
+  for (int i = threadIdx.x; i < p.m; i += 256) dyn[i] = min(max(p.qsl[i], 0), p.n);
+  __syncthreads();
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (t < p.n) grow_token(p, dyn, static_cast<int>(t));
 }
 
 // ---------------------------------------------------------------- free
@@ -418,7 +452,13 @@ int fold_grow_pages(int* refs, int num_pages, int* block_tables, int64_t block_t
   const int smem = 12 * (m > 0 ? m : 1);
   if (smem > 46 * 1024)
     if (int s = allow_smem(grow_pages_kernel, 12 * kMaxSeqs, configured, "cudaFuncSetAttribute(grow_pages)")) return s;
-  return launch_behind(grow_pages_kernel, dim3(1), kThreads, smem, static_cast<cudaStream_t>(stream), "grow_pages_kernel", p);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int s = launch_behind(grow_pages_kernel, dim3(1), kThreads, smem, st, "grow_pages_kernel", p)) return s;
+  if (n <= kFewTokens) return FOLD_OK;
+  static std::atomic<uint64_t> configured_tokens{0};
+  if (4 * m > 46 * 1024)
+    if (int s = allow_smem(grow_tokens_kernel, 4 * kMaxSeqs, configured_tokens, "cudaFuncSetAttribute(grow_tokens)")) return s;
+  return launch_behind(grow_tokens_kernel, dim3((n + 255) / 256), 256, 4 * m, st, "grow_tokens_kernel", p);
 }
 
 int fold_free_pages(int* refs, int num_pages, int* block_tables, int64_t block_tables_stride, int block_tables_len, int* lens,

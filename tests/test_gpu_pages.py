@@ -149,7 +149,14 @@ def test_grow_in_a_large_pool_and_of_many_sequences():
     rows = rng.sample(range(1500), 1300)
     p.free(rows, [rng.randint(0, 300) for _ in rows])
     rows = rng.sample(range(1500), 1100)
-    p.grow([rng.randint(0, 12) for _ in rows], rows=rows, spare=9)
+    p.grow([rng.randint(0, 12) for _ in rows], rows=rows, spare=9, lead=3)
+
+
+def test_refusals_among_many_tokens():
+    p = Pool(120, 6, 40, 16)
+    p.grow([500, 641, 500, 640, 3, 300], spare=5, err=DEVERR_CAPACITY | DEVERR_PAGES)  # too long; no pages for the last
+    assert p.tokens == [500, 0, 500, 640, 3, 0]
+    p.grow([600, 600, 7], rows=[4, 1, 4], lead=1, err=DEVERR_ROW | DEVERR_PAGES)
 
 
 def test_grow_of_the_most_sequences():
