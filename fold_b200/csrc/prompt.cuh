@@ -44,20 +44,28 @@ struct Tile {
   int seq, first, len, row0;  // row0: the tile's first row in the sequence
 };
 
-// Tile number x, found by a search of 32 probes a round (all lanes of a warp call this); false: idle.
-template <int T>
-__device__ __forceinline__ bool find_tile(const Shape& p, int x, Tile& t) {
+// The last sequence s with before(s, qsl[s]), which holds up to some sequence and not behind it; -1: none. A search
+// of 32 probes a round; all lanes of a warp call this.
+template <class F>
+__device__ __forceinline__ int last_sequence(const Shape& p, F before) {
   const int lane = threadIdx.x & 31;
   int lo = 0, hi = p.b;  // the sequence lies in [lo, hi)
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32, s = lo + lane * step;
-    const bool before = s < hi && min(max(__ldg(p.qsl + s), 0), p.n) / T + s <= x;
-    const uint32_t m = __ballot_sync(0xffffffffu, before);
-    if (m == 0) return false;
+    const uint32_t m = __ballot_sync(0xffffffffu, s < hi && before(s, min(max(__ldg(p.qsl + s), 0), p.n)));
+    if (m == 0) return -1;
     const int at = 31 - __clz(m);
     lo += at * step;
     hi = min(hi, lo + step);
   }
+  return lo;
+}
+
+// Tile number x; false: idle.
+template <int T>
+__device__ __forceinline__ bool find_tile(const Shape& p, int x, Tile& t) {
+  const int lo = last_sequence(p, [&](int s, int first) { return first / T + s <= x; });
+  if (lo < 0) return false;
   int first, last;
   seq_rows(p, lo, first, last);
   t.seq = lo, t.first = first, t.len = last - first;

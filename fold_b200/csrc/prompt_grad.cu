@@ -36,9 +36,16 @@ struct Shift {
   static constexpr float kDown = std::is_same<T, __nv_bfloat16>::value ? 1.f : 1.f / 1024.f;
 };
 
+// A row that sees up to this many keys has delta from them, as sum_j P_j (do.v_j) in float32, instead of from the
+// rounded out: where few keys share the weight, out's rounding is as large as what dP and delta leave of each other
+// (sequences of 2 to 6 tokens: dq off by 0.0028 of its norm, 0.0022 from the keys; rounding dq alone 0.0017).
+constexpr int kExactKeys = 8;
+
 // A warp a row and head: what the other kernels take of it. Memory bound (out and dout once).
+// (Registers for twelve blocks an SM, whatever the rare rows of few keys would take: with theirs 8192 rows of 32
+// heads took 80 us longer.)
 template <class T>
-__global__ void __launch_bounds__(128) prompt_delta_kernel(const GradParams p) {
+__global__ void __launch_bounds__(128, 12) prompt_delta_kernel(const GradParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int t = static_cast<int>(x / p.s.hq), h = static_cast<int>(x - static_cast<int64_t>(t) * p.s.hq);
@@ -57,6 +64,10 @@ __global__ void __launch_bounds__(128) prompt_delta_kernel(const GradParams p) {
     }
     return;
   }
+  const int seq = last_sequence(p.s, [&](int, int first) { return first <= t; });
+  int first, last, lo, hi;
+  seq_rows(p.s, max(seq, 0), first, last);
+  keys_of(p.s, last - first, t - first, t - first + 1, lo, hi);
   float sum = 0.f;
   for (int c = lane * 8; c < hd; c += 256) {
     const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out.ptr) + t * p.out.tok + h * p.out.head + c);
@@ -70,6 +81,45 @@ __global__ void __launch_bounds__(128) prompt_delta_kernel(const GradParams p) {
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (t >= first && t < last && hi - lo <= kExactKeys) {
+    float top = -INFINITY, num = 0.f, den = 0.f;
+    const int64_t hk = h / p.s.group;
+    for (int j0 = lo; j0 < hi; j0 += 4) {  // four at a time: their loads are under way together
+      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int c = lane * 8; c < hd; c += 256) {
+        uint4 in[2], kv[8];
+        in[0] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.ptr) + t * p.q.tok + h * p.q.head + c);
+        in[1] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout.ptr) + t * p.dout.tok + h * p.dout.head + c);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int64_t j = first + min(j0 + k, hi - 1);
+          kv[2 * k] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.k.ptr) + j * p.k.tok + hk * p.k.head + c);
+          kv[2 * k + 1] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v.ptr) + j * p.v.tok + hk * p.v.head + c);
+        }
+        const uint32_t *wi = reinterpret_cast<const uint32_t*>(in), *wk = reinterpret_cast<const uint32_t*>(kv);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 fq = unpack_pair<T>(wi[i]), fd = unpack_pair<T>(wi[4 + i]);
+            const float2 fk = unpack_pair<T>(wk[8 * k + i]), fv = unpack_pair<T>(wk[8 * k + 4 + i]);
+            x[k] = fmaf(fq.x, fk.x, fmaf(fq.y, fk.y, x[k])), y[k] = fmaf(fd.x, fv.x, fmaf(fd.y, fv.y, y[k]));
+          }
+      }
+#pragma unroll
+      for (int o = 16; o; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          x[k] += __shfl_xor_sync(0xffffffffu, x[k], o), y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (j0 + k < hi) {
+          const float z = x[k] * p.s.scale_log2, up = fmaxf(top, z), f = fast_exp2(top - up), e = fast_exp2(z - up);
+          num = fmaf(e, y[k], num * f), den = den * f + e, top = up;
+        }
+    }
+    if (den > 0.f) sum = num / den;
+  }
   if (lane == 0) {
     const int64_t at = static_cast<int64_t>(h) * p.s.n + t;
     const float lse = p.lse[at];
@@ -1022,6 +1072,10 @@ int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_st
       {"dk", dk, dk_stride_tok, dk_stride_head, hkv, true, &p.dk}, {"dv", dv, dv_stride_tok, dv_stride_head, hkv, true, &p.dv}};
   for (const auto& r : rows)
     if (int s = prompt_rows(what, r.name, r.ptr, r.tok, r.head, n, r.heads, hd, r.written, r.to)) return s;
+  for (int i = 5; i < 8; ++i)
+    for (int k = 0; k < i; ++k)
+      if (rows[i].ptr == rows[k].ptr)
+        return fail(FOLD_ERR_INVALID_ARGUMENT, std::string("prompt read grad: ") + rows[i].name + " must not be " + rows[k].name);
   if (!lse) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: null pointer");
   if (static_cast<int64_t>(n) * hq > (int64_t(1) << 32)) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: too many rows");
   p.splits = tensor_memory_size(hd) ? key_splits(n, hkv, p.s.group) : 1;

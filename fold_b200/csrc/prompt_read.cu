@@ -648,6 +648,7 @@ int fold_prompt_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   if (int s = prompt_rows(what, "k", k, k_stride_tok, k_stride_head, n, hkv, hd, false, &p.k)) return s;
   if (int s = prompt_rows(what, "v", v, v_stride_tok, v_stride_head, n, hkv, hd, false, &p.v)) return s;
   if (int s = prompt_rows(what, "out", out, o_stride_tok, o_stride_head, n, hq, hd, true, &p.out)) return s;
+  if (out == k || out == v) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read: out must not be k or v");
   p.lse = lse, p.err = err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == FOLD_BF16 ? launch_read<__nv_bfloat16>(p, st) : launch_read<__half>(p, st);

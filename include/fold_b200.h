@@ -243,7 +243,8 @@ int fold_prompt_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
 /* Gradient of fold_prompt_read: from dout [n, hq, hd] (and dlse [hq, n] of lse, may be NULL), its inputs
  * and its results out and lse, the gradients dq [n, hq, hd], dk and dv [n, hkv, hd], those of a key or
  * value summed over the heads of its group. Rows outside the sequences get zeros when `zero_rest`, else
- * they are left as they were. No sum depends on the order in which blocks run: equal calls give equal
+ * they are left as they were. As for values, a row of q and dout must be finite even for keys that it does not
+ * see, and a key and value for rows that do not see it. No sum depends on the order in which blocks run: equal calls give equal
  * bits. The gradients must not overlap the inputs. workspace: fold_prompt_read_grad_workspace bytes of
  * device memory, 16-byte aligned, not shared by calls that may overlap; nothing in it outlives the call. */
 int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_stride_head, const void* q,

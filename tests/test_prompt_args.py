@@ -15,8 +15,8 @@ def read(**kw):
 
 
 def grad(**kw):
-    a = dict(do=16, dos=(512, 128), q=16, qs=(512, 128), k=32, ks=(256, 128), v=48, vs=(256, 128), o=80, os=(512, 128),
-             lse=16, qsl=16, b=1, scale=1.0, dq=64, dqs=(512, 128), dk=64, dks=(256, 128), dv=64, dvs=(256, 128), ws=16,
+    a = dict(do=64, dos=(512, 128), q=16, qs=(512, 128), k=32, ks=(256, 128), v=48, vs=(256, 128), o=80, os=(512, 128),
+             lse=16, qsl=16, b=1, scale=1.0, dq=96, dqs=(512, 128), dk=112, dks=(256, 128), dv=128, dvs=(256, 128), ws=16,
              wb=1 << 30, n=2, hq=4, hkv=2, hd=128, dtype=0, rest=1)
     a.update(kw)
     _lib.call("fold_prompt_read_grad", a["do"], *a["dos"], a["q"], *a["qs"], a["k"], *a["ks"], a["v"], *a["vs"], a["o"],
@@ -31,7 +31,8 @@ SIZES = [dict(n=-1), dict(b=-1), dict(hq=3), dict(hq=0), dict(hkv=0), dict(hd=0)
 
 
 @pytest.mark.parametrize("bad", SIZES + [dict(out=None), dict(out=8), dict(os=(0, 128)), dict(os=(512, 0)),
-                                         dict(os=(256, 128)), dict(os=(512, 64)), dict(os=(-512, 128))], ids=str)
+                                         dict(os=(256, 128)), dict(os=(512, 64)), dict(os=(-512, 128)),
+                                         dict(out=32), dict(out=48)], ids=str)
 def test_read_refusals(bad):
     with pytest.raises(FoldError, match="prompt read"):
         read(**bad)
@@ -39,7 +40,8 @@ def test_read_refusals(bad):
 
 @pytest.mark.parametrize("bad", SIZES + [dict(do=None), dict(o=None), dict(lse=None), dict(dq=None), dict(dk=None),
                                          dict(dv=None), dict(dqs=(128, 128)), dict(dks=(256, 64)), dict(dvs=(0, 128)),
-                                         dict(ws=None), dict(wb=8), dict(ws=24), dict(do=2), dict(b=0)], ids=str)
+                                         dict(ws=None), dict(wb=8), dict(ws=24), dict(do=2), dict(b=0),
+                                         dict(dq=16), dict(dk=32), dict(dv=112), dict(dk=80), dict(dv=64)], ids=str)
 def test_grad_refusals(bad):
     with pytest.raises(FoldError, match="prompt read grad"):
         grad(**bad)
