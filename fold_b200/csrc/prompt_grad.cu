@@ -9,6 +9,13 @@
 // by the rows' tiles (dq) and once by the keys' (dk, dv): seven products where one pass with dq added up
 // in memory would take five, but no sum depends on the order in which blocks run, and nothing of the
 // size of P is written.
+//
+// Measured (bf16, head size 128, 32 query and 8 KV heads, one causal sequence; the GPU's time of captured calls):
+// 8192 tokens 1.59 ms (866 TFLOP/s of five products, 1.21 PFLOP/s of the seven made; 1.8 ms in a long run, where
+// the board is at its 1000 W), 2048 tokens 188 us, 64 tokens 19 us. A tile of 128 x 128 takes a key's item 3300
+// cycles and a row's 2700, of which the products are 2050 and 1540: what bounds it is the chain dP, dS, acc1, dP of
+// the next, and the energy of the products. At head size 64 (1.45 ms at 8192 tokens) the exponentials and dS, 2100
+// to 2800 cycles a tile.
 #include "prompt.cuh"
 #include "tcgen05.cuh"
 
@@ -38,95 +45,101 @@ struct Shift {
 
 // A row that sees up to this many keys has delta from them, as sum_j P_j (do.v_j) in float32, instead of from the
 // rounded out: where few keys share the weight, out's rounding is as large as what dP and delta leave of each other
-// (sequences of 2 to 6 tokens: dq off by 0.0028 of its norm, 0.0022 from the keys; rounding dq alone 0.0017).
+// (in sequences of a few tokens dq was off by 0.0028 of its norm, 1.65 times what rounding dq alone gives; for 2 to
+// 6 tokens it is now that rounding).
 constexpr int kExactKeys = 8;
 
-// A warp a row and head: what the other kernels take of it. Memory bound (out and dout once).
+// What the other kernels take of a row and head. A warp has one token and 32 / L of its heads, L lanes of eight
+// columns each a head, so that the sequence is looked up once for them. Memory bound (out and dout once).
 // (Registers for twelve blocks an SM, whatever the rare rows of few keys would take: with theirs 8192 rows of 32
 // heads took 80 us longer.)
-template <class T>
+template <int L, class T>
 __global__ void __launch_bounds__(128, 12) prompt_delta_kernel(const GradParams p) {
-  const int lane = threadIdx.x & 31;
+  constexpr int HEADS = 32 / L;
+  const int lane = threadIdx.x & 31, c = (lane % L) * 8, hd = p.s.hd;
+  const int groups = (p.s.hq + HEADS - 1) / HEADS;
   const int64_t x = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int t = static_cast<int>(x / p.s.hq), h = static_cast<int>(x - static_cast<int64_t>(t) * p.s.hq);
+  const int t = static_cast<int>(x / groups), own = static_cast<int>(x - static_cast<int64_t>(t) * groups) * HEADS + lane / L;
+  const int h = min(own, p.s.hq - 1);  // (lanes behind the last head repeat it)
+  const bool mine = own < p.s.hq && c < hd;
   wait_for_producer();
   if (t >= p.s.n) return;
-  const int hd = p.s.hd;
   if (t < __ldg(p.s.qsl) || t >= __ldg(p.s.qsl + p.s.b)) {
-    if (!p.zero_rest) return;
-    for (int c = lane * 8; c < hd; c += 256) {
-      const uint4 z = make_uint4(0, 0, 0, 0);
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.dq.ptr) + t * p.dq.tok + h * p.dq.head + c) = z;
-      if (h < p.s.hkv) {
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.dk.ptr) + t * p.dk.tok + h * p.dk.head + c) = z;
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.dv.ptr) + t * p.dv.tok + h * p.dv.head + c) = z;
-      }
+    if (!p.zero_rest || !mine) return;
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.dq.ptr) + t * p.dq.tok + h * p.dq.head + c) = z;
+    if (h < p.s.hkv) {
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.dk.ptr) + t * p.dk.tok + h * p.dk.head + c) = z;
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.dv.ptr) + t * p.dv.tok + h * p.dv.head + c) = z;
     }
     return;
   }
+  auto load = [&](const Rows& r, int64_t row, int64_t head, uint32_t (&w)[4]) {  // eight elements
+    const uint4 v = c < hd ? *reinterpret_cast<const uint4*>(static_cast<const T*>(r.ptr) + row * r.tok + head * r.head + c)
+                           : make_uint4(0, 0, 0, 0);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  };
+  auto dot = [](const uint32_t (&a)[4], const uint32_t (&b)[4]) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 fa = unpack_pair<T>(a[i]), fb = unpack_pair<T>(b[i]);
+      sum = fmaf(fa.x, fb.x, fmaf(fa.y, fb.y, sum));
+    }
+    return sum;
+  };
+  auto total = [](float v) {  // over a head's lanes
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  uint32_t wo[4], wd[4];
+  load(p.out, t, h, wo), load(p.dout, t, h, wd);
   const int seq = last_sequence(p.s, [&](int, int first) { return first <= t; });
   int first, last, lo, hi;
   seq_rows(p.s, max(seq, 0), first, last);
   keys_of(p.s, last - first, t - first, t - first + 1, lo, hi);
-  float sum = 0.f;
-  for (int c = lane * 8; c < hd; c += 256) {
-    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.out.ptr) + t * p.out.tok + h * p.out.head + c);
-    const uint4 b = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout.ptr) + t * p.dout.tok + h * p.dout.head + c);
-    const uint32_t ua[4] = {a.x, a.y, a.z, a.w}, ub[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 fa = unpack_pair<T>(ua[i]), fb = unpack_pair<T>(ub[i]);
-      sum = fmaf(fa.x, fb.x, sum), sum = fmaf(fa.y, fb.y, sum);
-    }
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  float sum = total(dot(wo, wd));
   if (t >= first && t < last && hi - lo <= kExactKeys) {
     float top = -INFINITY, num = 0.f, den = 0.f;
-    const int64_t hk = h / p.s.group;
+    const int hk = h / p.s.group;
+    uint32_t wq[4];
+    load(p.q, t, h, wq);
     for (int j0 = lo; j0 < hi; j0 += 4) {  // four at a time: their loads are under way together
-      float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int c = lane * 8; c < hd; c += 256) {
-        uint4 in[2], kv[8];
-        in[0] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q.ptr) + t * p.q.tok + h * p.q.head + c);
-        in[1] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout.ptr) + t * p.dout.tok + h * p.dout.head + c);
+      uint32_t wk[4][4], wv[4][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int64_t j = first + min(j0 + k, hi - 1);
-          kv[2 * k] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.k.ptr) + j * p.k.tok + hk * p.k.head + c);
-          kv[2 * k + 1] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.v.ptr) + j * p.v.tok + hk * p.v.head + c);
-        }
-        const uint32_t *wi = reinterpret_cast<const uint32_t*>(in), *wk = reinterpret_cast<const uint32_t*>(kv);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 fq = unpack_pair<T>(wi[i]), fd = unpack_pair<T>(wi[4 + i]);
-            const float2 fk = unpack_pair<T>(wk[8 * k + i]), fv = unpack_pair<T>(wk[8 * k + 4 + i]);
-            x[k] = fmaf(fq.x, fk.x, fmaf(fq.y, fk.y, x[k])), y[k] = fmaf(fd.x, fv.x, fmaf(fd.y, fv.y, y[k]));
-          }
+      for (int k = 0; k < 4; ++k) {
+        const int64_t j = first + min(j0 + k, hi - 1);
+        load(p.k, j, hk, wk[k]), load(p.v, j, hk, wv[k]);
       }
 #pragma unroll
-      for (int o = 16; o; o >>= 1)
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          x[k] += __shfl_xor_sync(0xffffffffu, x[k], o), y[k] += __shfl_xor_sync(0xffffffffu, y[k], o);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < 4; ++k) {
+        const float z = total(dot(wq, wk[k])) * p.s.scale_log2, y = total(dot(wd, wv[k]));
         if (j0 + k < hi) {
-          const float z = x[k] * p.s.scale_log2, up = fmaxf(top, z), f = fast_exp2(top - up), e = fast_exp2(z - up);
-          num = fmaf(e, y[k], num * f), den = den * f + e, top = up;
+          const float up = fmaxf(top, z), f = fast_exp2(top - up), e = fast_exp2(z - up);
+          num = fmaf(e, y, num * f), den = den * f + e, top = up;
         }
+      }
     }
     if (den > 0.f) sum = num / den;
   }
-  if (lane == 0) {
+  if (lane % L == 0 && own < p.s.hq) {
     const int64_t at = static_cast<int64_t>(h) * p.s.n + t;
     const float lse = p.lse[at];
     if (p.dlse) sum -= p.dlse[at];
     // a row without a key (lse -inf) has weights of zero
     p.row[at] = make_float2(lse == -INFINITY ? -INFINITY : Shift<T>::kUp - lse * kLog2e, -sum * Shift<T>::kDown);
   }
+}
+
+template <class T>
+int launch_delta(const GradParams& p, cudaStream_t stream) {
+  const int heads = p.s.hd <= 64 ? 4 : p.s.hd <= 128 ? 2 : 1;
+  const int64_t warps = static_cast<int64_t>(p.s.n) * ((p.s.hq + heads - 1) / heads);
+  const dim3 grid(static_cast<unsigned>((warps + 3) / 4));
+  if (heads == 4) return launch_behind(prompt_delta_kernel<8, T>, grid, 128, 0, stream, "prompt_delta_kernel", p);
+  if (heads == 2) return launch_behind(prompt_delta_kernel<16, T>, grid, 128, 0, stream, "prompt_delta_kernel", p);
+  return launch_behind(prompt_delta_kernel<32, T>, grid, 128, 0, stream, "prompt_delta_kernel", p);
 }
 
 // Whether row r sees one key, which then is its own: the weight is 1 whatever the logit, and dS is the
@@ -143,9 +156,10 @@ __device__ __forceinline__ float lone_ds(const GradParams& p, int h, int at, flo
 
 // Whether dS of the rows [row0, row0 + rows) is held in two parts: where the last one sees up to 512 keys, or 1024
 // if the rows before it see as many (behind a window, or without causality: gradients do not fall off there). Such
-// rows have the largest gradients, and delta, from the rounded out, is least exact for them. Against 64 bits dq of
-// 13 sequences of 30 to 1300 tokens is off by 0.0019 of its norm (bf16; rounding dq alone: 0.0017), 0.0026 with
-// one part.
+// rows have the largest gradients, and delta, from the rounded out, is least exact for them. Against 64 bits
+// dq of 100 to 300 tokens is off by 1.06 times the rounding of dq alone, by 1.5 times with one part; of 1500
+// tokens 1.15; of 4096 tokens 1.44 with one part throughout. The second part costs a product and its conversions, a
+// fifth of a tile's time.
 __device__ __forceinline__ bool two_parts(const Shape& p, int len, int row0, int rows) {
   const int r = min(row0 + rows, len) - 1;
   int lo, hi;
@@ -1026,10 +1040,7 @@ int launch_tc(const GradParams& p, cudaStream_t stream) {
 
 template <class T>
 int launch_grad(const GradParams& p, cudaStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(p.s.n) * p.s.hq;
-  if (int s = launch_behind(prompt_delta_kernel<T>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, stream,
-                            "prompt_delta_kernel", p))
-    return s;
+  if (int s = launch_delta<T>(p, stream)) return s;
   const int hd = p.s.hd;
   if (hd <= 64) return launch_tc<64, T>(p, stream);
   if (hd <= 128) return launch_tc<128, T>(p, stream);
