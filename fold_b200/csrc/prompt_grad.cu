@@ -154,7 +154,7 @@ __device__ __forceinline__ float lone_ds(const GradParams& p, int h, int at, flo
   return p.dlse ? weight * p.dlse[static_cast<int64_t>(h) * p.s.n + at] * Shift<T>::kDown : 0.f;
 }
 
-// Whether dS of the rows [row0, row0 + rows) is held in two parts: where the last one sees up to 512 keys, or 1024
+// Whether dS of the rows [row0, row0 + rows) is held in two parts: where the last one sees up to 512 keys, or 2048
 // if the rows before it see as many (behind a window, or without causality: gradients do not fall off there). Such
 // rows have the largest gradients, and delta, from the rounded out, is least exact for them. Against 64 bits
 // dq of 100 to 300 tokens is off by 1.06 times the rounding of dq alone, by 1.5 times with one part; of 1500
@@ -165,7 +165,7 @@ __device__ __forceinline__ bool two_parts(const Shape& p, int len, int row0, int
   int lo, hi;
   keys_of(p, len, r, r + 1, lo, hi);
   const bool grows = p.right == 0 && p.left >= r;
-  return hi - lo <= (grows ? 512 : 1024);
+  return hi - lo <= (grows ? 512 : 2048);
 }
 
 // Columns that a warp sums gradients of: halves, whose accumulators fit the registers. Two warpgroups find the same
