@@ -594,6 +594,12 @@ def _prompt_shape(what, q, k, qsl, lse):
     return n, hq, ks[1], d, code, qsl.shape[0] - 1
 
 
+def _window(window_size):
+    """(left, right) of a window, as C integers hold them."""
+    left, right = window_size
+    return max(-1, min(left, 1 << 30)), max(-1, min(right, 1 << 30))
+
+
 def _ptr(what, t, check):
     if t is None:
         return None
@@ -608,15 +614,15 @@ def prompt_read(q, k, v, qsl, out, *, softmax_scale, causal=True, window_size=(-
     [qsl[i], qsl[i + 1]) belong to sequence i (qsl int32 [b + 1] on the device). Row r of a sequence sees
     its keys [r - left, r + right] of window_size (left, right) (-1: unbounded), up to its own when
     causal. Writes out [n, Hq, D] (which may be q) and, when given, lse [Hq, n] float32; rows outside the
-    sequences are left alone. Keys and values go to a paged cache by append_paged; prompt_read_grad is the
-    gradient."""
+    sequences are left alone. Values must be finite, seen or not, within their sequence. Keys and values go to
+    a paged cache by append_paged; prompt_read_grad is the gradient."""
     dev = _check_devices("prompt_read", q, k, v, qsl, out, lse, err)
     n, hq, hkv, d, code, b = _prompt_shape("prompt_read", q, k, qsl, lse)
     os = _prompt_out("prompt_read", "out", out, n, hq, d, q.dtype)
     q, qs = _prompt_rows("prompt_read", "q", q, n, hq, d, out.dtype)
     k, ks = _prompt_rows("prompt_read", "k", k, n, hkv, d, out.dtype)
     v, vs = _prompt_rows("prompt_read", "v", v, n, hkv, d, out.dtype)
-    left, right = window_size
+    left, right = _window(window_size)
     _call_on(dev, "fold_prompt_read", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0],
              vs[1], qsl.data_ptr(), b, 1 if causal else 0, left, right, softmax_scale, out.data_ptr(), os[0], os[1],
              None if lse is None else lse.data_ptr(), n, hq, hkv, d, code, _ptr("prompt_read", err, _check_err))
@@ -671,7 +677,7 @@ def prompt_read_grad(dout, q, k, v, out, lse, qsl, *, softmax_scale, causal=True
         workspace = q.new_empty(max(size, 0), dtype=torch.uint8)
     elif workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
         raise FoldError("prompt_read_grad: workspace must be a contiguous uint8 tensor (prompt_grad_workspace)")
-    left, right = window_size
+    left, right = _window(window_size)
     _call_on(dev, "fold_prompt_read_grad", dout.data_ptr(), dos[0], dos[1], q.data_ptr(), qs[0], qs[1], k.data_ptr(),
              ks[0], ks[1], v.data_ptr(), vs[0], vs[1], out.data_ptr(), os[0], os[1], lse.data_ptr(),
              None if dlse is None else dlse.data_ptr(), qsl.data_ptr(), b, 1 if causal else 0, left, right,

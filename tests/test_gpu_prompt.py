@@ -94,6 +94,13 @@ def test_read_layouts(layout, hd):
     assert torch.equal(c.q, want)
 
 
+def test_windows_past_every_length():
+    c = Prompts([70, 130], 4, 2, 64, seed=4)
+    want = read(c, False)[0]
+    for window in ((1 << 40, 1 << 33), (-(1 << 40), 1 << 31), (2 ** 31 - 1, 2 ** 30)):
+        assert torch.equal(read(c, False, window)[0], want)
+
+
 def test_read_large_logits():
     for dtype in DT:
         check_read(Prompts([260], 4, 2, 128, dtype, seed=5, boost=6.0))
