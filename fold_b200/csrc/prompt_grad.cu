@@ -674,7 +674,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         }
       }
       __syncwarp();
-      tc_fence_before();  // the next item's products come behind its first tile's P or dS
+      tc_fence_before();  // the next item's acc0 comes behind its first tile's P, acc1 behind all reads of its dP
     }
     if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
   } else {
@@ -839,6 +839,9 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           __syncwarp();
         }
         if (next.valid) landed(next, 1);
+        // An item's first product overwrites acc1, which either warpgroup may still be reading for the item before:
+        // once all have read dP they are through with it (dS of one half tells of one warpgroup only).
+        if (now.first) ok = ok && warp_wait(&B.dp_read, g & 1);
 #pragma unroll
         for (int half = 0; ok && half < 2; ++half) {
           ok = warp_wait(&B.ds_full[half], g & 1);

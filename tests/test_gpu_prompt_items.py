@@ -1,0 +1,51 @@
+"""Attention over whole prompts and its gradient where every block takes several items of several tiles, against float64."""
+import random
+
+import pytest
+import torch
+
+from tests.prompt_cases import DT, Prompts, check
+from tests.test_gpu_prompt import grad, read
+
+pytestmark = pytest.mark.gpu
+
+# Sequences, their least and most rows, heads. With the SMs' 148 blocks an item is followed by others, keys' and
+# rows': 24 sequences of 2 KV heads split a group of four into its heads, 12 of 8 KV heads into pairs; where a
+# device's blocks have three key tiles each (tiles x KV heads >= 444) an item has all heads of its group.
+PACKS = [(24, 100, 700, 8, 2), (12, 100, 700, 32, 8), (7, 150, 550, 64, 32), (17, 60, 600, 48, 16)]
+
+
+def pack(shape, hd, dtype, layout="packed"):
+    b, lo, hi, hq, hkv = shape
+    rng = random.Random(b + hd)
+    lens = [rng.randint(lo, hi) for _ in range(b)]
+    lens[1], lens[3] = 1, 0
+    return Prompts(lens, hq, hkv, hd, dtype, seed=b + hd, lead=2, rest=3, layout=layout)
+
+
+def compare(c, causal=True, window=(-1, -1), dlse=None, rows=slice(None)):
+    """Forward and backward, at the given rows; the backward pass three times with equal bits."""
+    out, lse = read(c, causal, window)
+    want, tol = c.oracle(causal, window, dlse)
+    check(out[rows], want["out"][rows], tol["out"][rows], "out")
+    check(lse[:, rows], want["lse"][:, rows], tol["lse"][:, rows], "lse")
+    first = None
+    for _ in range(3):
+        got = [c.full(c.hq), c.full(c.hkv), c.full(c.hkv)]
+        grad(c, out, lse, causal, window, dlse=dlse, dq=got[0], dk=got[1], dv=got[2])
+        got = [x[rows] for x in got]
+        first = first or got
+        for name, x, y in zip(("dq", "dk", "dv"), got, first):
+            check(x, want[name][rows], tol[name][rows], name)
+            assert torch.equal(x, y), f"{name} has other bits in another call"
+
+
+@pytest.mark.parametrize("causal,window", [(True, (-1, -1)), (True, (200, -1)), (False, (90, 150))])
+@pytest.mark.parametrize("hd", [64, 80, 128])
+@pytest.mark.parametrize("shape", PACKS, ids=str)
+def test_items_behind_items(shape, hd, causal, window):
+    """Accumulators, tiles and places that one item leaves are the next one's."""
+    dtype = "fp16" if hd == 80 or window[1] > 0 else "bf16"
+    c = pack(shape, hd, dtype)
+    dlse = torch.randn(c.hq, c.n, device="cuda", generator=torch.Generator("cuda").manual_seed(7)) if window[0] > 0 else None
+    compare(c, causal, window, dlse)
