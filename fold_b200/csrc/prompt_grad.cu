@@ -550,8 +550,10 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           ok = warp_wait(&B.b_full[g % NB], (g / NB) & 1);
           if (!ok) break;
           unsigned char *ta = smem + (g % NA) * C::UNIT, *tb = smem + C::OFF_B + (g % NB) * C::UNIT;
-          for (int e = tid; e < (128 - left) * C::NCG * 8; e += NSW * 32) {
-            const int at = left + e / (C::NCG * 8), c = e % (C::NCG * 8);
+          // (each warpgroup those of its half: acc1 of a half waits for that half's dS alone)
+          const int zero0 = max(left, wg * CW), zeros = (wg + 1) * CW - zero0;
+          for (int e = tid & 127; e < zeros * C::NCG * 8; e += 128) {
+            const int at = zero0 + e / (C::NCG * 8), c = e % (C::NCG * 8);
             const int off = (c >> 3) * C::CG + at * 128 + (c & 7) * 16;
             *reinterpret_cast<uint4*>(ta + off) = make_uint4(0, 0, 0, 0);
             *reinterpret_cast<uint4*>(tb + off) = make_uint4(0, 0, 0, 0);

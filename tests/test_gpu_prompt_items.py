@@ -1,4 +1,5 @@
 """Attention over whole prompts and its gradient where every block takes several items of several tiles, against float64."""
+import math
 import random
 
 import pytest
@@ -49,3 +50,20 @@ def test_items_behind_items(shape, hd, causal, window):
     c = pack(shape, hd, dtype)
     dlse = torch.randn(c.hq, c.n, device="cuda", generator=torch.Generator("cuda").manual_seed(7)) if window[0] > 0 else None
     compare(c, causal, window, dlse)
+
+
+@pytest.mark.parametrize("window", [(-1, -1), (130, -1)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_neighbours_of_cut_tiles(hd, window):
+    """Tiles cut in either half, beside sequences of NaN and infinities: weights of zero meet zeros."""
+    for hq, hkv in ((8, 2), (10, 2)):
+        lens = [x for i in range(40) for x in (128 * (i % 4) + 3 * i + 1, 140)]
+        c = Prompts(lens, hq, hkv, hd, "bf16", seed=hd, layout="own", rest=130)
+        rows = torch.ones(c.n, dtype=torch.bool, device="cuda")
+        for i in range(1, len(lens), 2):
+            w = slice(c.starts[i], c.starts[i + 1])
+            rows[w] = False
+            for x, bad in ((c.q, math.nan), (c.k, math.inf), (c.v, -math.inf), (c.do, math.nan)):
+                x[w] = bad
+        rows[c.starts[-1]:] = False
+        compare(c, True, window, rows=rows)
