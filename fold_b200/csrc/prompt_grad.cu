@@ -683,7 +683,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
     regs_down<kOtherRegs>();
     if (warp == NSW) {
       // ------------------------------------------------------------ loads
-      uint32_t g = 0, items = 0;
+      uint32_t g = 0, a_sent = 0, b_sent = 0, r0_sent = 0, r1_sent = 0;  // tiles so far; copies of each kind
       bool ok = true;
       if (lane == 0) prefetch_tensormap(&qmap), prefetch_tensormap(&domap), prefetch_tensormap(&kmap), prefetch_tensormap(&vmap);
       // dP of tile n, and with it all products of the tiles before
@@ -709,24 +709,28 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             if (i > 0) ok = through(g - 1);
             if (!ok) break;
             load(keys ? &kmap : &qmap, C::OFF_R, &B.r_full[0], it.head, it.first + it.row0);
+            ++r0_sent;
           }
           if (g >= NA) ok = through(g - NA + 1);
           if (!ok) break;
           load(keys ? &qmap : &kmap, (g % NA) * C::UNIT, &B.a_full[g % NA], head, row);
+          ++a_sent;
           if (first) {
             load(keys ? &vmap : &domap, C::OFF_R + C::UNIT, &B.r_full[1], it.head, it.first + it.row0);
-            items = i + 1;
+            ++r1_sent;
           }
           if (g >= NB) ok = through(g - NB + 1);
           if (!ok) break;
           load(keys ? &domap : &vmap, C::OFF_B + (g % NB) * C::UNIT, &B.b_full[g % NB], head, row);
+          ++b_sent;
         }
       }
       if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
-      // copies land before exit
-      for (uint32_t w = g > NA ? g - NA : 0; w < g; ++w) warp_wait(&B.a_full[w % NA], (w / NA) & 1);
-      for (uint32_t w = g > NB ? g - NB : 0; w < g; ++w) warp_wait(&B.b_full[w % NB], (w / NB) & 1);
-      if (items > 0) warp_wait(&B.r_full[0], (items - 1) & 1), warp_wait(&B.r_full[1], (items - 1) & 1);
+      // copies land before exit, those of a tile that another wait gave up on too
+      for (uint32_t w = a_sent > NA ? a_sent - NA : 0; w < a_sent; ++w) warp_wait(&B.a_full[w % NA], (w / NA) & 1);
+      for (uint32_t w = b_sent > NB ? b_sent - NB : 0; w < b_sent; ++w) warp_wait(&B.b_full[w % NB], (w / NB) & 1);
+      if (r0_sent > 0) warp_wait(&B.r_full[0], (r0_sent - 1) & 1);
+      if (r1_sent > 0) warp_wait(&B.r_full[1], (r1_sent - 1) & 1);
     } else if (warp == NSW + 1) {
       // ------------------------------------------------------------ MMAs
       constexpr uint32_t idesc_s = idesc_of(C::F16, 128, 0), idesc_o = idesc_of(C::F16, HD, 1), hi = desc_hi(1024);
