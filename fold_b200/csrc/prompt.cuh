@@ -229,6 +229,9 @@ int prompt_shape(const char* what, const int* qsl, int b, int n, int hq, int hkv
 // An operand's pointer, alignment and strides; `written`: its rows must not share memory.
 int prompt_rows(const char* what, const char* name, const void* ptr, int64_t tok, int64_t head, int n, int heads,
                 int hd, bool written, prompt::Rows* out);
+// Whether two operands of n rows share memory: exact for views of one tensor, whose tokens (or heads, where those come
+// first) lie at one stride; operands at other strides that reach into each other are taken to.
+bool prompt_overlap(prompt::Rows a, int heads_a, prompt::Rows b, int heads_b, int n, int hd);
 // Map of an operand: columns, heads, rows; a box is 64 columns of `rows` rows of one head.
 int prompt_map(const char* what, const prompt::Rows& x, int heads, int n, int hd, int rows, bool f16, CUtensorMap* out);
 

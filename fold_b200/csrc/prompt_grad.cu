@@ -1094,8 +1094,9 @@ int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_st
     if (int s = prompt_rows(what, r.name, r.ptr, r.tok, r.head, n, r.heads, hd, r.written, r.to)) return s;
   for (int i = 5; i < 8; ++i)
     for (int k = 0; k < i; ++k)
-      if (rows[i].ptr == rows[k].ptr)
-        return fail(FOLD_ERR_INVALID_ARGUMENT, std::string("prompt read grad: ") + rows[i].name + " must not be " + rows[k].name);
+      if (prompt_overlap(*rows[i].to, rows[i].heads, *rows[k].to, rows[k].heads, n, hd))
+        return fail(FOLD_ERR_INVALID_ARGUMENT,
+                    std::string("prompt read grad: ") + rows[i].name + " must not share memory with " + rows[k].name);
   if (!lse) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: null pointer");
   if (static_cast<int64_t>(n) * hq > (int64_t(1) << 32)) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: too many rows");
   p.splits = tensor_memory_size(hd) ? key_splits(n, hkv, p.s.group) : 1;

@@ -641,6 +641,49 @@ int prompt_rows(const char* what, const char* name, const void* ptr, int64_t tok
   return FOLD_OK;
 }
 
+namespace {
+// na pieces of hd elements at stride sa, and nb at stride sb from `off` on: whether any two share an element.
+bool pieces_meet(int64_t off, int na, int64_t sa, int nb, int64_t sb, int hd) {
+  using wide = __int128;
+  if (off >= static_cast<wide>(na - 1) * sa + hd || -off >= static_cast<wide>(nb - 1) * sb + hd) return false;
+  // some k of lo .. hi with |x + k s| < hd
+  auto near = [&](int64_t x, int64_t s, int64_t lo, int64_t hi) {
+    if (s == 0) return x < hd && -x < hd;
+    const int64_t a = -x - hd + 1, k = a > 0 ? (a + s - 1) / s : -(-a / s);  // the least k with x + k s > -hd
+    const int64_t first = k > lo ? k : lo;
+    return first <= hi && x + static_cast<wide>(first) * s < hd;
+  };
+  if (na == 1 || sa == sb) return near(off, sb, na == 1 ? 0 : 1 - na, nb - 1);
+  if (nb > 65536) return true;  // (heads are fewer; tokens at two strides in one range)
+  for (int j = 0; j < nb; ++j)
+    if (near(-off - j * sb, sa, 0, na - 1)) return true;
+  return false;
+}
+}  // namespace
+
+bool prompt_overlap(prompt::Rows a, int heads_a, prompt::Rows b, int heads_b, int n, int hd) {
+  using wide = __int128;
+  const int64_t d = (static_cast<const char*>(b.ptr) - static_cast<const char*>(a.ptr)) / 2;
+  if (heads_a == 1) a.head = b.head;  // strides of a single head or row are free
+  if (heads_b == 1) b.head = a.head;
+  auto span = [&](const prompt::Rows& x, int heads) { return static_cast<wide>(n - 1) * x.tok + static_cast<wide>(heads - 1) * x.head + hd; };
+  if (d >= span(a, heads_a) || -d >= span(b, heads_b)) return false;
+  if (n == 1) return pieces_meet(d, heads_a, a.head, heads_b, b.head, hd);
+  // The outer dimension's pieces lie t apart: b's begin m behind one of a's, and t - m before the next.
+  auto outer = [&](int64_t t, int na, int nb, auto inner) {
+    int64_t k = d / t, m = d % t;
+    if (m < 0) m += t, --k;
+    return (k > -nb && k < na && inner(m)) || (k + 1 > -nb && k + 1 < na && inner(m - t));
+  };
+  auto in_token = [&](const prompt::Rows& x, int heads) { return static_cast<wide>(heads - 1) * x.head + hd <= x.tok; };
+  auto in_head = [&](const prompt::Rows& x) { return static_cast<wide>(n - 1) * x.tok + hd <= x.head; };
+  if (a.tok == b.tok && in_token(a, heads_a) && in_token(b, heads_b))
+    return outer(a.tok, n, n, [&](int64_t off) { return pieces_meet(off, heads_a, a.head, heads_b, b.head, hd); });
+  if (a.head == b.head && in_head(a) && in_head(b))
+    return outer(a.head, heads_a, heads_b, [&](int64_t off) { return pieces_meet(off, n, a.tok, n, b.tok, hd); });
+  return true;
+}
+
 }  // namespace fold
 
 extern "C" {
@@ -660,7 +703,11 @@ int fold_prompt_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
   if (int s = prompt_rows(what, "k", k, k_stride_tok, k_stride_head, n, hkv, hd, false, &p.k)) return s;
   if (int s = prompt_rows(what, "v", v, v_stride_tok, v_stride_head, n, hkv, hd, false, &p.v)) return s;
   if (int s = prompt_rows(what, "out", out, o_stride_tok, o_stride_head, n, hq, hd, true, &p.out)) return s;
-  if (out == k || out == v) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read: out must not be k or v");
+  if (prompt_overlap(p.out, hq, p.k, hkv, n, hd) || prompt_overlap(p.out, hq, p.v, hkv, n, hd))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read: out must not share memory with k or v");
+  const bool over_q = p.out.ptr == p.q.ptr && p.out.tok == p.q.tok && p.out.head == p.q.head;
+  if (!over_q && prompt_overlap(p.out, hq, p.q, hq, n, hd))
+    return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read: out must be q or share no memory with it");
   p.lse = lse, p.err = err;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == FOLD_BF16 ? launch_read<__nv_bfloat16>(p, st) : launch_read<__half>(p, st);

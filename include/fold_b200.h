@@ -232,8 +232,9 @@ int64_t fold_prefix_read_workspace(int n, int hq, int hkv, int hd);
  * of the sum of exp(softmax_scale * q.k). Keys and values of other sequences may hold anything; a value
  * row that some rows of its sequence see must be finite even for rows that do not. dtype FOLD_BF16 or
  * FOLD_FP16; hd a multiple of 8 up to 256 (up to 128 on the tensor-memory kernels); every row on a
- * 16-byte boundary; out must not overlap k or v, and q only as q itself. b and n are what a captured
- * call is fixed to. err (may be NULL) takes FOLD_DEVERR_TIMEOUT. */
+ * 16-byte boundary; out must not share memory with k or v, and with q only as q itself (refused; views of one
+ * tensor that lie side by side are fine, operands at different strides must lie apart). b and n are what a
+ * captured call is fixed to. err (may be NULL) takes FOLD_DEVERR_TIMEOUT. */
 int fold_prompt_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,
                      int64_t k_stride_head, const void* v, int64_t v_stride_tok, int64_t v_stride_head, const int* qsl,
                      int b, int causal, int window_left, int window_right, float softmax_scale, void* out,
@@ -245,7 +246,7 @@ int fold_prompt_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
  * value summed over the heads of its group. Rows outside the sequences get zeros when `zero_rest`, else
  * they are left as they were. As for values, a row of q and dout must be finite even for keys that it does not
  * see, and a key and value for rows that do not see it. No sum depends on the order in which blocks run: equal calls give equal
- * bits. The gradients must not overlap the inputs. workspace: fold_prompt_read_grad_workspace bytes of
+ * bits. The gradients must not share memory with the inputs or each other (refused, as above). workspace: fold_prompt_read_grad_workspace bytes of
  * device memory, 16-byte aligned, not shared by calls that may overlap; nothing in it outlives the call. */
 int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_stride_head, const void* q,
                           int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,

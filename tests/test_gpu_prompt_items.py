@@ -67,3 +67,21 @@ def test_neighbours_of_cut_tiles(hd, window):
                 x[w] = bad
         rows[c.starts[-1]:] = False
         compare(c, True, window, rows=rows)
+
+
+@pytest.mark.parametrize("first", [False, True])
+def test_results_beside_the_inputs(first):
+    """Outputs that are views of the inputs' tensor, tokens or heads first, and share no row with them."""
+    n, hq, hkv, hd = 200, 4, 2, 64
+    c = Prompts([150, 50], hq, hkv, hd, seed=3, layout="own")
+    out, lse = read(c)
+    want = grad(c, out, lse)
+    heads = [hq, hkv, hkv, hq, hq, hkv, hkv]
+    x = torch.zeros((sum(heads), n, hd) if first else (n, sum(heads), hd), device="cuda", dtype=c.dt)
+    parts = [p.transpose(0, 1) if first else p for p in x.split(heads, 0 if first else 1)]
+    for p, t in zip(parts, (c.q, c.k, c.v)):
+        p.copy_(t)
+    c.q, c.k, c.v = parts[:3]
+    assert torch.equal(read(c, out=parts[3])[0], out)
+    got = grad(c, parts[3], lse, dq=parts[4], dk=parts[5], dv=parts[6])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
