@@ -383,12 +383,22 @@ __global__ void __launch_bounds__(128) fork_copy_kernel(const __grid_constant__ 
       int bad = 0;
       for (int j = threadIdx.x; j < full; j += 128) {
         const int page = *pool.entry(s, j);
+        bad |= page < 0 || page >= pool.pages;
+      }
+      if (__syncthreads_or(bad)) {  // the child stays empty, and gives back the page it took
+        if (threadIdx.x == 0) {
+          pool.lens[d] = 0;
+          if (plan.z > 0) atomicSub(pool.refs + plan.y, 1);
+          set_error(pool.err, FOLD_DEVERR_BLOCK_TABLE);
+        }
+        return;
+      }
+      for (int j = threadIdx.x; j < full; j += 128) {
+        const int page = *pool.entry(s, j);
         *pool.entry(d, j) = page;
-        if (page < 0 || page >= pool.pages) bad |= FOLD_DEVERR_BLOCK_TABLE;
-        else atomicAdd(pool.refs + page, 1);
+        atomicAdd(pool.refs + page, 1);
       }
       if (threadIdx.x == 0 && plan.z > 0) *pool.entry(d, full) = plan.y;
-      if (bad) set_error(pool.err, bad);
       return;
     }
     x -= p.f.m;

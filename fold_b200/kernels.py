@@ -737,7 +737,7 @@ def grow_pages(refs, block_tables, lens, qsl, n, *, block_size, rows=None, posit
 def free_pages(refs, block_tables, lens, rows=None, *, block_size, keep=None, err=None):
     """Cuts rows (int32 [m]; None: all; a negative one is skipped) of a page pool (grow_pages) down to keep tokens
     (int32 [m]; None: none): drafted tokens that were not accepted, sequences that are done. Pages that their
-    last row leaves become free."""
+    last row leaves become free. Bad tables are reported in err; their rows are cut all the same."""
     dev = _check_devices("free_pages", refs, block_tables, lens, rows, keep, err)
     pool = _check_pool("free_pages", refs, block_tables, lens, (rows, keep), block_size)
     m = lens.shape[0] if rows is None else rows.shape[0]
@@ -751,8 +751,9 @@ def fork_pages(refs, block_tables, lens, src, dst, caches, *, workspace=None, er
     """Row dst[i] of a page pool (grow_pages) becomes a copy of row src[i] (int32 [m]; a negative row skips the
     pair): full pages are shared, the tokens of a partly filled last page are copied to a fresh one in every
     cache of the list `caches` (the layers' [pages, Hkv, block_size, width] tensors or planes, all of one
-    shape, type and strides). The rows dst must be empty (free_pages) and distinct; such that are not, and
-    children that find no free page, are reported in err."""
+    shape, type and strides). The rows dst must be empty (free_pages) and distinct; such that are not,
+    children that find no free page and those of a table that names no page are left as they were and
+    reported in err."""
     dev = _check_devices("fork_pages", refs, block_tables, lens, src, dst, workspace, err, *caches)
     if not caches or caches[0].dim() != 4:
         raise FoldError("fork_pages: caches is a list of [pages, Hkv, block_size, width] tensors")

@@ -281,7 +281,9 @@ int fold_grow_pages(int* refs, int num_pages, int* block_tables, int64_t block_t
                     void* positions, void* slots, int* err, void* stream);
 
 /* Cuts rows[i] (NULL: row i) down to keep[i] tokens (NULL: none); pages that are left by their last row
- * become free. A row named twice is cut to the smaller length, and gives each page back once. */
+ * become free. A row named twice is cut to the smaller length, and gives each page back once. An entry outside the
+ * pool (FOLD_DEVERR_BLOCK_TABLE), a page that nobody holds (FOLD_DEVERR_REFS) and a length past the table
+ * (FOLD_DEVERR_CAPACITY) are reported; the row is cut all the same and its other pages are given back. */
 int fold_free_pages(int* refs, int num_pages, int* block_tables, int64_t block_tables_stride, int block_tables_len,
                     int* lens, int num_rows, const int* rows, const int* keep, int m, int block_size, int* err,
                     void* stream);
@@ -290,7 +292,8 @@ int fold_free_pages(int* refs, int num_pages, int* block_tables, int64_t block_t
  * of a partly filled last page are copied to a fresh one in each of the caches, [num_pages, heads,
  * block_size] rows of row_bytes at the given strides (bytes), all alike (caches: host array of device
  * addresses). A negative row skips the pair. dst must be empty, else, or named before, it is left alone
- * (FOLD_DEVERR_ROW); a child that finds no free page stays empty (FOLD_DEVERR_PAGES). workspace:
+ * (FOLD_DEVERR_ROW); a child that finds no free page (FOLD_DEVERR_PAGES), or whose parent's table names a
+ * page outside the pool (FOLD_DEVERR_BLOCK_TABLE), stays empty. workspace:
  * fold_fork_pages_workspace bytes of device memory, 16-byte aligned, not shared by calls that overlap. */
 int fold_fork_pages(int* refs, int num_pages, int* block_tables, int64_t block_tables_stride, int block_tables_len,
                     int* lens, int num_rows, const int* src, const int* dst, int m, const int64_t* caches, int num_caches,
