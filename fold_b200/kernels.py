@@ -629,7 +629,8 @@ def prompt_read(q, k, v, qsl, out, *, softmax_scale, causal=True, window_size=(-
 
 
 def prompt_grad_workspace(n, hq, hkv, d, device):
-    """A workspace for prompt_read_grad calls of up to these sizes (one per call that may overlap another)."""
+    """A workspace for prompt_read_grad calls of up to n rows with these heads and this head size (other heads or
+    another head size, smaller ones too, may take more); one per call that may overlap another."""
     dev = torch.device(device)
     if dev.type != "cuda":
         raise FoldError("FOLD kernels take CUDA tensors (there is no CPU path)")

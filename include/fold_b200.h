@@ -258,7 +258,8 @@ int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_st
                           int64_t dv_stride_head, int zero_rest, void* workspace, int64_t workspace_bytes, int n,
                           int hq, int hkv, int hd, int dtype, int* err, void* stream);
 
-/* Bytes of workspace that calls of up to n rows take (-1: sizes fold_prompt_read_grad does not take). */
+/* Bytes of workspace that calls of up to n rows with these heads and this head size take (-1: sizes that
+ * fold_prompt_read_grad does not take). */
 int64_t fold_prompt_read_grad_workspace(int n, int hq, int hkv, int hd);
 
 /* Pages of a paged cache, kept on the device; no reference counterpart (vLLM's host keeps them).
