@@ -1016,6 +1016,8 @@ int64_t most_part_bytes(int n, int hkv, int group, int hd) {
   return most;
 }
 bool tensor_memory_size(int hd) { return hd <= 128; }
+// The kernel of the other head sizes has a head of keys or queries in each of the grid's y blocks.
+bool heads_fit(int hq, int hkv, int hd) { return tensor_memory_size(hd) || hq + hkv <= 65535; }
 
 template <int HD, class T>
 int launch_tc(const GradParams& p, cudaStream_t stream) {
@@ -1063,7 +1065,7 @@ int launch_grad(const GradParams& p, cudaStream_t stream) {
 extern "C" {
 
 int64_t fold_prompt_read_grad_workspace(int n, int hq, int hkv, int hd) {
-  if (n < 0 || hq < 1 || hkv < 1 || hq % hkv || hq > 65535 || hd < 8 || hd > 256 || hd % 8) return -1;
+  if (n < 0 || hq < 1 || hkv < 1 || hq % hkv || hq > 65535 || hd < 8 || hd > 256 || hd % 8 || !fold::heads_fit(hq, hkv, hd)) return -1;
   const int64_t rows = (static_cast<int64_t>(n) * hq * 8 + 15) / 16 * 16;
   return rows + 16 + (fold::tensor_memory_size(hd) ? fold::most_part_bytes(n, hkv, hq / hkv, hd) : 0);
 }
@@ -1082,6 +1084,7 @@ int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_st
   GradParams p{};
   if (int s = prompt_shape(what, qsl, b, n, hq, hkv, hd, dtype, causal, window_left, window_right, softmax_scale, &p.s))
     return s;
+  if (!heads_fit(hq, hkv, hd)) return fail(FOLD_ERR_UNSUPPORTED, "prompt read grad: too many heads for this head size");
   if (n == 0) return FOLD_OK;
   if (b == 0 && !zero_rest) return FOLD_OK;
   if (b == 0) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: no sequences");

@@ -12,12 +12,14 @@ def enough(size, n, hq, hkv, hd):
     there, before anything is launched."""
     ops = [x for i, heads in enumerate((hq, hq, hkv, hkv, hq)) for x in (FAR * (i + 2), heads * hd, hd)]
     outs = [x for i, heads in enumerate((hq, hkv, hkv)) for x in (FAR * (i + 10), heads * hd, hd)]
-    with pytest.raises(FoldError) as e:
+    try:
         _lib.call("fold_prompt_read_grad", *ops, 16, None, 16, 1, 1, -1, -1, 1.0, *outs, 0, 8, size, n, hq, hkv, hd, 0, None,
                   None)
-    text = str(e.value)
-    assert "16-byte aligned" in text or "workspace holds" in text, text
-    return "16-byte aligned" in text
+    except FoldError as e:
+        if "16-byte aligned" in str(e) or "workspace holds" in str(e):
+            return "16-byte aligned" in str(e)
+        raise
+    raise AssertionError("a workspace off a boundary was taken")
 
 
 @pytest.mark.parametrize("hq,hkv,hd", [(32, 8, 128), (32, 1, 64), (24, 4, 80), (12, 2, 128), (28, 4, 64), (16, 16, 128),
@@ -40,3 +42,13 @@ def test_other_heads_may_take_more():
     size = _lib.prompt_read_grad_workspace
     assert size(2048, 32, 8, 128) > size(2048, 32, 8, 256) and size(4096, 32, 8, 128) > size(4096, 32, 32, 128)
     assert not enough(size(2048, 32, 8, 256), 2048, 32, 8, 128) and not enough(size(4096, 32, 32, 128), 4096, 32, 8, 128)
+
+
+def test_heads_past_the_grid():
+    """Above head size 128 heads of queries and keys together are up to 65535."""
+    size = _lib.prompt_read_grad_workspace
+    for hq, hkv in ((40000, 40000), (65535, 1)):
+        assert size(1, hq, hkv, 256) == size(1, hq, hkv, 136) == -1 and size(1, hq, hkv, 128) > 0
+        with pytest.raises(FoldError, match="too many heads"):
+            enough(1 << 40, 1, hq, hkv, 256)
+    assert size(1, 65534, 1, 256) > 0
