@@ -29,6 +29,9 @@ struct GradParams {
   const float* lse;   // [hq, n]
   const float* dlse;  // [hq, n] or null
   float2* row;        // workspace [hq, n]: shift - lse log2(e), -delta 2^-shift (see Shift)
+  float* norm;        // workspace [hq + hkv, n], fp16: |do_r|^2 of a query head, |v_j|^2 of a KV head
+  float2* most;       // workspace [n, hq + hkv], fp16: the largest of them, and of |dlse_r|, in the sequence that starts at
+                      // a row (see held_up)
   float* part;        // workspace [splits][dk, dv][n, hkv, hd]: sums over some of a group's heads (splits > 1)
   int splits;
   int zero_rest;      // rows outside the sequences get gradients of zero
@@ -39,9 +42,73 @@ struct GradParams {
 // rows with many keys keep their bits; dS takes the factor back out.
 template <class T>
 struct Shift {
-  static constexpr float kUp = std::is_same<T, __nv_bfloat16>::value ? 0.f : 10.f;
-  static constexpr float kDown = std::is_same<T, __nv_bfloat16>::value ? 1.f : 1.f / 1024.f;
+  static constexpr bool F16 = std::is_same<T, __half>::value;
+  static constexpr float kUp = F16 ? 10.f : 0.f;
+  static constexpr float kDown = F16 ? 1.f / 1024.f : 1.f;
 };
+
+// dS of fp16 is held up too, by a power of two that dq and dk take back out: dS of thousands of keys and a small dout
+// lies below the type's normal numbers (2^-14) where dq and dk do not (4096 keys, dout of size 0.001: dq was off by
+// 3.5 to 4.5 times its own rounding, now by 1.25). The power follows a bound of dS in a sequence,
+//   |dS_rj| <= |do_r.v_j| + |delta_r| <= 2 max|do_r| max|v_j| + max|dlse_r|  (norms; o_r lies between the v_j),
+// so that nothing passes the type's range that did not before: 1 where the bound is 2^15 or more or not finite.
+// Typical dS of n keys lie some 2^5 n below the bound, which leaves 12 binades for smaller rows at 4096 keys. A NaN
+// makes its own results NaN whatever the bound, so it is left out. The norms come from the rows' first kernel, their
+// maxima from a launch of their own (5 us of 185 for 2048 rows of 32 heads): with the factor in the softmax fp16 takes
+// 192 us there where it took 185; 8192 rows 1.95 ms for 1.91, a batch of short sequences 6 to 10 percent more. Maxima by atomics in the first kernel took it from 15 to 33 us.
+// Rows' items hold dS up through P, which dq has no other use of; keys' need P for dv as it is.
+// Heads [h0, h0 + nh) with KV head hk of the sequence from row `first` on; all lanes of a warp call this.
+__device__ __forceinline__ float warp_most(float x) {  // of numbers that are not negative
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x)));
+}
+__device__ __forceinline__ float2* most_of(const GradParams& p, int first) {
+  return p.most + static_cast<int64_t>(first) * (p.s.hq + p.s.hkv);
+}
+template <class T>
+__device__ __forceinline__ float held_up(const GradParams& p, int first, int h0, int nh, int hk) {
+  if constexpr (!Shift<T>::F16) return 1.f;
+  const float2* at = most_of(p, first);
+  const float v = at[p.s.hq + hk].x;
+  float d = 0.f, l = 0.f;
+  for (int h = h0 + static_cast<int>(threadIdx.x & 31); h < h0 + nh; h += 32) {
+    const float2 b = at[h];
+    d = fmaxf(d, b.x), l = fmaxf(l, b.y);
+  }
+  const float m = fmaf(2.02f * sqrtf(warp_most(d)), sqrtf(v), warp_most(l));
+  const int e = min(max(141 - static_cast<int>(__float_as_uint(m) >> 23), 0), 60);  // m 2^e < 2^15
+  return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+__device__ __forceinline__ float log2_of_power(float x) {
+  return static_cast<float>(static_cast<int>(__float_as_uint(x) >> 23) - 127);
+}
+// GradParams::most from the rows' norms: a warp a sequence and head (8192 rows: four microseconds).
+__global__ void __launch_bounds__(256) prompt_most_kernel(const GradParams p) {
+  const int64_t x = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int heads = p.s.hq + p.s.hkv, s = static_cast<int>(x / heads), h = static_cast<int>(x - static_cast<int64_t>(s) * heads);
+  const int lane = threadIdx.x & 31;
+  wait_for_producer();
+  if (s >= p.s.b) return;
+  int first, last;
+  seq_rows(p.s, s, first, last);
+  if (first == last) return;
+  auto most = [&](const float* row) {  // of the sequence's sizes (fmaxf leaves NaN out)
+    float top = 0.f;
+    auto take = [&](float y) { top = fmaxf(top, fabsf(y)); };
+    const int lead = min(static_cast<int>(-(reinterpret_cast<uintptr_t>(row) >> 2) & 3), last - first);  // before whole quads
+    const int quads = (last - first - lead) / 4, rest = lead + quads * 4;
+    if (lane < lead) take(row[lane]);
+    if (rest + lane < last - first) take(row[rest + lane]);
+#pragma unroll 8
+    for (int q = lane; q < quads; q += 32) {
+      const float4 y = *reinterpret_cast<const float4*>(row + lead + q * 4);
+      take(y.x), take(y.y), take(y.z), take(y.w);
+    }
+    return warp_most(top);
+  };
+  const float size = most(p.norm + static_cast<int64_t>(h) * p.s.n + first);
+  const float slope = p.dlse && h < p.s.hq ? most(p.dlse + static_cast<int64_t>(h) * p.s.n + first) : 0.f;
+  if (lane == 0) most_of(p, first)[h] = make_float2(size, slope);
+}
 
 // A row that sees up to this many keys has delta from them, as sum_j P_j (do.v_j) in float32, instead of from the
 // rounded out: where few keys share the weight, out's rounding is as large as what dP and delta leave of each other
@@ -95,11 +162,22 @@ __global__ void __launch_bounds__(128, 12) prompt_delta_kernel(const GradParams 
   };
   uint32_t wo[4], wd[4];
   load(p.out, t, h, wo), load(p.dout, t, h, wd);
+  // (fp16) the values' norms by the warps of as many heads
+  const bool values = Shift<T>::F16 && own - lane / L < p.s.hkv;
+  uint32_t wn[4];
+  if (values) load(p.v, t, min(own, p.s.hkv - 1), wn);
   const int seq = last_sequence(p.s, [&](int, int first) { return first <= t; });
   int first, last, lo, hi;
   seq_rows(p.s, max(seq, 0), first, last);
   keys_of(p.s, last - first, t - first, t - first + 1, lo, hi);
   float sum = total(dot(wo, wd));
+  if constexpr (Shift<T>::F16) {
+    const float d = total(dot(wd, wd)), v = values ? total(dot(wn, wn)) : 0.f;
+    if (lane % L == 0) {
+      if (own < p.s.hq) p.norm[static_cast<int64_t>(h) * p.s.n + t] = d;
+      if (values && own < p.s.hkv) p.norm[static_cast<int64_t>(p.s.hq + own) * p.s.n + t] = v;
+    }
+  }
   if (t >= first && t < last && hi - lo <= kExactKeys) {
     float top = -INFINITY, num = 0.f, den = 0.f;
     const int hk = h / p.s.group;
@@ -197,6 +275,7 @@ __device__ __forceinline__ void keys_mma(const GradParams& p, const Tile& t, int
   const int rb = lo / 64, re = (hi + 63) / 64;
   stage_rows<DP, NT>(sk, p.k, t.first, t.len, t.row0, hk, hd);
   stage_rows<DP, NT>(sv, p.v, t.first, t.len, t.row0, hk, hd);
+  const float up = held_up<T>(p, t.first, hk * p.s.group, p.s.group, hk), down = Shift<T>::kDown * up;
   float dk[2 * NC][4], dv[2 * NC][4];
 #pragma unroll
   for (int i = 0; i < 2 * NC; ++i)
@@ -209,10 +288,11 @@ __device__ __forceinline__ void keys_mma(const GradParams& p, const Tile& t, int
       stage_rows<DP, NT>(sq, p.q, t.first, t.len, j * 64, h, hd);
       stage_rows<DP, NT>(sd, p.dout, t.first, t.len, j * 64, h, hd);
       cp_commit();
-      if (threadIdx.x < 64)
-        rows[threadIdx.x] = j * 64 + threadIdx.x < t.len
-                                ? p.row[static_cast<int64_t>(h) * p.s.n + t.first + j * 64 + threadIdx.x]
-                                : make_float2(-INFINITY, 0.f);
+      if (threadIdx.x < 64) {
+        float2 rr = make_float2(-INFINITY, 0.f);
+        if (j * 64 + threadIdx.x < t.len) rr = p.row[static_cast<int64_t>(h) * p.s.n + t.first + j * 64 + threadIdx.x];
+        rows[threadIdx.x] = make_float2(rr.x, rr.y * up);
+      }
       cp_wait<0>();
       __syncthreads();
       float x[8][4], d[8][4];
@@ -228,11 +308,11 @@ __device__ __forceinline__ void keys_mma(const GradParams& p, const Tile& t, int
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = i * 8 + 2 * t4 + (e & 1), row = j * 64 + r, key = key0 + (e >> 1) * 8;
-          const float2 rr = rows[r];
+          const float2 rr = rows[r];  // (-delta as dS is held)
           const bool in = row < t.len && key >= row - p.s.left && key <= row + p.s.right && key < t.len;
           pv[e] = in ? fast_exp2(fmaf(x[i][e], p.s.scale_log2, rr.x)) : 0.f;
-          sv4[e] = in ? pv[e] * fmaf(d[i][e], Shift<T>::kDown, rr.y) : 0.f;
-          if (row == key && in && lone(p.s, t.len, row)) sv4[e] = lone_ds<T>(p, h, t.first + row, pv[e]);
+          sv4[e] = in ? pv[e] * fmaf(d[i][e], down, rr.y) : 0.f;
+          if (row == key && in && lone(p.s, t.len, row)) sv4[e] = lone_ds<T>(p, h, t.first + row, pv[e]) * up;
         }
         pa[i >> 1][(i & 1) * 2] = pack_pair<T>(pv[0], pv[1]);
         pa[i >> 1][(i & 1) * 2 + 1] = pack_pair<T>(pv[2], pv[3]);
@@ -246,6 +326,7 @@ __device__ __forceinline__ void keys_mma(const GradParams& p, const Tile& t, int
       if (two) product<DP, NC, T>(dk, dl, sq, part * NC);
     }
   }
+  const float out_scale = p.s.scale / up;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int key = key0 + e * 8;
@@ -256,7 +337,7 @@ __device__ __forceinline__ void keys_mma(const GradParams& p, const Tile& t, int
     for (int i = 0; i < 2 * NC; ++i) {
       const int c = part * NC * 16 + i * 8;
       if (c >= hd) continue;
-      *reinterpret_cast<uint32_t*>(ok + c + 2 * t4) = pack_pair<T>(dk[i][2 * e] * p.s.scale, dk[i][2 * e + 1] * p.s.scale);
+      *reinterpret_cast<uint32_t*>(ok + c + 2 * t4) = pack_pair<T>(dk[i][2 * e] * out_scale, dk[i][2 * e + 1] * out_scale);
       *reinterpret_cast<uint32_t*>(ov + c + 2 * t4) =
           pack_pair<T>(dv[i][2 * e] * Shift<T>::kDown, dv[i][2 * e + 1] * Shift<T>::kDown);
     }
@@ -277,6 +358,7 @@ __device__ __forceinline__ void rows_mma(const GradParams& p, const Tile& t, int
   const int kb = lo / 64, ke = (hi + 63) / 64;
   stage_rows<DP, NT>(sq, p.q, t.first, t.len, t.row0, h, hd);
   stage_rows<DP, NT>(sd, p.dout, t.first, t.len, t.row0, h, hd);
+  const float up = held_up<T>(p, t.first, h, 1, hk);
   float dq[2 * NC][4];
 #pragma unroll
   for (int i = 0; i < 2 * NC; ++i)
@@ -291,6 +373,7 @@ __device__ __forceinline__ void rows_mma(const GradParams& p, const Tile& t, int
     keys_of(p.s, t.len, r, r + 1, klo[e], khi[e]);
     if (r >= t.len) khi[e] = 0;
     rr[e] = r < t.len ? p.row[static_cast<int64_t>(h) * p.s.n + t.first + r] : make_float2(-INFINITY, 0.f);
+    rr[e].x += log2_of_power(up);
   }
   for (int j = kb; j < ke; ++j) {
     __syncthreads();
@@ -324,6 +407,7 @@ __device__ __forceinline__ void rows_mma(const GradParams& p, const Tile& t, int
     product<DP, NC, T>(dq, da, sk, part * NC);
     if (two) product<DP, NC, T>(dq, dl, sk, part * NC);
   }
+  const float out_scale = p.s.scale / up;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int r = t.row0 + warp * 16 + e * 8 + g;
@@ -333,7 +417,7 @@ __device__ __forceinline__ void rows_mma(const GradParams& p, const Tile& t, int
     for (int i = 0; i < 2 * NC; ++i) {
       const int c = part * NC * 16 + i * 8;
       if (c < hd)
-        *reinterpret_cast<uint32_t*>(o + c + 2 * t4) = pack_pair<T>(dq[i][2 * e] * p.s.scale, dq[i][2 * e + 1] * p.s.scale);
+        *reinterpret_cast<uint32_t*>(o + c + 2 * t4) = pack_pair<T>(dq[i][2 * e] * out_scale, dq[i][2 * e + 1] * out_scale);
     }
   }
 }
@@ -372,7 +456,7 @@ int launch_mma(const GradParams& p, cudaStream_t stream) {
 // Order of the products: S of the next tile, acc0 of this one, acc1, dP of the next; dS runs beside S and acc0,
 // the exponentials of the next tile beside acc1 and dP.
 //
-// P of dv is rounded once to the type. dS of a row that sees few keys is held as two numbers of the type, its
+// P of dv is rounded once to the type. dS (in fp16 held up, held_up) of a row that sees few keys is held as two numbers of the type, its
 // rounding and what that leaves: such rows have the largest gradients, and delta, from the rounded out, is least
 // exact for them (two_parts). Of other rows it is rounded once.
 template <int HD_, class T_>
@@ -414,6 +498,9 @@ struct GradBars {
   uint4 answer;
   uint32_t tmem;
   GradItem item[kItems];
+  // fp16: what dS of an item is held up by. One place more than items are published ahead, so that an item's stays
+  // until all warps have taken the next one.
+  float up[kItems + 1];
 };
 static_assert(sizeof(GradBars) <= 1024, "barriers fit their place");
 
@@ -506,6 +593,9 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       const bool own = lone(p.s, it.len, r);
       float2 rr = make_float2(0.f, 0.f);
       if (!keys) rr = p.row[static_cast<int64_t>(it.head) * p.s.n + it.first + r];
+      // (read from shared memory where it is used: the registers are full)
+      auto up = [&] { return C::F16 ? B.up[i % (kItems + 1)] : 1.f; };
+      if (C::F16 && !keys) rr.x += log2_of_power(up());
       bool two = !keys && two_parts(p.s, it.len, it.row0, 128);
       for (int h = 0, j = it.jb; h < it.nh; ++g) {
         const int col0 = j * 128;  // stream row of column 0
@@ -573,6 +663,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           __syncwarp();
           if (lane == 0) mbar_arrive(&B.p_full[gk & 1]);
         }
+        const float down = Shift<T>::kDown * (keys ? up() : 1.f);
         ok = warp_wait(&B.dp_full[g & 3], (g >> 2) & 1);
         if (!ok) break;
         tc_fence_after();
@@ -587,8 +678,8 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
 #pragma unroll
           for (int c = 0; c < CW; c += 4) {
             const float4 a = *reinterpret_cast<const float4*>(nl + 128 + c);
-            ffma2(d[c], d[c + 1], Shift<T>::kDown, a.x, a.y);
-            ffma2(d[c + 2], d[c + 3], Shift<T>::kDown, a.z, a.w);
+            ffma2(d[c], d[c + 1], down, a.x, a.y);
+            ffma2(d[c + 2], d[c + 3], down, a.z, a.w);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&B.st_empty[gk & 1]);
@@ -606,7 +697,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           const int self = r - col0 - wg * CW, head = keys ? it.h0 + h : it.head;
 #pragma unroll
           for (int c = 0; c < CW; ++c)
-            if (own && c == self) d[c] = lone_ds<T>(p, head, it.first + r, v[c]);
+            if (own && c == self) d[c] = lone_ds<T>(p, head, it.first + r, keys ? v[c] * up() : v[c]);
         }
 #pragma unroll
         for (int c = 0; c < CW; c += 32) {
@@ -651,7 +742,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       const bool dv = keys && wg < C::NWG / 2;
       const int cols = keys ? HD * 2 / C::NWG : HD / C::NWG, c0 = (keys ? wg % (C::NWG / 2) : wg) * cols;
       const uint32_t acc = lanes + (dv ? C::TMEM_ACC0 : C::TMEM_ACC1) + c0;
-      const float f = dv ? Shift<T>::kDown : p.s.scale;
+      const float f = dv ? Shift<T>::kDown : p.s.scale / up();
       const Rows& to = dv ? p.dv : keys ? p.dk : p.dq;
       const int64_t row = it.first + r;
       T* out = static_cast<T*>(to.ptr) + row * to.tok + it.head * to.head + c0;
@@ -893,6 +984,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         ok = next_item(i, it);
         if (!ok || it.keys < 0) break;
         if (it.keys == 0) continue;
+        const float up = C::F16 ? B.up[i % (kItems + 1)] : 1.f;
         for (int h = 0, j = it.jb; h < it.nh; ++gk) {
           const int r0 = j * 128;
           const float2* src = p.row + static_cast<int64_t>(it.h0 + h) * p.s.n + it.first + r0;
@@ -905,7 +997,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (!ok) break;
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            stat[(gk & 1) * 256 + k * 32 + lane] = v[k].x, stat[(gk & 1) * 256 + 128 + k * 32 + lane] = v[k].y;
+            stat[(gk & 1) * 256 + k * 32 + lane] = v[k].x, stat[(gk & 1) * 256 + 128 + k * 32 + lane] = v[k].y * up;
           __syncwarp();
           if (lane == 0) mbar_arrive(&B.st_full[gk & 1]);
         }
@@ -917,11 +1009,12 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       uint32_t asked = 0;
       int out = 0;
       bool ok = true;
-      auto publish = [&](const GradItem& it) {
+      auto publish = [&](const GradItem& it, float up) {
         if (out >= kItems) ok = warp_wait(&B.item_empty[out % kItems], (out / kItems - 1) & 1);
         if (!ok) return;
         if (lane == 0) {
           B.item[out % kItems] = it;
+          if (C::F16) B.up[out % (kItems + 1)] = up;
           mbar_arrive(&B.item_full[out % kItems]);
         }
         __syncwarp();
@@ -948,7 +1041,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
             keys_of(p.s, t.len, t.row0, min(t.row0 + 128, t.len), lo, hi);
           }
           it.jb = lo / 128, it.je = (hi + 127) / 128;
-          publish(it);
+          publish(it, held_up<T>(p, t.first, keys ? it.h0 : h, it.nh, keys ? it.head : it.h0));
         }
         ok = warp_wait(&B.asked, asked++ & 1) && ok;  // (an answer lands before exit, too)
         if (!ok) break;
@@ -958,7 +1051,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       if (ok) {
         GradItem it{};
         it.keys = -1;
-        publish(it);
+        publish(it, 1.f);
       }
       if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
     }
@@ -1015,6 +1108,9 @@ int64_t most_part_bytes(int n, int hkv, int group, int hd) {
   }
   return most;
 }
+// Bytes of the workspace's other parts: GradParams::row, and most and norm (fp16).
+int64_t row_bytes(int64_t n, int hq) { return (n * hq * 8 + 15) / 16 * 16; }
+int64_t most_bytes(int64_t n, int hq, int hkv) { return (n * (hq + hkv) * 12 + 15) / 16 * 16; }
 bool tensor_memory_size(int hd) { return hd <= 128; }
 // The kernel of the other head sizes has a head of keys or queries in each of the grid's y blocks.
 bool heads_fit(int hq, int hkv, int hd) { return tensor_memory_size(hd) || hq + hkv <= 65535; }
@@ -1052,6 +1148,11 @@ int launch_tc(const GradParams& p, cudaStream_t stream) {
 template <class T>
 int launch_grad(const GradParams& p, cudaStream_t stream) {
   if (int s = launch_delta<T>(p, stream)) return s;
+  if constexpr (Shift<T>::F16) {
+    const int64_t warps = static_cast<int64_t>(p.s.b) * (p.s.hq + p.s.hkv);
+    if (warps / 8 >= 0x7fffffff) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: too many sequences");
+    if (int s = launch_behind(prompt_most_kernel, dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, stream, "prompt_most_kernel", p)) return s;
+  }
   const int hd = p.s.hd;
   if (hd <= 64) return launch_tc<64, T>(p, stream);
   if (hd <= 128) return launch_tc<128, T>(p, stream);
@@ -1066,8 +1167,7 @@ extern "C" {
 
 int64_t fold_prompt_read_grad_workspace(int n, int hq, int hkv, int hd) {
   if (n < 0 || hq < 1 || hkv < 1 || hq % hkv || hq > 65535 || hd < 8 || hd > 256 || hd % 8 || !fold::heads_fit(hq, hkv, hd)) return -1;
-  const int64_t rows = (static_cast<int64_t>(n) * hq * 8 + 15) / 16 * 16;
-  return rows + 16 + (fold::tensor_memory_size(hd) ? fold::most_part_bytes(n, hkv, hq / hkv, hd) : 0);
+  return fold::row_bytes(n, hq) + fold::most_bytes(n, hq, hkv) + 16 + (fold::tensor_memory_size(hd) ? fold::most_part_bytes(n, hkv, hq / hkv, hd) : 0);
 }
 
 int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_stride_head, const void* q,
@@ -1103,11 +1203,14 @@ int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_st
   if (!lse) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: null pointer");
   if (static_cast<int64_t>(n) * hq > (int64_t(1) << 32)) return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: too many rows");
   p.splits = tensor_memory_size(hd) ? key_splits(n, hkv, p.s.group) : 1;
-  if (!workspace || workspace_bytes < (static_cast<int64_t>(n) * hq * 8 + 15) / 16 * 16 + part_bytes(n, p.splits, hkv, hd))
+  const int64_t part_at = row_bytes(n, hq) + (dtype == FOLD_FP16 ? most_bytes(n, hq, hkv) : 0);
+  if (!workspace || workspace_bytes < part_at + part_bytes(n, p.splits, hkv, hd))
     return fail(FOLD_ERR_INVALID_ARGUMENT, "prompt read grad: the workspace holds fold_prompt_read_grad_workspace bytes");
   if (!aligned16(workspace)) return fail(FOLD_ERR_ALIGNMENT, "prompt read grad: the workspace must be 16-byte aligned");
   p.lse = lse, p.dlse = dlse, p.row = static_cast<float2*>(workspace), p.zero_rest = zero_rest, p.err = err;
-  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + (static_cast<int64_t>(n) * hq * 8 + 15) / 16 * 16);
+  p.most = reinterpret_cast<float2*>(static_cast<char*>(workspace) + row_bytes(n, hq));
+  p.norm = reinterpret_cast<float*>(p.most + static_cast<int64_t>(n) * (hq + hkv));
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_at);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == FOLD_BF16 ? launch_grad<__nv_bfloat16>(p, st) : launch_grad<__half>(p, st);
 }

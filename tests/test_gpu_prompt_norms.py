@@ -89,3 +89,32 @@ def test_few_tokens(lens, hd, dtype):
                                                 ([3100], True, (2047, -1)), ([2500], True, (-1, -1))])
 def test_longer_rows(lens, causal, window, hd, dtype):
     compare(Prompts(lens, 4, 2, hd, dtype, seed=hd), causal, window)
+
+
+@pytest.mark.parametrize("size", [100.0, 1.0, 1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n,causal", [(4096, True), (3000, False), (300, True)])
+def test_small_gradients(n, causal, hd, size):
+    """A gradient that a mean over many tokens leaves: dS of thousands of keys is far below the smallest normal number
+    of fp16 where dq and dk are not."""
+    c = Prompts([n], 4, 2, hd, "fp16", seed=hd)
+    c.do = (c.do.float() * size).to(c.dt)
+    compare(c, causal)
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+def test_gradients_of_different_sizes(hd):
+    """One sequence's large gradient does not take the bits of another's, nor do rows without one."""
+    c = Prompts([700, 900, 1000], 4, 2, hd, "fp16", seed=hd)
+    size = torch.ones(c.n, 1, 1, device="cuda")
+    size[:700], size[700:1600], size[1000:1400] = 300.0, 1e-3, 0.0
+    c.do = (c.do.float() * size).to(c.dt)
+    out, lse = read(c)
+    got = grad(c, out, lse)
+    for i, L in enumerate(c.lens):
+        w = slice(c.starts[i], c.starts[i] + L)
+        one = Prompts([L], 4, 2, hd, "fp16")
+        one.q, one.k, one.v, one.do = c.q[w], c.k[w], c.v[w], c.do[w]
+        want, norm = errors(one, out[w], True, (-1, -1))
+        ratio = {k: float((x[w].double() - want[k]).norm()) / norm[k] for k, x in zip(("dq", "dk", "dv"), got)}
+        assert max(ratio.values()) <= ROOM, (i, ratio)

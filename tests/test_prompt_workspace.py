@@ -7,13 +7,13 @@ from fold_b200.errors import FoldError
 FAR = 1 << 40
 
 
-def enough(size, n, hq, hkv, hd):
+def enough(size, n, hq, hkv, hd, dtype=0):
     """Whether a call of n rows takes a workspace of `size` bytes. Its address is off a boundary, so that the call ends
     there, before anything is launched."""
     ops = [x for i, heads in enumerate((hq, hq, hkv, hkv, hq)) for x in (FAR * (i + 2), heads * hd, hd)]
     outs = [x for i, heads in enumerate((hq, hkv, hkv)) for x in (FAR * (i + 10), heads * hd, hd)]
     try:
-        _lib.call("fold_prompt_read_grad", *ops, 16, None, 16, 1, 1, -1, -1, 1.0, *outs, 0, 8, size, n, hq, hkv, hd, 0, None,
+        _lib.call("fold_prompt_read_grad", *ops, 16, None, 16, 1, 1, -1, -1, 1.0, *outs, 0, 8, size, n, hq, hkv, hd, dtype, None,
                   None)
     except FoldError as e:
         if "16-byte aligned" in str(e) or "workspace holds" in str(e):
@@ -33,7 +33,7 @@ def test_fewer_rows(hq, hkv, hd):
     rows = sorted(rows)
     for most in rows:
         size = _lib.prompt_read_grad_workspace(most, hq, hkv, hd)
-        assert all(enough(size, n, hq, hkv, hd) for n in rows if n <= most)
+        assert all(enough(size, n, hq, hkv, hd, dtype) for n in rows if n <= most for dtype in (0, 1))
         assert not enough(size // 4 if hd > 128 else 8 * most * hq - 16, most, hq, hkv, hd)
 
 
