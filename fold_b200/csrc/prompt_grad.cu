@@ -501,6 +501,7 @@ struct GradBars {
   // fp16: what dS of an item is held up by. One place more than items are published ahead, so that an item's stays
   // until all warps have taken the next one.
   float up[kItems + 1];
+  int gave_up;  // a role's wait ran out
 };
 static_assert(sizeof(GradBars) <= 1024, "barriers fit their place");
 
@@ -546,6 +547,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       mbar_init(&B.p_full[0], NSW), mbar_init(&B.p_full[1], NSW), mbar_init(&B.dp_read, NSW);
       for (int i = 0; i < kItems; ++i) mbar_init(&B.item_full[i], 1), mbar_init(&B.item_empty[i], 3 + NSW);
       mbar_init(&B.asked, 1), mbar_init(&B.drained, 1);
+      B.gave_up = 0;
       fence_mbar_init();
     }
     __syncwarp();
@@ -558,6 +560,10 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
   __syncthreads();  // barriers and the address of tensor memory are visible
   tc_fence_after();
   const uint32_t tmem = B.tmem;
+  auto give_up = [&] {
+    *const_cast<volatile int*>(&B.gave_up) = 1;
+    set_error(p.err, FOLD_DEVERR_TIMEOUT);
+  };
   // Every role walks the items in the scheduler's order.
   auto next_item = [&](int i, GradItem& it) {
     if (!warp_wait(&B.item_full[i % kItems], (i / kItems) & 1)) return false;
@@ -769,7 +775,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       __syncwarp();
       tc_fence_before();  // the next item's acc0 comes behind its first tile's P, acc1 behind all reads of its dP
     }
-    if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+    if (!ok && lane == 0) give_up();
   } else {
     regs_down<kOtherRegs>();
     if (warp == NSW) {
@@ -816,7 +822,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           ++b_sent;
         }
       }
-      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+      if (!ok && lane == 0) give_up();
       // copies land before exit, those of a tile that another wait gave up on too
       for (uint32_t w = a_sent > NA ? a_sent - NA : 0; w < a_sent; ++w) warp_wait(&B.a_full[w % NA], (w / NA) & 1);
       for (uint32_t w = b_sent > NB ? b_sent - NB : 0; w < b_sent; ++w) warp_wait(&B.b_full[w % NB], (w / NB) & 1);
@@ -968,7 +974,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       }
       if (!ok) {  // let what was issued finish before tensor memory goes
         if (elect_one()) {
-          set_error(p.err, FOLD_DEVERR_TIMEOUT);
+          give_up();
           tc_commit(&B.drained);
         }
         __syncwarp();
@@ -1002,7 +1008,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
           if (lane == 0) mbar_arrive(&B.st_full[gk & 1]);
         }
       }
-      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+      if (!ok && lane == 0) give_up();
     } else {
       // ------------------------------------------------------------ scheduler
       const int key_heads = p.s.hkv * p.splits, numbers = key_items / key_heads;
@@ -1010,7 +1016,11 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
       int out = 0;
       bool ok = true;
       auto publish = [&](const GradItem& it, float up) {
-        if (out >= kItems) ok = warp_wait(&B.item_empty[out % kItems], (out / kItems - 1) & 1);
+        // An item lasts for seconds where many heads share a KV head and a million rows (128 heads: 1.8 s), so this
+        // wait goes on while no other role has given up.
+        if (out >= kItems)
+          for (int tries = 0; !(ok = warp_wait(&B.item_empty[out % kItems], (out / kItems - 1) & 1)) && tries < 64; ++tries)
+            if (__any_sync(0xffffffffu, *const_cast<const volatile int*>(&B.gave_up))) break;
         if (!ok) return;
         if (lane == 0) {
           B.item[out % kItems] = it;
@@ -1053,7 +1063,7 @@ __global__ void __launch_bounds__(C::NTHREADS, 1)
         it.keys = -1;
         publish(it, 1.f);
       }
-      if (!ok && lane == 0) set_error(p.err, FOLD_DEVERR_TIMEOUT);
+      if (!ok && lane == 0) give_up();
     }
   }
   tc_fence_before();
