@@ -12,7 +12,7 @@
 // search reads refs from the start until it has found enough free pages (16K counts a round). The copy of
 // a fork is memory bound. Measured (the GPU's time): five tokens of one sequence grown and trimmed 7 us (two
 // launches), 20000 tokens of 250 sequences 17.5 us; 160 children of 40 sequences in 24 layers, 237 MB copied, with
-// their rows freed before, 78 us (6.1 TB/s, 0.93 of the measured copy rate).
+// their rows freed before, 80 us (5.9 TB/s, 0.90 of the measured copy rate).
 #include "common.cuh"
 #include "host_common.h"
 

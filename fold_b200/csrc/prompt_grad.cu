@@ -10,11 +10,11 @@
 // in memory would take five, but no sum depends on the order in which blocks run, and nothing of the
 // size of P is written.
 //
-// Measured (bf16, head size 128, 32 query and 8 KV heads, one causal sequence; the GPU's time of captured calls):
-// 8192 tokens 1.59 ms (866 TFLOP/s of five products, 1.21 PFLOP/s of the seven made; 1.8 ms in a long run, where
-// the board is at its 1000 W), 2048 tokens 188 us, 64 tokens 19 us. A tile of 128 x 128 takes a key's item 3300
+// Measured (bf16, head size 128, 32 query and 8 KV heads, one causal sequence; the GPU's time of captured calls, a dozen
+// in a row): 8192 tokens 1.62 ms (848 TFLOP/s of five products, 1.19 PFLOP/s of the seven made; 1.8-1.9 ms in a long
+// run, where the board is at its 1000 W), 2048 tokens 186 us, 64 tokens 19 us; fp16 1.69 ms, 192 us, 23-29 us. A tile of 128 x 128 takes a key's item 3300
 // cycles and a row's 2700, of which the products are 2050 and 1540: what bounds it is the chain dP, dS, acc1, dP of
-// the next, and the energy of the products. At head size 64 (1.45 ms at 8192 tokens) the exponentials and dS, 2100
+// the next, and the energy of the products. At head size 64 (1.36 ms at 8192 tokens) the exponentials and dS, 2100
 // to 2800 cycles a tile.
 #include "prompt.cuh"
 #include "tcgen05.cuh"
@@ -54,8 +54,9 @@ struct Shift {
 // so that nothing passes the type's range that did not before: 1 where the bound is 2^15 or more or not finite.
 // Typical dS of n keys lie some 2^5 n below the bound, which leaves 12 binades for smaller rows at 4096 keys. A NaN
 // makes its own results NaN whatever the bound, so it is left out. The norms come from the rows' first kernel, their
-// maxima from a launch of their own (5 us of 185 for 2048 rows of 32 heads): with the factor in the softmax fp16 takes
-// 192 us there where it took 185; 8192 rows 1.95 ms for 1.91, a batch of short sequences 6 to 10 percent more. Maxima by atomics in the first kernel took it from 15 to 33 us.
+// maxima from a launch of their own (5 us for 2048 rows of 32 heads): with the factor in the softmax 2048 rows take
+// 192 us where they took 185, 8192 rows in a long run 1.95 ms for 1.91, a batch of short sequences 6 to 10 percent
+// more. Maxima by atomics in the first kernel took that from 15 to 33 us.
 // Rows' items hold dS up through P, which dq has no other use of; keys' need P for dv as it is.
 // Heads [h0, h0 + nh) with KV head hk of the sequence from row `first` on; all lanes of a warp call this.
 __device__ __forceinline__ float warp_most(float x) {  // of numbers that are not negative
@@ -235,9 +236,10 @@ __device__ __forceinline__ float lone_ds(const GradParams& p, int h, int at, flo
 // Whether dS of the rows [row0, row0 + rows) is held in two parts: where the last one sees up to 512 keys, or 2048
 // if the rows before it see as many (behind a window, or without causality: gradients do not fall off there). Such
 // rows have the largest gradients, and delta, from the rounded out, is least exact for them. Against 64 bits
-// dq of 100 to 300 tokens is off by 1.06 times the rounding of dq alone, by 1.5 times with one part; of 1500
-// tokens 1.15; of 4096 tokens 1.44 with one part throughout. The second part costs a product and its conversions, a
-// fifth of a tile's time.
+// dq of 100 to 300 tokens is off by 1.07 (heads of 128) to 1.17 times (64) the rounding of dq alone, by 1.5 times with
+// one part; of 1500 tokens 1.18 to 1.26, of 4096 tokens, most rows of which have one, 1.24 to 1.38. The limits are
+// where that ratio was found to pass 1.5 for the last rows; beyond them it does so without causality alone (4096
+// tokens 1.46 to 1.58). The second part costs a product and its conversions, a fifth of a tile's time.
 __device__ __forceinline__ bool two_parts(const Shape& p, int len, int row0, int rows) {
   const int r = min(row0 + rows, len) - 1;
   int lo, hi;

@@ -10,9 +10,9 @@
 // the output alone is 0.0016 and 0.0002.
 //
 // Measured (bf16, head size 128, 32 query and 8 KV heads, causal; the GPU's time): one sequence of 16384 tokens
-// 1.97 ms in a long run (1116 TFLOP/s, 0.80 of the measured sustained GEMM rate; the board is at its 1000 W), of 8192
-// tokens 465 us (1184 TFLOP/s), of 2048 53 us, of 512 15 us, of 40 9 us; 24 sequences of up to 2100 tokens
-// 449 us. A tile's turn is a chain (softmax 1500-1600 cycles, P V and the next S 1024) which the other tile
+// 1.99 ms in a long run (1107 TFLOP/s, 0.79 of the measured sustained GEMM rate; the board is at its 1000 W), 1.74 ms
+// a dozen times in a row, of 8192 tokens 475 us (1157 TFLOP/s), of 2048 52 us, of 512 15 us, of 40 9 us; 24 sequences
+// of up to 2100 tokens 452 us. A tile's turn is a chain (softmax 1500-1600 cycles, P V and the next S 1024) which the other tile
 // fills: 1840 cycles a tile for 1024 of products. Short sequences lose half of the diagonal tiles and some 4 us a
 // block's tile for its start and its result. Exponentials by polynomial beside the special unit were slower (8192
 // tokens 537 us for 474).

@@ -615,7 +615,7 @@ def prompt_read(q, k, v, qsl, out, *, softmax_scale, causal=True, window_size=(-
     its keys [r - left, r + right] of window_size (left, right) (-1: unbounded), up to its own when
     causal. Writes out [n, Hq, D] (which may be q) and, when given, lse [Hq, n] float32; rows outside the
     sequences are left alone. Values must be finite, seen or not, within their sequence. Keys and values go to
-    a paged cache by append_paged; prompt_read_grad is the gradient."""
+    a paged cache by append_paged; prompt_read_grad is the gradient (the result has no autograd history)."""
     dev = _check_devices("prompt_read", q, k, v, qsl, out, lse, err)
     n, hq, hkv, d, code, b = _prompt_shape("prompt_read", q, k, qsl, lse)
     os = _prompt_out("prompt_read", "out", out, n, hq, d, q.dtype)
