@@ -12,10 +12,10 @@
 //
 // Measured (bf16, head size 128, 32 query and 8 KV heads, one causal sequence; the GPU's time of captured calls, a dozen
 // in a row): 8192 tokens 1.62 ms (848 TFLOP/s of five products, 1.19 PFLOP/s of the seven made; 1.8-1.9 ms in a long
-// run, where the board is at its 1000 W), 2048 tokens 186 us, 64 tokens 19 us; fp16 1.69 ms, 192 us, 23-29 us. A tile of 128 x 128 takes a key's item 3300
-// cycles and a row's 2700, of which the products are 2050 and 1540: what bounds it is the chain dP, dS, acc1, dP of
-// the next, and the energy of the products. At head size 64 (1.36 ms at 8192 tokens) the exponentials and dS, 2100
-// to 2800 cycles a tile.
+// run, where the board is at its 1000 W), 2048 tokens 186 us, 64 tokens 19 us; fp16 1.69 ms, 192 us, 23-29 us. A tile
+// of 128 x 128 takes a key's item 3300 cycles and a row's 2700, of which the products are 2050 and 1540: what bounds it
+// is the chain dP, dS, acc1, dP of the next, and the energy of the products. At head size 64 (1.36 ms at 8192 tokens)
+// the exponentials and dS, 2100 to 2800 cycles a tile.
 #include "prompt.cuh"
 #include "tcgen05.cuh"
 
@@ -47,6 +47,13 @@ struct Shift {
   static constexpr float kDown = F16 ? 1.f / 1024.f : 1.f;
 };
 
+__device__ __forceinline__ float warp_most(float x) {  // of numbers that are not negative
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x)));
+}
+__device__ __forceinline__ float2* most_of(const GradParams& p, int first) {
+  return p.most + static_cast<int64_t>(first) * (p.s.hq + p.s.hkv);
+}
+
 // dS of fp16 is held up too, by a power of two that dq and dk take back out: dS of thousands of keys and a small dout
 // lies below the type's normal numbers (2^-14) where dq and dk do not (4096 keys, dout of size 0.001: dq was off by
 // 3.5 to 4.5 times its own rounding, now by 1.25). The power follows a bound of dS in a sequence,
@@ -59,12 +66,6 @@ struct Shift {
 // more. Maxima by atomics in the first kernel took that from 15 to 33 us.
 // Rows' items hold dS up through P, which dq has no other use of; keys' need P for dv as it is.
 // Heads [h0, h0 + nh) with KV head hk of the sequence from row `first` on; all lanes of a warp call this.
-__device__ __forceinline__ float warp_most(float x) {  // of numbers that are not negative
-  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(x)));
-}
-__device__ __forceinline__ float2* most_of(const GradParams& p, int first) {
-  return p.most + static_cast<int64_t>(first) * (p.s.hq + p.s.hkv);
-}
 template <class T>
 __device__ __forceinline__ float held_up(const GradParams& p, int first, int h0, int nh, int hk) {
   if constexpr (!Shift<T>::F16) return 1.f;
@@ -458,9 +459,9 @@ int launch_mma(const GradParams& p, cudaStream_t stream) {
 // Order of the products: S of the next tile, acc0 of this one, acc1, dP of the next; dS runs beside S and acc0,
 // the exponentials of the next tile beside acc1 and dP.
 //
-// P of dv is rounded once to the type. dS (in fp16 held up, held_up) of a row that sees few keys is held as two numbers of the type, its
-// rounding and what that leaves: such rows have the largest gradients, and delta, from the rounded out, is least
-// exact for them (two_parts). Of other rows it is rounded once.
+// P of dv is rounded once to the type. dS (in fp16 held up, held_up) of a row that sees few keys is held as two numbers
+// of the type, its rounding and what that leaves: such rows have the largest gradients, and delta, from the rounded
+// out, is least exact for them (two_parts). Of other rows it is rounded once.
 template <int HD_, class T_>
 struct GradCfg {
   using T = T_;

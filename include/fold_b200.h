@@ -245,9 +245,9 @@ int fold_prompt_read(const void* q, int64_t q_stride_tok, int64_t q_stride_head,
  * and its results out and lse, the gradients dq [n, hq, hd], dk and dv [n, hkv, hd], those of a key or
  * value summed over the heads of its group. Rows outside the sequences get zeros when `zero_rest`, else
  * they are left as they were. As for values, a row of q and dout must be finite even for keys that it does not
- * see, and a key and value for rows that do not see it. No sum depends on the order in which blocks run: equal calls give equal
- * bits. The gradients must not share memory with the inputs or each other (refused, as above). workspace: fold_prompt_read_grad_workspace bytes of
- * device memory, 16-byte aligned, not shared by calls that may overlap; nothing in it outlives the call. */
+ * see, and a key and value for rows that do not see it. No sum depends on the order in which blocks run: equal
+ * calls give equal bits. The gradients must not share memory with the inputs or each other (refused, as above).
+ * workspace: fold_prompt_read_grad_workspace bytes of device memory, 16-byte aligned, not shared by calls that may overlap; nothing in it outlives the call. */
 int fold_prompt_read_grad(const void* dout, int64_t do_stride_tok, int64_t do_stride_head, const void* q,
                           int64_t q_stride_tok, int64_t q_stride_head, const void* k, int64_t k_stride_tok,
                           int64_t k_stride_head, const void* v, int64_t v_stride_tok, int64_t v_stride_head,
